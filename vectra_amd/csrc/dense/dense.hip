@@ -1,0 +1,705 @@
+// The dense operators' C ABI (include/vectra_dense.h): argument checks, the
+// plan of a call (which products, on which tiles, through which scratch) and
+// the small kernels around the products.
+//
+// A backward pass is
+//   [x^ = the 8-bit rows' values]       where the input was kept in 8 bits
+//   [dz, sums of dz] = slope epilogue of x W^T      (an activation or a gate)
+//   dx = dz W;   dW = dz^T x;   db = the sums, added up.
+// z is computed again rather than kept: that is one more product, but no
+// [rows, width_out] tensor lives from the forward to the backward pass, and at
+// the price model's widths (128 to 256) reading x again is cheaper than
+// reading z back.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "dense_common.h"
+#include "dense_kernels.h"
+
+namespace vectra_dense {
+namespace {
+
+constexpr int kBlock = 32;  // elements that share a power of two
+
+// ----------------------------------------------------------------- kernels
+
+// Copies rows into rows of whole 16-byte chunks (zero padded): operands whose
+// rows are not 16-byte aligned or hold part of a chunk at their end.  One
+// thread per output chunk.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* x, int64_t stride, int64_t rows, int64_t width, T* out,
+                                                   int64_t chunks) {
+  constexpr int kPer = 16 / sizeof(T);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * chunks) return;
+  const int64_t row = at / chunks, first = (at - row * chunks) * kPer;
+  const T* p = x + row * stride + first;
+  T v[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) v[e] = first + e < width ? p[e] : static_cast<T>(0.f);
+  u32x4 w;
+  __builtin_memcpy(&w, v, 16);
+  *reinterpret_cast<u32x4*>(out + at * kPer) = w;
+}
+
+// Zeros columns [from, stride) of a matrix.
+template <typename T>
+__global__ __launch_bounds__(256) void zero_tail_kernel(T* x, int64_t rows, int64_t from, int64_t stride) {
+  const int64_t n = stride - from;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at < rows * n) x[at / n * stride + from + at % n] = static_cast<T>(0.f);
+}
+
+// Adds up the planes of a split product in order and finishes it:
+// act(sum + bias) + residual.  One thread per four columns.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float* parts, int splits, int64_t m, int64_t n, int64_t ld,
+                                                   GemmParams p) {
+  const int64_t quads = ld / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= m * quads) return;
+  const int64_t row = at / quads, col = (at - row * quads) * 4;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(parts + k * m * ld + row * ld + col);
+  const int left = static_cast<int>(min<int64_t>(n - col, 4));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (p.bias && e < left) s[e] += load_bias(p.bias, col + e, p.bias_dtype);
+    s[e] = act_value(s[e], p.activation);
+  }
+  if (p.residual) s += load4(static_cast<const T*>(p.residual) + row * p.ldr + col, left, p.vec & kVecResidual);
+  store4(static_cast<T*>(p.out) + row * p.ldo + col, s, left, p.vec & kVecOut);
+}
+
+// Sums of 64 columns over the rows [blockIdx.y * per, ...): 16 row lanes of 64
+// columns, joined in LDS in a fixed order.  In: T or float; out: one row of
+// partial sums per blockIdx.y, or with one block the bias gradient itself.
+template <typename In>
+__global__ __launch_bounds__(1024) void column_sums_kernel(const In* x, int64_t stride, int64_t rows, int64_t n,
+                                                           int64_t per, void* out, int64_t out_stride,
+                                                           int32_t out_dtype) {
+  __shared__ float part[16][64];
+  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + c;
+  const int64_t first = blockIdx.y * per, last = min(first + per, rows);
+  float s = 0.f;
+  if (col < n)
+    for (int64_t row = first + r; row < last; row += 16) s += widen(x[row * stride + col]);
+  part[r][c] = s;
+  __syncthreads();
+  if (r != 0 || col >= n) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) s += part[k][c];
+  const int64_t at = blockIdx.y * out_stride + col;
+  if (out_dtype == VECTRA_DENSE_F32)
+    static_cast<float*>(out)[at] = s;
+  else if (out_dtype == VECTRA_DENSE_F16)
+    static_cast<_Float16*>(out)[at] = narrow<_Float16>(s);
+  else
+    static_cast<__bf16*>(out)[at] = narrow<__bf16>(s);
+}
+
+// ------------------------------------------------------------- 8-bit rows
+
+// The exponent byte of a block whose largest finite magnitude is `largest`:
+// the smallest e with largest <= 448 * 2^e, at least `lowest`, plus 127.
+// largest = f * 2^x with f in [1, 2): 448 = 1.75 * 2^8.
+__device__ __forceinline__ int block_exponent(float largest, int lowest) {
+  const uint32_t bits = __float_as_uint(largest);
+  int e;
+  if (bits < 0x00800000u) {
+    e = lowest;  // zero or an fp32 subnormal: far below the lowest exponent
+  } else {
+    e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x007fffffu) > 0x00600000u ? 1 : 0);
+  }
+  return max(e, lowest) + 127;
+}
+
+// 2^e as fp32 for e in [-126, 127].
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// fp32 in [-448, 448] to e4m3, ties to even (v_cvt_pk_fp8_f32); NaN to NaN.
+__device__ __forceinline__ uint32_t to_e4m3x4(f32x4 v) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true));
+}
+
+__device__ __forceinline__ f32x4 from_e4m3x4(uint32_t w) {
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
+  return f32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Eight lanes per block of 32, four elements per lane.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows, int64_t width, int64_t stride,
+                                                       uint8_t* codes, int64_t codes_stride, uint8_t* scales,
+                                                       int64_t scales_stride, int64_t blocks, int vec) {
+  constexpr int kLowest = sizeof(T) == 2 && !__is_same(T, __bf16) ? -15 : -117;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
+  const bool live = at < rows * blocks;
+  const int64_t row = live ? at / blocks : 0, block = live ? at - row * blocks : 0;
+  const int64_t col = block * kBlock + (threadIdx.x & 7) * 4;
+  const int left = live ? static_cast<int>(max<int64_t>(min<int64_t>(width - col, 4), 0)) : 0;
+  f32x4 v = load4(x + row * stride + col, left, vec & 1);
+  float largest = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = __builtin_fabsf(v[e]);
+    if (a <= 3.4028234663852886e38f) {
+      largest = a > largest ? a : largest;
+    } else {
+      v[e] = __builtin_nanf("");
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+  const int byte = block_exponent(largest, kLowest);
+  const int e = byte - 127;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] *= power_of_two(-e);  // e in [-117, 120]
+  if constexpr (__is_same(T, _Float16)) {
+    // 65504 = 255.875 * 2^8 would round to 256 * 2^8, which fp16 lacks: at
+    // e = 8, magnitudes of 248 and more take the code below, 240.
+    if (e == 8)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (__builtin_fabsf(v[k]) >= 248.f) v[k] = __builtin_copysignf(240.f, v[k]);
+  }
+  const uint32_t w = to_e4m3x4(v);
+  uint8_t* const out = codes + row * codes_stride + col;
+  if (left == 4 && (vec & 2)) {
+    *reinterpret_cast<uint32_t*>(out) = w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < left) out[k] = static_cast<uint8_t>(w >> (8 * k));
+  }
+  if (live && (threadIdx.x & 7) == 0) scales[row * scales_stride + block] = static_cast<uint8_t>(byte);
+}
+
+// One thread per four columns of the output's `ld` columns; columns from
+// `width` on are zeros (the workspace's padded rows).
+template <typename T>
+__global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, int64_t codes_stride,
+                                                         const uint8_t* scales, int64_t scales_stride, int64_t rows,
+                                                         int64_t width, T* out, int64_t out_stride, int64_t columns,
+                                                         int vec) {
+  const int64_t quads = (columns + 3) / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * quads) return;
+  const int64_t row = at / quads, col = (at - row * quads) * 4;
+  const int left = static_cast<int>(max<int64_t>(min<int64_t>(width - col, 4), 0));
+  const uint8_t* const p = codes + row * codes_stride + col;
+  uint32_t w = 0;
+  if (left == 4 && (vec & 2)) {
+    w = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < left) w |= static_cast<uint32_t>(p[k]) << (8 * k);
+  }
+  f32x4 v = from_e4m3x4(w);
+  if (left > 0) {
+    const int e = static_cast<int>(scales[row * scales_stride + col / kBlock]) - 127;
+    const float s = e == 128 ? __builtin_nanf("") : e == -127 ? 5.877471754111438e-39f : power_of_two(e);
+    v *= s;
+  }
+  store4(out + row * out_stride + col, v, static_cast<int>(min<int64_t>(columns - col, 4)), vec & 1);
+}
+
+// -------------------------------------------------------------------- host
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int64_t element_size(int32_t dtype) { return dtype == VECTRA_DENSE_F32 ? 4 : 2; }
+
+// CUs of the current device (an atomic per device id, filled once).
+int compute_units() {
+  static std::atomic<int> known[64];
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) return 256;
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n <= 0) n = 256;
+    known[device].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Scratch memory in order of use.  Without a base only the size is found.
+struct Scratch {
+  char* base;
+  int64_t used;
+  void* take(int64_t bytes) {
+    void* const p = base ? base + used : nullptr;
+    used += (bytes + 255) & ~int64_t{255};
+    return p;
+  }
+};
+
+struct Matrix {
+  const void* p;
+  int64_t ld;
+};
+
+// One call: the element type, the scratch and whether kernels are launched.
+struct Call {
+  int32_t dtype;
+  Scratch scratch;
+  bool launch;
+  hipStream_t stream;
+  int cus;
+  int status = VECTRA_DENSE_OK;
+
+  int64_t esize() const { return element_size(dtype); }
+  int64_t per() const { return 16 / esize(); }
+  void check() {
+    if (hipGetLastError() != hipSuccess && status == VECTRA_DENSE_OK) status = VECTRA_DENSE_ERR_LAUNCH;
+  }
+  bool go() const { return launch && status == VECTRA_DENSE_OK; }
+
+  template <typename F>
+  void typed(F&& f) {
+    switch (dtype) {
+      case VECTRA_DENSE_F32: f(static_cast<float*>(nullptr)); break;
+      case VECTRA_DENSE_F16: f(static_cast<_Float16*>(nullptr)); break;
+      default: f(static_cast<__bf16*>(nullptr)); break;
+    }
+    check();
+  }
+
+  bool whole_chunks(const void* p, int64_t ld, int64_t width) const {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % per() == 0 && width % per() == 0;
+  }
+
+  int64_t padded(int64_t width) const { return ceil_div(width, per()) * per(); }
+
+  // The operand as the products read it: itself where its rows are 16-byte
+  // aligned and of whole chunks, else a zero-padded copy.
+  Matrix operand(const void* p, int64_t ld, int64_t rows, int64_t width) {
+    if (rows == 0 || width == 0 || whole_chunks(p, ld, width)) return {p, ld};
+    const int64_t out_ld = padded(width), chunks = out_ld / per();
+    void* const out = scratch.take(rows * out_ld * esize());
+    if (go())
+      typed([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        pack_kernel<T><<<static_cast<uint32_t>(ceil_div(rows * chunks, 256)), 256, 0, stream>>>(
+            static_cast<const T*>(p), ld, rows, width, static_cast<T*>(out), chunks);
+      });
+    return {out, out_ld};
+  }
+
+  int vec4(const void* p, int64_t ld, int flag) const {
+    return (reinterpret_cast<uintptr_t>(p) & (4 * esize() - 1)) == 0 && ld % 4 == 0 ? flag : 0;
+  }
+
+  // A product through the tile whose workgroups fill the CUs; where even the
+  // smallest tile leaves most CUs idle and the contraction is long, it is
+  // split and joined.
+  void product(GemmParams p, int layout, int epi) {
+    const bool gated = epi == kEpiGated || epi == kEpiGatedSlope;
+    const int64_t columns = gated ? 2 * p.n : p.n;
+    const int deep = static_cast<int>(128 / esize());
+    p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
+    int tile = kTileCount - 1;
+    for (int t = 0; t < kTileCount; ++t) {
+      const int64_t tiles = ceil_div(p.m, kTileM[t]) * ceil_div(columns, kTileN[t]);
+      if (tiles >= cus * 3 / 4) {
+        tile = t;
+        break;
+      }
+    }
+    int splits = 1;
+    if (epi == kEpiStore) {
+      // Medium tiles on parts of the contraction rather than small ones on all of it.
+      const int64_t medium = ceil_div(p.m, 128) * ceil_div(columns, 128);
+      if (tile == kTileCount - 1 && p.k_tiles >= 8) {
+        if (medium * p.k_tiles / 4 >= cus / 2) tile = kTileMedium;
+        const int64_t tiles = ceil_div(p.m, kTileM[tile]) * ceil_div(columns, kTileN[tile]);
+        splits = static_cast<int>(std::min<int64_t>(ceil_div(2 * cus, tiles), p.k_tiles / 4));
+        splits = std::max(1, std::min(splits, 256));
+      }
+    }
+    p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileM[tile]));
+    p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileN[tile]));
+    last_tiles_m = p.tiles_m;
+    p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
+    splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
+    if (splits == 1) {
+      run(p, layout, tile, epi, 1);
+      return;
+    }
+    const int64_t ld = ceil_div(p.n, 4) * 4, kept = scratch.used;
+    float* const parts = static_cast<float*>(scratch.take(splits * p.m * ld * 4));
+    GemmParams q = p;
+    q.out = parts;
+    q.ldo = ld;
+    run(q, layout, tile, kEpiPartial, splits);
+    if (go())
+      typed([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        join_kernel<T><<<static_cast<uint32_t>(ceil_div(p.m * (ld / 4), 256)), 256, 0, stream>>>(parts, splits, p.m, p.n,
+                                                                                               ld, p);
+      });
+    most = std::max(most, scratch.used);
+    scratch.used = kept;  // the next product may use it again: launches of one stream run in order
+  }
+  int64_t most = 0;          // of scratch, over all products
+  int64_t last_tiles_m = 0;  // tile rows of the last product
+
+  void run(const GemmParams& p, int layout, int tile, int epi, int splits) {
+    if (!go()) return;
+    const auto f = dtype == VECTRA_DENSE_F32 ? launch_gemm_f32 : dtype == VECTRA_DENSE_F16 ? launch_gemm_f16 : launch_gemm_bf16;
+    const int st = f(p, layout, tile, epi, splits, stream);
+    if (st != VECTRA_DENSE_OK) status = st;
+  }
+
+  // Column sums of [rows, n] into the bias's gradient.
+  template <typename In>
+  void column_sums(const In* x, int64_t stride, int64_t rows, int64_t n, void* out, int32_t out_dtype) {
+    const uint32_t across = static_cast<uint32_t>(ceil_div(n, 64));
+    int64_t parts = std::min<int64_t>(ceil_div(rows, 128), std::max<int64_t>(1, 4 * cus / across));
+    parts = std::max<int64_t>(1, std::min<int64_t>(parts, 1024));
+    if (parts == 1) {
+      if (go()) column_sums_kernel<In><<<dim3(across, 1), 1024, 0, stream>>>(x, stride, rows, n, rows, out, 0, out_dtype);
+    } else {
+      const int64_t per = ceil_div(rows, parts);
+      float* const sums = static_cast<float*>(scratch.take(parts * n * 4));
+      if (go()) {
+        column_sums_kernel<In><<<dim3(across, static_cast<uint32_t>(parts)), 1024, 0, stream>>>(
+            x, stride, rows, n, per, sums, n, VECTRA_DENSE_F32);
+        column_sums_kernel<float><<<dim3(across, 1), 1024, 0, stream>>>(sums, n, parts, n, parts, out, 0, out_dtype);
+      }
+    }
+    check();
+  }
+};
+
+constexpr int64_t kMostRows = int64_t{1} << 30;
+constexpr int64_t kMostWidth = int64_t{1} << 21;
+
+bool known_dtype(int32_t t) { return t == VECTRA_DENSE_F32 || t == VECTRA_DENSE_F16 || t == VECTRA_DENSE_BF16; }
+
+// Sizes that the kernels' 32-bit offsets within a tile and their grids cover.
+int check_sizes(int64_t rows, int64_t width_in, int64_t width_out, int gated) {
+  if (rows < 0 || width_in < 0 || width_out < 0) return VECTRA_DENSE_ERR_BAD_SHAPE;
+  if (rows > kMostRows || width_in > kMostWidth || width_out > kMostWidth) return VECTRA_DENSE_ERR_TOO_LARGE;
+  // Elementwise kernels: a thread per four elements, fewer than 2^32 threads.
+  const int64_t widest = std::max(width_in, width_out * (1 + gated)) + 64;
+  if (rows * widest >= int64_t{1} << 34) return VECTRA_DENSE_ERR_TOO_LARGE;
+  return VECTRA_DENSE_OK;
+}
+
+// A row stride covers the row, and 256 rows (a gated weight's tile: a whole
+// half and 256 rows) span less than 2^31 bytes.
+int check_stride(int64_t stride, int64_t width, int64_t rows, int64_t span_rows, int64_t esize) {
+  if (rows > 1 && stride < width) return VECTRA_DENSE_ERR_BAD_SHAPE;
+  if (stride < 0) return VECTRA_DENSE_ERR_BAD_SHAPE;
+  if (stride > (int64_t{1} << 40) || span_rows * std::max<int64_t>(stride, 64) * esize >= (int64_t{1} << 31))
+    return VECTRA_DENSE_ERR_TOO_LARGE;
+  return VECTRA_DENSE_OK;
+}
+
+bool known_activation(int32_t a) { return a >= VECTRA_DENSE_NONE && a <= VECTRA_DENSE_SILU; }
+
+int check_forward(const vectra_dense_args* a) {
+  if (!a) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  if (a->struct_size != static_cast<int64_t>(sizeof(vectra_dense_args))) return VECTRA_DENSE_ERR_BAD_STRUCT;
+  if (!known_dtype(a->dtype)) return VECTRA_DENSE_ERR_BAD_DTYPE;
+  if (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != VECTRA_DENSE_F32) return VECTRA_DENSE_ERR_BAD_DTYPE;
+  if (!known_activation(a->activation)) return VECTRA_DENSE_ERR_BAD_ACTIVATION;
+  if (a->gated != 0 && a->gated != 1) return VECTRA_DENSE_ERR_BAD_SHAPE;
+  if (a->gated && a->residual) return VECTRA_DENSE_ERR_BAD_SHAPE;
+  const int64_t es = element_size(a->dtype);
+  if (int st = check_sizes(a->rows, a->width_in, a->width_out, a->gated)) return st;
+  if (a->rows == 0 || a->width_out == 0) return VECTRA_DENSE_OK;
+  if (!a->out || (a->width_in && (!a->x || !a->weight))) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  const int64_t n_w = a->width_out * (1 + a->gated);
+  if (int st = check_stride(a->x_stride, a->width_in, a->rows, 256, es)) return st;
+  if (int st = check_stride(a->weight_stride, a->width_in, n_w, a->gated ? a->width_out + 256 : 256, es)) return st;
+  if (int st = check_stride(a->out_stride, a->width_out, a->rows, 1, es)) return st;
+  if (a->residual)
+    if (int st = check_stride(a->residual_stride, a->width_out, a->rows, 1, es)) return st;
+  return VECTRA_DENSE_OK;
+}
+
+void forward(const vectra_dense_args& a, Call& c) {
+  if (a.rows == 0 || a.width_out == 0) return;
+  const int64_t n_w = a.width_out * (1 + a.gated);
+  const Matrix x = c.operand(a.x, a.x_stride, a.rows, a.width_in);
+  const Matrix w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
+  GemmParams p{};
+  p.a = x.p;
+  p.lda = x.ld;
+  p.b = w.p;
+  p.ldb = w.ld;
+  p.m = a.rows;
+  p.n = a.width_out;
+  p.depth = p.depth_b = c.padded(a.width_in);
+  p.out = a.out;
+  p.ldo = a.out_stride;
+  p.bias = a.bias;
+  p.bias_dtype = a.bias_dtype;
+  p.activation = a.activation;
+  p.residual = a.residual;
+  p.ldr = a.residual_stride;
+  p.vec = c.vec4(a.out, a.out_stride, kVecOut) | c.vec4(a.residual, a.residual_stride, kVecResidual);
+  c.product(p, kLayoutForward, a.gated ? kEpiGated : kEpiStore);
+}
+
+int check_backward(const vectra_dense_grad_args* a) {
+  if (!a) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  if (a->struct_size != static_cast<int64_t>(sizeof(vectra_dense_grad_args))) return VECTRA_DENSE_ERR_BAD_STRUCT;
+  if (!known_dtype(a->dtype)) return VECTRA_DENSE_ERR_BAD_DTYPE;
+  if ((a->bias || a->dbias) && a->bias_dtype != a->dtype && a->bias_dtype != VECTRA_DENSE_F32)
+    return VECTRA_DENSE_ERR_BAD_DTYPE;
+  if (!known_activation(a->activation)) return VECTRA_DENSE_ERR_BAD_ACTIVATION;
+  if (a->gated != 0 && a->gated != 1) return VECTRA_DENSE_ERR_BAD_SHAPE;
+  const int64_t es = element_size(a->dtype);
+  if (int st = check_sizes(a->rows, a->width_in, a->width_out, a->gated)) return st;
+  const int64_t n_w = a->width_out * (1 + a->gated);
+  const bool any = a->rows && a->width_out;
+  if (any && !a->grad) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  if (any && a->width_in) {
+    if (!a->weight) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+    if (!a->x && !(a->codes && a->scales)) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  }
+  if (any) {
+    if (a->x) {
+      if (int st = check_stride(a->x_stride, a->width_in, a->rows, 256, es)) return st;
+    } else {
+      if (int st = check_stride(a->codes_stride, a->width_in, a->rows, 1, 1)) return st;
+      if (int st = check_stride(a->scales_stride, ceil_div(a->width_in, kBlock), a->rows, 1, 1)) return st;
+    }
+    if (int st = check_stride(a->weight_stride, a->width_in, n_w, a->gated ? a->width_out + 256 : 256, es)) return st;
+    if (int st = check_stride(a->grad_stride, a->width_out, a->rows, 256, es)) return st;
+  }
+  if (a->dx && a->rows && a->width_in)
+    if (int st = check_stride(a->dx_stride, a->width_in, a->rows, 1, es)) return st;
+  if (a->dweight && n_w && a->width_in)
+    if (int st = check_stride(a->dweight_stride, a->width_in, n_w, 1, es)) return st;
+  return VECTRA_DENSE_OK;
+}
+
+void backward(const vectra_dense_grad_args& a, Call& c) {
+  const int64_t n_w = a.width_out * (1 + a.gated);
+  const bool slope = a.gated || a.activation != VECTRA_DENSE_NONE;
+  const bool want_dx = a.dx && a.rows && a.width_in, want_dw = a.dweight && n_w && a.width_in;
+  const bool want_db = a.dbias && n_w;
+  if (!want_dx && !want_dw && !want_db) return;
+  const bool use_x = slope || want_dw, use_w = slope || want_dx;
+  Matrix x{nullptr, 0}, w{nullptr, 0}, dz{nullptr, 0};
+  const int64_t depth = c.padded(a.width_in);
+  if (use_x && a.rows && a.width_in) {
+    if (a.x) {
+      x = c.operand(a.x, a.x_stride, a.rows, a.width_in);
+    } else {
+      x = {c.scratch.take(a.rows * depth * c.esize()), depth};
+      if (c.go())
+        c.typed([&](auto* t) {
+          using T = std::remove_pointer_t<decltype(t)>;
+          const int vec = 1 | ((reinterpret_cast<uintptr_t>(a.codes) & 3) == 0 && a.codes_stride % 4 == 0 ? 2 : 0);
+          dequantize_kernel<T><<<static_cast<uint32_t>(ceil_div(a.rows * (depth / 4), 256)), 256, 0, c.stream>>>(
+              static_cast<const uint8_t*>(a.codes), a.codes_stride, static_cast<const uint8_t*>(a.scales),
+              a.scales_stride, a.rows, a.width_in, const_cast<T*>(static_cast<const T*>(x.p)), depth, depth, vec);
+        });
+    }
+  }
+  if (use_w && a.rows && a.width_in && n_w) w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
+  const int64_t n_pad = c.padded(n_w);
+  float* sums = nullptr;
+  int64_t sum_rows = 0;
+  if (slope && a.rows && n_w) {
+    dz = {c.scratch.take(a.rows * n_pad * c.esize()), n_pad};
+    // Tile rows of the smallest tile: at least as many as the product uses.
+    sum_rows = ceil_div(a.rows, kTileM[kTileCount - 1]);
+    if (want_db) sums = static_cast<float*>(c.scratch.take(sum_rows * n_w * 4));
+    GemmParams p{};
+    p.a = x.p;
+    p.lda = x.ld;
+    p.b = w.p;
+    p.ldb = w.ld;
+    p.m = a.rows;
+    p.n = a.width_out;
+    p.depth = p.depth_b = depth;
+    p.out = const_cast<void*>(dz.p);
+    p.ldo = n_pad;
+    p.bias = a.bias;
+    p.bias_dtype = a.bias_dtype;
+    p.activation = a.activation;
+    p.grad = a.grad;
+    p.ldg = a.grad_stride;
+    p.sums = sums;
+    p.sums_stride = n_w;
+    p.vec = kVecOut | (a.width_out % 4 == 0 ? kVecOutUp : 0) | c.vec4(a.grad, a.grad_stride, kVecGrad);
+    c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope);
+    sum_rows = c.last_tiles_m;
+    if (n_pad != n_w && c.go())
+      c.typed([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        zero_tail_kernel<T><<<static_cast<uint32_t>(ceil_div(a.rows * (n_pad - n_w), 256)), 256, 0, c.stream>>>(
+            static_cast<T*>(const_cast<void*>(dz.p)), a.rows, n_w, n_pad);
+      });
+  } else if (want_dx || want_dw) {
+    dz = c.operand(a.grad, a.grad_stride, a.rows, n_w);
+  }
+  if (want_db) {
+    if (sums || a.rows == 0 || n_w == 0)
+      c.column_sums<float>(sums, n_w, sums ? sum_rows : 0, n_w, a.dbias, a.bias_dtype);
+    else
+      c.typed([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        c.column_sums<T>(static_cast<const T*>(a.grad), a.grad_stride, a.rows, n_w, a.dbias, a.bias_dtype);
+      });
+  }
+  if (want_dx) {
+    GemmParams p{};
+    p.a = dz.p;
+    p.lda = dz.ld;
+    p.b = w.p;
+    p.ldb = w.ld;
+    p.b_width = depth;
+    p.m = a.rows;
+    p.n = a.width_in;
+    p.depth = n_pad;
+    p.depth_b = n_w;
+    p.out = a.dx;
+    p.ldo = a.dx_stride;
+    p.vec = c.vec4(a.dx, a.dx_stride, kVecOut);
+    c.product(p, kLayoutInput, kEpiStore);
+  }
+  if (want_dw) {
+    GemmParams p{};
+    p.a = dz.p;
+    p.lda = dz.ld;
+    p.a_width = n_pad;
+    p.b = x.p;
+    p.ldb = x.ld;
+    p.b_width = depth;
+    p.m = n_w;
+    p.n = a.width_in;
+    p.depth = p.depth_b = a.rows;
+    p.out = a.dweight;
+    p.ldo = a.dweight_stride;
+    p.vec = c.vec4(a.dweight, a.dweight_stride, kVecOut);
+    c.product(p, kLayoutWeight, kEpiStore);
+  }
+}
+
+// Runs a plan twice where a workspace is needed: once to find its size, once
+// to launch.  Launches nothing before the size is known to fit.
+template <typename Args, typename F>
+int run_call(const Args& a, F&& plan, void* workspace, int64_t workspace_bytes, vectra_dense_stream_t stream) {
+  Call sized{a.dtype, {nullptr, 0}, false, nullptr, compute_units()};
+  plan(a, sized);
+  const int64_t need = std::max(sized.most, sized.scratch.used);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return VECTRA_DENSE_ERR_WORKSPACE;
+  Call c{a.dtype, {static_cast<char*>(workspace), 0}, true, reinterpret_cast<hipStream_t>(stream), sized.cus};
+  (void)hipGetLastError();  // an error left by other work is not this call's
+  plan(a, c);
+  return c.status;
+}
+
+template <typename Args, typename F>
+int64_t need_of(const Args& a, F&& plan) {
+  Call sized{a.dtype, {nullptr, 0}, false, nullptr, compute_units()};
+  plan(a, sized);
+  return std::max(sized.most, sized.scratch.used);
+}
+
+}  // namespace
+}  // namespace vectra_dense
+
+using namespace vectra_dense;
+
+extern "C" {
+
+int vectra_dense_forward(const vectra_dense_args* args, void* workspace, int64_t workspace_bytes,
+                         vectra_dense_stream_t stream) {
+  if (int st = check_forward(args)) return st;
+  return run_call(*args, forward, workspace, workspace_bytes, stream);
+}
+
+int64_t vectra_dense_forward_workspace_bytes(const vectra_dense_args* args) {
+  if (int st = check_forward(args)) return -st;
+  return need_of(*args, forward);
+}
+
+int vectra_dense_backward(const vectra_dense_grad_args* args, void* workspace, int64_t workspace_bytes,
+                          vectra_dense_stream_t stream) {
+  if (int st = check_backward(args)) return st;
+  return run_call(*args, backward, workspace, workspace_bytes, stream);
+}
+
+int64_t vectra_dense_backward_workspace_bytes(const vectra_dense_grad_args* args) {
+  if (int st = check_backward(args)) return -st;
+  return need_of(*args, backward);
+}
+
+int vectra_rows_quantize(const void* x, int32_t dtype, int64_t rows, int64_t width, int64_t x_stride, void* codes,
+                         int64_t codes_stride, void* scales, int64_t scales_stride, vectra_dense_stream_t stream) {
+  if (!known_dtype(dtype)) return VECTRA_DENSE_ERR_BAD_DTYPE;
+  if (int st = check_sizes(rows, width, 0, 0)) return st;
+  if (rows == 0 || width == 0) return VECTRA_DENSE_OK;
+  if (!x || !codes || !scales) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  const int64_t blocks = ceil_div(width, kBlock);
+  if (int st = check_stride(x_stride, width, rows, 1, element_size(dtype))) return st;
+  if (int st = check_stride(codes_stride, width, rows, 1, 1)) return st;
+  if (int st = check_stride(scales_stride, blocks, rows, 1, 1)) return st;
+  Call c{dtype, {nullptr, 0}, true, reinterpret_cast<hipStream_t>(stream), 0};
+  (void)hipGetLastError();
+  const int vec = c.vec4(x, x_stride, 1) |
+                  ((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && codes_stride % 4 == 0 ? 2 : 0);
+  c.typed([&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    quantize_kernel<T><<<static_cast<uint32_t>(ceil_div(rows * blocks, 32)), 256, 0, c.stream>>>(
+        static_cast<const T*>(x), rows, width, x_stride, static_cast<uint8_t*>(codes), codes_stride,
+        static_cast<uint8_t*>(scales), scales_stride, blocks, vec);
+  });
+  return c.status;
+}
+
+int vectra_rows_dequantize(const void* codes, int64_t codes_stride, const void* scales, int64_t scales_stride,
+                           int32_t dtype, int64_t rows, int64_t width, void* out, int64_t out_stride,
+                           vectra_dense_stream_t stream) {
+  if (!known_dtype(dtype)) return VECTRA_DENSE_ERR_BAD_DTYPE;
+  if (int st = check_sizes(rows, width, 0, 0)) return st;
+  if (rows == 0 || width == 0) return VECTRA_DENSE_OK;
+  if (!out || !codes || !scales) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+  if (int st = check_stride(out_stride, width, rows, 1, element_size(dtype))) return st;
+  if (int st = check_stride(codes_stride, width, rows, 1, 1)) return st;
+  if (int st = check_stride(scales_stride, ceil_div(width, kBlock), rows, 1, 1)) return st;
+  Call c{dtype, {nullptr, 0}, true, reinterpret_cast<hipStream_t>(stream), 0};
+  (void)hipGetLastError();
+  const int vec = c.vec4(out, out_stride, 1) |
+                  ((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && codes_stride % 4 == 0 ? 2 : 0);
+  c.typed([&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    dequantize_kernel<T><<<static_cast<uint32_t>(ceil_div(rows * ceil_div(width, 4), 256)), 256, 0, c.stream>>>(
+        static_cast<const uint8_t*>(codes), codes_stride, static_cast<const uint8_t*>(scales), scales_stride, rows,
+        width, static_cast<T*>(out), out_stride, width, vec);
+  });
+  return c.status;
+}
+
+const char* vectra_dense_status_string(int status) {
+  switch (status) {
+    case VECTRA_DENSE_OK: return "ok";
+    case VECTRA_DENSE_ERR_NULL_ARGUMENT: return "a required pointer is NULL";
+    case VECTRA_DENSE_ERR_BAD_DTYPE: return "unsupported dtype combination";
+    case VECTRA_DENSE_ERR_BAD_SHAPE: return "negative or inconsistent sizes or strides";
+    case VECTRA_DENSE_ERR_BAD_STRUCT: return "struct_size does not match this build of the library";
+    case VECTRA_DENSE_ERR_TOO_LARGE: return "a size exceeds the kernels' index range";
+    case VECTRA_DENSE_ERR_LAUNCH: return "HIP kernel launch failed";
+    case VECTRA_DENSE_ERR_BAD_ACTIVATION: return "unknown activation";
+    case VECTRA_DENSE_ERR_WORKSPACE: return "workspace missing, too small or not 256-byte aligned";
+    default: return "unknown status";
+  }
+}
+
+int vectra_dense_abi_version(void) { return (1 << 16) | 0; }
+
+}  // extern "C"

@@ -1,0 +1,59 @@
+// What the dense library's host code launches.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "vectra_dense.h"
+
+namespace vectra_dense {
+
+// Epilogues of the tiled product.
+enum {
+  kEpiStore = 0,       // act(D + bias) + residual, in the element type
+  kEpiPartial = 1,     // D in fp32, one plane per split of the contraction
+  kEpiGated = 2,       // act(D_gate + bias) * (D_up + bias)
+  kEpiSlope = 3,       // grad * act'(D + bias), and its column sums
+  kEpiGatedSlope = 4,  // both factors' gradients, and their column sums
+};
+
+// GemmParams::vec: rows that start at multiples of four elements.
+enum { kVecOut = 1, kVecResidual = 2, kVecGrad = 4, kVecOutUp = 8 };
+
+struct GemmParams {
+  const void* a;  // row operand
+  const void* b;  // column operand
+  int64_t lda, ldb;
+  int64_t a_width, b_width;  // wide operands: elements per stored row (whole chunks)
+  int64_t m, n;              // output rows and columns (gated: outputs)
+  int64_t depth;             // contraction, as A's rows hold it (zero padded to whole chunks)
+  int64_t depth_b;           // contraction rows of a wide B (at most depth: rows past it are zeros)
+  int32_t tiles_m, tiles_n;
+  int32_t k_tiles, k_tiles_per_split;
+  void* out;
+  int64_t ldo;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  const void* grad;
+  int64_t ldg;
+  float* sums;  // column sums per tile row, or NULL
+  int64_t sums_stride;
+  int32_t bias_dtype;
+  int32_t activation;
+  int32_t vec;
+};
+
+// The shapes of one tiled product's kernels.
+enum { kLayoutForward = 0, kLayoutInput = 1, kLayoutWeight = 2 };
+enum { kTileLarge = 0, kTileMedium = 1, kTileSmall = 2, kTileCount = 3 };
+constexpr int kTileM[kTileCount] = {256, 128, 64};
+constexpr int kTileN[kTileCount] = {256, 128, 64};
+
+// Launches the product with the given layout, tile and epilogue on `splits`
+// contraction parts.  One definition per element type.
+int launch_gemm_bf16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
+int launch_gemm_f16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
+int launch_gemm_f32(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
+
+}  // namespace vectra_dense

@@ -1,0 +1,8 @@
+// Tiled products of _Float16 operands.
+#include "gemm_launch.h"
+
+namespace vectra_dense {
+int launch_gemm_f16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream) {
+  return launch_gemm<_Float16>(p, layout, tile, epi, splits, stream);
+}
+}  // namespace vectra_dense

@@ -1,0 +1,420 @@
+// Tiled matrix products on gfx950 matrix cores, with the operators' epilogues:
+// the kernel template, instantiated per element type in gemm_<type>.hip.
+//
+//   D[m, n] = sum_c A(m, c) B(n, c)
+//
+// A is the row operand and B the column operand.  Each is stored either with
+// the contraction c contiguous ("deep" rows: element (m, c) at m ld + c) or
+// with it strided ("wide" rows: element (m, c) at c ld + m), which covers
+//   forward  x W^T     both deep
+//   dx       dz W      A deep, B wide
+//   dW       dz^T x    both wide
+//
+// A workgroup of kWM x kWN waves computes a kBM x kBN tile of D, a wave
+// kTM x kTN tiles of 16 x 16.  B is the matrix instruction's first operand and
+// A its second, so a lane holds four consecutive n of one m: rows of D are
+// stored in 8- or 16-byte pieces.
+//
+// Staging: the tiles go from global memory straight into LDS in 16-byte chunks
+// (buffer loads with the LDS bit: no registers, no LDS write instructions),
+// one tile ahead of the one being multiplied.  Such a load writes LDS in lane
+// order, so the swizzle that keeps LDS reads free of bank conflicts is applied
+// to the global address each lane loads: LDS chunk p of a row holds the row's
+// chunk p ^ f(row).  Buffer bounds turn rows past the operand into zeros;
+// chunks past the contraction's end are sent out of bounds on the last tile.
+// Operands have 16-byte aligned rows of whole chunks (others are copied into
+// the workspace first, zero padded).
+//
+// LDS reads: deep 16-bit and 32-bit operands read 16 bytes per lane.  Wide
+// 16-bit operands are read with the transposing LDS read (rbf_mfma_ops.h
+// describes its lane mapping), wide fp32 operands element by element.  fp32
+// products use a permuted contraction (lane group g takes elements 4g .. 4g+3
+// of 16), the same for both operands.
+#pragma once
+
+#include "dense_common.h"
+#include "dense_kernels.h"
+
+namespace vectra_dense {
+
+typedef short lds_v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+// What one lane feeds a matrix instruction: 16 bytes.
+struct Frag {
+  u32x4 w;
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+  typedef __bf16 V __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a.w), __builtin_bit_cast(V, b.w), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> {
+  typedef _Float16 V __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a.w), __builtin_bit_cast(V, b.w), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[j]), __uint_as_float(b.w[j]), c, 0, 0, 0);
+    return c;
+  }
+};
+
+// One operand's tile in LDS: kRows rows of the output dimension, kDeep of the
+// contraction.
+template <typename T, bool kWide, int kRows, int kDeep, int kThreads>
+struct Tile {
+  static constexpr int kPer = 16 / sizeof(T);                       // elements per chunk
+  static constexpr int kLdsRows = kWide ? kDeep : kRows;            // rows as stored
+  static constexpr int kChunks = (kWide ? kRows : kDeep) / kPer;    // chunks per stored row
+  static constexpr int kRowBytes = kChunks * 16;
+  static constexpr int kBytes = kLdsRows * kRowBytes;
+  static constexpr int kSlots = kLdsRows * kChunks / kThreads;      // loads per thread
+  static constexpr int kStep = 4 * kPer;                            // contraction per fragment
+  static_assert(kSlots * kThreads == kLdsRows * kChunks, "whole loads");
+  static_assert(kWide || kChunks == 8 || kChunks == 4, "64- or 128-byte deep rows");
+
+  // The chunk XOR of a stored row.
+  //  deep, 128-byte rows: 16 lanes read one chunk of 16 consecutive rows; with
+  //    64 banks (256 bytes) two rows share a bank line, so rows r and r + 1
+  //    differ already and (r >> 1) & 7 separates the pairs.
+  //  deep, 64-byte rows: four rows share a line; (r >> 2) & 3 likewise.
+  //  wide, 16-bit: a transposing read takes 32-byte pieces of rows {0..3} and
+  //    {8..11} (then {4..7}, {12..15}) at once: piece index ^ f, f from row
+  //    bits 0, 1 and 3 (a 128-byte row holds two of those bits by parity).
+  //  wide, fp32: 64-byte pieces of the rows 4g + j, g = 0..3: piece ^ g.
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (!kWide) {
+      return kChunks == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+    } else if constexpr (sizeof(T) == 2) {
+      if constexpr (kRowBytes >= 256) return ((row & 3) | ((row >> 1) & 4)) << 1;
+      return (((row >> 1) & 1) | ((row >> 2) & 2)) << 1;
+    } else {
+      return kRowBytes >= 256 ? ((row >> 2) & 3) << 2 : ((row >> 3) & 1) << 2;
+    }
+  }
+
+  // Slot s of a thread: the stored row and the row's chunk that it loads.
+  static __device__ __forceinline__ void slot(int s, int tid, int& row, int& chunk) {
+    const int at = s * kThreads + tid;
+    row = at / kChunks;
+    chunk = (at % kChunks) ^ swizzle(row);
+  }
+
+  // The fragment of 16 rows from `row0` (a multiple of 16) of contraction step
+  // `step`, for lane group g, lane i of it.
+  static __device__ __forceinline__ Frag read(const lds_char* tile, int row0, int step, int g, int i) {
+    Frag f;
+    if constexpr (!kWide) {
+      const int row = row0 + i;
+      f.w = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
+          tile + row * kRowBytes + (((step * 4 + g) ^ swizzle(i)) * 16));
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = step * 32 + 8 * g + 4 * h + i / 4;
+        const int chunk = (row0 / 8 + (i % 4) / 2) ^ swizzle(8 * g + i / 4);
+        const lds_v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) lds_v4s*)(const_cast<lds_char*>(tile) + row * kRowBytes + chunk * 16 +
+                                                         (i & 1) * 8));
+        const uint2 u = __builtin_bit_cast(uint2, v);
+        f.w[2 * h] = u.x;
+        f.w[2 * h + 1] = u.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = step * 16 + 4 * g + j;
+        const int chunk = (row0 / 4 + i / 4) ^ swizzle(4 * g);
+        f.w[j] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(tile + row * kRowBytes +
+                                                                                      chunk * 16 + (i % 4) * 4);
+      }
+    }
+    return f;
+  }
+};
+
+// Tile `id` of `tiles_m` x `tiles_n`.  Workgroups are dealt round-robin to the
+// 8 XCDs: each XCD takes one contiguous run of tiles, and within the run
+// bands of kBand tile rows are walked column by column, so that the operands
+// of the tiles in flight on an XCD stay in its L2.
+constexpr int kBand = 4;
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int total = tiles_m * tiles_n;
+  const int xcd = id & 7, each = total >> 3, more = total & 7;
+  const int t = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+  const int per_band = kBand * tiles_n;
+  const int band = t / per_band, in = t - band * per_band;
+  const int height = min(kBand, tiles_m - band * kBand);
+  tn = in / height;
+  tm = band * kBand + (in - tn * height);
+}
+
+// Waits for this wave's loads into LDS (they count as vector memory
+// operations; a workgroup barrier by itself orders LDS instructions only).
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+constexpr uint32_t kOutside = 0x80000000u;  // past any buffer (host checks: tiles span less than 2^31 bytes)
+
+// Loads the tile of one operand.  `base`: the operand's element (first row of
+// the tile, first contraction element of the tile), wave-uniform.
+template <typename TileT, typename T, bool kWide, int kThreads>
+__device__ __forceinline__ void stage(lds_char* tile, const T* base, const uint32_t (&offset)[TileT::kSlots],
+                                      int64_t bytes, int valid_chunks, const uint32_t (&chunk)[TileT::kSlots],
+                                      int wave) {
+  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<T*>(base), 0, static_cast<int>(bytes > 0 ? bytes : 0), 0x00020000);
+#pragma unroll
+  for (int s = 0; s < TileT::kSlots; ++s) {
+    uint32_t at = offset[s];
+    if constexpr (!kWide) {
+      if (valid_chunks < TileT::kChunks) at = static_cast<int>(chunk[s]) < valid_chunks ? at : kOutside;
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rsrc, (__attribute__((address_space(3))) void*)(tile + (s * kThreads + wave * 64) * 16), 16, at, 0, 0, 0);
+  }
+}
+
+template <typename T, int kBM_, int kBN_, int kWM_, int kWN_, bool kWideA_, bool kWideB_, int kEpi_>
+struct GemmConfig {
+  static constexpr int kBM = kBM_, kBN = kBN_, kWM = kWM_, kWN = kWN_, kEpi = kEpi_;
+  static constexpr bool kWideA = kWideA_, kWideB = kWideB_;
+  static constexpr int kThreads = 64 * kWM * kWN;
+  static constexpr int kDeep = 128 / sizeof(T);  // contraction per tile
+  static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
+  static constexpr bool kGated = kEpi == kEpiGated || kEpi == kEpiGatedSlope;
+  using A = Tile<T, kWideA, kBM, kDeep, kThreads>;
+  using B = Tile<T, kWideB, kBN, kDeep, kThreads>;
+  static constexpr int kStageBytes = A::kBytes + B::kBytes;
+  static constexpr int kLdsBytes = 2 * kStageBytes;
+};
+
+template <typename T, typename C>
+__global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
+  __shared__ __attribute__((aligned(256))) char smem_generic[C::kLdsBytes];
+  lds_char* const smem = (lds_char*)smem_generic;
+  using A = typename C::A;
+  using B = typename C::B;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, i = lane & 15;
+  const int wm = wave / C::kWN, wn = wave % C::kWN;
+
+  int tm, tn;
+  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * C::kBM;
+  constexpr int kOutN = C::kGated ? C::kBN / 2 : C::kBN;  // output columns per tile
+  const int64_t n0 = static_cast<int64_t>(tn) * kOutN;
+  const int k_first = blockIdx.y * p.k_tiles_per_split;
+  const int k_last = min(k_first + p.k_tiles_per_split, p.k_tiles);
+
+  // ---- per-lane load offsets (bytes from the tile's base) and base pointers
+  const T* a = static_cast<const T*>(p.a);
+  const T* b = static_cast<const T*>(p.b);
+  uint32_t a_off[A::kSlots], b_off[B::kSlots], a_chunk[A::kSlots], b_chunk[B::kSlots];
+  int64_t a_bytes, b_bytes, a_step, b_step;  // bytes left in the operand from the base, bytes per contraction tile
+  if constexpr (C::kWideA) {
+    a += static_cast<int64_t>(k_first) * C::kDeep * p.lda + m0;
+    a_bytes = ((p.depth - static_cast<int64_t>(k_first) * C::kDeep - 1) * p.lda + (p.a_width - m0)) * sizeof(T);
+    a_step = static_cast<int64_t>(C::kDeep) * p.lda * sizeof(T);
+  } else {
+    a += m0 * p.lda + static_cast<int64_t>(k_first) * C::kDeep;
+    const int64_t rows = min<int64_t>(p.m - m0, C::kBM);
+    a_bytes = ((rows - 1) * p.lda + p.depth - static_cast<int64_t>(k_first) * C::kDeep) * sizeof(T);
+    a_step = C::kDeep * sizeof(T);
+  }
+  if constexpr (C::kWideB) {
+    b += static_cast<int64_t>(k_first) * C::kDeep * p.ldb + n0;
+    b_bytes = ((p.depth_b - static_cast<int64_t>(k_first) * C::kDeep - 1) * p.ldb + (p.b_width - n0)) * sizeof(T);
+    b_step = static_cast<int64_t>(C::kDeep) * p.ldb * sizeof(T);
+  } else {
+    b += n0 * p.ldb + static_cast<int64_t>(k_first) * C::kDeep;
+    const int64_t rows = (C::kGated ? p.n : 0) + min<int64_t>(p.n - n0, kOutN);
+    b_bytes = ((rows - 1) * p.ldb + p.depth - static_cast<int64_t>(k_first) * C::kDeep) * sizeof(T);
+    b_step = C::kDeep * sizeof(T);
+  }
+#pragma unroll
+  for (int s = 0; s < A::kSlots; ++s) {
+    int row, chunk;
+    A::slot(s, tid, row, chunk);
+    a_off[s] = static_cast<uint32_t>(row * p.lda * sizeof(T)) + chunk * 16;
+    a_chunk[s] = chunk;
+    if constexpr (C::kWideA) {
+      if (m0 + chunk * A::kPer >= p.a_width) a_off[s] = kOutside;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < B::kSlots; ++s) {
+    int row, chunk;
+    B::slot(s, tid, row, chunk);
+    b_chunk[s] = chunk;
+    if constexpr (C::kGated) {
+      // A wave's columns are kTN / 2 tiles of gate rows, then the up rows of
+      // the same outputs: one wave holds both factors of its outputs.
+      constexpr int kSeg = C::kTN * 16, kHalf = kSeg / 2;
+      const int seg = row / kSeg, in = row % kSeg;
+      const int out = seg * kHalf + in % kHalf;
+      const int64_t w_row = out + (in >= kHalf ? p.n : 0);
+      b_off[s] = n0 + out < p.n ? static_cast<uint32_t>(w_row * p.ldb * sizeof(T)) + chunk * 16 : kOutside;
+    } else {
+      b_off[s] = static_cast<uint32_t>(row * p.ldb * sizeof(T)) + chunk * 16;
+      if constexpr (C::kWideB) {
+        if (n0 + chunk * B::kPer >= p.b_width) b_off[s] = kOutside;
+      }
+    }
+  }
+  const auto load = [&](int kt, int buf) {
+    lds_char* const at = smem + buf * C::kStageBytes;
+    const int left = static_cast<int>((min<int64_t>(p.depth - static_cast<int64_t>(kt) * C::kDeep, C::kDeep) + A::kPer - 1) / A::kPer);
+    stage<A, T, C::kWideA, C::kThreads>(at, a, a_off, min<int64_t>(a_bytes, 0x7fffffff), left, a_chunk, wave);
+    stage<B, T, C::kWideB, C::kThreads>(at + A::kBytes, b, b_off, min<int64_t>(b_bytes, 0x7fffffff), left, b_chunk, wave);
+    a = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a) + a_step);
+    b = reinterpret_cast<const T*>(reinterpret_cast<const char*>(b) + b_step);
+    a_bytes -= a_step;
+    b_bytes -= b_step;
+  };
+
+  f32x4 acc[C::kTN][C::kTM];
+#pragma unroll
+  for (int tn_ = 0; tn_ < C::kTN; ++tn_)
+#pragma unroll
+    for (int tm_ = 0; tm_ < C::kTM; ++tm_) acc[tn_][tm_] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (k_first < k_last) load(k_first, 0);
+  for (int kt = k_first; kt < k_last; ++kt) {
+    const int buf = (kt - k_first) & 1;
+    wait_loads();
+    __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
+    if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
+    const lds_char* const ta = smem + buf * C::kStageBytes;
+    const lds_char* const tb = ta + A::kBytes;
+#pragma unroll
+    for (int step = 0; step < C::kDeep / A::kStep; ++step) {
+      Frag fa[C::kTM], fb[C::kTN];
+#pragma unroll
+      for (int t = 0; t < C::kTN; ++t) fb[t] = B::read(tb, (wn * C::kTN + t) * 16, step, g, i);
+#pragma unroll
+      for (int t = 0; t < C::kTM; ++t) fa[t] = A::read(ta, (wm * C::kTM + t) * 16, step, g, i);
+#pragma unroll
+      for (int t = 0; t < C::kTM; ++t)
+#pragma unroll
+        for (int u = 0; u < C::kTN; ++u) acc[u][t] = Mma<T>::run(fb[u], fa[t], acc[u][t]);
+    }
+  }
+
+  // ---- epilogue: lane holds D[m, n .. n + 3] of every 16 x 16 tile
+  constexpr int kPairs = C::kGated ? C::kTN / 2 : C::kTN;
+  constexpr bool kSlope = C::kEpi == kEpiSlope || C::kEpi == kEpiGatedSlope;
+  const int64_t n_wave = n0 + wn * kPairs * 16;
+  f32x4 sum_a[kSlope ? kPairs : 1], sum_b[kSlope && C::kGated ? kPairs : 1];
+#pragma unroll
+  for (int u = 0; u < kPairs; ++u) {
+    const int64_t n = n_wave + u * 16 + 4 * g;
+    const int left = static_cast<int>(min<int64_t>(p.n - n, 4));
+    f32x4 bias = {0.f, 0.f, 0.f, 0.f}, bias_up = {0.f, 0.f, 0.f, 0.f};
+    if (C::kEpi != kEpiPartial && p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) {
+          bias[e] = load_bias(p.bias, n + e, p.bias_dtype);
+          if constexpr (C::kGated) bias_up[e] = load_bias(p.bias, p.n + n + e, p.bias_dtype);
+        }
+    }
+    if constexpr (kSlope) {
+      sum_a[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (C::kGated) sum_b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int t = 0; t < C::kTM; ++t) {
+      const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
+      if (m >= p.m || left <= 0) continue;
+      if constexpr (C::kEpi == kEpiPartial) {
+        float* const out = static_cast<float*>(p.out) + (static_cast<int64_t>(blockIdx.y) * p.m + m) * p.ldo + n;
+        *reinterpret_cast<f32x4*>(out) = acc[u][t];  // ldo is a multiple of 4
+      } else if constexpr (C::kEpi == kEpiStore) {
+        f32x4 y = acc[u][t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = act_value(y[e] + bias[e], p.activation);
+        if (p.residual) y += load4(static_cast<const T*>(p.residual) + m * p.ldr + n, left, p.vec & kVecResidual);
+        store4(static_cast<T*>(p.out) + m * p.ldo + n, y, left, p.vec & kVecOut);
+      } else if constexpr (C::kEpi == kEpiGated) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[e] = act_value(acc[u][t][e] + bias[e], p.activation) * (acc[u + kPairs][t][e] + bias_up[e]);
+        store4(static_cast<T*>(p.out) + m * p.ldo + n, y, left, p.vec & kVecOut);
+      } else {
+        const f32x4 dy = load4(static_cast<const T*>(p.grad) + m * p.ldg + n, left, p.vec & kVecGrad);
+        f32x4 da, db;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float value, slope;
+          act_slope(acc[u][t][e] + bias[e], p.activation, value, slope);
+          da[e] = dy[e] * slope;
+          if constexpr (C::kGated) {
+            da[e] *= acc[u + kPairs][t][e] + bias_up[e];
+            db[e] = dy[e] * value;
+          }
+        }
+        T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
+        store4(out, da, left, p.vec & kVecOut);
+        sum_a[u] += da;
+        if constexpr (C::kGated) {
+          store4(out + p.n, db, left, p.vec & kVecOutUp);
+          sum_b[u] += db;
+        }
+      }
+    }
+  }
+
+  // Column sums of dz over this tile's rows, for the bias's gradient: over the
+  // 16 lanes of a group, then over the waves of a column through LDS, in a
+  // fixed order.  Row `tm` of p.sums receives them.
+  if constexpr (kSlope) {
+    if (p.sums) {
+      __syncthreads();  // all waves are done with the tiles
+      __attribute__((address_space(3))) float* const sums = (__attribute__((address_space(3))) float*)smem;
+      constexpr int kCols = C::kBN;  // gated: kBN / 2 gate columns, then as many up columns
+#pragma unroll
+      for (int u = 0; u < kPairs; ++u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float s = sum_a[u][e], s2 = 0.f;
+          if constexpr (C::kGated) s2 = sum_b[u][e];
+#pragma unroll
+          for (int d = 1; d < 16; d <<= 1) {
+            s += __shfl_xor(s, d);
+            if constexpr (C::kGated) s2 += __shfl_xor(s2, d);
+          }
+          if (i == 0) {
+            const int col = (wn * kPairs + u) * 16 + 4 * g + e;
+            sums[wm * kCols + col] = s;
+            if constexpr (C::kGated) sums[wm * kCols + kOutN + col] = s2;
+          }
+        }
+      }
+      __syncthreads();
+      for (int col = tid; col < kCols; col += C::kThreads) {
+        const bool up = C::kGated && col >= kOutN;
+        const int64_t n = n0 + (up ? col - kOutN : col);
+        if (n >= p.n) continue;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::kWM; ++w) s += sums[w * kCols + col];
+        p.sums[static_cast<int64_t>(tm) * p.sums_stride + (up ? p.n : 0) + n] = s;
+      }
+    }
+  }
+}
+
+}  // namespace vectra_dense

@@ -1,0 +1,45 @@
+// Host side of the tiled product: from layout, tile and epilogue to a kernel.
+#pragma once
+
+#include "gemm_impl.h"
+
+namespace vectra_dense {
+
+template <typename T, typename C>
+int launch_one(const GemmParams& p, int splits, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(splits));
+  gemm_kernel<T, C><<<grid, C::kThreads, 0, stream>>>(p);
+  return hipGetLastError() == hipSuccess ? VECTRA_DENSE_OK : VECTRA_DENSE_ERR_LAUNCH;
+}
+
+template <typename T, bool kWideA, bool kWideB, int kEpi>
+int launch_tile(const GemmParams& p, int tile, int splits, hipStream_t stream) {
+  switch (tile) {
+    case kTileLarge:
+      return launch_one<T, GemmConfig<T, 256, 256, 2, 4, kWideA, kWideB, kEpi>>(p, splits, stream);
+    case kTileMedium:
+      return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi>>(p, splits, stream);
+    default:
+      return launch_one<T, GemmConfig<T, 64, 64, 2, 2, kWideA, kWideB, kEpi>>(p, splits, stream);
+  }
+}
+
+template <typename T>
+int launch_gemm(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream) {
+  if (layout == kLayoutForward) {
+    switch (epi) {
+      case kEpiStore: return launch_tile<T, false, false, kEpiStore>(p, tile, splits, stream);
+      case kEpiPartial: return launch_tile<T, false, false, kEpiPartial>(p, tile, splits, stream);
+      case kEpiGated: return launch_tile<T, false, false, kEpiGated>(p, tile, splits, stream);
+      case kEpiSlope: return launch_tile<T, false, false, kEpiSlope>(p, tile, splits, stream);
+      default: return launch_tile<T, false, false, kEpiGatedSlope>(p, tile, splits, stream);
+    }
+  }
+  if (layout == kLayoutInput)
+    return epi == kEpiStore ? launch_tile<T, false, true, kEpiStore>(p, tile, splits, stream)
+                            : launch_tile<T, false, true, kEpiPartial>(p, tile, splits, stream);
+  return epi == kEpiStore ? launch_tile<T, true, true, kEpiStore>(p, tile, splits, stream)
+                          : launch_tile<T, true, true, kEpiPartial>(p, tile, splits, stream);
+}
+
+}  // namespace vectra_dense

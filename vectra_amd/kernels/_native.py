@@ -1,8 +1,9 @@
 """Locates and loads the native libraries built in-tree.
 
 * ``libvectra_rbf.so``   -- the C-ABI HIP library (include/vectra_rbf.h);
+* ``libvectra_dense.so`` -- the C-ABI dense operators (include/vectra_dense.h);
 * ``libvectra_torch.so`` -- the torch.library extension that registers
-  ``vectra::rbf_attention`` and links the first one;
+  ``vectra::rbf_attention`` and the dense operators and links the first two;
 * ``libvectra_scan.so``  -- the C-ABI distance scans (include/vectra_scan.h),
   used by vectra_amd.index.
 
@@ -23,6 +24,7 @@ LIB_DIR = os.environ.get('VECTRA_LIB_DIR') or os.path.join(
     os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'lib')
 HIP_LIBRARY = os.path.join(LIB_DIR, 'libvectra_rbf.so')
 TORCH_LIBRARY = os.path.join(LIB_DIR, 'libvectra_torch.so')
+DENSE_LIBRARY = os.path.join(LIB_DIR, 'libvectra_dense.so')
 SCAN_LIBRARY = os.path.join(LIB_DIR, 'libvectra_scan.so')
 
 
@@ -70,6 +72,34 @@ def hip_library() -> ctypes.CDLL:
     lib.vectra_rbf_status_string.restype = ctypes.c_char_p
     lib.vectra_rbf_abi_version.argtypes = []
     lib.vectra_rbf_abi_version.restype = ctypes.c_int
+    return lib
+
+
+@functools.cache
+def dense_library() -> ctypes.CDLL:
+    """The dense-operator library as a ctypes handle (shared with the extension)."""
+    lib = ctypes.CDLL(_require(DENSE_LIBRARY))
+    for name in ('vectra_dense_forward', 'vectra_dense_backward'):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+        size = getattr(lib, name + '_workspace_bytes')
+        size.argtypes = [ctypes.c_void_p]
+        size.restype = ctypes.c_int64
+    lib.vectra_rows_quantize.argtypes = [
+        ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+    ]
+    lib.vectra_rows_quantize.restype = ctypes.c_int
+    lib.vectra_rows_dequantize.argtypes = [
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+    ]
+    lib.vectra_rows_dequantize.restype = ctypes.c_int
+    lib.vectra_dense_status_string.argtypes = [ctypes.c_int]
+    lib.vectra_dense_status_string.restype = ctypes.c_char_p
+    lib.vectra_dense_abi_version.argtypes = []
+    lib.vectra_dense_abi_version.restype = ctypes.c_int
     return lib
 
 
