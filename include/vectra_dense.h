@@ -23,8 +23,8 @@
  * smallest for which no finite element exceeds 448 2^e in magnitude (e >= -117; for
  * fp16 rows e >= -15), and an element x is kept as x / 2^e rounded to OCP e4m3 (ties
  * to even).  codes [rows, width] holds e4m3 bytes, scales [rows, ceil(width / 32)]
- * holds e + 127 as bytes.  A non-finite element becomes e4m3's NaN.  An fp16 element
- * whose rounding would pass 65504 takes the next code below.
+ * holds e + 127 as bytes.  A non-finite element becomes e4m3's NaN.  An element
+ * whose rounding would pass its type's largest value takes the next code below.
  *
  * Contract (as vectra_rbf.h):
  *  - Plain pointers, sizes and strides; matrices are row-major with unit element

@@ -136,7 +136,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows, int64_t width, int64_t stride,
                                                        uint8_t* codes, int64_t codes_stride, uint8_t* scales,
                                                        int64_t scales_stride, int64_t blocks, int vec) {
-  constexpr int kLowest = sizeof(T) == 2 && !__is_same(T, __bf16) ? -15 : -117;
+  constexpr int kLowest = __is_same(T, _Float16) ? -15 : -117, kHighest = __is_same(T, _Float16) ? 8 : 120;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
   const bool live = at < rows * blocks;
   const int64_t row = live ? at / blocks : 0, block = live ? at - row * blocks : 0;
@@ -159,14 +159,13 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
   const int e = byte - 127;
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] *= power_of_two(-e);  // e in [-117, 120]
-  if constexpr (__is_same(T, _Float16)) {
-    // 65504 = 255.875 * 2^8 would round to 256 * 2^8, which fp16 lacks: at
-    // e = 8, magnitudes of 248 and more take the code below, 240.
-    if (e == 8)
+  // The type's largest value, 255.9 * 2^8 (fp16) or 2^120, would round to 256
+  // times that, which the type lacks: at its exponent, magnitudes of 248 and
+  // more take the code below, 240.
+  if (e == kHighest)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (__builtin_fabsf(v[k]) >= 248.f) v[k] = __builtin_copysignf(240.f, v[k]);
-  }
+    for (int k = 0; k < 4; ++k)
+      if (__builtin_fabsf(v[k]) >= 248.f) v[k] = __builtin_copysignf(240.f, v[k]);
   const uint32_t w = to_e4m3x4(v);
   uint8_t* const out = codes + row * codes_stride + col;
   if (left == 4 && (vec & 2)) {

@@ -366,7 +366,8 @@ Tensor gated_linear_cpu(const Tensor& x, const Tensor& weight, const OptTensor& 
 std::tuple<Tensor, Tensor> quantize_rows_cpu(const Tensor& x) {
   check_rows(x);
   const int64_t width = x.size(-1), rows = rows_of(x), blocks = (width + kBlock - 1) / kBlock;
-  const int32_t lowest = x.scalar_type() == at::kHalf ? -15 : -117;
+  const bool half = x.scalar_type() == at::kHalf;
+  const int32_t lowest = half ? -15 : -117, highest = half ? 8 : 120;
   const Tensor xf = x.to(at::kFloat).reshape({rows, width}).contiguous();
   Tensor values = at::empty({rows, width}, xf.options());
   Tensor scales = at::empty({rows, blocks}, x.options().dtype(at::kByte));
@@ -387,7 +388,7 @@ std::tuple<Tensor, Tensor> quantize_rows_cpu(const Tensor& x) {
       }
       for (int64_t i = first; i < last; ++i) {
         float y = std::isfinite(p[i]) ? std::ldexp(p[i], -e) : std::nanf("");
-        if (x.scalar_type() == at::kHalf && e == 8 && std::fabs(y) >= 248.f) y = std::copysign(240.f, y);
+        if (e == highest && std::fabs(y) >= 248.f) y = std::copysign(240.f, y);
         v[i] = y;
       }
       s[r * blocks + b] = static_cast<uint8_t>(e + 127);
