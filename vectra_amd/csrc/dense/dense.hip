@@ -12,6 +12,7 @@
 // reading z back.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "dense_common.h"
@@ -51,18 +52,45 @@ __global__ __launch_bounds__(256) void zero_tail_kernel(T* x, int64_t rows, int6
   if (at < rows * n) x[at / n * stride + from + at % n] = static_cast<T>(0.f);
 }
 
-// Adds up the planes of a split product in order and finishes it:
-// act(sum + bias) + residual.  One thread per four columns.
-template <typename T>
+// Adds up the planes of a split product in a fixed order and finishes it:
+// act(sum + bias) + residual.  A thread adds every kLanes-th plane of four
+// columns, four planes in flight; the kLanes threads of a quad are joined in
+// LDS.  One lane per quad where there are few planes or many quads; 16 where
+// one thread would walk hundreds of planes (a [256, 128] weight gradient of
+// 208 parts: 57.8 us with one lane, each load waiting for the one before).
+template <typename T, int kLanes>
 __global__ __launch_bounds__(256) void join_kernel(const float* parts, int splits, int64_t m, int64_t n, int64_t ld,
                                                    GemmParams p) {
+  constexpr int kQuads = 256 / kLanes;
+  __shared__ f32x4 part[kLanes > 1 ? kLanes : 1][kQuads];
+  const int q = threadIdx.x % kQuads, lane = threadIdx.x / kQuads;
   const int64_t quads = ld / 4;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= m * quads) return;
-  const int64_t row = at / quads, col = (at - row * quads) * 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kQuads + q;
+  const bool live = at < m * quads;
+  const int64_t row = live ? at / quads : 0, col = live ? (at - row * quads) * 4 : 0;
+  const float* const from = parts + row * ld + col;
+  const int64_t plane = m * ld;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(parts + k * m * ld + row * ld + col);
-  const int left = static_cast<int>(min<int64_t>(n - col, 4));
+  if (live) {
+    int k = lane;
+    for (; k + 3 * kLanes < splits; k += 4 * kLanes) {
+      f32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(from + (k + j * kLanes) * plane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += v[j];
+    }
+    for (; k < splits; k += kLanes) s += *reinterpret_cast<const f32x4*>(from + k * plane);
+  }
+  if constexpr (kLanes > 1) {
+    part[lane][q] = s;
+    __syncthreads();
+    if (lane != 0) return;
+#pragma unroll
+    for (int k = 1; k < kLanes; ++k) s += part[k][q];
+  }
+  if (!live) return;
+  const int left = static_cast<int>(least(n - col, 4));
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (p.bias && e < left) s[e] += load_bias(p.bias, col + e, p.bias_dtype);
@@ -82,7 +110,7 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const In* x, int64_t 
   __shared__ float part[16][64];
   const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + c;
-  const int64_t first = blockIdx.y * per, last = min(first + per, rows);
+  const int64_t first = blockIdx.y * per, last = least(first + per, rows);
   float s = 0.f;
   if (col < n)
     for (int64_t row = first + r; row < last; row += 16) s += widen(x[row * stride + col]);
@@ -141,7 +169,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
   const bool live = at < rows * blocks;
   const int64_t row = live ? at / blocks : 0, block = live ? at - row * blocks : 0;
   const int64_t col = block * kBlock + (threadIdx.x & 7) * 4;
-  const int left = live ? static_cast<int>(max<int64_t>(min<int64_t>(width - col, 4), 0)) : 0;
+  const int left = live ? static_cast<int>(most(least(width - col, 4), 0)) : 0;
   f32x4 v = load4(x + row * stride + col, left, vec & 1);
   float largest = 0.f;
 #pragma unroll
@@ -189,7 +217,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, i
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (at >= rows * quads) return;
   const int64_t row = at / quads, col = (at - row * quads) * 4;
-  const int left = static_cast<int>(max<int64_t>(min<int64_t>(width - col, 4), 0));
+  const int left = static_cast<int>(most(least(width - col, 4), 0));
   const uint8_t* const p = codes + row * codes_stride + col;
   uint32_t w = 0;
   if (left == 4 && (vec & 2)) {
@@ -205,7 +233,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, i
     const float s = e == 128 ? __builtin_nanf("") : e == -127 ? 5.877471754111438e-39f : power_of_two(e);
     v *= s;
   }
-  store4(out + row * out_stride + col, v, static_cast<int>(min<int64_t>(columns - col, 4)), vec & 1);
+  store4(out + row * out_stride + col, v, static_cast<int>(least(columns - col, 4)), vec & 1);
 }
 
 // -------------------------------------------------------------------- host
@@ -294,33 +322,50 @@ struct Call {
     return (reinterpret_cast<uintptr_t>(p) & (4 * esize() - 1)) == 0 && ld % 4 == 0 ? flag : 0;
   }
 
-  // A product through the tile whose workgroups fill the CUs; where even the
-  // smallest tile leaves most CUs idle and the contraction is long, it is
-  // split and joined.
+  // The tile and the number of contraction parts with the least estimated time.
+  //
+  // Workgroups resident per CU by LDS (1, 2 and 5), the rate of a CU full of
+  // them (16 bits: 1.15, 0.95 and 0.7 PFLOP/s over 256 CUs; fp32: 0.12 for
+  // each), and the work counted in whole tiles and whole rounds of the chip:
+  //   2051 x 2048 -> 11264 fp16: 118 / 105 / 145 us for the large, medium and
+  //   small tile (estimated in this order, too); 10007 x 5464 -> 1000 bf16 with
+  //   a wide operand: 193 / 206 / 229.
+  // A split costs its fp32 planes, written and read once at 5 TB/s, and the
+  // joining launch.  Contractions of at most four tiles have no steady state:
+  // the small tile's five workgroups per CU hide each other's loads and
+  // stores (66560 x 128 -> 256 bf16: 42 / 31 / 23 us).
+  void choose(const GemmParams& p, int64_t columns, int epi, int& tile, int& splits) const {
+    static constexpr double kRate16[kTileCount] = {1.15e15, 0.95e15, 0.7e15}, kRate32 = 0.12e15;
+    static constexpr int kResident[kTileCount] = {1, 2, 5};
+    splits = 1;
+    tile = kTileCount - 1;
+    if (p.k_tiles <= 4) return;
+    double best = 1e30;
+    const int most_splits = epi == kEpiStore ? std::min(256, p.k_tiles / 2) : 1;
+    for (int t = 0; t < kTileCount; ++t) {
+      const double tiles = static_cast<double>(ceil_div(p.m, kTileM[t])) * ceil_div(columns, kTileN[t]);
+      const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : kRate16[t]) / cus / kResident[t];  // of one workgroup
+      for (int k = 1; k <= most_splits; k *= 2) {
+        const double rounds = std::ceil(tiles * k / (cus * kResident[t]));
+        const double one = 2.0 * kTileM[t] * kTileN[t] * (128 / esize()) * ceil_div(p.k_tiles, k) / rate + 2e-6;
+        const double join = k > 1 ? 8.0 * k * p.m * p.n / 5e12 + 4e-6 : 0;
+        const double time = rounds * one + join;
+        if (time < best * 0.98) {
+          best = time;
+          tile = t;
+          splits = k;
+        }
+      }
+    }
+  }
+
   void product(GemmParams p, int layout, int epi) {
     const bool gated = epi == kEpiGated || epi == kEpiGatedSlope;
     const int64_t columns = gated ? 2 * p.n : p.n;
     const int deep = static_cast<int>(128 / esize());
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
-    int tile = kTileCount - 1;
-    for (int t = 0; t < kTileCount; ++t) {
-      const int64_t tiles = ceil_div(p.m, kTileM[t]) * ceil_div(columns, kTileN[t]);
-      if (tiles >= cus * 3 / 4) {
-        tile = t;
-        break;
-      }
-    }
-    int splits = 1;
-    if (epi == kEpiStore) {
-      // Medium tiles on parts of the contraction rather than small ones on all of it.
-      const int64_t medium = ceil_div(p.m, 128) * ceil_div(columns, 128);
-      if (tile == kTileCount - 1 && p.k_tiles >= 8) {
-        if (medium * p.k_tiles / 4 >= cus / 2) tile = kTileMedium;
-        const int64_t tiles = ceil_div(p.m, kTileM[tile]) * ceil_div(columns, kTileN[tile]);
-        splits = static_cast<int>(std::min<int64_t>(ceil_div(2 * cus, tiles), p.k_tiles / 4));
-        splits = std::max(1, std::min(splits, 256));
-      }
-    }
+    int tile, splits;
+    choose(p, columns, epi, tile, splits);
     p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileM[tile]));
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileN[tile]));
     last_tiles_m = p.tiles_m;
@@ -339,8 +384,11 @@ struct Call {
     if (go())
       typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        join_kernel<T><<<static_cast<uint32_t>(ceil_div(p.m * (ld / 4), 256)), 256, 0, stream>>>(parts, splits, p.m, p.n,
-                                                                                               ld, p);
+        const int64_t quads = p.m * (ld / 4);
+        if (splits > 8 && quads < 64 * 256 * 4)
+          join_kernel<T, 16><<<static_cast<uint32_t>(ceil_div(quads, 16)), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p);
+        else
+          join_kernel<T, 1><<<static_cast<uint32_t>(ceil_div(quads, 256)), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p);
       });
     most = std::max(most, scratch.used);
     scratch.used = kept;  // the next product may use it again: launches of one stream run in order

@@ -229,7 +229,7 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
     a_step = static_cast<int64_t>(C::kDeep) * p.lda * sizeof(T);
   } else {
     a += m0 * p.lda + static_cast<int64_t>(k_first) * C::kDeep;
-    const int64_t rows = min<int64_t>(p.m - m0, C::kBM);
+    const int64_t rows = least(p.m - m0, C::kBM);
     a_bytes = ((rows - 1) * p.lda + p.depth - static_cast<int64_t>(k_first) * C::kDeep) * sizeof(T);
     a_step = C::kDeep * sizeof(T);
   }
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
     b_step = static_cast<int64_t>(C::kDeep) * p.ldb * sizeof(T);
   } else {
     b += n0 * p.ldb + static_cast<int64_t>(k_first) * C::kDeep;
-    const int64_t rows = (C::kGated ? p.n : 0) + min<int64_t>(p.n - n0, kOutN);
+    const int64_t rows = (C::kGated ? p.n : 0) + least(p.n - n0, kOutN);
     b_bytes = ((rows - 1) * p.ldb + p.depth - static_cast<int64_t>(k_first) * C::kDeep) * sizeof(T);
     b_step = C::kDeep * sizeof(T);
   }
@@ -275,9 +275,9 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
   }
   const auto load = [&](int kt, int buf) {
     lds_char* const at = smem + buf * C::kStageBytes;
-    const int left = static_cast<int>((min<int64_t>(p.depth - static_cast<int64_t>(kt) * C::kDeep, C::kDeep) + A::kPer - 1) / A::kPer);
-    stage<A, T, C::kWideA, C::kThreads>(at, a, a_off, min<int64_t>(a_bytes, 0x7fffffff), left, a_chunk, wave);
-    stage<B, T, C::kWideB, C::kThreads>(at + A::kBytes, b, b_off, min<int64_t>(b_bytes, 0x7fffffff), left, b_chunk, wave);
+    const int left = static_cast<int>((least(p.depth - static_cast<int64_t>(kt) * C::kDeep, C::kDeep) + A::kPer - 1) / A::kPer);
+    stage<A, T, C::kWideA, C::kThreads>(at, a, a_off, least(a_bytes, 0x7fffffff), left, a_chunk, wave);
+    stage<B, T, C::kWideB, C::kThreads>(at + A::kBytes, b, b_off, least(b_bytes, 0x7fffffff), left, b_chunk, wave);
     a = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a) + a_step);
     b = reinterpret_cast<const T*>(reinterpret_cast<const char*>(b) + b_step);
     a_bytes -= a_step;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
 #pragma unroll
   for (int u = 0; u < kPairs; ++u) {
     const int64_t n = n_wave + u * 16 + 4 * g;
-    const int left = static_cast<int>(min<int64_t>(p.n - n, 4));
+    const int left = static_cast<int>(least(p.n - n, 4));
     f32x4 bias = {0.f, 0.f, 0.f, 0.f}, bias_up = {0.f, 0.f, 0.f, 0.f};
     if (C::kEpi != kEpiPartial && p.bias) {
 #pragma unroll
