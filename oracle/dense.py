@@ -132,7 +132,7 @@ class Layer:
             return value, e + rounding(value, e, dtype)
 
         bias = dz.sum(0)
-        bias_err = err.sum(0) + (m + 1) * U * SLACK * size.sum(0)
+        bias_err = kept.sum(0) + (m + 1) * U * SLACK * size.sum(0)
         return {
             'x': product(dz @ self.weight, dz, kept, self.weight),
             'weight': product(dz.t() @ self.x, dz.t(), kept.t(), self.x),

@@ -44,6 +44,8 @@ SIZES = [
     (63, 65, 31), (64, 64, 64), (65, 128, 384), (127, 72, 129), (128, 128, 128), (129, 136, 257), (255, 200, 256),
     (256, 64, 512), (300, 33, 7), (1, 4096, 520), (4, 2048, 77), (40, 1000, 200), (513, 264, 1000), (2048, 8, 8),
     (5000, 24, 40),
+    # Many rows by a weight that fits LDS.
+    (16384, 128, 256), (16391, 141, 33), (17000, 72, 100), (16500, 256, 128), (16400, 30, 65),
 ]
 
 

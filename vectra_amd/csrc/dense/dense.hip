@@ -60,8 +60,17 @@ __global__ __launch_bounds__(256) void zero_tail_kernel(T* x, int64_t rows, int6
 // 208 parts: 57.8 us with one lane, each load waiting for the one before).
 template <typename T, int kLanes>
 __global__ __launch_bounds__(256) void join_kernel(const float* parts, int splits, int64_t m, int64_t n, int64_t ld,
-                                                   GemmParams p) {
+                                                   GemmParams p, const float* sum_parts, int quad_blocks) {
   constexpr int kQuads = 256 / kLanes;
+  if (static_cast<int>(blockIdx.x) >= quad_blocks) {  // the sums' planes: a thread per sum
+    const int64_t at = static_cast<int64_t>(blockIdx.x - quad_blocks) * 256 + threadIdx.x;
+    if (at >= m) return;
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += sum_parts[k * m + at];
+    store_as(p.sums, at, p.sums_dtype, s);
+    return;
+  }
   __shared__ f32x4 part[kLanes > 1 ? kLanes : 1][kQuads];
   const int q = threadIdx.x % kQuads, lane = threadIdx.x / kQuads;
   const int64_t quads = ld / 4;
@@ -119,13 +128,7 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const In* x, int64_t 
   if (r != 0 || col >= n) return;
 #pragma unroll
   for (int k = 1; k < 16; ++k) s += part[k][c];
-  const int64_t at = blockIdx.y * out_stride + col;
-  if (out_dtype == VECTRA_DENSE_F32)
-    static_cast<float*>(out)[at] = s;
-  else if (out_dtype == VECTRA_DENSE_F16)
-    static_cast<_Float16*>(out)[at] = narrow<_Float16>(s);
-  else
-    static_cast<__bf16*>(out)[at] = narrow<__bf16>(s);
+  store_as(out, blockIdx.y * out_stride + col, out_dtype, s);
 }
 
 // ------------------------------------------------------------- 8-bit rows
@@ -322,6 +325,11 @@ struct Call {
     return (reinterpret_cast<uintptr_t>(p) & (4 * esize() - 1)) == 0 && ld % 4 == 0 ? flag : 0;
   }
 
+  // Rows that start on 16 bytes (resident kernels move eight 16-bit elements at once).
+  int vec8(const void* p, int64_t ld, int flag) const {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % per() == 0 ? flag : 0;
+  }
+
   // The tile and the number of contraction parts with the least estimated time.
   //
   // Workgroups resident per CU by LDS (1, 2 and 5), the rate of a CU full of
@@ -368,7 +376,6 @@ struct Call {
     choose(p, columns, epi, tile, splits);
     p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileM[tile]));
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileN[tile]));
-    last_tiles_m = p.tiles_m;
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
     splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
     if (splits == 1) {
@@ -377,29 +384,60 @@ struct Call {
     }
     const int64_t ld = ceil_div(p.n, 4) * 4, kept = scratch.used;
     float* const parts = static_cast<float*>(scratch.take(splits * p.m * ld * 4));
+    float* const sum_parts = p.sums ? static_cast<float*>(scratch.take(splits * p.m * 4)) : nullptr;
     GemmParams q = p;
     q.out = parts;
+    q.sums = sum_parts;
     q.ldo = ld;
     run(q, layout, tile, kEpiPartial, splits);
     if (go())
       typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const int64_t quads = p.m * (ld / 4);
-        if (splits > 8 && quads < 64 * 256 * 4)
-          join_kernel<T, 16><<<static_cast<uint32_t>(ceil_div(quads, 16)), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p);
-        else
-          join_kernel<T, 1><<<static_cast<uint32_t>(ceil_div(quads, 256)), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p);
+        const bool lanes = splits > 8 && quads < 64 * 256 * 4;
+        const int64_t blocks = ceil_div(quads, lanes ? 16 : 256), sum_blocks = sum_parts ? ceil_div(p.m, 256) : 0;
+        const auto kernel = lanes ? join_kernel<T, 16> : join_kernel<T, 1>;
+        kernel<<<static_cast<uint32_t>(blocks + sum_blocks), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p, sum_parts,
+                                                                               static_cast<int>(blocks));
       });
     most = std::max(most, scratch.used);
     scratch.used = kept;  // the next product may use it again: launches of one stream run in order
   }
   int64_t most = 0;          // of scratch, over all products
-  int64_t last_tiles_m = 0;  // tile rows of the last product
 
   void run(const GemmParams& p, int layout, int tile, int epi, int splits) {
     if (!go()) return;
     const auto f = dtype == VECTRA_DENSE_F32 ? launch_gemm_f32 : dtype == VECTRA_DENSE_F16 ? launch_gemm_f16 : launch_gemm_bf16;
     const int st = f(p, layout, tile, epi, splits, stream);
+    if (st != VECTRA_DENSE_OK) status = st;
+  }
+
+  // Contraction steps of the resident kernel that serves these sizes, or 0.
+  // Its workgroups copy the whole weight first, so it needs rows enough that
+  // every CU's 16 waves have a unit of 16 rows.
+  int resident_steps(int64_t rows, int64_t width, int64_t n, bool gated) const {
+    if (rows < 16 * 16 * cus / 4) return 0;
+    const int64_t bytes = width * esize(), n_pad = ceil_div(n, 32) * 32 * (1 + gated);
+    const auto fits = [&](int steps) {
+      const int64_t row = steps * 64 + ((steps & (steps - 1)) ? 16 : 0) + 4;  // and the bias
+      return bytes <= steps * 64 && n_pad * row <= kResidentLds;
+    };
+    if (esize() == 2) {
+      for (int s : kResidentSteps16)
+        if (fits(s)) return s;
+    } else {
+      for (int s : kResidentSteps32)
+        if (fits(s)) return s;
+    }
+    return 0;
+  }
+
+  void resident(ResidentParams p, int steps, int epi, bool with_dx) {
+    if (!go()) return;
+    p.n_pad = static_cast<int32_t>(ceil_div(p.n, 32) * 32);
+    const auto f = dtype == VECTRA_DENSE_F32 ? launch_resident_f32 : dtype == VECTRA_DENSE_F16 ? launch_resident_f16 : launch_resident_bf16;
+    const int workgroups = static_cast<int>(std::min<int64_t>(cus, ceil_div(ceil_div(p.rows, 16), 16)));
+    const int st = f(p, steps, epi, with_dx, workgroups, stream);
     if (st != VECTRA_DENSE_OK) status = st;
   }
 
@@ -475,6 +513,26 @@ int check_forward(const vectra_dense_args* a) {
 void forward(const vectra_dense_args& a, Call& c) {
   if (a.rows == 0 || a.width_out == 0) return;
   const int64_t n_w = a.width_out * (1 + a.gated);
+  if (const int steps = a.width_in ? c.resident_steps(a.rows, a.width_in, a.width_out, a.gated) : 0) {
+    ResidentParams p{};
+    p.x = a.x;
+    p.ldx = a.x_stride;
+    p.rows = a.rows;
+    p.width = a.width_in;
+    p.w = a.weight;
+    p.ldw = a.weight_stride;
+    p.n = static_cast<int32_t>(a.width_out);
+    p.bias = a.bias;
+    p.bias_dtype = a.bias_dtype;
+    p.activation = a.activation;
+    p.residual = a.residual;
+    p.ldr = a.residual_stride;
+    p.out = a.out;
+    p.ldo = a.out_stride;
+    p.vec = c.vec8(a.out, a.out_stride, kVecOut) | c.vec8(a.residual, a.residual_stride, kVecResidual);
+    c.resident(p, steps, a.gated ? kEpiGated : kEpiStore, false);
+    return;
+  }
   const Matrix x = c.operand(a.x, a.x_stride, a.rows, a.width_in);
   const Matrix w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
   GemmParams p{};
@@ -537,11 +595,17 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
   const bool want_db = a.dbias && n_w;
   if (!want_dx && !want_dw && !want_db) return;
   const bool use_x = slope || want_dw, use_w = slope || want_dx;
+  const bool use_dz = want_dw || want_db;
   Matrix x{nullptr, 0}, w{nullptr, 0}, dz{nullptr, 0};
   const int64_t depth = c.padded(a.width_in);
-  if (use_x && a.rows && a.width_in) {
+  const int64_t n_pad = c.padded(n_w);
+  const bool any = a.rows && a.width_in && n_w;
+  // A layer with a slope whose weight fits LDS: dz and dx in one pass over x and grad.
+  const int steps = slope && any ? c.resident_steps(a.rows, a.width_in, a.width_out, a.gated) : 0;
+  const bool dx_with_dz = steps > 0 && want_dx && c.esize() == 2 && steps <= kResidentDxSteps;
+  if (use_x && any) {
     if (a.x) {
-      x = c.operand(a.x, a.x_stride, a.rows, a.width_in);
+      x = steps > 0 && !want_dw ? Matrix{a.x, a.x_stride} : c.operand(a.x, a.x_stride, a.rows, a.width_in);
     } else {
       x = {c.scratch.take(a.rows * depth * c.esize()), depth};
       if (c.go())
@@ -554,36 +618,52 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
         });
     }
   }
-  if (use_w && a.rows && a.width_in && n_w) w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
-  const int64_t n_pad = c.padded(n_w);
-  float* sums = nullptr;
-  int64_t sum_rows = 0;
-  if (slope && a.rows && n_w) {
-    dz = {c.scratch.take(a.rows * n_pad * c.esize()), n_pad};
-    // Tile rows of the smallest tile: at least as many as the product uses.
-    sum_rows = ceil_div(a.rows, kTileM[kTileCount - 1]);
-    if (want_db) sums = static_cast<float*>(c.scratch.take(sum_rows * n_w * 4));
-    GemmParams p{};
-    p.a = x.p;
-    p.lda = x.ld;
-    p.b = w.p;
-    p.ldb = w.ld;
-    p.m = a.rows;
-    p.n = a.width_out;
-    p.depth = p.depth_b = depth;
-    p.out = const_cast<void*>(dz.p);
-    p.ldo = n_pad;
-    p.bias = a.bias;
-    p.bias_dtype = a.bias_dtype;
-    p.activation = a.activation;
-    p.grad = a.grad;
-    p.ldg = a.grad_stride;
-    p.sums = sums;
-    p.sums_stride = n_w;
-    p.vec = kVecOut | (a.width_out % 4 == 0 ? kVecOutUp : 0) | c.vec4(a.grad, a.grad_stride, kVecGrad);
-    c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope);
-    sum_rows = c.last_tiles_m;
-    if (n_pad != n_w && c.go())
+  if (use_w && any && (steps == 0 || (want_dx && !dx_with_dz)))
+    w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
+  if (slope && a.rows && n_w && (use_dz || want_dx)) {
+    const bool keep_dz = use_dz || !dx_with_dz;
+    if (keep_dz) dz = {c.scratch.take(a.rows * n_pad * c.esize()), n_pad};
+    if (steps > 0) {
+      ResidentParams p{};
+      p.x = x.p;
+      p.ldx = x.ld;
+      p.rows = a.rows;
+      p.width = a.width_in;
+      p.w = a.weight;
+      p.ldw = a.weight_stride;
+      p.n = static_cast<int32_t>(a.width_out);
+      p.bias = a.bias;
+      p.bias_dtype = a.bias_dtype;
+      p.activation = a.activation;
+      p.grad = a.grad;
+      p.ldg = a.grad_stride;
+      p.out = keep_dz ? const_cast<void*>(dz.p) : nullptr;
+      p.ldo = n_pad;
+      p.dx = dx_with_dz ? a.dx : nullptr;
+      p.lddx = a.dx_stride;
+      p.vec = kVecOut | (a.width_out % 8 == 0 ? kVecOutUp : 0) | c.vec8(a.grad, a.grad_stride, kVecGrad) |
+              c.vec4(a.dx, a.dx_stride, kVecDx);
+      c.resident(p, steps, a.gated ? kEpiGatedSlope : kEpiSlope, dx_with_dz);
+    } else {
+      GemmParams p{};
+      p.a = x.p;
+      p.lda = x.ld;
+      p.b = w.p;
+      p.ldb = w.ld;
+      p.m = a.rows;
+      p.n = a.width_out;
+      p.depth = p.depth_b = depth;
+      p.out = const_cast<void*>(dz.p);
+      p.ldo = n_pad;
+      p.bias = a.bias;
+      p.bias_dtype = a.bias_dtype;
+      p.activation = a.activation;
+      p.grad = a.grad;
+      p.ldg = a.grad_stride;
+      p.vec = kVecOut | (a.width_out % 4 == 0 ? kVecOutUp : 0) | c.vec4(a.grad, a.grad_stride, kVecGrad);
+      c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope);
+    }
+    if (keep_dz && n_pad != n_w && c.go())
       c.typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         zero_tail_kernel<T><<<static_cast<uint32_t>(ceil_div(a.rows * (n_pad - n_w), 256)), 256, 0, c.stream>>>(
@@ -591,17 +671,16 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       });
   } else if (want_dx || want_dw) {
     dz = c.operand(a.grad, a.grad_stride, a.rows, n_w);
+  } else {
+    dz = {a.grad, a.grad_stride};
   }
-  if (want_db) {
-    if (sums || a.rows == 0 || n_w == 0)
-      c.column_sums<float>(sums, n_w, sums ? sum_rows : 0, n_w, a.dbias, a.bias_dtype);
-    else
-      c.typed([&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        c.column_sums<T>(static_cast<const T*>(a.grad), a.grad_stride, a.rows, n_w, a.dbias, a.bias_dtype);
-      });
-  }
-  if (want_dx) {
+  // db: with dW where that is formed too (the sums of its first operand).
+  if (want_db && !want_dw)
+    c.typed([&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      c.column_sums<T>(static_cast<const T*>(dz.p), dz.ld, a.rows, n_w, a.dbias, a.bias_dtype);
+    });
+  if (want_dx && !dx_with_dz) {
     GemmParams p{};
     p.a = dz.p;
     p.lda = dz.ld;
@@ -628,6 +707,8 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
     p.m = n_w;
     p.n = a.width_in;
     p.depth = p.depth_b = a.rows;
+    p.sums = want_db ? a.dbias : nullptr;
+    p.sums_dtype = a.bias_dtype;
     p.out = a.dweight;
     p.ldo = a.dweight_stride;
     p.vec = c.vec4(a.dweight, a.dweight_stride, kVecOut);

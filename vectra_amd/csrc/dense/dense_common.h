@@ -170,4 +170,14 @@ __device__ __forceinline__ float load_bias(const void* bias, int64_t i, int32_t 
   }
 }
 
+// Writes element i of a vector in the given type.
+__device__ __forceinline__ void store_as(void* out, int64_t i, int32_t dtype, float v) {
+  if (dtype == VECTRA_DENSE_F32)
+    static_cast<float*>(out)[i] = v;
+  else if (dtype == VECTRA_DENSE_F16)
+    static_cast<_Float16*>(out)[i] = narrow<_Float16>(v);
+  else
+    static_cast<__bf16*>(out)[i] = narrow<__bf16>(v);
+}
+
 }  // namespace vectra_dense

@@ -13,12 +13,12 @@ enum {
   kEpiStore = 0,       // act(D + bias) + residual, in the element type
   kEpiPartial = 1,     // D in fp32, one plane per split of the contraction
   kEpiGated = 2,       // act(D_gate + bias) * (D_up + bias)
-  kEpiSlope = 3,       // grad * act'(D + bias), and its column sums
-  kEpiGatedSlope = 4,  // both factors' gradients, and their column sums
+  kEpiSlope = 3,       // grad * act'(D + bias)
+  kEpiGatedSlope = 4,  // both factors' gradients
 };
 
 // GemmParams::vec: rows that start at multiples of four elements.
-enum { kVecOut = 1, kVecResidual = 2, kVecGrad = 4, kVecOutUp = 8 };
+enum { kVecOut = 1, kVecResidual = 2, kVecGrad = 4, kVecOutUp = 8, kVecDx = 16 };
 
 struct GemmParams {
   const void* a;  // row operand
@@ -37,8 +37,11 @@ struct GemmParams {
   int64_t ldr;
   const void* grad;
   int64_t ldg;
-  float* sums;  // column sums per tile row, or NULL
-  int64_t sums_stride;
+  // Weight layout: sums of A over the contraction (the bias's gradient), [m]
+  // in sums_dtype where the product is whole, fp32 [splits, m] where it is
+  // split; NULL: not wanted.
+  void* sums;
+  int32_t sums_dtype;
   int32_t bias_dtype;
   int32_t activation;
   int32_t vec;
@@ -55,5 +58,36 @@ constexpr int kTileN[kTileCount] = {256, 128, 64};
 int launch_gemm_bf16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
 int launch_gemm_f16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
 int launch_gemm_f32(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
+
+// A product with a weight that stays in LDS (resident_impl.h).
+struct ResidentParams {
+  const void* x;
+  int64_t ldx, rows, width;  // width: contraction
+  const void* w;
+  int64_t ldw;
+  int32_t w_wide;    // 0: W [n, width]; 1: W [width, n]
+  int32_t n, n_pad;  // outputs (gated: of a half), and rounded up to 32
+  const void* bias;
+  int32_t bias_dtype, activation, vec;
+  const void* residual;
+  int64_t ldr;
+  const void* grad;  // slope epilogues
+  int64_t ldg;
+  void* out;  // y, or dz (NULL: not wanted)
+  int64_t ldo;
+  void* dx;
+  int64_t lddx;
+};
+
+// Contraction steps (of 64 bytes) that a resident kernel exists for, the LDS a
+// workgroup may use, and the steps up to which it can form dx as well.
+constexpr int kResidentSteps16[] = {2, 4, 8};
+constexpr int kResidentSteps32[] = {2, 4, 6, 9, 12, 16};
+constexpr int kResidentLds = 160 * 1024;
+constexpr int kResidentDxSteps = 4;
+
+int launch_resident_bf16(const ResidentParams& p, int steps, int epi, bool with_dx, int workgroups, hipStream_t stream);
+int launch_resident_f16(const ResidentParams& p, int steps, int epi, bool with_dx, int workgroups, hipStream_t stream);
+int launch_resident_f32(const ResidentParams& p, int steps, int epi, bool with_dx, int workgroups, hipStream_t stream);
 
 }  // namespace vectra_dense

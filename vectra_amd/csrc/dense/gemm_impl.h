@@ -53,12 +53,24 @@ struct Mma<__bf16> {
   static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a.w), __builtin_bit_cast(V, b.w), c, 0, 0, 0);
   }
+  // s + the fragment's elements, in fp32.
+  static __device__ __forceinline__ float sum(Frag a, float s) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += __uint_as_float(a.w[j] << 16) + __uint_as_float(a.w[j] & 0xffff0000u);
+    return s;
+  }
 };
 template <>
 struct Mma<_Float16> {
   typedef _Float16 V __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a.w), __builtin_bit_cast(V, b.w), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum(Frag a, float s) {
+    const V v = __builtin_bit_cast(V, a.w);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) s += static_cast<float>(v[j]) + static_cast<float>(v[j + 1]);
+    return s;
   }
 };
 template <>
@@ -68,6 +80,11 @@ struct Mma<float> {
     for (int j = 0; j < 4; ++j)
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[j]), __uint_as_float(b.w[j]), c, 0, 0, 0);
     return c;
+  }
+  static __device__ __forceinline__ float sum(Frag a, float s) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += __uint_as_float(a.w[j]);
+    return s;
   }
 };
 
@@ -194,6 +211,7 @@ struct GemmConfig {
   static constexpr int kDeep = 128 / sizeof(T);  // contraction per tile
   static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
   static constexpr bool kGated = kEpi == kEpiGated || kEpi == kEpiGatedSlope;
+  static constexpr bool kSums = kWideA && kWideB;  // the weight's gradient, and with it the bias's
   using A = Tile<T, kWideA, kBM, kDeep, kThreads>;
   using B = Tile<T, kWideB, kBN, kDeep, kThreads>;
   static constexpr int kStageBytes = A::kBytes + B::kBytes;
@@ -290,6 +308,11 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
 #pragma unroll
     for (int tm_ = 0; tm_ < C::kTM; ++tm_) acc[tn_][tm_] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  const bool sum_here = C::kSums && p.sums && tn == 0 && wn == 0;
+  float sums[C::kSums ? C::kTM : 1];
+#pragma unroll
+  for (int t = 0; t < (C::kSums ? C::kTM : 1); ++t) sums[t] = 0.f;
+
   if (k_first < k_last) load(k_first, 0);
   for (int kt = k_first; kt < k_last; ++kt) {
     const int buf = (kt - k_first) & 1;
@@ -309,14 +332,17 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
       for (int t = 0; t < C::kTM; ++t)
 #pragma unroll
         for (int u = 0; u < C::kTN; ++u) acc[u][t] = Mma<T>::run(fb[u], fa[t], acc[u][t]);
+      if constexpr (C::kSums) {
+        if (sum_here)
+#pragma unroll
+          for (int t = 0; t < C::kTM; ++t) sums[t] = Mma<T>::sum(fa[t], sums[t]);
+      }
     }
   }
 
   // ---- epilogue: lane holds D[m, n .. n + 3] of every 16 x 16 tile
   constexpr int kPairs = C::kGated ? C::kTN / 2 : C::kTN;
-  constexpr bool kSlope = C::kEpi == kEpiSlope || C::kEpi == kEpiGatedSlope;
   const int64_t n_wave = n0 + wn * kPairs * 16;
-  f32x4 sum_a[kSlope ? kPairs : 1], sum_b[kSlope && C::kGated ? kPairs : 1];
 #pragma unroll
   for (int u = 0; u < kPairs; ++u) {
     const int64_t n = n_wave + u * 16 + 4 * g;
@@ -329,10 +355,6 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
           bias[e] = load_bias(p.bias, n + e, p.bias_dtype);
           if constexpr (C::kGated) bias_up[e] = load_bias(p.bias, p.n + n + e, p.bias_dtype);
         }
-    }
-    if constexpr (kSlope) {
-      sum_a[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (C::kGated) sum_b[u] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (int t = 0; t < C::kTM; ++t) {
@@ -368,50 +390,27 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
         }
         T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
         store4(out, da, left, p.vec & kVecOut);
-        sum_a[u] += da;
-        if constexpr (C::kGated) {
-          store4(out + p.n, db, left, p.vec & kVecOutUp);
-          sum_b[u] += db;
-        }
+        if constexpr (C::kGated) store4(out + p.n, db, left, p.vec & kVecOutUp);
       }
     }
   }
 
-  // Column sums of dz over this tile's rows, for the bias's gradient: over the
-  // 16 lanes of a group, then over the waves of a column through LDS, in a
-  // fixed order.  Row `tm` of p.sums receives them.
-  if constexpr (kSlope) {
-    if (p.sums) {
-      __syncthreads();  // all waves are done with the tiles
-      __attribute__((address_space(3))) float* const sums = (__attribute__((address_space(3))) float*)smem;
-      constexpr int kCols = C::kBN;  // gated: kBN / 2 gate columns, then as many up columns
+  // The sums of A over the contraction, gathered by the waves of the first
+  // column of tiles: lane group g holds those of its own elements.
+  if constexpr (C::kSums) {
+    if (sum_here) {
 #pragma unroll
-      for (int u = 0; u < kPairs; ++u) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float s = sum_a[u][e], s2 = 0.f;
-          if constexpr (C::kGated) s2 = sum_b[u][e];
-#pragma unroll
-          for (int d = 1; d < 16; d <<= 1) {
-            s += __shfl_xor(s, d);
-            if constexpr (C::kGated) s2 += __shfl_xor(s2, d);
-          }
-          if (i == 0) {
-            const int col = (wn * kPairs + u) * 16 + 4 * g + e;
-            sums[wm * kCols + col] = s;
-            if constexpr (C::kGated) sums[wm * kCols + kOutN + col] = s2;
-          }
+      for (int t = 0; t < C::kTM; ++t) {
+        float s = sums[t];
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
+        if (g == 0 && m < p.m) {
+          if constexpr (C::kEpi == kEpiPartial)
+            static_cast<float*>(p.sums)[blockIdx.y * p.m + m] = s;
+          else
+            store_as(p.sums, m, p.sums_dtype, s);
         }
-      }
-      __syncthreads();
-      for (int col = tid; col < kCols; col += C::kThreads) {
-        const bool up = C::kGated && col >= kOutN;
-        const int64_t n = n0 + (up ? col - kOutN : col);
-        if (n >= p.n) continue;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < C::kWM; ++w) s += sums[w * kCols + col];
-        p.sums[static_cast<int64_t>(tm) * p.sums_stride + (up ? p.n : 0) + n] = s;
       }
     }
   }
