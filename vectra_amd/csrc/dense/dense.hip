@@ -162,81 +162,93 @@ __device__ __forceinline__ f32x4 from_e4m3x4(uint32_t w) {
   return f32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
-// Eight lanes per block of 32, four elements per lane.
-template <typename T>
+// Both kernels move eight elements per thread and turn, 16 bytes of a 16-bit
+// row, and turn their work's index into a row and a column by 32-bit division
+// (Index) where the counts allow: a 64-bit one costs more than the rest of a
+// turn (66560 x 256 bf16: 16.6 us with it and four elements per thread).
+
+// Four lanes per block of 32.
+template <typename T, typename Index>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows, int64_t width, int64_t stride,
                                                        uint8_t* codes, int64_t codes_stride, uint8_t* scales,
                                                        int64_t scales_stride, int64_t blocks, int vec) {
   constexpr int kLowest = __is_same(T, _Float16) ? -15 : -117, kHighest = __is_same(T, _Float16) ? 8 : 120;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
-  const bool live = at < rows * blocks;
-  const int64_t row = live ? at / blocks : 0, block = live ? at - row * blocks : 0;
-  const int64_t col = block * kBlock + (threadIdx.x & 7) * 4;
-  const int left = live ? static_cast<int>(most(least(width - col, 4), 0)) : 0;
-  f32x4 v = load4(x + row * stride + col, left, vec & 1);
+  const Index at = static_cast<Index>(blockIdx.x) * 64 + (threadIdx.x >> 2);
+  const bool live = at < static_cast<Index>(rows * blocks);
+  const Index row = live ? at / static_cast<Index>(blocks) : 0;
+  const int64_t block = live ? at - row * static_cast<Index>(blocks) : 0;
+  const int64_t col = block * kBlock + (threadIdx.x & 3) * 8;
+  const int left = live ? static_cast<int>(most(least(width - col, 8), 0)) : 0;
+  f32x4 v[2] = {};
+  if (left > 0) load8(x + row * stride + col, left, vec & 1, v[0], v[1]);
   float largest = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float a = __builtin_fabsf(v[e]);
+  for (int k = 0; k < 8; ++k) {
+    const float a = __builtin_fabsf(v[k / 4][k % 4]);
     if (a <= 3.4028234663852886e38f) {
       largest = a > largest ? a : largest;
     } else {
-      v[e] = __builtin_nanf("");
+      v[k / 4][k % 4] = __builtin_nanf("");
     }
   }
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+  for (int d = 1; d < 4; d <<= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
   const int byte = block_exponent(largest, kLowest);
   const int e = byte - 127;
+  uint32_t w[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] *= power_of_two(-e);  // e in [-117, 120]
-  // The type's largest value, 255.9 * 2^8 (fp16) or 2^120, would round to 256
-  // times that, which the type lacks: at its exponent, magnitudes of 248 and
-  // more take the code below, 240.
-  if (e == kHighest)
+  for (int h = 0; h < 2; ++h) {
+    v[h] *= power_of_two(-e);  // e in [-117, 120]
+    // The type's largest value, 255.9 * 2^8 (fp16) or 2^120, would round to
+    // 256 times that, which the type lacks: at its exponent, magnitudes of
+    // 248 and more take the code below, 240.
+    if (e == kHighest)
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (__builtin_fabsf(v[k]) >= 248.f) v[k] = __builtin_copysignf(240.f, v[k]);
-  const uint32_t w = to_e4m3x4(v);
+      for (int k = 0; k < 4; ++k)
+        if (__builtin_fabsf(v[h][k]) >= 248.f) v[h][k] = __builtin_copysignf(240.f, v[h][k]);
+    w[h] = to_e4m3x4(v[h]);
+  }
   uint8_t* const out = codes + row * codes_stride + col;
-  if (left == 4 && (vec & 2)) {
-    *reinterpret_cast<uint32_t*>(out) = w;
+  if (left == 8 && (vec & 2)) {
+    *reinterpret_cast<uint2*>(out) = uint2{w[0], w[1]};
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < left) out[k] = static_cast<uint8_t>(w >> (8 * k));
+    for (int k = 0; k < 8; ++k)
+      if (k < left) out[k] = static_cast<uint8_t>(w[k / 4] >> (8 * (k % 4)));
   }
-  if (live && (threadIdx.x & 7) == 0) scales[row * scales_stride + block] = static_cast<uint8_t>(byte);
+  if (live && (threadIdx.x & 3) == 0) scales[row * scales_stride + block] = static_cast<uint8_t>(byte);
 }
 
-// One thread per four columns of the output's `ld` columns; columns from
-// `width` on are zeros (the workspace's padded rows).
-template <typename T>
+// The output has `columns` columns; those from `width` on are zeros (the
+// workspace's padded rows).
+template <typename T, typename Index>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, int64_t codes_stride,
                                                          const uint8_t* scales, int64_t scales_stride, int64_t rows,
                                                          int64_t width, T* out, int64_t out_stride, int64_t columns,
                                                          int vec) {
-  const int64_t quads = (columns + 3) / 4;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= rows * quads) return;
-  const int64_t row = at / quads, col = (at - row * quads) * 4;
-  const int left = static_cast<int>(most(least(width - col, 4), 0));
+  const Index eights = static_cast<Index>((columns + 7) / 8);
+  const Index at = static_cast<Index>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= static_cast<Index>(rows) * eights) return;
+  const Index row = at / eights;
+  const int64_t col = static_cast<int64_t>(at - row * eights) * 8;
+  const int left = static_cast<int>(most(least(width - col, 8), 0));
   const uint8_t* const p = codes + row * codes_stride + col;
-  uint32_t w = 0;
-  if (left == 4 && (vec & 2)) {
-    w = *reinterpret_cast<const uint32_t*>(p);
+  uint2 w = {0, 0};
+  if (left == 8 && (vec & 2)) {
+    w = *reinterpret_cast<const uint2*>(p);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < left) w |= static_cast<uint32_t>(p[k]) << (8 * k);
+    for (int k = 0; k < 8; ++k)
+      if (k < left) (k < 4 ? w.x : w.y) |= static_cast<uint32_t>(p[k]) << (8 * (k % 4));
   }
-  f32x4 v = from_e4m3x4(w);
+  f32x4 a = from_e4m3x4(w.x), b = from_e4m3x4(w.y);
   if (left > 0) {
     const int e = static_cast<int>(scales[row * scales_stride + col / kBlock]) - 127;
     const float s = e == 128 ? __builtin_nanf("") : e == -127 ? 5.877471754111438e-39f : power_of_two(e);
-    v *= s;
+    a *= s;
+    b *= s;
   }
-  store4(out + row * out_stride + col, v, static_cast<int>(least(columns - col, 4)), vec & 1);
+  store8(out + row * out_stride + col, a, b, static_cast<int>(least(columns - col, 8)), vec & 1);
 }
 
 // -------------------------------------------------------------------- host
@@ -462,6 +474,29 @@ struct Call {
   }
 };
 
+// The 8-bit form's kernels, for the operators and for a backward pass.
+template <typename T>
+void quantize(const void* x, int64_t rows, int64_t width, int64_t stride, void* codes, int64_t codes_stride, void* scales,
+              int64_t scales_stride, Call& c) {
+  const int64_t blocks = ceil_div(width, kBlock), grid = ceil_div(rows * blocks, 64);
+  const int vec = c.vec8(x, stride, 1) | ((reinterpret_cast<uintptr_t>(codes) & 7) == 0 && codes_stride % 8 == 0 ? 2 : 0);
+  const auto kernel = rows * blocks < (int64_t{1} << 31) - 64 ? quantize_kernel<T, uint32_t> : quantize_kernel<T, int64_t>;
+  kernel<<<static_cast<uint32_t>(grid), 256, 0, c.stream>>>(
+      static_cast<const T*>(x), rows, width, stride, static_cast<uint8_t*>(codes), codes_stride,
+      static_cast<uint8_t*>(scales), scales_stride, blocks, vec);
+}
+
+template <typename T>
+void dequantize(const void* codes, int64_t codes_stride, const void* scales, int64_t scales_stride, int64_t rows,
+                int64_t width, const void* out, int64_t out_stride, int64_t columns, Call& c) {
+  const int64_t work = rows * ceil_div(columns, 8);
+  const int vec = c.vec8(out, out_stride, 1) | ((reinterpret_cast<uintptr_t>(codes) & 7) == 0 && codes_stride % 8 == 0 ? 2 : 0);
+  const auto kernel = work < (int64_t{1} << 31) - 256 ? dequantize_kernel<T, uint32_t> : dequantize_kernel<T, int64_t>;
+  kernel<<<static_cast<uint32_t>(ceil_div(work, 256)), 256, 0, c.stream>>>(
+      static_cast<const uint8_t*>(codes), codes_stride, static_cast<const uint8_t*>(scales), scales_stride, rows, width,
+      const_cast<T*>(static_cast<const T*>(out)), out_stride, columns, vec);
+}
+
 constexpr int64_t kMostRows = int64_t{1} << 30;
 constexpr int64_t kMostWidth = int64_t{1} << 21;
 
@@ -531,6 +566,28 @@ void forward(const vectra_dense_args& a, Call& c) {
     p.ldo = a.out_stride;
     p.vec = c.vec8(a.out, a.out_stride, kVecOut) | c.vec8(a.residual, a.residual_stride, kVecResidual);
     c.resident(p, steps, a.gated ? kEpiGated : kEpiStore, false);
+    return;
+  }
+  if (a.rows <= kFewRows && a.width_in) {
+    if (!c.go()) return;
+    FewRowsParams p{};
+    p.x = a.x;
+    p.ldx = a.x_stride;
+    p.rows = static_cast<int32_t>(a.rows);
+    p.w = a.weight;
+    p.ldw = a.weight_stride;
+    p.n = a.width_out;
+    p.width = a.width_in;
+    p.bias = a.bias;
+    p.bias_dtype = a.bias_dtype;
+    p.activation = a.activation;
+    p.residual = a.residual;
+    p.ldr = a.residual_stride;
+    p.out = a.out;
+    p.ldo = a.out_stride;
+    p.vec = c.vec4(a.out, a.out_stride, kVecOut) | c.vec4(a.residual, a.residual_stride, kVecResidual);
+    const auto f = a.dtype == VECTRA_DENSE_F32 ? launch_few_rows_f32 : a.dtype == VECTRA_DENSE_F16 ? launch_few_rows_f16 : launch_few_rows_bf16;
+    c.status = f(p, a.gated, c.stream);
     return;
   }
   const Matrix x = c.operand(a.x, a.x_stride, a.rows, a.width_in);
@@ -611,10 +668,7 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       if (c.go())
         c.typed([&](auto* t) {
           using T = std::remove_pointer_t<decltype(t)>;
-          const int vec = 1 | ((reinterpret_cast<uintptr_t>(a.codes) & 3) == 0 && a.codes_stride % 4 == 0 ? 2 : 0);
-          dequantize_kernel<T><<<static_cast<uint32_t>(ceil_div(a.rows * (depth / 4), 256)), 256, 0, c.stream>>>(
-              static_cast<const uint8_t*>(a.codes), a.codes_stride, static_cast<const uint8_t*>(a.scales),
-              a.scales_stride, a.rows, a.width_in, const_cast<T*>(static_cast<const T*>(x.p)), depth, depth, vec);
+          dequantize<T>(a.codes, a.codes_stride, a.scales, a.scales_stride, a.rows, a.width_in, x.p, depth, depth, c);
         });
     }
   }
@@ -779,13 +833,9 @@ int vectra_rows_quantize(const void* x, int32_t dtype, int64_t rows, int64_t wid
   if (int st = check_stride(scales_stride, blocks, rows, 1, 1)) return st;
   Call c{dtype, {nullptr, 0}, true, reinterpret_cast<hipStream_t>(stream), 0};
   (void)hipGetLastError();
-  const int vec = c.vec4(x, x_stride, 1) |
-                  ((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && codes_stride % 4 == 0 ? 2 : 0);
   c.typed([&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    quantize_kernel<T><<<static_cast<uint32_t>(ceil_div(rows * blocks, 32)), 256, 0, c.stream>>>(
-        static_cast<const T*>(x), rows, width, x_stride, static_cast<uint8_t*>(codes), codes_stride,
-        static_cast<uint8_t*>(scales), scales_stride, blocks, vec);
+    quantize<T>(x, rows, width, x_stride, codes, codes_stride, scales, scales_stride, c);
   });
   return c.status;
 }
@@ -802,13 +852,9 @@ int vectra_rows_dequantize(const void* codes, int64_t codes_stride, const void* 
   if (int st = check_stride(scales_stride, ceil_div(width, kBlock), rows, 1, 1)) return st;
   Call c{dtype, {nullptr, 0}, true, reinterpret_cast<hipStream_t>(stream), 0};
   (void)hipGetLastError();
-  const int vec = c.vec4(out, out_stride, 1) |
-                  ((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && codes_stride % 4 == 0 ? 2 : 0);
   c.typed([&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    dequantize_kernel<T><<<static_cast<uint32_t>(ceil_div(rows * ceil_div(width, 4), 256)), 256, 0, c.stream>>>(
-        static_cast<const uint8_t*>(codes), codes_stride, static_cast<const uint8_t*>(scales), scales_stride, rows,
-        width, static_cast<T*>(out), out_stride, width, vec);
+    dequantize<T>(codes, codes_stride, scales, scales_stride, rows, width, out, out_stride, width, c);
   });
   return c.status;
 }

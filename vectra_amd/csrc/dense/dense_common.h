@@ -158,6 +158,39 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int left, bool vec) {
   }
 }
 
+// Eight consecutive elements of one row (two quads), `left` of which exist;
+// `vec`: the row's eights are aligned to 16 bytes.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, f32x4 a, f32x4 b, int left, bool vec) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec && left >= 8) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      asm volatile("" : "+v"(a), "+v"(b));
+      const uint2 lo = __builtin_bit_cast(uint2, __builtin_convertvector(a, T4));
+      const uint2 hi = __builtin_bit_cast(uint2, __builtin_convertvector(b, T4));
+      *reinterpret_cast<u32x4*>(p) = u32x4{lo.x, lo.y, hi.x, hi.y};
+      return;
+    }
+  }
+  store4(p, a, left, vec);
+  store4(p + 4, b, left - 4, vec);
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, bool vec, f32x4& a, f32x4& b) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec && left >= 8) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+      a = __builtin_convertvector(__builtin_bit_cast(T4, uint2{w[0], w[1]}), f32x4);
+      b = __builtin_convertvector(__builtin_bit_cast(T4, uint2{w[2], w[3]}), f32x4);
+      return;
+    }
+  }
+  a = load4(p, left, vec);
+  b = load4(p + 4, left - 4, vec);
+}
+
 // Element i of a bias, in its own type.
 __device__ __forceinline__ float load_bias(const void* bias, int64_t i, int32_t dtype) {
   switch (dtype) {

@@ -90,4 +90,24 @@ int launch_resident_bf16(const ResidentParams& p, int steps, int epi, bool with_
 int launch_resident_f16(const ResidentParams& p, int steps, int epi, bool with_dx, int workgroups, hipStream_t stream);
 int launch_resident_f32(const ResidentParams& p, int steps, int epi, bool with_dx, int workgroups, hipStream_t stream);
 
+// A product of a few rows (few_rows_impl.h).
+struct FewRowsParams {
+  const void* x;
+  int64_t ldx;
+  int32_t rows;
+  const void* w;
+  int64_t ldw, n, width;  // outputs (gated: of a half), contraction
+  const void* bias;
+  int32_t bias_dtype, activation, vec;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  int64_t ldo;
+};
+constexpr int kFewRows = 32;
+
+int launch_few_rows_bf16(const FewRowsParams& p, bool gated, hipStream_t stream);
+int launch_few_rows_f16(const FewRowsParams& p, bool gated, hipStream_t stream);
+int launch_few_rows_f32(const FewRowsParams& p, bool gated, hipStream_t stream);
+
 }  // namespace vectra_dense

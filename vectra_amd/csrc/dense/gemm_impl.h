@@ -53,10 +53,18 @@ struct Mma<__bf16> {
   static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a.w), __builtin_bit_cast(V, b.w), c, 0, 0, 0);
   }
-  // s + the fragment's elements, in fp32.
+  // s + the fragment's elements, in fp32: one v_dot2 per pair.  The ones come
+  // from a scalar register: as an inline constant the compiler encodes a bf16
+  // pair as the 32-bit constant of one of its halves.
   static __device__ __forceinline__ float sum(Frag a, float s) {
+    typedef __bf16 V2 __attribute__((ext_vector_type(2)));
+    uint32_t ones;
+    asm("s_mov_b32 %0, 0x3f803f80" : "=s"(ones));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s += __uint_as_float(a.w[j] << 16) + __uint_as_float(a.w[j] & 0xffff0000u);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t pair = a.w[j];  // (a bit cast of the element itself takes element 0)
+      s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, pair), __builtin_bit_cast(V2, ones), s, false);
+    }
     return s;
   }
 };
@@ -67,9 +75,13 @@ struct Mma<_Float16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a.w), __builtin_bit_cast(V, b.w), c, 0, 0, 0);
   }
   static __device__ __forceinline__ float sum(Frag a, float s) {
-    const V v = __builtin_bit_cast(V, a.w);
+    typedef _Float16 V2 __attribute__((ext_vector_type(2)));
+    const V2 ones = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) s += static_cast<float>(v[j]) + static_cast<float>(v[j + 1]);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t pair = a.w[j];
+      s = __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, pair), ones, s, false);
+    }
     return s;
   }
 };
@@ -308,7 +320,9 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
 #pragma unroll
     for (int tm_ = 0; tm_ < C::kTM; ++tm_) acc[tn_][tm_] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const bool sum_here = C::kSums && p.sums && tn == 0 && wn == 0;
+  // Sums of A: by the workgroups of the first tile column, tile t of a wave's
+  // rows by the wave t % kWN of that row.
+  const bool sum_here = C::kSums && p.sums && tn == 0;
   float sums[C::kSums ? C::kTM : 1];
 #pragma unroll
   for (int t = 0; t < (C::kSums ? C::kTM : 1); ++t) sums[t] = 0.f;
@@ -335,7 +349,8 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
       if constexpr (C::kSums) {
         if (sum_here)
 #pragma unroll
-          for (int t = 0; t < C::kTM; ++t) sums[t] = Mma<T>::sum(fa[t], sums[t]);
+          for (int t = 0; t < C::kTM; ++t)
+            if (t % C::kWN == wn) sums[t] = Mma<T>::sum(fa[t], sums[t]);
       }
     }
   }
@@ -395,8 +410,8 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
     }
   }
 
-  // The sums of A over the contraction, gathered by the waves of the first
-  // column of tiles: lane group g holds those of its own elements.
+  // The sums of A over the contraction: lane group g holds those of its own
+  // elements.
   if constexpr (C::kSums) {
     if (sum_here) {
 #pragma unroll
@@ -405,7 +420,7 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
-        if (g == 0 && m < p.m) {
+        if (g == 0 && m < p.m && t % C::kWN == wn) {
           if constexpr (C::kEpi == kEpiPartial)
             static_cast<float*>(p.sums)[blockIdx.y * p.m + m] = s;
           else

@@ -62,50 +62,20 @@ __device__ __forceinline__ int resident_swizzle(int row) {
   return (row >> 2) & 3;
 }
 
-template <typename T, typename C>
+// Elements first .. of a row of `width`, zeros past its end.
+template <typename T>
 __device__ __forceinline__ Frag load_row_chunk(const T* row, int64_t width, int first) {
+  constexpr int kPer = 16 / sizeof(T);
   Frag f;
-  if (first + C::kPer <= width) {
+  if (first + kPer <= width) {
     __builtin_memcpy(&f.w, row + first, 16);  // unaligned
   } else {
-    T v[C::kPer];
+    T v[kPer];
 #pragma unroll
-    for (int e = 0; e < C::kPer; ++e) v[e] = first + e < width ? row[first + e] : static_cast<T>(0.f);
+    for (int e = 0; e < kPer; ++e) v[e] = first + e < width ? row[first + e] : static_cast<T>(0.f);
     __builtin_memcpy(&f.w, v, 16);
   }
   return f;
-}
-
-// Eight consecutive results of one row (two quads), `left` of which exist.
-template <typename T>
-__device__ __forceinline__ void store8(T* p, f32x4 a, f32x4 b, int left, bool vec) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec && left >= 8) {
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      asm volatile("" : "+v"(a), "+v"(b));
-      const uint2 lo = __builtin_bit_cast(uint2, __builtin_convertvector(a, T4));
-      const uint2 hi = __builtin_bit_cast(uint2, __builtin_convertvector(b, T4));
-      *reinterpret_cast<u32x4*>(p) = u32x4{lo.x, lo.y, hi.x, hi.y};
-      return;
-    }
-  }
-  store4(p, a, left, vec);
-  store4(p + 4, b, left - 4, vec);
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, bool vec, f32x4& a, f32x4& b) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec && left >= 8) {
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-      a = __builtin_convertvector(__builtin_bit_cast(T4, uint2{w[0], w[1]}), f32x4);
-      b = __builtin_convertvector(__builtin_bit_cast(T4, uint2{w[2], w[3]}), f32x4);
-      return;
-    }
-  }
-  a = load4(p, left, vec);
-  b = load4(p + 4, left - 4, vec);
 }
 
 // kAct: the activation, fixed per instantiation of the body so that no branch
@@ -127,7 +97,7 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
     Frag fx[C::kSteps];
 #pragma unroll
     for (int s = 0; s < C::kSteps; ++s)
-      fx[s] = load_row_chunk<T, C>(x + row_read * p.ldx, p.width, (s * 4 + g) * C::kPer);
+      fx[s] = load_row_chunk<T>(x + row_read * p.ldx, p.width, (s * 4 + g) * C::kPer);
 
     f32x4 dx[C::kDx ? C::kDeep / 16 : 1];
     if constexpr (C::kDx) {
@@ -288,7 +258,7 @@ __global__ __launch_bounds__(64 * kResidentWaves) void resident_kernel(const Res
         }
         __builtin_memcpy(&f.w, v, 16);
       } else {
-        f = load_row_chunk<T, C>(w + w_row * p.ldw, p.width, chunk * C::kPer);
+        f = load_row_chunk<T>(w + w_row * p.ldw, p.width, chunk * C::kPer);
       }
     }
     const int to = C::kPowerOfTwo ? chunk ^ resident_swizzle<C::kChunks>(r & 15) : chunk;
