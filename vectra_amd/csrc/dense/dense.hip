@@ -105,8 +105,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
     if (p.bias && e < left) s[e] += load_bias(p.bias, col + e, p.bias_dtype);
     s[e] = act_value(s[e], p.activation);
   }
-  if (p.residual) s += load4(static_cast<const T*>(p.residual) + row * p.ldr + col, left, p.vec & kVecResidual);
-  store4(static_cast<T*>(p.out) + row * p.ldo + col, s, left, p.vec & kVecOut);
+  if (p.residual) s += load4(static_cast<const T*>(p.residual) + row * p.ldr + col, left);
+  store4(static_cast<T*>(p.out) + row * p.ldo + col, s, left);
 }
 
 // Sums of 64 columns over the rows [blockIdx.y * per, ...): 16 row lanes of 64
@@ -171,7 +171,7 @@ __device__ __forceinline__ f32x4 from_e4m3x4(uint32_t w) {
 template <typename T, typename Index>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows, int64_t width, int64_t stride,
                                                        uint8_t* codes, int64_t codes_stride, uint8_t* scales,
-                                                       int64_t scales_stride, int64_t blocks, int vec) {
+                                                       int64_t scales_stride, int64_t blocks) {
   constexpr int kLowest = __is_same(T, _Float16) ? -15 : -117, kHighest = __is_same(T, _Float16) ? 8 : 120;
   const Index at = static_cast<Index>(blockIdx.x) * 64 + (threadIdx.x >> 2);
   const bool live = at < static_cast<Index>(rows * blocks);
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
   const int64_t col = block * kBlock + (threadIdx.x & 3) * 8;
   const int left = live ? static_cast<int>(most(least(width - col, 8), 0)) : 0;
   f32x4 v[2] = {};
-  if (left > 0) load8(x + row * stride + col, left, vec & 1, v[0], v[1]);
+  if (left > 0) load8(x + row * stride + col, left, v[0], v[1]);
   float largest = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
@@ -209,8 +209,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
     w[h] = to_e4m3x4(v[h]);
   }
   uint8_t* const out = codes + row * codes_stride + col;
-  if (left == 8 && (vec & 2)) {
-    *reinterpret_cast<uint2*>(out) = uint2{w[0], w[1]};
+  if (left == 8) {
+    __builtin_memcpy(out, w, 8);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -224,8 +224,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
 template <typename T, typename Index>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, int64_t codes_stride,
                                                          const uint8_t* scales, int64_t scales_stride, int64_t rows,
-                                                         int64_t width, T* out, int64_t out_stride, int64_t columns,
-                                                         int vec) {
+                                                         int64_t width, T* out, int64_t out_stride, int64_t columns) {
   const Index eights = static_cast<Index>((columns + 7) / 8);
   const Index at = static_cast<Index>(blockIdx.x) * 256 + threadIdx.x;
   if (at >= static_cast<Index>(rows) * eights) return;
@@ -234,8 +233,8 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, i
   const int left = static_cast<int>(most(least(width - col, 8), 0));
   const uint8_t* const p = codes + row * codes_stride + col;
   uint2 w = {0, 0};
-  if (left == 8 && (vec & 2)) {
-    w = *reinterpret_cast<const uint2*>(p);
+  if (left == 8) {
+    __builtin_memcpy(&w, p, 8);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -248,7 +247,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, i
     a *= s;
     b *= s;
   }
-  store8(out + row * out_stride + col, a, b, static_cast<int>(least(columns - col, 8)), vec & 1);
+  store8(out + row * out_stride + col, a, b, static_cast<int>(least(columns - col, 8)));
 }
 
 // -------------------------------------------------------------------- host
@@ -331,15 +330,6 @@ struct Call {
             static_cast<const T*>(p), ld, rows, width, static_cast<T*>(out), chunks);
       });
     return {out, out_ld};
-  }
-
-  int vec4(const void* p, int64_t ld, int flag) const {
-    return (reinterpret_cast<uintptr_t>(p) & (4 * esize() - 1)) == 0 && ld % 4 == 0 ? flag : 0;
-  }
-
-  // Rows that start on 16 bytes (resident kernels move eight 16-bit elements at once).
-  int vec8(const void* p, int64_t ld, int flag) const {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % per() == 0 ? flag : 0;
   }
 
   // The tile and the number of contraction parts with the least estimated time.
@@ -479,22 +469,20 @@ template <typename T>
 void quantize(const void* x, int64_t rows, int64_t width, int64_t stride, void* codes, int64_t codes_stride, void* scales,
               int64_t scales_stride, Call& c) {
   const int64_t blocks = ceil_div(width, kBlock), grid = ceil_div(rows * blocks, 64);
-  const int vec = c.vec8(x, stride, 1) | ((reinterpret_cast<uintptr_t>(codes) & 7) == 0 && codes_stride % 8 == 0 ? 2 : 0);
   const auto kernel = rows * blocks < (int64_t{1} << 31) - 64 ? quantize_kernel<T, uint32_t> : quantize_kernel<T, int64_t>;
   kernel<<<static_cast<uint32_t>(grid), 256, 0, c.stream>>>(
       static_cast<const T*>(x), rows, width, stride, static_cast<uint8_t*>(codes), codes_stride,
-      static_cast<uint8_t*>(scales), scales_stride, blocks, vec);
+      static_cast<uint8_t*>(scales), scales_stride, blocks);
 }
 
 template <typename T>
 void dequantize(const void* codes, int64_t codes_stride, const void* scales, int64_t scales_stride, int64_t rows,
                 int64_t width, const void* out, int64_t out_stride, int64_t columns, Call& c) {
   const int64_t work = rows * ceil_div(columns, 8);
-  const int vec = c.vec8(out, out_stride, 1) | ((reinterpret_cast<uintptr_t>(codes) & 7) == 0 && codes_stride % 8 == 0 ? 2 : 0);
   const auto kernel = work < (int64_t{1} << 31) - 256 ? dequantize_kernel<T, uint32_t> : dequantize_kernel<T, int64_t>;
   kernel<<<static_cast<uint32_t>(ceil_div(work, 256)), 256, 0, c.stream>>>(
       static_cast<const uint8_t*>(codes), codes_stride, static_cast<const uint8_t*>(scales), scales_stride, rows, width,
-      const_cast<T*>(static_cast<const T*>(out)), out_stride, columns, vec);
+      const_cast<T*>(static_cast<const T*>(out)), out_stride, columns);
 }
 
 constexpr int64_t kMostRows = int64_t{1} << 30;
@@ -564,7 +552,6 @@ void forward(const vectra_dense_args& a, Call& c) {
     p.ldr = a.residual_stride;
     p.out = a.out;
     p.ldo = a.out_stride;
-    p.vec = c.vec8(a.out, a.out_stride, kVecOut) | c.vec8(a.residual, a.residual_stride, kVecResidual);
     c.resident(p, steps, a.gated ? kEpiGated : kEpiStore, false);
     return;
   }
@@ -585,7 +572,6 @@ void forward(const vectra_dense_args& a, Call& c) {
     p.ldr = a.residual_stride;
     p.out = a.out;
     p.ldo = a.out_stride;
-    p.vec = c.vec4(a.out, a.out_stride, kVecOut) | c.vec4(a.residual, a.residual_stride, kVecResidual);
     const auto f = a.dtype == VECTRA_DENSE_F32 ? launch_few_rows_f32 : a.dtype == VECTRA_DENSE_F16 ? launch_few_rows_f16 : launch_few_rows_bf16;
     c.status = f(p, a.gated, c.stream);
     return;
@@ -607,7 +593,6 @@ void forward(const vectra_dense_args& a, Call& c) {
   p.activation = a.activation;
   p.residual = a.residual;
   p.ldr = a.residual_stride;
-  p.vec = c.vec4(a.out, a.out_stride, kVecOut) | c.vec4(a.residual, a.residual_stride, kVecResidual);
   c.product(p, kLayoutForward, a.gated ? kEpiGated : kEpiStore);
 }
 
@@ -695,8 +680,6 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       p.ldo = n_pad;
       p.dx = dx_with_dz ? a.dx : nullptr;
       p.lddx = a.dx_stride;
-      p.vec = kVecOut | (a.width_out % 8 == 0 ? kVecOutUp : 0) | c.vec8(a.grad, a.grad_stride, kVecGrad) |
-              c.vec4(a.dx, a.dx_stride, kVecDx);
       c.resident(p, steps, a.gated ? kEpiGatedSlope : kEpiSlope, dx_with_dz);
     } else {
       GemmParams p{};
@@ -714,7 +697,6 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       p.activation = a.activation;
       p.grad = a.grad;
       p.ldg = a.grad_stride;
-      p.vec = kVecOut | (a.width_out % 4 == 0 ? kVecOutUp : 0) | c.vec4(a.grad, a.grad_stride, kVecGrad);
       c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope);
     }
     if (keep_dz && n_pad != n_w && c.go())
@@ -747,7 +729,6 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
     p.depth_b = n_w;
     p.out = a.dx;
     p.ldo = a.dx_stride;
-    p.vec = c.vec4(a.dx, a.dx_stride, kVecOut);
     c.product(p, kLayoutInput, kEpiStore);
   }
   if (want_dw) {
@@ -765,7 +746,6 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
     p.sums_dtype = a.bias_dtype;
     p.out = a.dweight;
     p.ldo = a.dweight_stride;
-    p.vec = c.vec4(a.dweight, a.dweight_stride, kVecOut);
     c.product(p, kLayoutWeight, kEpiStore);
   }
 }

@@ -114,6 +114,22 @@ __device__ __forceinline__ void act_slope(float z, int act, float& value, float&
   }
 }
 
+// f with the activation as a constant: its element loops hold no branch.
+template <int kAct>
+struct Activation {
+  static constexpr int value = kAct;
+};
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  switch (act) {
+    case VECTRA_DENSE_RELU: return f(Activation<VECTRA_DENSE_RELU>{});
+    case VECTRA_DENSE_GELU: return f(Activation<VECTRA_DENSE_GELU>{});
+    case VECTRA_DENSE_GELU_TANH: return f(Activation<VECTRA_DENSE_GELU_TANH>{});
+    case VECTRA_DENSE_SILU: return f(Activation<VECTRA_DENSE_SILU>{});
+    default: return f(Activation<VECTRA_DENSE_NONE>{});
+  }
+}
+
 // ------------------------------------------------------------ element types
 
 template <typename T>
@@ -128,14 +144,17 @@ __device__ __forceinline__ T narrow(float x) {
   return static_cast<T>(x);
 }
 
-// Four consecutive elements p[0..3] of which those at n .. n_end - 1 exist.
-// `vec`: p is aligned to four elements.
+// Runs of four and eight consecutive elements of a row, of which `left` exist.
+// Whole runs move as one 8- or 16-byte access (fp32: 16 bytes, twice for
+// eight) at whatever alignment the row has: gfx950's vector memory accesses
+// need none.
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, int left, bool vec) {
+__device__ __forceinline__ f32x4 load4(const T* p, int left) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (vec && left >= 4) {
+  if (left >= 4) {
     typedef T T4 __attribute__((ext_vector_type(4)));
-    const T4 v = *reinterpret_cast<const T4*>(p);
+    T4 v;
+    __builtin_memcpy(&v, p, sizeof(v));
     r = __builtin_convertvector(v, f32x4);
   } else {
 #pragma unroll
@@ -146,11 +165,12 @@ __device__ __forceinline__ f32x4 load4(const T* p, int left, bool vec) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* p, f32x4 v, int left, bool vec) {
-  if (vec && left >= 4) {
+__device__ __forceinline__ void store4(T* p, f32x4 v, int left) {
+  if (left >= 4) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     if constexpr (sizeof(T) < 4) asm volatile("" : "+v"(v));
-    *reinterpret_cast<T4*>(p) = __builtin_convertvector(v, T4);
+    const T4 t = __builtin_convertvector(v, T4);
+    __builtin_memcpy(p, &t, sizeof(t));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -158,37 +178,37 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int left, bool vec) {
   }
 }
 
-// Eight consecutive elements of one row (two quads), `left` of which exist;
-// `vec`: the row's eights are aligned to 16 bytes.
 template <typename T>
-__device__ __forceinline__ void store8(T* p, f32x4 a, f32x4 b, int left, bool vec) {
+__device__ __forceinline__ void load8(const T* p, int left, f32x4& a, f32x4& b) {
   if constexpr (sizeof(T) == 2) {
-    if (vec && left >= 8) {
+    if (left >= 8) {
       typedef T T4 __attribute__((ext_vector_type(4)));
-      asm volatile("" : "+v"(a), "+v"(b));
-      const uint2 lo = __builtin_bit_cast(uint2, __builtin_convertvector(a, T4));
-      const uint2 hi = __builtin_bit_cast(uint2, __builtin_convertvector(b, T4));
-      *reinterpret_cast<u32x4*>(p) = u32x4{lo.x, lo.y, hi.x, hi.y};
-      return;
-    }
-  }
-  store4(p, a, left, vec);
-  store4(p + 4, b, left - 4, vec);
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, bool vec, f32x4& a, f32x4& b) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec && left >= 8) {
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+      u32x4 w;
+      __builtin_memcpy(&w, p, 16);
       a = __builtin_convertvector(__builtin_bit_cast(T4, uint2{w[0], w[1]}), f32x4);
       b = __builtin_convertvector(__builtin_bit_cast(T4, uint2{w[2], w[3]}), f32x4);
       return;
     }
   }
-  a = load4(p, left, vec);
-  b = load4(p + 4, left - 4, vec);
+  a = load4(p, left);
+  b = load4(p + 4, left - 4);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, f32x4 a, f32x4 b, int left) {
+  if constexpr (sizeof(T) == 2) {
+    if (left >= 8) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      asm volatile("" : "+v"(a), "+v"(b));
+      const uint2 lo = __builtin_bit_cast(uint2, __builtin_convertvector(a, T4));
+      const uint2 hi = __builtin_bit_cast(uint2, __builtin_convertvector(b, T4));
+      const u32x4 w = {lo.x, lo.y, hi.x, hi.y};
+      __builtin_memcpy(p, &w, 16);
+      return;
+    }
+  }
+  store4(p, a, left);
+  store4(p + 4, b, left - 4);
 }
 
 // Element i of a bias, in its own type.

@@ -17,9 +17,6 @@ enum {
   kEpiGatedSlope = 4,  // both factors' gradients
 };
 
-// GemmParams::vec: rows that start at multiples of four elements.
-enum { kVecOut = 1, kVecResidual = 2, kVecGrad = 4, kVecOutUp = 8, kVecDx = 16 };
-
 struct GemmParams {
   const void* a;  // row operand
   const void* b;  // column operand
@@ -44,7 +41,6 @@ struct GemmParams {
   int32_t sums_dtype;
   int32_t bias_dtype;
   int32_t activation;
-  int32_t vec;
 };
 
 // The shapes of one tiled product's kernels.
@@ -68,7 +64,7 @@ struct ResidentParams {
   int32_t w_wide;    // 0: W [n, width]; 1: W [width, n]
   int32_t n, n_pad;  // outputs (gated: of a half), and rounded up to 32
   const void* bias;
-  int32_t bias_dtype, activation, vec;
+  int32_t bias_dtype, activation;
   const void* residual;
   int64_t ldr;
   const void* grad;  // slope epilogues
@@ -98,7 +94,7 @@ struct FewRowsParams {
   const void* w;
   int64_t ldw, n, width;  // outputs (gated: of a half), contraction
   const void* bias;
-  int32_t bias_dtype, activation, vec;
+  int32_t bias_dtype, activation;
   const void* residual;
   int64_t ldr;
   void* out;

@@ -99,8 +99,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const FewRowsP
     z[e] = act_value(z[e], p.activation);
     if constexpr (kGated) z[e] *= u[e];
   }
-  if (!kGated && p.residual) z += load4(static_cast<const T*>(p.residual) + m * p.ldr + n, left, p.vec & kVecResidual);
-  store4(static_cast<T*>(p.out) + m * p.ldo + n, z, left, p.vec & kVecOut);
+  if (!kGated && p.residual) z += load4(static_cast<const T*>(p.residual) + m * p.ldr + n, left);
+  store4(static_cast<T*>(p.out) + m * p.ldo + n, z, left);
 }
 
 template <typename T>

@@ -111,6 +111,7 @@ struct Tile {
   static constexpr int kBytes = kLdsRows * kRowBytes;
   static constexpr int kSlots = kLdsRows * kChunks / kThreads;      // loads per thread
   static constexpr int kStep = 4 * kPer;                            // contraction per fragment
+  static constexpr int kReads = !kWide ? 1 : sizeof(T) == 2 ? 2 : 4;  // LDS reads per fragment
   static_assert(kSlots * kThreads == kLdsRows * kChunks, "whole loads");
   static_assert(kWide || kChunks == 8 || kChunks == 4, "64- or 128-byte deep rows");
 
@@ -194,6 +195,27 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& t
 // operations; a workgroup barrier by itself orders LDS instructions only).
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
+// The same, and for LDS reads.
+__device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(0x0070); }  // vmcnt(0) lgkmcnt(0)
+
+// Asks the scheduler to spread a phase's LDS reads (and loads) over its
+// products.
+template <typename C, bool kLoads>
+__device__ __forceinline__ void interleave() {
+  constexpr int kReads = C::kTM * C::A::kReads + C::kTN * C::B::kReads;
+  constexpr int kProducts = C::kTM * C::kTN * C::kMmas;
+  constexpr int kLoadCount = kLoads ? C::A::kSlots + C::B::kSlots : 0;
+  constexpr int kGroups = kReads;
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+    constexpr int kEach = kProducts / kGroups;
+    __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);  // matrix
+    if (kLoadCount > 0 && j * kLoadCount / kGroups != (j + 1) * kLoadCount / kGroups)
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // load
+  }
+}
+
 constexpr uint32_t kOutside = 0x80000000u;  // past any buffer (host checks: tiles span less than 2^31 bytes)
 
 // Loads the tile of one operand.  `base`: the operand's element (first row of
@@ -207,15 +229,14 @@ __device__ __forceinline__ void stage(lds_char* tile, const T* base, const uint3
 #pragma unroll
   for (int s = 0; s < TileT::kSlots; ++s) {
     uint32_t at = offset[s];
-    if constexpr (!kWide) {
-      if (valid_chunks < TileT::kChunks) at = static_cast<int>(chunk[s]) < valid_chunks ? at : kOutside;
-    }
+    if constexpr (!kWide) at = static_cast<int>(chunk[s]) < valid_chunks ? at : kOutside;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         rsrc, (__attribute__((address_space(3))) void*)(tile + (s * kThreads + wave * 64) * 16), 16, at, 0, 0, 0);
   }
 }
 
-template <typename T, int kBM_, int kBN_, int kWM_, int kWN_, bool kWideA_, bool kWideB_, int kEpi_>
+template <typename T, int kBM_, int kBN_, int kWM_, int kWN_, bool kWideA_, bool kWideB_, int kEpi_,
+          bool kPhased_ = false>
 struct GemmConfig {
   static constexpr int kBM = kBM_, kBN = kBN_, kWM = kWM_, kWN = kWN_, kEpi = kEpi_;
   static constexpr bool kWideA = kWideA_, kWideB = kWideB_;
@@ -227,11 +248,17 @@ struct GemmConfig {
   using A = Tile<T, kWideA, kBM, kDeep, kThreads>;
   using B = Tile<T, kWideB, kBN, kDeep, kThreads>;
   static constexpr int kStageBytes = A::kBytes + B::kBytes;
-  static constexpr int kLdsBytes = 2 * kStageBytes;
+  static constexpr int kMmas = sizeof(T) == 2 ? 1 : 4;  // matrix instructions per fragment pair
+  static constexpr bool kPhased = kPhased_;
+  static constexpr int kBandTiles = kTM < 4 ? kTM : 4;  // 16-row tiles per epilogue band
+  static constexpr int kBandStride = kTN * 16 + 4;      // rows 16 bytes apart in the banks
+  static constexpr int kBandBytes = kEpi == kEpiPartial ? 0 : kWM * kWN * kBandTiles * 16 * kBandStride * 4;
+  static constexpr int kLdsBytes = 2 * kStageBytes > kBandBytes ? 2 * kStageBytes : kBandBytes;
+  static_assert(kLdsBytes <= 160 * 1024, "LDS");
 };
 
 template <typename T, typename C>
-__global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
+__global__ __launch_bounds__(C::kThreads, C::kPhased && C::kThreads == 256 ? 1 : 2) void gemm_kernel(const GemmParams p) {
   __shared__ __attribute__((aligned(256))) char smem_generic[C::kLdsBytes];
   lds_char* const smem = (lds_char*)smem_generic;
   using A = typename C::A;
@@ -303,11 +330,14 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
       }
     }
   }
+  // (The chunks of a tile that hold contraction elements: all but on the last.)
+  const int depth_chunks = static_cast<int>((p.depth + A::kPer - 1) / A::kPer);
   const auto load = [&](int kt, int buf) {
     lds_char* const at = smem + buf * C::kStageBytes;
-    const int left = static_cast<int>((least(p.depth - static_cast<int64_t>(kt) * C::kDeep, C::kDeep) + A::kPer - 1) / A::kPer);
-    stage<A, T, C::kWideA, C::kThreads>(at, a, a_off, least(a_bytes, 0x7fffffff), left, a_chunk, wave);
-    stage<B, T, C::kWideB, C::kThreads>(at + A::kBytes, b, b_off, least(b_bytes, 0x7fffffff), left, b_chunk, wave);
+    const int left = depth_chunks - kt * (C::kDeep / A::kPer);
+    const bool there = kt < k_last;
+    stage<A, T, C::kWideA, C::kThreads>(at, a, a_off, there ? least(a_bytes, 0x7fffffff) : 0, left, a_chunk, wave);
+    stage<B, T, C::kWideB, C::kThreads>(at + A::kBytes, b, b_off, there ? least(b_bytes, 0x7fffffff) : 0, left, b_chunk, wave);
     a = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a) + a_step);
     b = reinterpret_cast<const T*>(reinterpret_cast<const char*>(b) + b_step);
     a_bytes -= a_step;
@@ -327,86 +357,167 @@ __global__ __launch_bounds__(C::kThreads) void gemm_kernel(const GemmParams p) {
 #pragma unroll
   for (int t = 0; t < (C::kSums ? C::kTM : 1); ++t) sums[t] = 0.f;
 
-  if (k_first < k_last) load(k_first, 0);
-  for (int kt = k_first; kt < k_last; ++kt) {
-    const int buf = (kt - k_first) & 1;
-    wait_loads();
-    __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
-    if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
+  const auto read = [&](Frag(&fa)[C::kTM], Frag(&fb)[C::kTN], int buf, int step) {
     const lds_char* const ta = smem + buf * C::kStageBytes;
     const lds_char* const tb = ta + A::kBytes;
 #pragma unroll
-    for (int step = 0; step < C::kDeep / A::kStep; ++step) {
-      Frag fa[C::kTM], fb[C::kTN];
+    for (int t = 0; t < C::kTN; ++t) fb[t] = B::read(tb, (wn * C::kTN + t) * 16, step, g, i);
 #pragma unroll
-      for (int t = 0; t < C::kTN; ++t) fb[t] = B::read(tb, (wn * C::kTN + t) * 16, step, g, i);
+    for (int t = 0; t < C::kTM; ++t) fa[t] = A::read(ta, (wm * C::kTM + t) * 16, step, g, i);
+  };
+  const auto multiply = [&](const Frag(&fa)[C::kTM], const Frag(&fb)[C::kTN]) {
 #pragma unroll
-      for (int t = 0; t < C::kTM; ++t) fa[t] = A::read(ta, (wm * C::kTM + t) * 16, step, g, i);
+    for (int t = 0; t < C::kTM; ++t)
 #pragma unroll
-      for (int t = 0; t < C::kTM; ++t)
+      for (int u = 0; u < C::kTN; ++u) acc[u][t] = Mma<T>::run(fb[u], fa[t], acc[u][t]);
+  };
+  const auto add_sums = [&](const Frag(&fa)[C::kTM]) {
+    if constexpr (C::kSums) {
+      if (sum_here)
 #pragma unroll
-        for (int u = 0; u < C::kTN; ++u) acc[u][t] = Mma<T>::run(fb[u], fa[t], acc[u][t]);
-      if constexpr (C::kSums) {
-        if (sum_here)
+        for (int t = 0; t < C::kTM; ++t)
+          if (t % C::kWN == wn) sums[t] = Mma<T>::sum(fa[t], sums[t]);
+    }
+  };
+
+  if constexpr (C::kPhased) {
+    // Two tiles in LDS, two steps per tile, the fragments of one step ahead in
+    // registers.  While the products of step 0 run, step 1 is read; then one
+    // barrier, after which nobody reads this tile any more and the next one is
+    // there; while the products of step 1 run, the tile after next is loaded
+    // over this one and step 0 of the next is read.  Loads past the last tile
+    // go out of bounds (zeros, never multiplied).
+    static_assert(C::kDeep / A::kStep == 2, "two steps per tile");
+    if (k_first < k_last) {
+      Frag fa0[C::kTM], fb0[C::kTN], fa1[C::kTM], fb1[C::kTN];
+      load(k_first, 0);
+      wait_loads();
+      __builtin_amdgcn_s_barrier();
+      load(k_first + 1, 1);
+      read(fa0, fb0, 0, 0);
+      for (int kt = k_first; kt < k_last; ++kt) {
+        const int buf = (kt - k_first) & 1;
+        read(fa1, fb1, buf, 1);
+        multiply(fa0, fb0);
+        add_sums(fa0);
+        interleave<C, false>();
+        wait_all();
+        __builtin_amdgcn_s_barrier();
+        load(kt + 2, buf);
+        read(fa0, fb0, buf ^ 1, 0);
+        multiply(fa1, fb1);
+        add_sums(fa1);
+        interleave<C, true>();
+      }
+      wait_all();  // nothing is on its way into LDS when it is used again
+    }
+  } else {
+    if (k_first < k_last) load(k_first, 0);
+    for (int kt = k_first; kt < k_last; ++kt) {
+      const int buf = (kt - k_first) & 1;
+      wait_loads();
+      __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
+      if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
 #pragma unroll
-          for (int t = 0; t < C::kTM; ++t)
-            if (t % C::kWN == wn) sums[t] = Mma<T>::sum(fa[t], sums[t]);
+      for (int step = 0; step < C::kDeep / A::kStep; ++step) {
+        Frag fa[C::kTM], fb[C::kTN];
+        read(fa, fb, buf, step);
+        multiply(fa, fb);
+        add_sums(fa);
       }
     }
   }
 
-  // ---- epilogue: lane holds D[m, n .. n + 3] of every 16 x 16 tile
-  constexpr int kPairs = C::kGated ? C::kTN / 2 : C::kTN;
-  const int64_t n_wave = n0 + wn * kPairs * 16;
+  // ---- epilogue
+  if constexpr (C::kEpi == kEpiPartial) {
+    // A lane holds D[m, n .. n + 3] of every 16 x 16 tile; ldo is a multiple of 4.
+    float* const out = static_cast<float*>(p.out) + static_cast<int64_t>(blockIdx.y) * p.m * p.ldo;
 #pragma unroll
-  for (int u = 0; u < kPairs; ++u) {
-    const int64_t n = n_wave + u * 16 + 4 * g;
-    const int left = static_cast<int>(least(p.n - n, 4));
-    f32x4 bias = {0.f, 0.f, 0.f, 0.f}, bias_up = {0.f, 0.f, 0.f, 0.f};
-    if (C::kEpi != kEpiPartial && p.bias) {
+    for (int u = 0; u < C::kTN; ++u) {
+      const int64_t n = n0 + (wn * C::kTN + u) * 16 + 4 * g;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int t = 0; t < C::kTM; ++t) {
+        const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
+        if (m < p.m && n < p.n) *reinterpret_cast<f32x4*>(out + m * p.ldo + n) = acc[u][t];
+      }
+    }
+  } else {
+    // Through LDS, a band of up to 64 rows of the wave's tile at a time (each
+    // wave in its own part: no barrier but the first): afterwards a lane holds
+    // eight consecutive columns, so rows of the result, the residual and the
+    // gradient move in whole cache lines.
+    constexpr int kBandTiles = C::kBandTiles, kCols = C::kTN * 16;
+    constexpr int kStride = C::kBandStride;  // floats per row
+    constexpr int kOut = C::kGated ? kCols / 2 : kCols, kLanes = kOut / 8, kRows = 64 / kLanes;
+    __attribute__((address_space(3))) float* const band =
+        (__attribute__((address_space(3))) float*)smem + wave * kBandTiles * 16 * kStride;
+    const int col = (lane % kLanes) * 8;
+    const int64_t n = n0 + wn * kOut + col;
+    const int left = static_cast<int>(least(p.n - n, 8));
+    f32x4 bias[2] = {}, bias_up[2] = {};
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
         if (e < left) {
-          bias[e] = load_bias(p.bias, n + e, p.bias_dtype);
-          if constexpr (C::kGated) bias_up[e] = load_bias(p.bias, p.n + n + e, p.bias_dtype);
+          bias[e / 4][e % 4] = load_bias(p.bias, n + e, p.bias_dtype);
+          if constexpr (C::kGated) bias_up[e / 4][e % 4] = load_bias(p.bias, p.n + n + e, p.bias_dtype);
         }
     }
+    __syncthreads();  // all waves are done with the tiles
 #pragma unroll
-    for (int t = 0; t < C::kTM; ++t) {
-      const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
-      if (m >= p.m || left <= 0) continue;
-      if constexpr (C::kEpi == kEpiPartial) {
-        float* const out = static_cast<float*>(p.out) + (static_cast<int64_t>(blockIdx.y) * p.m + m) * p.ldo + n;
-        *reinterpret_cast<f32x4*>(out) = acc[u][t];  // ldo is a multiple of 4
-      } else if constexpr (C::kEpi == kEpiStore) {
-        f32x4 y = acc[u][t];
+    for (int first = 0; first < C::kTM; first += kBandTiles) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = act_value(y[e] + bias[e], p.activation);
-        if (p.residual) y += load4(static_cast<const T*>(p.residual) + m * p.ldr + n, left, p.vec & kVecResidual);
-        store4(static_cast<T*>(p.out) + m * p.ldo + n, y, left, p.vec & kVecOut);
-      } else if constexpr (C::kEpi == kEpiGated) {
-        f32x4 y;
+      for (int t = 0; t < kBandTiles; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = act_value(acc[u][t][e] + bias[e], p.activation) * (acc[u + kPairs][t][e] + bias_up[e]);
-        store4(static_cast<T*>(p.out) + m * p.ldo + n, y, left, p.vec & kVecOut);
-      } else {
-        const f32x4 dy = load4(static_cast<const T*>(p.grad) + m * p.ldg + n, left, p.vec & kVecGrad);
-        f32x4 da, db;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float value, slope;
-          act_slope(acc[u][t][e] + bias[e], p.activation, value, slope);
-          da[e] = dy[e] * slope;
+        for (int u = 0; u < C::kTN; ++u)
+          *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(band + (t * 16 + i) * kStride + u * 16 + 4 * g) =
+              acc[u][first + t];
+      const int64_t m_band = m0 + (wm * C::kTM + first) * 16 + lane / kLanes;
+      with_activation(p.activation, [&](auto act) {
+        constexpr int kAct = decltype(act)::value;
+#pragma unroll 2
+        for (int r = 0; r < kBandTiles * 16; r += kRows) {
+          const int64_t m = m_band + r;
+          const __attribute__((address_space(3))) f32x4* const from =
+              (const __attribute__((address_space(3))) f32x4*)(band + (r + lane / kLanes) * kStride + col);
+          f32x4 z[2] = {from[0] + bias[0], from[1] + bias[1]}, u[2];
           if constexpr (C::kGated) {
-            da[e] *= acc[u + kPairs][t][e] + bias_up[e];
-            db[e] = dy[e] * value;
+            u[0] = from[kOut / 4] + bias_up[0];
+            u[1] = from[kOut / 4 + 1] + bias_up[1];
+          }
+          if (m >= p.m || left <= 0) continue;
+          if constexpr (C::kEpi == kEpiStore || C::kEpi == kEpiGated) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              z[e / 4][e % 4] = act_value(z[e / 4][e % 4], kAct);
+              if constexpr (C::kGated) z[e / 4][e % 4] *= u[e / 4][e % 4];
+            }
+            if (C::kEpi == kEpiStore && p.residual) {
+              f32x4 ra, rb;
+              load8(static_cast<const T*>(p.residual) + m * p.ldr + n, left, ra, rb);
+              z[0] += ra;
+              z[1] += rb;
+            }
+            store8(static_cast<T*>(p.out) + m * p.ldo + n, z[0], z[1], left);
+          } else {
+            f32x4 dy[2], up[2];
+            load8(static_cast<const T*>(p.grad) + m * p.ldg + n, left, dy[0], dy[1]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float value, slope;
+              act_slope(z[e / 4][e % 4], kAct, value, slope);
+              z[e / 4][e % 4] = dy[e / 4][e % 4] * slope;
+              if constexpr (C::kGated) {
+                z[e / 4][e % 4] *= u[e / 4][e % 4];
+                up[e / 4][e % 4] = dy[e / 4][e % 4] * value;
+              }
+            }
+            T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
+            store8(out, z[0], z[1], left);
+            if constexpr (C::kGated) store8(out + p.n, up[0], up[1], left);
           }
         }
-        T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
-        store4(out, da, left, p.vec & kVecOut);
-        if constexpr (C::kGated) store4(out + p.n, db, left, p.vec & kVecOutUp);
-      }
+      });
     }
   }
 

@@ -16,7 +16,7 @@ template <typename T, bool kWideA, bool kWideB, int kEpi>
 int launch_tile(const GemmParams& p, int tile, int splits, hipStream_t stream) {
   switch (tile) {
     case kTileLarge:
-      return launch_one<T, GemmConfig<T, 256, 256, 2, 4, kWideA, kWideB, kEpi>>(p, splits, stream);
+      return launch_one<T, GemmConfig<T, 256, 256, 2, 4, kWideA, kWideB, kEpi, true>>(p, splits, stream);
     case kTileMedium:
       return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi>>(p, splits, stream);
     default:

@@ -175,16 +175,16 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         if (live && left > 0) {
           if (!C::kGated && p.residual) {
             f32x4 ra, rb;
-            load8(static_cast<const T*>(p.residual) + row * p.ldr + n, left, p.vec & kVecResidual, ra, rb);
+            load8(static_cast<const T*>(p.residual) + row * p.ldr + n, left, ra, rb);
             ya += ra;
             yb += rb;
           }
-          store8(static_cast<T*>(p.out) + row * p.ldo + n, ya, yb, left, p.vec & kVecOut);
+          store8(static_cast<T*>(p.out) + row * p.ldo + n, ya, yb, left);
         }
       } else {
         f32x4 ga = {0.f, 0.f, 0.f, 0.f}, gb = {0.f, 0.f, 0.f, 0.f};
         if (live && left > 0)
-          load8(static_cast<const T*>(p.grad) + row * p.ldg + n, left, p.vec & kVecGrad, ga, gb);
+          load8(static_cast<const T*>(p.grad) + row * p.ldg + n, left, ga, gb);
         f32x4 da, db, ea, eb;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -212,8 +212,8 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         if constexpr (C::kGated) gradient(p.n_pad + pair * 32, ea, eb);
         if (p.out && live && left > 0) {
           T* const out = static_cast<T*>(p.out) + row * p.ldo + n;
-          store8(out, da, db, left, p.vec & kVecOut);
-          if constexpr (C::kGated) store8(out + p.n, ea, eb, left, p.vec & kVecOutUp);
+          store8(out, da, db, left);
+          if constexpr (C::kGated) store8(out + p.n, ea, eb, left);
         }
       }
     }
@@ -222,7 +222,7 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         T* const out = static_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
         for (int t = 0; t < C::kDeep / 16; ++t)
-          store4(out + t * 16 + 4 * g, dx[t], static_cast<int>(p.width) - (t * 16 + 4 * g), p.vec & kVecDx);
+          store4(out + t * 16 + 4 * g, dx[t], static_cast<int>(p.width) - (t * 16 + 4 * g));
       }
     }
   }
