@@ -218,20 +218,53 @@ __device__ __forceinline__ void interleave() {
 
 constexpr uint32_t kOutside = 0x80000000u;  // past any buffer (host checks: tiles span less than 2^31 bytes)
 
+// The 16-byte load into LDS that stage() issues.
+//
+// kOpaque: written as an instruction rather than through the builtin.  The
+// compiler waits for every outstanding load of the builtin's kind before a
+// transposing LDS read, whose address it cannot tell apart from theirs: the
+// loads just issued for the tile after next would be waited for at once.
+// Here the kernel's own waits (wait_loads, wait_all before the barrier that
+// hands a tile over) order them.  The instruction writes no register; M0
+// holds the wave's LDS address (one wait state before its use, five for a
+// scalar register of the descriptor that a vector instruction wrote).
+template <bool kOpaque>
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, u32x4 words, lds_char* to, uint32_t at) {
+  if constexpr (kOpaque) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to))), "v"(at), "s"(words)
+        : "memory", "m0");
+  } else {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
+  }
+}
+
 // Loads the tile of one operand.  `base`: the operand's element (first row of
 // the tile, first contraction element of the tile), wave-uniform.
-template <typename TileT, typename T, bool kWide, int kThreads>
+template <typename TileT, typename T, bool kWide, int kThreads, bool kOpaque>
 __device__ __forceinline__ void stage(lds_char* tile, const T* base, const uint32_t (&offset)[TileT::kSlots],
                                       int64_t bytes, int valid_chunks, const uint32_t (&chunk)[TileT::kSlots],
                                       int wave) {
-  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<T*>(base), 0, static_cast<int>(bytes > 0 ? bytes : 0), 0x00020000);
+  const uint32_t size = static_cast<uint32_t>(bytes > 0 ? bytes : 0);
+  __amdgpu_buffer_rsrc_t rsrc;
+  u32x4 words;
+  if constexpr (kOpaque) {
+    const uint64_t address = reinterpret_cast<uintptr_t>(base);
+    const auto uniform = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); };
+    words = u32x4{uniform(static_cast<uint32_t>(address)), uniform(static_cast<uint32_t>(address >> 32)), uniform(size),
+                  0x00020000u};
+  } else {
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, static_cast<int>(size), 0x00020000);
+  }
 #pragma unroll
   for (int s = 0; s < TileT::kSlots; ++s) {
     uint32_t at = offset[s];
     if constexpr (!kWide) at = static_cast<int>(chunk[s]) < valid_chunks ? at : kOutside;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rsrc, (__attribute__((address_space(3))) void*)(tile + (s * kThreads + wave * 64) * 16), 16, at, 0, 0, 0);
+    load_to_lds<kOpaque>(rsrc, words, tile + (s * kThreads + wave * 64) * 16, at);
   }
 }
 
@@ -250,11 +283,17 @@ struct GemmConfig {
   static constexpr int kStageBytes = A::kBytes + B::kBytes;
   static constexpr int kMmas = sizeof(T) == 2 ? 1 : 4;  // matrix instructions per fragment pair
   static constexpr bool kPhased = kPhased_;
+  static constexpr bool kOpaque = kPhased && sizeof(T) == 2 && (kWideA || kWideB);
   static constexpr int kBandTiles = kTM < 4 ? kTM : 4;  // 16-row tiles per epilogue band
   static constexpr int kBandStride = kTN * 16 + 4;      // rows 16 bytes apart in the banks
   static constexpr int kBandBytes = kEpi == kEpiPartial ? 0 : kWM * kWN * kBandTiles * 16 * kBandStride * 4;
   static constexpr int kLdsBytes = 2 * kStageBytes > kBandBytes ? 2 * kStageBytes : kBandBytes;
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
+};
+
+template <bool kFlag>
+struct Flag {
+  static constexpr bool value = kFlag;
 };
 
 template <typename T, typename C>
@@ -336,8 +375,8 @@ __global__ __launch_bounds__(C::kThreads, C::kPhased && C::kThreads == 256 ? 1 :
     lds_char* const at = smem + buf * C::kStageBytes;
     const int left = depth_chunks - kt * (C::kDeep / A::kPer);
     const bool there = kt < k_last;
-    stage<A, T, C::kWideA, C::kThreads>(at, a, a_off, there ? least(a_bytes, 0x7fffffff) : 0, left, a_chunk, wave);
-    stage<B, T, C::kWideB, C::kThreads>(at + A::kBytes, b, b_off, there ? least(b_bytes, 0x7fffffff) : 0, left, b_chunk, wave);
+    stage<A, T, C::kWideA, C::kThreads, C::kOpaque>(at, a, a_off, there ? least(a_bytes, 0x7fffffff) : 0, left, a_chunk, wave);
+    stage<B, T, C::kWideB, C::kThreads, C::kOpaque>(at + A::kBytes, b, b_off, there ? least(b_bytes, 0x7fffffff) : 0, left, b_chunk, wave);
     a = reinterpret_cast<const T*>(reinterpret_cast<const char*>(a) + a_step);
     b = reinterpret_cast<const T*>(reinterpret_cast<const char*>(b) + b_step);
     a_bytes -= a_step;
@@ -350,8 +389,7 @@ __global__ __launch_bounds__(C::kThreads, C::kPhased && C::kThreads == 256 ? 1 :
 #pragma unroll
     for (int tm_ = 0; tm_ < C::kTM; ++tm_) acc[tn_][tm_] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Sums of A: by the workgroups of the first tile column, tile t of a wave's
-  // rows by the wave t % kWN of that row.
+  // Sums of A: by the workgroups of the first tile column.
   const bool sum_here = C::kSums && p.sums && tn == 0;
   float sums[C::kSums ? C::kTM : 1];
 #pragma unroll
@@ -371,61 +409,70 @@ __global__ __launch_bounds__(C::kThreads, C::kPhased && C::kThreads == 256 ? 1 :
 #pragma unroll
       for (int u = 0; u < C::kTN; ++u) acc[u][t] = Mma<T>::run(fb[u], fa[t], acc[u][t]);
   };
-  const auto add_sums = [&](const Frag(&fa)[C::kTM]) {
-    if constexpr (C::kSums) {
-      if (sum_here)
+  // The loop over the contraction, with or without the sums of A.
+  const auto products = [&](auto with_sums) {
+    constexpr bool kSum = decltype(with_sums)::value;
+    const auto add_sums = [&](const Frag(&fa)[C::kTM]) {
+      if constexpr (kSum) {
 #pragma unroll
-        for (int t = 0; t < C::kTM; ++t)
-          if (t % C::kWN == wn) sums[t] = Mma<T>::sum(fa[t], sums[t]);
-    }
-  };
-
-  if constexpr (C::kPhased) {
-    // Two tiles in LDS, two steps per tile, the fragments of one step ahead in
-    // registers.  While the products of step 0 run, step 1 is read; then one
-    // barrier, after which nobody reads this tile any more and the next one is
-    // there; while the products of step 1 run, the tile after next is loaded
-    // over this one and step 0 of the next is read.  Loads past the last tile
-    // go out of bounds (zeros, never multiplied).
-    static_assert(C::kDeep / A::kStep == 2, "two steps per tile");
-    if (k_first < k_last) {
-      Frag fa0[C::kTM], fb0[C::kTN], fa1[C::kTM], fb1[C::kTN];
-      load(k_first, 0);
-      wait_loads();
-      __builtin_amdgcn_s_barrier();
-      load(k_first + 1, 1);
-      read(fa0, fb0, 0, 0);
+        for (int t = 0; t < C::kTM; ++t) sums[t] = Mma<T>::sum(fa[t], sums[t]);
+      }
+    };
+    if constexpr (C::kPhased) {
+      // Two tiles in LDS, two steps per tile, the fragments of one step ahead in
+      // registers.  While the products of step 0 run, step 1 is read; then one
+      // barrier, after which nobody reads this tile any more and the next one is
+      // there; while the products of step 1 run, the tile after next is loaded
+      // over this one and step 0 of the next is read.  Loads past the last tile
+      // go out of bounds (zeros, never multiplied).
+      static_assert(C::kDeep / A::kStep == 2, "two steps per tile");
+      if (k_first < k_last) {
+        Frag fa0[C::kTM], fb0[C::kTN], fa1[C::kTM], fb1[C::kTN];
+        load(k_first, 0);
+        wait_loads();
+        __builtin_amdgcn_s_barrier();
+        load(k_first + 1, 1);
+        read(fa0, fb0, 0, 0);
+        for (int kt = k_first; kt < k_last; ++kt) {
+          const int buf = (kt - k_first) & 1;
+          read(fa1, fb1, buf, 1);
+          multiply(fa0, fb0);
+          add_sums(fa0);
+          interleave<C, false>();
+          wait_all();
+          __builtin_amdgcn_s_barrier();
+          load(kt + 2, buf);
+          read(fa0, fb0, buf ^ 1, 0);
+          multiply(fa1, fb1);
+          add_sums(fa1);
+          interleave<C, true>();
+        }
+        wait_all();  // nothing is on its way into LDS when it is used again
+      }
+    } else {
+      if (k_first < k_last) load(k_first, 0);
       for (int kt = k_first; kt < k_last; ++kt) {
         const int buf = (kt - k_first) & 1;
-        read(fa1, fb1, buf, 1);
-        multiply(fa0, fb0);
-        add_sums(fa0);
-        interleave<C, false>();
-        wait_all();
-        __builtin_amdgcn_s_barrier();
-        load(kt + 2, buf);
-        read(fa0, fb0, buf ^ 1, 0);
-        multiply(fa1, fb1);
-        add_sums(fa1);
-        interleave<C, true>();
-      }
-      wait_all();  // nothing is on its way into LDS when it is used again
-    }
-  } else {
-    if (k_first < k_last) load(k_first, 0);
-    for (int kt = k_first; kt < k_last; ++kt) {
-      const int buf = (kt - k_first) & 1;
-      wait_loads();
-      __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
-      if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
+        wait_loads();
+        __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
+        if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
 #pragma unroll
-      for (int step = 0; step < C::kDeep / A::kStep; ++step) {
-        Frag fa[C::kTM], fb[C::kTN];
-        read(fa, fb, buf, step);
-        multiply(fa, fb);
-        add_sums(fa);
+        for (int step = 0; step < C::kDeep / A::kStep; ++step) {
+          Frag fa[C::kTM], fb[C::kTN];
+          read(fa, fb, buf, step);
+          multiply(fa, fb);
+          add_sums(fa);
+        }
       }
     }
+  };
+  if constexpr (C::kSums) {
+    if (sum_here)
+      products(Flag<true>{});
+    else
+      products(Flag<false>{});
+  } else {
+    products(Flag<false>{});
   }
 
   // ---- epilogue
@@ -531,7 +578,7 @@ __global__ __launch_bounds__(C::kThreads, C::kPhased && C::kThreads == 256 ? 1 :
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
-        if (g == 0 && m < p.m && t % C::kWN == wn) {
+        if (wn == 0 && g == 0 && m < p.m) {
           if constexpr (C::kEpi == kEpiPartial)
             static_cast<float*>(p.sums)[blockIdx.y * p.m + m] = s;
           else
