@@ -62,12 +62,20 @@ template <typename T, int kLanes>
 __global__ __launch_bounds__(256) void join_kernel(const float* parts, int splits, int64_t m, int64_t n, int64_t ld,
                                                    GemmParams p, const float* sum_parts, int quad_blocks) {
   constexpr int kQuads = 256 / kLanes;
-  if (static_cast<int>(blockIdx.x) >= quad_blocks) {  // the sums' planes: a thread per sum
-    const int64_t at = static_cast<int64_t>(blockIdx.x - quad_blocks) * 256 + threadIdx.x;
-    if (at >= m) return;
+  if (static_cast<int>(blockIdx.x) >= quad_blocks) {  // the sums' planes: 16 lanes per sum, 16 sums
+    __shared__ float sum_part[16][16];
+    const int c = threadIdx.x % 16, lane = threadIdx.x / 16;
+    const int64_t at = static_cast<int64_t>(blockIdx.x - quad_blocks) * 16 + c;
     float s = 0.f;
+    if (at < m) {
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) s += sum_parts[k * m + at];
+      for (int k = lane; k < splits; k += 16) s += sum_parts[k * m + at];
+    }
+    sum_part[lane][c] = s;
+    __syncthreads();
+    if (lane != 0 || at >= m) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sum_part[k][c];
     store_as(p.sums, at, p.sums_dtype, s);
     return;
   }
@@ -332,34 +340,40 @@ struct Call {
     return {out, out_ld};
   }
 
-  // The tile and the number of contraction parts with the least estimated time.
-  //
-  // Workgroups resident per CU by LDS (1, 2 and 5), the rate of a CU full of
-  // them (16 bits: 1.15, 0.95 and 0.7 PFLOP/s over 256 CUs; fp32: 0.12 for
-  // each), and the work counted in whole tiles and whole rounds of the chip:
-  //   2051 x 2048 -> 11264 fp16: 118 / 105 / 145 us for the large, medium and
-  //   small tile (estimated in this order, too); 10007 x 5464 -> 1000 bf16 with
-  //   a wide operand: 193 / 206 / 229.
-  // A split costs its fp32 planes, written and read once at 5 TB/s, and the
-  // joining launch.  Contractions of at most four tiles have no steady state:
-  // the small tile's five workgroups per CU hide each other's loads and
-  // stores (66560 x 128 -> 256 bf16: 42 / 31 / 23 us).
+  // The tile and the number of contraction parts with the least estimated
+  // time.  Measured, 16 bits, 8192 x K -> 4096 (the slope over K, and what a
+  // workgroup costs besides its products, stores above all):
+  //   tile 256: 1.5 PFLOP/s and 9.5 us, one workgroup per CU (LDS)
+  //   tile 128: 1.14 PFLOP/s and 2.2 us per two workgroups of a CU
+  //   tile 64: 0.79 PFLOP/s and 2.2 us per five
+  // fp32 products run at 0.12 PFLOP/s on any of them.  A CU holding fewer
+  // workgroups than it could runs at a part of its rate (kPart).  The tiles'
+  // operands pass from L2 to LDS at 8 TB/s.  A split costs its fp32 planes,
+  // written and read at 5 TB/s, and the joining launch.
+  //   estimated / measured, us: 8192 x 1024 -> 4096 bf16 64 / 64 on the chosen
+  //   256 (77 on 128); 2051 x 2048 -> 2 x 5632 fp16 98 / 99 on 128 (101 on
+  //   256); 300 x 1024 -> 1024 11 / 10 on 64 (14 on 128); 66560 x 128 -> 256
+  //   weight gradient 24 / 21 on 128 in 128 parts (25 on 64).
   void choose(const GemmParams& p, int64_t columns, int epi, int& tile, int& splits) const {
-    static constexpr double kRate16[kTileCount] = {1.15e15, 0.95e15, 0.7e15}, kRate32 = 0.12e15;
+    static constexpr double kRate16[kTileCount] = {1.5e15, 1.14e15, 0.79e15}, kRate32 = 0.12e15;
+    static constexpr double kBatch[kTileCount] = {9.5e-6, 2.2e-6, 2.2e-6};
     static constexpr int kResident[kTileCount] = {1, 2, 5};
+    static constexpr double kPart[kTileCount][5] = {{1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
+    double best = 1e30;
     splits = 1;
     tile = kTileCount - 1;
-    if (p.k_tiles <= 4) return;
-    double best = 1e30;
     const int most_splits = epi == kEpiStore ? std::min(256, p.k_tiles / 2) : 1;
     for (int t = 0; t < kTileCount; ++t) {
-      const double tiles = static_cast<double>(ceil_div(p.m, kTileM[t])) * ceil_div(columns, kTileN[t]);
-      const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : kRate16[t]) / cus / kResident[t];  // of one workgroup
-      for (int k = 1; k <= most_splits; k *= 2) {
-        const double rounds = std::ceil(tiles * k / (cus * kResident[t]));
-        const double one = 2.0 * kTileM[t] * kTileN[t] * (128 / esize()) * ceil_div(p.k_tiles, k) / rate + 2e-6;
-        const double join = k > 1 ? 8.0 * k * p.m * p.n / 5e12 + 4e-6 : 0;
-        const double time = rounds * one + join;
+      const int64_t tiles = ceil_div(p.m, kTileSize[t]) * ceil_div(columns, kTileSize[t]);
+      const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : kRate16[t]) / 256;  // of a full CU
+      for (int k = 1; k <= std::max(1, most_splits); k *= 2) {
+        const int64_t depth = ceil_div(p.k_tiles, k) * (128 / esize());
+        const int64_t per_cu = ceil_div(tiles * k, cus);
+        const int together = static_cast<int>(std::min<int64_t>(per_cu, kResident[t]));
+        const double products = per_cu * 2.0 * kTileSize[t] * kTileSize[t] * depth / (rate * kPart[t][together - 1]);
+        const double traffic = tiles * k * 2.0 * kTileSize[t] * depth * esize() / 8e12;
+        const double join = k > 1 ? 8.0 * k * p.m * p.n / 5e12 + 6e-6 : 0;
+        const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
         if (time < best * 0.98) {
           best = time;
           tile = t;
@@ -376,8 +390,8 @@ struct Call {
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
     int tile, splits;
     choose(p, columns, epi, tile, splits);
-    p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileM[tile]));
-    p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileN[tile]));
+    p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileSize[tile]));
+    p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileSize[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
     splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
     if (splits == 1) {
@@ -397,7 +411,7 @@ struct Call {
         using T = std::remove_pointer_t<decltype(t)>;
         const int64_t quads = p.m * (ld / 4);
         const bool lanes = splits > 8 && quads < 64 * 256 * 4;
-        const int64_t blocks = ceil_div(quads, lanes ? 16 : 256), sum_blocks = sum_parts ? ceil_div(p.m, 256) : 0;
+        const int64_t blocks = ceil_div(quads, lanes ? 16 : 256), sum_blocks = sum_parts ? ceil_div(p.m, 16) : 0;
         const auto kernel = lanes ? join_kernel<T, 16> : join_kernel<T, 1>;
         kernel<<<static_cast<uint32_t>(blocks + sum_blocks), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p, sum_parts,
                                                                                static_cast<int>(blocks));
@@ -416,7 +430,8 @@ struct Call {
 
   // Contraction steps of the resident kernel that serves these sizes, or 0.
   // Its workgroups copy the whole weight first, so it needs rows enough that
-  // every CU's 16 waves have a unit of 16 rows.
+  // every CU's 8 waves have a unit of 32 rows at least (a quarter of them
+  // still pays).
   int resident_steps(int64_t rows, int64_t width, int64_t n, bool gated) const {
     if (rows < 16 * 16 * cus / 4) return 0;
     const int64_t bytes = width * esize(), n_pad = ceil_div(n, 32) * 32 * (1 + gated);

@@ -46,8 +46,7 @@ struct GemmParams {
 // The shapes of one tiled product's kernels.
 enum { kLayoutForward = 0, kLayoutInput = 1, kLayoutWeight = 2 };
 enum { kTileLarge = 0, kTileMedium = 1, kTileSmall = 2, kTileCount = 3 };
-constexpr int kTileM[kTileCount] = {256, 128, 64};
-constexpr int kTileN[kTileCount] = {256, 128, 64};
+constexpr int kTileSize[kTileCount] = {256, 128, 64};  // square
 
 // Launches the product with the given layout, tile and epilogue on `splits`
 // contraction parts.  One definition per element type.

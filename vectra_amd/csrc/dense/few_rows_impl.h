@@ -3,10 +3,11 @@
 //
 //   y = act(x W^T + b) + r,  or the gated product
 //
-// Such a call is the weight's bytes.  A workgroup of 8 waves takes 16 rows of
-// W (16 of the gate and the same 16 of the up projection), and its waves share
-// out the contraction: wave w takes the 64-byte steps w, w + 8, ... of those
-// rows, so the workgroup reads 512 consecutive bytes of each row at a time.  A
+// Such a call is the weight's bytes.  A workgroup of 8 or 16 waves takes 16
+// rows of W (16 of the gate and the same 16 of the up projection), and its
+// waves share out the contraction: of 8, wave w takes the 64-byte steps w,
+// w + 8, ... of those rows, so the workgroup reads 512 consecutive bytes of
+// each row at a time.  A
 // wave loads a batch of steps straight into the registers of the matrix
 // instruction's first operand (lane l: row l % 16, 16-byte chunk l / 16), x
 // likewise into the second's (from L2 after the first workgroups), and has up
@@ -21,9 +22,8 @@
 
 namespace vectra_dense {
 
-constexpr int kFewWaves = 8;
 
-template <typename T, int kRowTiles, bool kGated>
+template <typename T, int kRowTiles, bool kGated, int kFewWaves>
 __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const FewRowsParams p) {
   constexpr int kHalves = kGated ? 2 : 1;
   constexpr int kBatch = kGated || kRowTiles > 1 ? 4 : 8;
@@ -106,9 +106,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const FewRowsP
 template <typename T>
 int launch_few_rows(const FewRowsParams& p, bool gated, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>((p.n + 15) / 16));
-  const auto kernel = p.rows <= 16 ? (gated ? few_rows_kernel<T, 1, true> : few_rows_kernel<T, 1, false>)
-                                   : (gated ? few_rows_kernel<T, 2, true> : few_rows_kernel<T, 2, false>);
-  kernel<<<grid, 64 * kFewWaves, 0, stream>>>(p);
+  // 16 waves where at most one workgroup of 8 would be on a CU.
+  const int waves = p.n <= 16 * 256 ? 16 : 8;
+  const auto kernel = p.rows <= 16 ? (gated ? (waves == 16 ? few_rows_kernel<T, 1, true, 16> : few_rows_kernel<T, 1, true, 8>)
+                                            : (waves == 16 ? few_rows_kernel<T, 1, false, 16> : few_rows_kernel<T, 1, false, 8>))
+                                   : (gated ? (waves == 16 ? few_rows_kernel<T, 2, true, 16> : few_rows_kernel<T, 2, true, 8>)
+                                            : (waves == 16 ? few_rows_kernel<T, 2, false, 16> : few_rows_kernel<T, 2, false, 8>));
+  kernel<<<grid, 64 * waves, 0, stream>>>(p);
   return hipGetLastError() == hipSuccess ? VECTRA_DENSE_OK : VECTRA_DENSE_ERR_LAUNCH;
 }
 

@@ -297,7 +297,7 @@ struct Flag {
 };
 
 template <typename T, typename C>
-__global__ __launch_bounds__(C::kThreads, C::kPhased && C::kThreads == 256 ? 1 : 2) void gemm_kernel(const GemmParams p) {
+__global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p) {
   __shared__ __attribute__((aligned(256))) char smem_generic[C::kLdsBytes];
   lds_char* const smem = (lds_char*)smem_generic;
   using A = typename C::A;

@@ -14,13 +14,20 @@ int launch_one(const GemmParams& p, int splits, hipStream_t stream) {
 
 template <typename T, bool kWideA, bool kWideB, int kEpi>
 int launch_tile(const GemmParams& p, int tile, int splits, hipStream_t stream) {
+  // One or two workgroups per CU need the phased loop; so do the transposing
+  // reads of wide operands at any tile (10007 x 1000 -> 5464 bf16 weight
+  // gradient on medium tiles: 174 us with the plain loop, 123 phased).
+  // Forward products on medium and small tiles keep the plain loop: their
+  // workgroups overlap each other (8192 x 4096 -> 4096: 245 us either way,
+  // 10007 x 1000 -> 2 x 2730 gated: 143 plain, 151 phased).
+  constexpr bool kWide = kWideA || kWideB;
   switch (tile) {
     case kTileLarge:
       return launch_one<T, GemmConfig<T, 256, 256, 2, 4, kWideA, kWideB, kEpi, true>>(p, splits, stream);
     case kTileMedium:
-      return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi>>(p, splits, stream);
+      return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi, kWide>>(p, splits, stream);
     default:
-      return launch_one<T, GemmConfig<T, 64, 64, 2, 2, kWideA, kWideB, kEpi>>(p, splits, stream);
+      return launch_one<T, GemmConfig<T, 64, 64, 2, 2, kWideA, kWideB, kEpi, kWide>>(p, splits, stream);
   }
 }
 

@@ -64,7 +64,7 @@ __device__ __forceinline__ int resident_swizzle(int row) {
 
 // Elements first .. of a row of `width`, zeros past its end.
 template <typename T>
-__device__ __forceinline__ Frag load_row_chunk(const T* row, int64_t width, int first) {
+__device__ __forceinline__ Frag load_row_chunk(const T* row, int64_t width, int64_t first) {
   constexpr int kPer = 16 / sizeof(T);
   Frag f;
   if (first + kPer <= width) {
