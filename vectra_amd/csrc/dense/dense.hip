@@ -344,19 +344,23 @@ struct Call {
   // time.  Measured, 16 bits, 8192 x K -> 4096 (the slope over K, and what a
   // workgroup costs besides its products, stores above all):
   //   tile 256: 1.5 PFLOP/s and 9.5 us, one workgroup per CU (LDS)
-  //   tile 128: 1.14 PFLOP/s and 2.2 us per two workgroups of a CU
+  //   tile 128: 1.14 PFLOP/s (1.0 with a wide operand) and 2.2 us per two
+  //   workgroups of a CU
   //   tile 64: 0.79 PFLOP/s and 2.2 us per five
-  // fp32 products run at 0.12 PFLOP/s on any of them.  A CU holding fewer
+  // and 12, 5 and 5 us where the epilogue evaluates activations.  fp32
+  // products run at 0.12 PFLOP/s on any of them.  A CU holding fewer
   // workgroups than it could runs at a part of its rate (kPart).  The tiles'
-  // operands pass from L2 to LDS at 8 TB/s.  A split costs its fp32 planes,
+  // operands pass from L2 to LDS at 16 TB/s.  A split costs its fp32 planes,
   // written and read at 5 TB/s, and the joining launch.
-  //   estimated / measured, us: 8192 x 1024 -> 4096 bf16 64 / 64 on the chosen
-  //   256 (77 on 128); 2051 x 2048 -> 2 x 5632 fp16 98 / 99 on 128 (101 on
-  //   256); 300 x 1024 -> 1024 11 / 10 on 64 (14 on 128); 66560 x 128 -> 256
-  //   weight gradient 24 / 21 on 128 in 128 parts (25 on 64).
-  void choose(const GemmParams& p, int64_t columns, int epi, int& tile, int& splits) const {
+  //   chosen / other tiles, us: 8192 x 1024 -> 4096 bf16 62 on 256 (73 on 128);
+  //   2051 x 2048 -> 2 x 5632 fp16 gated 97 on 128 (102 on 256); 10007 x 1000
+  //   -> 2 x 2730 bf16 gated 123 on 256 (144 on 128); 300 x 1024 -> 1024 10 on
+  //   64 (14 on 128); 66560 x 128 -> 256 weight gradient 18 on 64 in 64 parts
+  //   (20 on 128 in 128).
+  void choose(const GemmParams& p, int64_t columns, int layout, int epi, int& tile, int& splits) const {
     static constexpr double kRate16[kTileCount] = {1.5e15, 1.14e15, 0.79e15}, kRate32 = 0.12e15;
-    static constexpr double kBatch[kTileCount] = {9.5e-6, 2.2e-6, 2.2e-6};
+    static constexpr double kBatch[2][kTileCount] = {{9.5e-6, 2.2e-6, 2.2e-6}, {12e-6, 5e-6, 5e-6}};
+    const bool busy = epi > kEpiPartial || p.activation != VECTRA_DENSE_NONE;
     static constexpr int kResident[kTileCount] = {1, 2, 5};
     static constexpr double kPart[kTileCount][5] = {{1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
     double best = 1e30;
@@ -365,15 +369,16 @@ struct Call {
     const int most_splits = epi == kEpiStore ? std::min(256, p.k_tiles / 2) : 1;
     for (int t = 0; t < kTileCount; ++t) {
       const int64_t tiles = ceil_div(p.m, kTileSize[t]) * ceil_div(columns, kTileSize[t]);
-      const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : kRate16[t]) / 256;  // of a full CU
+      const double rate16 = t == kTileMedium && layout != kLayoutForward ? 1.0e15 : kRate16[t];
+      const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : rate16) / 256;  // of a full CU
       for (int k = 1; k <= std::max(1, most_splits); k *= 2) {
         const int64_t depth = ceil_div(p.k_tiles, k) * (128 / esize());
         const int64_t per_cu = ceil_div(tiles * k, cus);
         const int together = static_cast<int>(std::min<int64_t>(per_cu, kResident[t]));
         const double products = per_cu * 2.0 * kTileSize[t] * kTileSize[t] * depth / (rate * kPart[t][together - 1]);
-        const double traffic = tiles * k * 2.0 * kTileSize[t] * depth * esize() / 8e12;
+        const double traffic = tiles * k * 2.0 * kTileSize[t] * depth * esize() / 16e12;
         const double join = k > 1 ? 8.0 * k * p.m * p.n / 5e12 + 6e-6 : 0;
-        const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
+        const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[busy][t] + join;
         if (time < best * 0.98) {
           best = time;
           tile = t;
@@ -389,7 +394,7 @@ struct Call {
     const int deep = static_cast<int>(128 / esize());
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
     int tile, splits;
-    choose(p, columns, epi, tile, splits);
+    choose(p, columns, layout, epi, tile, splits);
     p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileSize[tile]));
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileSize[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));

@@ -175,15 +175,18 @@ struct Tile {
   }
 };
 
-// Tile `id` of `tiles_m` x `tiles_n`.  Workgroups are dealt round-robin to the
-// 8 XCDs: each XCD takes one contiguous run of tiles, and within the run
-// bands of kBand tile rows are walked column by column, so that the operands
-// of the tiles in flight on an XCD stay in its L2.
+// The part of the contraction and the tile that workgroup `id` computes.
+// Workgroups are dealt round-robin to the 8 XCDs: each XCD takes one contiguous
+// run of the tiles of all parts, part by part (the tiles of a part read the
+// same operand rows), and within a part bands of kBand tile rows are walked
+// column by column, so that the operands of the tiles in flight on an XCD stay
+// in its L2.
 constexpr int kBand = 4;
-__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int total = tiles_m * tiles_n;
+__device__ __forceinline__ void tile_of(int id, int total, int tiles_m, int tiles_n, int& part, int& tm, int& tn) {
   const int xcd = id & 7, each = total >> 3, more = total & 7;
-  const int t = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+  int t = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+  part = t / (tiles_m * tiles_n);
+  t -= part * tiles_m * tiles_n;
   const int per_band = kBand * tiles_n;
   const int band = t / per_band, in = t - band * per_band;
   const int height = min(kBand, tiles_m - band * kBand);
@@ -306,12 +309,12 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
   const int g = lane >> 4, i = lane & 15;
   const int wm = wave / C::kWN, wn = wave % C::kWN;
 
-  int tm, tn;
-  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  int part, tm, tn;
+  tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, part, tm, tn);
   const int64_t m0 = static_cast<int64_t>(tm) * C::kBM;
   constexpr int kOutN = C::kGated ? C::kBN / 2 : C::kBN;  // output columns per tile
   const int64_t n0 = static_cast<int64_t>(tn) * kOutN;
-  const int k_first = blockIdx.y * p.k_tiles_per_split;
+  const int k_first = part * p.k_tiles_per_split;
   const int k_last = min(k_first + p.k_tiles_per_split, p.k_tiles);
 
   // ---- per-lane load offsets (bytes from the tile's base) and base pointers
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
   // ---- epilogue
   if constexpr (C::kEpi == kEpiPartial) {
     // A lane holds D[m, n .. n + 3] of every 16 x 16 tile; ldo is a multiple of 4.
-    float* const out = static_cast<float*>(p.out) + static_cast<int64_t>(blockIdx.y) * p.m * p.ldo;
+    float* const out = static_cast<float*>(p.out) + static_cast<int64_t>(part) * p.m * p.ldo;
 #pragma unroll
     for (int u = 0; u < C::kTN; ++u) {
       const int64_t n = n0 + (wn * C::kTN + u) * 16 + 4 * g;
@@ -580,7 +583,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
         const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
         if (wn == 0 && g == 0 && m < p.m) {
           if constexpr (C::kEpi == kEpiPartial)
-            static_cast<float*>(p.sums)[blockIdx.y * p.m + m] = s;
+            static_cast<float*>(p.sums)[part * p.m + m] = s;
           else
             store_as(p.sums, m, p.sums_dtype, s);
         }

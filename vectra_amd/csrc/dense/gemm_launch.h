@@ -7,7 +7,7 @@ namespace vectra_dense {
 
 template <typename T, typename C>
 int launch_one(const GemmParams& p, int splits, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(splits));
+  const uint32_t grid = static_cast<uint32_t>(p.tiles_m) * static_cast<uint32_t>(p.tiles_n) * static_cast<uint32_t>(splits);
   gemm_kernel<T, C><<<grid, C::kThreads, 0, stream>>>(p);
   return hipGetLastError() == hipSuccess ? VECTRA_DENSE_OK : VECTRA_DENSE_ERR_LAUNCH;
 }
