@@ -17,6 +17,7 @@
 
 #include "dense_common.h"
 #include "dense_kernels.h"
+#include "row_chunk.h"
 
 namespace vectra_dense {
 namespace {
@@ -60,7 +61,8 @@ __global__ __launch_bounds__(256) void zero_tail_kernel(T* x, int64_t rows, int6
 // 208 parts: 57.8 us with one lane, each load waiting for the one before).
 template <typename T, int kLanes>
 __global__ __launch_bounds__(256) void join_kernel(const float* parts, int splits, int64_t m, int64_t n, int64_t ld,
-                                                   GemmParams p, const float* sum_parts, int quad_blocks) {
+                                                   GemmParams p, int quad_blocks, void* sums_out,
+                                                   int32_t sums_dtype) {
   constexpr int kQuads = 256 / kLanes;
   if (static_cast<int>(blockIdx.x) >= quad_blocks) {  // the sums' planes: 16 lanes per sum, 16 sums
     __shared__ float sum_part[16][16];
@@ -69,14 +71,14 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
     float s = 0.f;
     if (at < m) {
 #pragma unroll 4
-      for (int k = lane; k < splits; k += 16) s += sum_parts[k * m + at];
+      for (int k = lane; k < splits; k += 16) s += p.sums[k * m + at];
     }
     sum_part[lane][c] = s;
     __syncthreads();
     if (lane != 0 || at >= m) return;
 #pragma unroll
     for (int k = 1; k < 16; ++k) s += sum_part[k][c];
-    store_as(p.sums, at, p.sums_dtype, s);
+    store_as(sums_out, at, sums_dtype, s);
     return;
   }
   __shared__ f32x4 part[kLanes > 1 ? kLanes : 1][kQuads];
@@ -117,26 +119,49 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
   store4(static_cast<T*>(p.out) + row * p.ldo + col, s, left);
 }
 
-// Sums of 64 columns over the rows [blockIdx.y * per, ...): 16 row lanes of 64
-// columns, joined in LDS in a fixed order.  In: T or float; out: one row of
-// partial sums per blockIdx.y, or with one block the bias gradient itself.
+// Column sums of rows [blockIdx.y * per, ...): a thread adds up a 16-byte
+// chunk of every kRows-th row, four rows in flight; 2^lanes_log2 threads side by
+// side cover a row's chunks (64 at most, as many as a narrow row has), and the
+// block's row lanes are joined in LDS in a fixed order.  Out: one row of
+// partial sums per blockIdx.y, or with one of them the result itself.
 template <typename In>
-__global__ __launch_bounds__(1024) void column_sums_kernel(const In* x, int64_t stride, int64_t rows, int64_t n,
-                                                           int64_t per, void* out, int64_t out_stride,
-                                                           int32_t out_dtype) {
-  __shared__ float part[16][64];
-  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + c;
+__global__ __launch_bounds__(256) void column_sums_kernel(const In* x, int64_t stride, int64_t rows, int64_t n,
+                                                          int64_t per, int lanes_log2, void* out, int64_t out_stride,
+                                                          int32_t out_dtype) {
+  constexpr int kPer = 16 / sizeof(In);
+  __shared__ float part[256][kPer + 1];
+  const int lanes = 1 << lanes_log2, row_lanes = 256 >> lanes_log2;
+  const int c = threadIdx.x & (lanes - 1), r = threadIdx.x >> lanes_log2;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + c) * kPer;
   const int64_t first = blockIdx.y * per, last = least(first + per, rows);
-  float s = 0.f;
-  if (col < n)
-    for (int64_t row = first + r; row < last; row += 16) s += widen(x[row * stride + col]);
-  part[r][c] = s;
-  __syncthreads();
-  if (r != 0 || col >= n) return;
+  float s[kPer] = {};
+  const auto add = [&](const Frag& f) {
+    In v[kPer];
+    __builtin_memcpy(v, &f.w, 16);
 #pragma unroll
-  for (int k = 1; k < 16; ++k) s += part[k][c];
-  store_as(out, blockIdx.y * out_stride + col, out_dtype, s);
+    for (int e = 0; e < kPer; ++e) s[e] += widen(v[e]);
+  };
+  if (col < n) {
+    int64_t row = first + r;
+    for (; row + 3 * row_lanes < last; row += 4 * row_lanes) {
+      Frag f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = load_row_chunk(x + (row + j * row_lanes) * stride, n, col);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add(f[j]);
+    }
+    for (; row < last; row += row_lanes) add(load_row_chunk(x + row * stride, n, col));
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) part[threadIdx.x][e] = s[e];
+  __syncthreads();
+  for (int at = threadIdx.x; at < lanes * kPer; at += 256) {
+    const int64_t to = static_cast<int64_t>(blockIdx.x) * lanes * kPer + at;
+    if (to >= n) continue;
+    float total = 0.f;
+    for (int k = 0; k < row_lanes; ++k) total += part[k * lanes + at / kPer][at % kPer];
+    store_as(out, blockIdx.y * out_stride + to, out_dtype, total);
+  }
 }
 
 // ------------------------------------------------------------- 8-bit rows
@@ -388,7 +413,8 @@ struct Call {
     }
   }
 
-  void product(GemmParams p, int layout, int epi) {
+  // sums_out: where the sums of A over the contraction go (weight layout), or NULL.
+  void product(GemmParams p, int layout, int epi, void* sums_out = nullptr, int32_t sums_dtype = 0) {
     const bool gated = epi == kEpiGated || epi == kEpiGatedSlope;
     const int64_t columns = gated ? 2 * p.n : p.n;
     const int deep = static_cast<int>(128 / esize());
@@ -399,28 +425,38 @@ struct Call {
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileSize[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
     splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
-    if (splits == 1) {
-      run(p, layout, tile, epi, 1);
-      return;
-    }
-    const int64_t ld = ceil_div(p.n, 4) * 4, kept = scratch.used;
-    float* const parts = static_cast<float*>(scratch.take(splits * p.m * ld * 4));
-    float* const sum_parts = p.sums ? static_cast<float*>(scratch.take(splits * p.m * 4)) : nullptr;
-    GemmParams q = p;
-    q.out = parts;
-    q.sums = sum_parts;
-    q.ldo = ld;
-    run(q, layout, tile, kEpiPartial, splits);
-    if (go())
+    const int64_t kept = scratch.used;
+    // The large tile leaves the sums to a pass of their own: their few adds per
+    // product cost its loop 85 us of 325 (8192 x 4096 -> 4096 bf16), the pass 20.
+    if (sums_out && tile == kTileLarge) {
       typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const int64_t quads = p.m * (ld / 4);
-        const bool lanes = splits > 8 && quads < 64 * 256 * 4;
-        const int64_t blocks = ceil_div(quads, lanes ? 16 : 256), sum_blocks = sum_parts ? ceil_div(p.m, 16) : 0;
-        const auto kernel = lanes ? join_kernel<T, 16> : join_kernel<T, 1>;
-        kernel<<<static_cast<uint32_t>(blocks + sum_blocks), 256, 0, stream>>>(parts, splits, p.m, p.n, ld, p, sum_parts,
-                                                                               static_cast<int>(blocks));
+        column_sums<T>(static_cast<const T*>(p.a), p.lda, p.depth, p.m, sums_out, sums_dtype);
       });
+      sums_out = nullptr;
+    }
+    if (sums_out) p.sums = static_cast<float*>(scratch.take(static_cast<int64_t>(splits) * p.m * 4));
+    if (splits == 1) {
+      run(p, layout, tile, epi, 1);
+      if (sums_out) column_sums<float>(p.sums, p.m, 1, p.m, sums_out, sums_dtype);
+    } else {
+      const int64_t ld = ceil_div(p.n, 4) * 4;
+      GemmParams q = p;
+      q.out = scratch.take(splits * p.m * ld * 4);
+      q.ldo = ld;
+      run(q, layout, tile, kEpiPartial, splits);
+      if (go())
+        typed([&](auto* t) {
+          using T = std::remove_pointer_t<decltype(t)>;
+          const int64_t quads = p.m * (ld / 4);
+          const bool lanes = splits > 8 && quads < 64 * 256 * 4;
+          const int64_t blocks = ceil_div(quads, lanes ? 16 : 256), sum_blocks = sums_out ? ceil_div(p.m, 16) : 0;
+          const auto kernel = lanes ? join_kernel<T, 16> : join_kernel<T, 1>;
+          kernel<<<static_cast<uint32_t>(blocks + sum_blocks), 256, 0, stream>>>(
+              static_cast<const float*>(q.out), splits, p.m, p.n, ld, p, static_cast<int>(blocks),
+              sums_out, sums_dtype);
+        });
+    }
     most = std::max(most, scratch.used);
     scratch.used = kept;  // the next product may use it again: launches of one stream run in order
   }
@@ -466,21 +502,28 @@ struct Call {
   // Column sums of [rows, n] into the bias's gradient.
   template <typename In>
   void column_sums(const In* x, int64_t stride, int64_t rows, int64_t n, void* out, int32_t out_dtype) {
-    const uint32_t across = static_cast<uint32_t>(ceil_div(n, 64));
-    int64_t parts = std::min<int64_t>(ceil_div(rows, 128), std::max<int64_t>(1, 4 * cus / across));
-    parts = std::max<int64_t>(1, std::min<int64_t>(parts, 1024));
+    const int64_t chunks = ceil_div(n, 16 / static_cast<int64_t>(sizeof(In)));
+    int lanes_log2 = 0;
+    while (lanes_log2 < 6 && (1 << lanes_log2) < chunks) ++lanes_log2;
+    const uint32_t across = static_cast<uint32_t>(ceil_div(chunks, 1 << lanes_log2));
+    // Enough parts for four blocks per CU, of at least eight turns of four rows.
+    int64_t parts = std::min<int64_t>(ceil_div(rows, 32 * (256 >> lanes_log2)), ceil_div(4 * cus, across));
+    parts = std::max<int64_t>(1, parts);
     if (parts == 1) {
-      if (go()) column_sums_kernel<In><<<dim3(across, 1), 1024, 0, stream>>>(x, stride, rows, n, rows, out, 0, out_dtype);
-    } else {
-      const int64_t per = ceil_div(rows, parts);
-      float* const sums = static_cast<float*>(scratch.take(parts * n * 4));
-      if (go()) {
-        column_sums_kernel<In><<<dim3(across, static_cast<uint32_t>(parts)), 1024, 0, stream>>>(
-            x, stride, rows, n, per, sums, n, VECTRA_DENSE_F32);
-        column_sums_kernel<float><<<dim3(across, 1), 1024, 0, stream>>>(sums, n, parts, n, parts, out, 0, out_dtype);
-      }
+      if (go())
+        column_sums_kernel<In><<<dim3(across, 1), 256, 0, stream>>>(x, stride, rows, n, rows, lanes_log2, out, 0, out_dtype);
+      check();
+      return;
     }
+    const int64_t per = ceil_div(rows, parts), kept = scratch.used;
+    float* const sums = static_cast<float*>(scratch.take(parts * n * 4));
+    if (go())
+      column_sums_kernel<In><<<dim3(across, static_cast<uint32_t>(parts)), 256, 0, stream>>>(
+          x, stride, rows, n, per, lanes_log2, sums, n, VECTRA_DENSE_F32);
     check();
+    column_sums<float>(sums, n, parts, n, out, out_dtype);
+    most = std::max(most, scratch.used);
+    scratch.used = kept;
   }
 };
 
@@ -762,11 +805,9 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
     p.m = n_w;
     p.n = a.width_in;
     p.depth = p.depth_b = a.rows;
-    p.sums = want_db ? a.dbias : nullptr;
-    p.sums_dtype = a.bias_dtype;
     p.out = a.dweight;
     p.ldo = a.dweight_stride;
-    c.product(p, kLayoutWeight, kEpiStore);
+    c.product(p, kLayoutWeight, kEpiStore, want_db ? a.dbias : nullptr, a.bias_dtype);
   }
 }
 

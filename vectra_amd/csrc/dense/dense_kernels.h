@@ -34,11 +34,9 @@ struct GemmParams {
   int64_t ldr;
   const void* grad;
   int64_t ldg;
-  // Weight layout: sums of A over the contraction (the bias's gradient), [m]
-  // in sums_dtype where the product is whole, fp32 [splits, m] where it is
-  // split; NULL: not wanted.
-  void* sums;
-  int32_t sums_dtype;
+  // Weight layout: sums of A over the contraction (the bias's gradient), fp32
+  // [parts, m], to be added up; NULL: not wanted (always on the large tile).
+  float* sums;
   int32_t bias_dtype;
   int32_t activation;
 };

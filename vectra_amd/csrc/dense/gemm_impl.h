@@ -34,16 +34,12 @@
 
 #include "dense_common.h"
 #include "dense_kernels.h"
+#include "row_chunk.h"
 
 namespace vectra_dense {
 
 typedef short lds_v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
-
-// What one lane feeds a matrix instruction: 16 bytes.
-struct Frag {
-  u32x4 w;
-};
 
 template <typename T>
 struct Mma;
@@ -280,7 +276,9 @@ struct GemmConfig {
   static constexpr int kDeep = 128 / sizeof(T);  // contraction per tile
   static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
   static constexpr bool kGated = kEpi == kEpiGated || kEpi == kEpiGatedSlope;
-  static constexpr bool kSums = kWideA && kWideB;  // the weight's gradient, and with it the bias's
+  // The weight's gradient, and with it the bias's: where the registers have
+  // room for it (the large tile has none).
+  static constexpr bool kSums = kWideA && kWideB && kTM * kTN <= 16;
   using A = Tile<T, kWideA, kBM, kDeep, kThreads>;
   using B = Tile<T, kWideB, kBN, kDeep, kThreads>;
   static constexpr int kStageBytes = A::kBytes + B::kBytes;
@@ -392,11 +390,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
 #pragma unroll
     for (int tm_ = 0; tm_ < C::kTM; ++tm_) acc[tn_][tm_] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Sums of A: by the workgroups of the first tile column.
-  const bool sum_here = C::kSums && p.sums && tn == 0;
-  float sums[C::kSums ? C::kTM : 1];
-#pragma unroll
-  for (int t = 0; t < (C::kSums ? C::kTM : 1); ++t) sums[t] = 0.f;
+  float sums[C::kSums ? C::kTM : 1] = {};
 
   const auto read = [&](Frag(&fa)[C::kTM], Frag(&fb)[C::kTN], int buf, int step) {
     const lds_char* const ta = smem + buf * C::kStageBytes;
@@ -412,70 +406,65 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
 #pragma unroll
       for (int u = 0; u < C::kTN; ++u) acc[u][t] = Mma<T>::run(fb[u], fa[t], acc[u][t]);
   };
-  // The loop over the contraction, with or without the sums of A.
-  const auto products = [&](auto with_sums) {
-    constexpr bool kSum = decltype(with_sums)::value;
-    const auto add_sums = [&](const Frag(&fa)[C::kTM]) {
-      if constexpr (kSum) {
+  const auto add_sums = [&](const Frag(&fa)[C::kTM]) {
 #pragma unroll
-        for (int t = 0; t < C::kTM; ++t) sums[t] = Mma<T>::sum(fa[t], sums[t]);
-      }
-    };
-    if constexpr (C::kPhased) {
-      // Two tiles in LDS, two steps per tile, the fragments of one step ahead in
-      // registers.  While the products of step 0 run, step 1 is read; then one
-      // barrier, after which nobody reads this tile any more and the next one is
-      // there; while the products of step 1 run, the tile after next is loaded
-      // over this one and step 0 of the next is read.  Loads past the last tile
-      // go out of bounds (zeros, never multiplied).
-      static_assert(C::kDeep / A::kStep == 2, "two steps per tile");
-      if (k_first < k_last) {
-        Frag fa0[C::kTM], fb0[C::kTN], fa1[C::kTM], fb1[C::kTN];
-        load(k_first, 0);
-        wait_loads();
-        __builtin_amdgcn_s_barrier();
-        load(k_first + 1, 1);
-        read(fa0, fb0, 0, 0);
-        for (int kt = k_first; kt < k_last; ++kt) {
-          const int buf = (kt - k_first) & 1;
-          read(fa1, fb1, buf, 1);
-          multiply(fa0, fb0);
-          add_sums(fa0);
-          interleave<C, false>();
-          wait_all();
-          __builtin_amdgcn_s_barrier();
-          load(kt + 2, buf);
-          read(fa0, fb0, buf ^ 1, 0);
-          multiply(fa1, fb1);
-          add_sums(fa1);
-          interleave<C, true>();
-        }
-        wait_all();  // nothing is on its way into LDS when it is used again
-      }
-    } else {
-      if (k_first < k_last) load(k_first, 0);
-      for (int kt = k_first; kt < k_last; ++kt) {
+    for (int t = 0; t < C::kTM; ++t) sums[t] = Mma<T>::sum(fa[t], sums[t]);
+  };
+
+  if constexpr (C::kPhased) {
+    // Two tiles in LDS, two steps per tile, the fragments of one step ahead in
+    // registers.  While the products of step 0 run, step 1 is read; then one
+    // barrier, after which nobody reads this tile any more and the next one is
+    // there; while the products of step 1 run, the tile after next is loaded
+    // over this one and step 0 of the next is read.  Loads past the last tile
+    // go out of bounds (zeros, never multiplied).
+    static_assert(C::kDeep / A::kStep == 2, "two steps per tile");
+    if (k_first < k_last) {
+      Frag fa0[C::kTM], fb0[C::kTN], fa1[C::kTM], fb1[C::kTN];
+      load(k_first, 0);
+      wait_loads();
+      __builtin_amdgcn_s_barrier();
+      load(k_first + 1, 1);
+      read(fa0, fb0, 0, 0);
+      const auto one = [&](int kt, auto with_sums) {
         const int buf = (kt - k_first) & 1;
-        wait_loads();
-        __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
-        if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
+        read(fa1, fb1, buf, 1);
+        multiply(fa0, fb0);
+        if constexpr (decltype(with_sums)::value) add_sums(fa0);
+        interleave<C, false>();
+        wait_all();
+        __builtin_amdgcn_s_barrier();
+        load(kt + 2, buf);
+        read(fa0, fb0, buf ^ 1, 0);
+        multiply(fa1, fb1);
+        if constexpr (decltype(with_sums)::value) add_sums(fa1);
+        interleave<C, true>();
+      };
+      bool with_sums = false;
+      if constexpr (C::kSums) with_sums = p.sums && tn == 0;
+      if constexpr (C::kSums) {
+        if (with_sums)
+          for (int kt = k_first; kt < k_last; ++kt) one(kt, Flag<true>{});
+      }
+      if (!with_sums)
+        for (int kt = k_first; kt < k_last; ++kt) one(kt, Flag<false>{});
+      wait_all();  // nothing is on its way into LDS when it is used again
+    }
+  } else {
+    static_assert(!C::kSums);
+    if (k_first < k_last) load(k_first, 0);
+    for (int kt = k_first; kt < k_last; ++kt) {
+      const int buf = (kt - k_first) & 1;
+      wait_loads();
+      __syncthreads();  // tile kt is in LDS, and nobody reads the other buffer any more
+      if (kt + 1 < k_last) load(kt + 1, buf ^ 1);
 #pragma unroll
-        for (int step = 0; step < C::kDeep / A::kStep; ++step) {
-          Frag fa[C::kTM], fb[C::kTN];
-          read(fa, fb, buf, step);
-          multiply(fa, fb);
-          add_sums(fa);
-        }
+      for (int step = 0; step < C::kDeep / A::kStep; ++step) {
+        Frag fa[C::kTM], fb[C::kTN];
+        read(fa, fb, buf, step);
+        multiply(fa, fb);
       }
     }
-  };
-  if constexpr (C::kSums) {
-    if (sum_here)
-      products(Flag<true>{});
-    else
-      products(Flag<false>{});
-  } else {
-    products(Flag<false>{});
   }
 
   // ---- epilogue
@@ -571,22 +560,17 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
     }
   }
 
-  // The sums of A over the contraction: lane group g holds those of its own
-  // elements.
+  // The sums of A, by the workgroups of the first tile column: lane group g
+  // holds those of its own elements.
   if constexpr (C::kSums) {
-    if (sum_here) {
+    if (p.sums && tn == 0 && wn == 0) {
 #pragma unroll
       for (int t = 0; t < C::kTM; ++t) {
         float s = sums[t];
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
-        if (wn == 0 && g == 0 && m < p.m) {
-          if constexpr (C::kEpi == kEpiPartial)
-            static_cast<float*>(p.sums)[part * p.m + m] = s;
-          else
-            store_as(p.sums, m, p.sums_dtype, s);
-        }
+        if (g == 0 && m < p.m) p.sums[static_cast<int64_t>(part) * p.m + m] = s;
       }
     }
   }

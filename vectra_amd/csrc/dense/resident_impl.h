@@ -62,22 +62,6 @@ __device__ __forceinline__ int resident_swizzle(int row) {
   return (row >> 2) & 3;
 }
 
-// Elements first .. of a row of `width`, zeros past its end.
-template <typename T>
-__device__ __forceinline__ Frag load_row_chunk(const T* row, int64_t width, int64_t first) {
-  constexpr int kPer = 16 / sizeof(T);
-  Frag f;
-  if (first + kPer <= width) {
-    __builtin_memcpy(&f.w, row + first, 16);  // unaligned
-  } else {
-    T v[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = first + e < width ? row[first + e] : static_cast<T>(0.f);
-    __builtin_memcpy(&f.w, v, 16);
-  }
-  return f;
-}
-
 // kAct: the activation, fixed per instantiation of the body so that no branch
 // sits in the element loops.
 template <typename T, typename C, int kAct>
