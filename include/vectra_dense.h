@@ -16,7 +16,8 @@
  *   linear   dz = g * act'(z), z = x W^T + b
  *   gated    dz = [g * u * act'(a), g * act(a)], [a, u] = x W^T + b
  *   dx = dz W      dW = dz^T x      db = column sums of dz      (dr = g)
- * dz is kept in the operands' type (one rounding), and all three are formed from that.
+ * dz is kept in the operands' type (one rounding) for the products; db sums it in fp32
+ * before that rounding where the product that forms it can, else after.
  * z is computed again from x (or from x's 8-bit form): nothing but the inputs is needed.
  *
  * 8-bit rows: every 32 consecutive elements of a row share a power of two 2^e, the

@@ -413,7 +413,8 @@ struct Call {
     }
   }
 
-  // sums_out: where the sums of A over the contraction go (weight layout), or NULL.
+  // sums_out: where the sums of A over the contraction go (weight layout), or the
+  // column sums of dz (slope epilogues); NULL: not wanted.
   void product(GemmParams p, int layout, int epi, void* sums_out = nullptr, int32_t sums_dtype = 0) {
     const bool gated = epi == kEpiGated || epi == kEpiGatedSlope;
     const int64_t columns = gated ? 2 * p.n : p.n;
@@ -428,17 +429,21 @@ struct Call {
     const int64_t kept = scratch.used;
     // The large tile leaves the sums to a pass of their own: their few adds per
     // product cost its loop 85 us of 325 (8192 x 4096 -> 4096 bf16), the pass 20.
-    if (sums_out && tile == kTileLarge) {
+    if (sums_out && layout == kLayoutWeight && tile == kTileLarge) {
       typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         column_sums<T>(static_cast<const T*>(p.a), p.lda, p.depth, p.m, sums_out, sums_dtype);
       });
       sums_out = nullptr;
     }
-    if (sums_out) p.sums = static_cast<float*>(scratch.take(static_cast<int64_t>(splits) * p.m * 4));
+    if (sums_out) {  // the planes: of the contraction's parts, or of the tile rows
+      const int64_t planes = layout == kLayoutWeight ? splits : p.tiles_m, width = layout == kLayoutWeight ? p.m : columns;
+      p.sums = static_cast<float*>(scratch.take(planes * width * 4));
+    }
     if (splits == 1) {
       run(p, layout, tile, epi, 1);
-      if (sums_out) column_sums<float>(p.sums, p.m, 1, p.m, sums_out, sums_dtype);
+      if (sums_out && layout == kLayoutWeight) column_sums<float>(p.sums, p.m, 1, p.m, sums_out, sums_dtype);
+      if (sums_out && layout == kLayoutForward) column_sums<float>(p.sums, columns, p.tiles_m, columns, sums_out, sums_dtype);
     } else {
       const int64_t ld = ceil_div(p.n, 4) * 4;
       GemmParams q = p;
@@ -722,6 +727,7 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
   }
   if (use_w && any && (steps == 0 || (want_dx && !dx_with_dz)))
     w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
+  bool db_done = false;
   if (slope && a.rows && n_w && (use_dz || want_dx)) {
     const bool keep_dz = use_dz || !dx_with_dz;
     if (keep_dz) dz = {c.scratch.take(a.rows * n_pad * c.esize()), n_pad};
@@ -760,7 +766,8 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       p.activation = a.activation;
       p.grad = a.grad;
       p.ldg = a.grad_stride;
-      c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope);
+      c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope, want_db ? a.dbias : nullptr, a.bias_dtype);
+      db_done = want_db;
     }
     if (keep_dz && n_pad != n_w && c.go())
       c.typed([&](auto* t) {
@@ -773,8 +780,9 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
   } else {
     dz = {a.grad, a.grad_stride};
   }
-  // db: with dW where that is formed too (the sums of its first operand).
-  if (want_db && !want_dw)
+  // db, where the product that made dz has not summed it: with dW where that is
+  // formed too (the sums of its first operand).
+  if (want_db && !db_done && !want_dw)
     c.typed([&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       c.column_sums<T>(static_cast<const T*>(dz.p), dz.ld, a.rows, n_w, a.dbias, a.bias_dtype);
@@ -807,7 +815,7 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
     p.depth = p.depth_b = a.rows;
     p.out = a.dweight;
     p.ldo = a.dweight_stride;
-    c.product(p, kLayoutWeight, kEpiStore, want_db ? a.dbias : nullptr, a.bias_dtype);
+    c.product(p, kLayoutWeight, kEpiStore, want_db && !db_done ? a.dbias : nullptr, a.bias_dtype);
   }
 }
 

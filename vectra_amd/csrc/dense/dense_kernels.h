@@ -34,6 +34,7 @@ struct GemmParams {
   int64_t ldr;
   const void* grad;
   int64_t ldg;
+  // Slope epilogues: column sums of dz, fp32 [tiles_m, columns], to be added up.
   // Weight layout: sums of A over the contraction (the bias's gradient), fp32
   // [parts, m], to be added up; NULL: not wanted (always on the large tile).
   float* sums;

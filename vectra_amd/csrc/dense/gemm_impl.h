@@ -502,6 +502,10 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
           if constexpr (C::kGated) bias_up[e / 4][e % 4] = load_bias(p.bias, p.n + n + e, p.bias_dtype);
         }
     }
+    // Slope epilogues: the lane's columns of dz (and of the up half's), added up
+    // over the wave's rows.
+    constexpr bool kSlope = C::kEpi == kEpiSlope || C::kEpi == kEpiGatedSlope;
+    f32x4 column[kSlope ? (C::kGated ? 4 : 2) : 1] = {};
     __syncthreads();  // all waves are done with the tiles
 #pragma unroll
     for (int first = 0; first < C::kTM; first += kBandTiles) {
@@ -554,9 +558,46 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
             T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
             store8(out, z[0], z[1], left);
             if constexpr (C::kGated) store8(out + p.n, up[0], up[1], left);
+            if constexpr (kSlope) {
+              column[0] += z[0];
+              column[1] += z[1];
+              if constexpr (C::kGated) {
+                column[2] += up[0];
+                column[3] += up[1];
+              }
+            }
           }
         }
       });
+    }
+    // Over the lanes of a column, then over the rows of waves, in a fixed
+    // order: row tm of p.sums.
+    if constexpr (kSlope) {
+      if (p.sums) {
+        constexpr int kSumCols = C::kWN * kOut;  // of one half
+        __attribute__((address_space(3))) float* const sums_lds = (__attribute__((address_space(3))) float*)smem;
+        __syncthreads();  // the bands are read
+#pragma unroll
+        for (int q = 0; q < (C::kGated ? 4 : 2); ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = column[q][e];
+#pragma unroll
+            for (int d = kLanes; d < 64; d <<= 1) v += __shfl_xor(v, d);
+            if (lane < kLanes)
+              sums_lds[(wm * (C::kGated ? 2 : 1) + q / 2) * kSumCols + wn * kOut + col + (q % 2) * 4 + e] = v;
+          }
+        __syncthreads();
+        for (int at = tid; at < kSumCols * (C::kGated ? 2 : 1); at += C::kThreads) {
+          const int half = at / kSumCols;
+          const int64_t to = n0 + at % kSumCols;
+          if (to >= p.n) continue;
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < C::kWM; ++w) v += sums_lds[(w * (C::kGated ? 2 : 1) + half) * kSumCols + at % kSumCols];
+          p.sums[static_cast<int64_t>(tm) * (C::kGated ? 2 * p.n : p.n) + half * p.n + to] = v;
+        }
+      }
     }
   }
 
