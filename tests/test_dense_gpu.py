@@ -72,6 +72,44 @@ def test_integers_are_exact(size, dtype):
             assert torch.equal(g.cpu(), v.to(dtype)), (activation, name)
 
 
+# Products of many large tiles, with rows, columns and contractions that end
+# inside one: forward, dx and dW each take them at one of these.
+LARGE = [(1100, 4104, 4104), (8200, 264, 4104), (8200, 4104, 264), (2051, 1000, 2056), (4096, 4096, 1024),
+         (4090, 2056, 4090), (8190, 1543, 4090)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('size', LARGE, ids=str)
+@pytest.mark.parametrize('gated', [False, True])
+def test_large_integers_are_exact(size, dtype, gated):
+    """As below 2^24 as the small ones: at most 8200 terms of at most 12.  The
+    64-bit reference runs on the GPU, as matrix products of doubles."""
+    rows, width_in, width_out = size
+    n = width_out * (1 + gated)
+    x, w = integers(rows, width_in, most=2, seed=1, dtype=dtype), integers(n, width_in, most=1, seed=2, dtype=dtype)
+    b = integers(n, most=9, seed=3, dtype=dtype)
+    if gated:  # an up projection of one-hot rows and a gate that passes all: dz stays a small integer
+        w.zero_()
+        w[torch.arange(n), torch.randint(0, width_in, (n,), generator=torch.Generator().manual_seed(6))] = 1
+    dy = integers(rows, width_out, most=3, seed=5, dtype=dtype)
+    r = None if gated else integers(rows, width_out, most=9, seed=4, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = dense.gated_linear(*leaves, 'relu') if gated else dense.linear(*leaves, r, 'relu')
+    got = torch.autograd.grad(y, leaves, dy)
+    xd, wd, bd, dyd = (t.double() for t in (x, w, b, dy))
+    z = xd @ wd.t() + bd
+    if gated:
+        gate, up = z.chunk(2, 1)
+        want_y = gate.clamp_min(0) * up
+        dz = torch.cat([dyd * up * (gate > 0), dyd * gate.clamp_min(0)], 1)
+    else:
+        want_y = z.clamp_min(0) + r.double()
+        dz = dyd * (z > 0)
+    assert torch.equal(y, want_y.to(dtype))
+    for name, g, v in zip(('x', 'weight', 'bias'), got, (dz @ wd, dz.t() @ xd, dz.sum(0))):
+        assert torch.equal(g, v.to(dtype)), name
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('size', SIZES, ids=str)
 def test_gated_integers_are_exact(size, dtype):

@@ -12,6 +12,7 @@ whole price model at the serving batch (config 5: d_model 128, 8 heads, 3 or
 Modes: `eager` (the baseline), `inductor` (torch.compile without the rewrite,
 which separates Inductor's own fusion from the HIP operator) and `vectra`
 (the deployment compile: every attention site on vectra::rbf_attention).
+`--dense-kernels` puts the model's linear layers on vectra::linear in any mode.
 Each run first gates its numerics against the eager model (rtol 1e-3), then
 times `--iters` forward passes after `--warmup` with events, as the median of
 `--trials` trials.  `--compare` checks a candidate against a baseline: same
@@ -20,6 +21,7 @@ throughput ratio of at least --min-ratio (the design's 3.0x).
 """
 
 import argparse
+import copy
 import json
 import os
 import statistics
@@ -57,25 +59,28 @@ def timed(fn, inputs, iters: int, warmup: int, trials: int) -> list[float]:
 
 
 def run(mode: str, batch_size: int, layers: int, block_dtype: str, iters: int, warmup: int,
-        trials: int) -> dict:
+        trials: int, dense_kernels: bool = False) -> dict:
     device = 'cuda'
     spec = compile_entry.ServingSpec(device, batch_size, block_dtype)
     torch.manual_seed(0)
     eager = compile_entry.prepare(model_lib.PriceTransformer(config_5(layers)), spec)
     inputs = tuple(model_lib.box_inputs(eager.config, batch_size, device=device, seed=0))
     sites = 0
+    model = eager
+    if dense_kernels:  # the same weights, their linear layers on the dense operators
+        model = copy.deepcopy(eager).set_dense_kernels()
     if mode == 'eager':
-        fn = eager
+        fn = model
     elif mode == 'inductor':
-        fn = torch.compile(eager, fullgraph=True, dynamic=False)
+        fn = torch.compile(model, fullgraph=True, dynamic=False)
     else:
-        fn, report, _ = compile_entry.compile_model(eager, spec)
+        fn, report, _ = compile_entry.compile_model(model, spec)
         sites = report.sites
     worst, _ = compile_entry.max_abs_error(fn, eager, eager.config, spec, batches=2)
     seconds = timed(fn, inputs, iters, warmup, trials)
     per_batch = statistics.median(seconds)
     return {
-        'mode': mode,
+        'mode': mode + ('+dense' if dense_kernels else ''),
         'device': torch.cuda.get_device_name(device),
         'batch_size': batch_size,
         'block_dtype': block_dtype,
@@ -116,6 +121,8 @@ def main(argv=None) -> int:
     p.add_argument('--iters', type=int, default=50)
     p.add_argument('--warmup', type=int, default=10)
     p.add_argument('--trials', type=int, default=5)
+    p.add_argument('--dense-kernels', action='store_true',
+                   help='run the linear layers through vectra::linear (PriceTransformer.set_dense_kernels)')
     p.add_argument('--out', default='')
     p.add_argument('--compare', nargs=2, metavar=('BASELINE', 'CANDIDATE'))
     p.add_argument('--min-ratio', type=float, default=3.0)
@@ -135,7 +142,7 @@ def main(argv=None) -> int:
         print('model_throughput needs a GPU', file=sys.stderr)
         return 2
     result = run(args.mode, args.batch_size, args.layers, args.block_dtype, args.iters, args.warmup,
-                 args.trials)
+                 args.trials, args.dense_kernels)
     text = json.dumps(result)
     if args.out:
         os.makedirs(os.path.dirname(args.out) or '.', exist_ok=True)

@@ -218,7 +218,7 @@ def export_bundle(checkpoint_dir: str, out_dir: str, spec: ServingSpec, numerics
     manifest = {
         'format_version': FORMAT_VERSION,
         'files': digests,
-        'model': dataclasses.asdict(eager.config),
+        'model': eager.config.to_dict(),
         'serving': {**dataclasses.asdict(spec), 'device_name': _device_label(spec.device)},
         'compile': {
             'backend': backend.BACKEND_NAME,

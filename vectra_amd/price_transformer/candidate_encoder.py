@@ -19,6 +19,15 @@ def _mlp(n_in: int, hidden: int, n_out: int) -> nn.Sequential:
     return nn.Sequential(nn.Linear(n_in, hidden), nn.GELU(), nn.Linear(hidden, n_out))
 
 
+def _run_mlp(mlp: nn.Sequential, x: torch.Tensor, dense_kernels: bool) -> torch.Tensor:
+    """The MLP, layer by layer or on torch.ops.vectra.linear."""
+    if not dense_kernels:
+        return mlp(x)
+    first, _, second = mlp
+    hidden = torch.ops.vectra.linear(x, first.weight, first.bias, None, 'gelu')
+    return torch.ops.vectra.linear(hidden, second.weight, second.bias)
+
+
 class QueryEncoder(nn.Module):
     """[B, E], [B, A] -> [B, d_model]."""
 
@@ -26,9 +35,10 @@ class QueryEncoder(nn.Module):
         super().__init__()
         self.mlp = _mlp(embedding_dim + attribute_dim, 2 * d_model, d_model)
         self.role = nn.Parameter(torch.zeros(d_model))
+        self.dense_kernels = False
 
     def forward(self, embedding, attributes):
-        return self.mlp(torch.cat([embedding, attributes], dim=-1)) + self.role
+        return _run_mlp(self.mlp, torch.cat([embedding, attributes], dim=-1), self.dense_kernels) + self.role
 
 
 class CandidateEncoder(nn.Module):
@@ -37,6 +47,7 @@ class CandidateEncoder(nn.Module):
     def __init__(self, embedding_dim: int, attribute_dim: int, d_model: int):
         super().__init__()
         self.mlp = _mlp(embedding_dim + attribute_dim + _EXTRA_FEATURES, 2 * d_model, d_model)
+        self.dense_kernels = False
 
     def forward(self, embedding, attributes, log_price, sale_age_days, offsets_km, distance_km,
                 radius_km, cell_flags):
@@ -53,4 +64,4 @@ class CandidateEncoder(nn.Module):
             ],
             dim=-1,
         )
-        return self.mlp(features)
+        return _run_mlp(self.mlp, features, self.dense_kernels)

@@ -6,7 +6,6 @@ Same files and layout as the reference's models/training/checkpoint.py:
 tensors only, so loading a checkpoint executes nothing from the file.
 """
 
-import dataclasses
 import json
 import os
 
@@ -25,7 +24,7 @@ def save(directory: str, model: model_lib.PriceTransformer, metadata: dict | Non
     state = {name: t.detach().float().cpu().contiguous() for name, t in model.state_dict().items()}
     safetensors_torch.save_file(state, os.path.join(directory, WEIGHTS))
     with open(os.path.join(directory, CONFIG), 'w', encoding='utf-8') as f:
-        json.dump({'model': dataclasses.asdict(model.config), 'metadata': metadata or {}}, f,
+        json.dump({'model': model.config.to_dict(), 'metadata': metadata or {}}, f,
                   indent=2, sort_keys=True)
         f.write('\n')
 

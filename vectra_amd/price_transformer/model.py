@@ -34,11 +34,19 @@ class ModelConfig:
     ffn_dim: int = 256
     num_candidates: int = 64
     min_candidates: int = 4  # kept when no comparable lies inside the radius
+    ffn_gate: bool = False  # a gated (SiLU) feed-forward block; no counterpart in the reference
 
     @classmethod
     def from_dict(cls, values: Mapping[str, typing.Any]) -> 'ModelConfig':
         names = {f.name for f in dataclasses.fields(cls)}
         return cls(**{k: v for k, v in values.items() if k in names})
+
+    def to_dict(self) -> dict[str, typing.Any]:
+        """The fields as the reference writes them; `ffn_gate` only where it is set."""
+        values = dataclasses.asdict(self)
+        if not self.ffn_gate:
+            del values['ffn_gate']
+        return values
 
 
 class PricingInputs(typing.NamedTuple):
@@ -81,6 +89,20 @@ def trim_to_radius(distance_km, radius_km, valid, min_keep: int) -> torch.Tensor
     return torch.where(inside.any(-1, keepdim=True), inside, fallback)
 
 
+class GatedFeedForward(nn.Module):
+    """down(silu(gate(x)) * up(x)); the gate's and the up projection's rows lie
+    in one weight, as torch.ops.vectra.gated_linear takes them."""
+
+    def __init__(self, d_model: int, hidden: int):
+        super().__init__()
+        self.gate_up = nn.Linear(d_model, 2 * hidden)
+        self.down = nn.Linear(hidden, d_model)
+
+    def forward(self, x):
+        gate, up = self.gate_up(x).chunk(2, dim=-1)
+        return self.down(nn.functional.silu(gate) * up)
+
+
 class Block(nn.Module):
     """Pre-norm Transformer block with spatial attention."""
 
@@ -89,15 +111,31 @@ class Block(nn.Module):
         self.norm1 = nn.LayerNorm(config.d_model)
         self.attention = spatial_attention.SpatialAttention(config.d_model, config.num_heads)
         self.norm2 = nn.LayerNorm(config.d_model)
-        self.ffn = nn.Sequential(
-            nn.Linear(config.d_model, config.ffn_dim),
-            nn.GELU(),
-            nn.Linear(config.ffn_dim, config.d_model),
-        )
+        if config.ffn_gate:
+            self.ffn = GatedFeedForward(config.d_model, config.ffn_dim)
+        else:
+            self.ffn = nn.Sequential(
+                nn.Linear(config.d_model, config.ffn_dim),
+                nn.GELU(),
+                nn.Linear(config.ffn_dim, config.d_model),
+            )
 
     def forward(self, x, key_bias):
-        x = x + self.attention(self.norm1(x), key_bias)
-        return x + self.ffn(self.norm2(x))
+        if self.attention.dense_checkpoint is None:
+            x = x + self.attention(self.norm1(x), key_bias)
+            return x + self.ffn(self.norm2(x))
+        x = self.attention(self.norm1(x), key_bias, residual=x)
+        return self._feed_forward(self.norm2(x), x, self.attention.dense_checkpoint)
+
+    def _feed_forward(self, x, residual, checkpoint):
+        """The feed-forward block on the dense operators, onto the residual."""
+        if isinstance(self.ffn, GatedFeedForward):
+            first, second = self.ffn.gate_up, self.ffn.down
+            hidden = torch.ops.vectra.gated_linear(x, first.weight, first.bias, 'silu', checkpoint)
+        else:
+            first, second = self.ffn[0], self.ffn[2]
+            hidden = torch.ops.vectra.linear(x, first.weight, first.bias, None, 'gelu', checkpoint)
+        return torch.ops.vectra.linear(hidden, second.weight, second.bias, residual, 'none', checkpoint)
 
 
 class PriceTransformer(nn.Module):
@@ -120,6 +158,23 @@ class PriceTransformer(nn.Module):
         read-out stay fp32 (coordinates in half precision would lose km)."""
         self.blocks.to(dtype)
         self._block_dtype = dtype
+        return self
+
+    def set_dense_kernels(self, enabled: bool = True, checkpoint: str = 'none') -> 'PriceTransformer':
+        """Runs the linear layers of the blocks and encoders through
+        torch.ops.vectra.linear and gated_linear: bias, activation and residual
+        in the product's epilogue, for training with the operators' own
+        gradients.  `checkpoint='e4m3'`: the blocks keep their layers' inputs
+        in 8 bits for the backward pass (the encoders' inputs, prices and
+        distances, stay as they are).  The parameters are the same either way."""
+        if enabled:
+            from vectra_amd.kernels import dense  # pylint: disable=import-outside-toplevel
+
+            if checkpoint not in dense.CHECKPOINTS:
+                raise ValueError(f'checkpoint must be one of {dense.CHECKPOINTS}, not {checkpoint!r}')
+        for block in self.blocks:
+            block.attention.dense_checkpoint = checkpoint if enabled else None
+        self.query_encoder.dense_kernels = self.candidate_encoder.dense_kernels = enabled
         return self
 
     def forward(self, query_embedding, query_attributes, query_location, query_cell6,

@@ -6,6 +6,10 @@ with a learned bandwidth per head, written as the plain eager chain on
 purpose (reference: models/price_transformer/spatial_attention.py:68-88) so
 that torch.compile(backend='vectra') finds it and substitutes
 torch.ops.vectra.rbf_attention.
+
+The projections around it are plain linear layers, or, after
+PriceTransformer.set_dense_kernels, torch.ops.vectra.linear calls (the output
+projection with the residual in its epilogue).
 """
 
 import math
@@ -27,15 +31,24 @@ class SpatialAttention(nn.Module):
         self.log_sigma = nn.Parameter(
             torch.full((1, num_heads, 1, 1), 0.5 * math.log(self.head_dim))
         )
+        # None: nn.Linear's own forward; else the form in which
+        # torch.ops.vectra.linear keeps its input for the backward pass.
+        self.dense_checkpoint: str | None = None
 
-    def forward(self, x: torch.Tensor, key_bias: torch.Tensor) -> torch.Tensor:
-        """x [B, N, d_model], key_bias [B, 1, 1, N] (0 or -inf) -> [B, N, d_model]."""
+    def _project(self, layer: nn.Linear, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if self.dense_checkpoint is None:
+            return layer(x) if residual is None else residual + layer(x)
+        return torch.ops.vectra.linear(x, layer.weight, layer.bias, residual, 'none', self.dense_checkpoint)
+
+    def forward(self, x: torch.Tensor, key_bias: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """x [B, N, d_model], key_bias [B, 1, 1, N] (0 or -inf) -> [B, N, d_model],
+        onto `residual` if one is given."""
         batch, tokens, width = x.shape
         q, k, v = (
             t.view(batch, tokens, self.num_heads, self.head_dim).transpose(1, 2)
-            for t in self.qkv(x).split(width, dim=-1)
+            for t in self._project(self.qkv, x).split(width, dim=-1)
         )
         sq_dist = (q.unsqueeze(-2) - k.unsqueeze(-3)).pow(2).sum(-1)
         logits = -sq_dist / (2 * self.log_sigma.exp() ** 2) + key_bias
         mixed = torch.softmax(logits, dim=-1) @ v
-        return self.out(mixed.transpose(1, 2).reshape(batch, tokens, width))
+        return self._project(self.out, mixed.transpose(1, 2).reshape(batch, tokens, width), residual)
