@@ -53,17 +53,20 @@ __global__ __launch_bounds__(256) void zero_tail_kernel(T* x, int64_t rows, int6
   if (at < rows * n) x[at / n * stride + from + at % n] = static_cast<T>(0.f);
 }
 
-// Adds up the planes of a split product in a fixed order and finishes it:
-// act(sum + bias) + residual.  A thread adds every kLanes-th plane of four
-// columns, four planes in flight; the kLanes threads of a quad are joined in
-// LDS.  One lane per quad where there are few planes or many quads; 16 where
-// one thread would walk hundreds of planes (a [256, 128] weight gradient of
-// 208 parts: 57.8 us with one lane, each load waiting for the one before).
-template <typename T, int kLanes>
+// Adds up the planes of a split product in a fixed order and finishes it with
+// the product's epilogue.  A thread adds every kLanes-th plane of four columns
+// (a gated layer: of both halves), four planes in flight; the kLanes threads of
+// a quad are joined in LDS.  One lane per quad where there are few planes or
+// many quads; 16 where one thread would walk hundreds of planes (a [256, 128]
+// weight gradient of 208 parts: 57.8 us with one lane, each load waiting for
+// the one before; 5 with 16).
+template <typename T, int kLanes, int kEpi>
 __global__ __launch_bounds__(256) void join_kernel(const float* parts, int splits, int64_t m, int64_t n, int64_t ld,
                                                    GemmParams p, int quad_blocks, void* sums_out,
                                                    int32_t sums_dtype) {
   constexpr int kQuads = 256 / kLanes;
+  constexpr bool kGated = kEpi == kEpiGated || kEpi == kEpiGatedSlope;
+  constexpr int kHalves = kGated ? 2 : 1;
   if (static_cast<int>(blockIdx.x) >= quad_blocks) {  // the sums' planes: 16 lanes per sum, 16 sums
     __shared__ float sum_part[16][16];
     const int c = threadIdx.x % 16, lane = threadIdx.x / 16;
@@ -81,42 +84,86 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
     store_as(sums_out, at, sums_dtype, s);
     return;
   }
-  __shared__ f32x4 part[kLanes > 1 ? kLanes : 1][kQuads];
+  __shared__ f32x4 part[kLanes > 1 ? kLanes : 1][kHalves][kQuads];
   const int q = threadIdx.x % kQuads, lane = threadIdx.x / kQuads;
-  const int64_t quads = ld / 4;
+  const int64_t quads = (n + 3) / 4;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kQuads + q;
   const bool live = at < m * quads;
   const int64_t row = live ? at / quads : 0, col = live ? (at - row * quads) * 4 : 0;
-  const float* const from = parts + row * ld + col;
   const int64_t plane = m * ld;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  f32x4 s[kHalves] = {};
   if (live) {
-    int k = lane;
-    for (; k + 3 * kLanes < splits; k += 4 * kLanes) {
-      f32x4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(from + (k + j * kLanes) * plane);
+    for (int h = 0; h < kHalves; ++h) {
+      const float* const from = parts + row * ld + h * n + col;
+      const auto load = [&](int k) {  // (the up half starts at any column)
+        f32x4 v;
+        __builtin_memcpy(&v, from + k * plane, 16);
+        return v;
+      };
+      int k = lane;
+      for (; k + 3 * kLanes < splits; k += 4 * kLanes) {
+        f32x4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s += v[j];
+        for (int j = 0; j < 4; ++j) v[j] = load(k + j * kLanes);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[h] += v[j];
+      }
+      for (; k < splits; k += kLanes) s[h] += load(k);
     }
-    for (; k < splits; k += kLanes) s += *reinterpret_cast<const f32x4*>(from + k * plane);
   }
   if constexpr (kLanes > 1) {
-    part[lane][q] = s;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) part[lane][h][q] = s[h];
     __syncthreads();
     if (lane != 0) return;
 #pragma unroll
-    for (int k = 1; k < kLanes; ++k) s += part[k][q];
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int k = 1; k < kLanes; ++k) s[h] += part[k][h][q];
   }
   if (!live) return;
   const int left = static_cast<int>(least(n - col, 4));
+  if (p.bias) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (p.bias && e < left) s[e] += load_bias(p.bias, col + e, p.bias_dtype);
-    s[e] = act_value(s[e], p.activation);
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) s[h][e] += load_bias(p.bias, h * n + col + e, p.bias_dtype);
   }
-  if (p.residual) s += load4(static_cast<const T*>(p.residual) + row * p.ldr + col, left);
-  store4(static_cast<T*>(p.out) + row * p.ldo + col, s, left);
+  T* const out = static_cast<T*>(p.out) + row * p.ldo + col;
+  if constexpr (kEpi == kEpiStore || kEpi == kEpiGated) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[0][e] = act_value(s[0][e], p.activation);
+      if constexpr (kGated) s[0][e] *= s[1][e];
+    }
+    if (p.residual) s[0] += load4(static_cast<const T*>(p.residual) + row * p.ldr + col, left);
+    store4(out, s[0], left);
+  } else {
+    const f32x4 dy = load4(static_cast<const T*>(p.grad) + row * p.ldg + col, left);
+    f32x4 up;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float value, slope;
+      act_slope(s[0][e], p.activation, value, slope);
+      s[0][e] = dy[e] * slope;
+      if constexpr (kGated) {
+        s[0][e] *= s[1][e];
+        up[e] = dy[e] * value;
+      }
+    }
+    store4(out, s[0], left);
+    if constexpr (kGated) store4(out + n, up, left);
+  }
+}
+
+template <typename T, int kLanes>
+auto join_for(int epi) {
+  return epi == kEpiStore   ? join_kernel<T, kLanes, kEpiStore>
+         : epi == kEpiGated ? join_kernel<T, kLanes, kEpiGated>
+         : epi == kEpiSlope ? join_kernel<T, kLanes, kEpiSlope>
+                            : join_kernel<T, kLanes, kEpiGatedSlope>;
 }
 
 // Column sums of rows [blockIdx.y * per, ...): a thread adds up a 16-byte
@@ -313,9 +360,14 @@ struct Scratch {
   }
 };
 
-struct Matrix {
-  const void* p;
-  int64_t ld;
+// An operand of products as the caller (or this call) has it, and, once a
+// product needs it, its zero-padded copy with whole 16-byte chunks per row.
+struct Operand {
+  const void* p = nullptr;
+  int64_t ld = 0, rows = 0, width = 0;
+  int64_t zeros_from = -1;  // a padded matrix of this call's own: columns to be zeroed before they are read, or -1
+  const void* packed = nullptr;
+  int64_t packed_ld = 0;
 };
 
 // One call: the element type, the scratch and whether kernels are launched.
@@ -350,19 +402,32 @@ struct Call {
 
   int64_t padded(int64_t width) const { return ceil_div(width, per()) * per(); }
 
-  // The operand as the products read it: itself where its rows are 16-byte
-  // aligned and of whole chunks, else a zero-padded copy.
-  Matrix operand(const void* p, int64_t ld, int64_t rows, int64_t width) {
-    if (rows == 0 || width == 0 || whole_chunks(p, ld, width)) return {p, ld};
-    const int64_t out_ld = padded(width), chunks = out_ld / per();
-    void* const out = scratch.take(rows * out_ld * esize());
+  bool whole(const Operand& o) const { return o.rows == 0 || o.width == 0 || o.zeros_from >= 0 || whole_chunks(o.p, o.ld, o.width); }
+
+  // Makes `o` readable in whole chunks: as it is, with its padding zeroed, or
+  // by a copy that later products of this call use too.
+  void pack(Operand& o) {
+    if (o.packed) return;
+    o.packed = o.p;
+    o.packed_ld = o.ld;
+    if (o.zeros_from >= 0 && o.zeros_from < o.ld && go())
+      typed([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const int64_t n = o.rows * (o.ld - o.zeros_from);
+        zero_tail_kernel<T><<<static_cast<uint32_t>(ceil_div(n, 256)), 256, 0, stream>>>(
+            const_cast<T*>(static_cast<const T*>(o.p)), o.rows, o.zeros_from, o.ld);
+      });
+    if (whole(o)) return;
+    o.packed_ld = padded(o.width);
+    const int64_t chunks = o.packed_ld / per();
+    o.packed = scratch.take(o.rows * o.packed_ld * esize());
     if (go())
       typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        pack_kernel<T><<<static_cast<uint32_t>(ceil_div(rows * chunks, 256)), 256, 0, stream>>>(
-            static_cast<const T*>(p), ld, rows, width, static_cast<T*>(out), chunks);
+        pack_kernel<T><<<static_cast<uint32_t>(ceil_div(o.rows * chunks, 256)), 256, 0, stream>>>(
+            static_cast<const T*>(o.p), o.ld, o.rows, o.width, const_cast<T*>(static_cast<const T*>(o.packed)), chunks);
       });
-    return {out, out_ld};
+    if (!launch) o.packed = &o;  // sizing: only that there is one counts
   }
 
   // The tile and the number of contraction parts with the least estimated
@@ -391,7 +456,7 @@ struct Call {
     double best = 1e30;
     splits = 1;
     tile = kTileCount - 1;
-    const int most_splits = epi == kEpiStore ? std::min(256, p.k_tiles / 2) : 1;
+    const int most_splits = std::min(256, p.k_tiles / 2);
     for (int t = 0; t < kTileCount; ++t) {
       const int64_t tiles = ceil_div(p.m, kTileSize[t]) * ceil_div(columns, kTileSize[t]);
       const double rate16 = t == kTileMedium && layout != kLayoutForward ? 1.0e15 : kRate16[t];
@@ -402,7 +467,7 @@ struct Call {
         const int together = static_cast<int>(std::min<int64_t>(per_cu, kResident[t]));
         const double products = per_cu * 2.0 * kTileSize[t] * kTileSize[t] * depth / (rate * kPart[t][together - 1]);
         const double traffic = tiles * k * 2.0 * kTileSize[t] * depth * esize() / 16e12;
-        const double join = k > 1 ? 8.0 * k * p.m * p.n / 5e12 + 6e-6 : 0;
+        const double join = k > 1 ? 8.0 * k * p.m * columns / 5e12 + 6e-6 : 0;
         const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[busy][t] + join;
         if (time < best * 0.98) {
           best = time;
@@ -413,10 +478,14 @@ struct Call {
     }
   }
 
-  // sums_out: where the sums of A over the contraction go (weight layout), or the
-  // column sums of dz (slope epilogues); NULL: not wanted.
-  void product(GemmParams p, int layout, int epi, void* sums_out = nullptr, int32_t sums_dtype = 0) {
+  // One product: A [p.m or contraction rows], B, the contraction p.depth, all in
+  // true sizes.  sums_out: where the sums of A over the contraction go (weight
+  // layout), or the column sums of dz (slope epilogues); NULL: not wanted.
+  // False where they were wanted and are left to the caller.
+  bool product(GemmParams p, Operand& a, Operand& b, int layout, int epi, void* sums_out = nullptr,
+               int32_t sums_dtype = 0) {
     const bool gated = epi == kEpiGated || epi == kEpiGatedSlope;
+    const bool slope = epi == kEpiSlope || epi == kEpiGatedSlope;
     const int64_t columns = gated ? 2 * p.n : p.n;
     const int deep = static_cast<int>(128 / esize());
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
@@ -426,51 +495,78 @@ struct Call {
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileSize[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
     splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
+    const bool any = tile != kTileLarge && !(whole(a) && whole(b));
+    p.depth_b = p.depth;
+    if (any) {
+      p.a = a.p;
+      p.lda = a.ld;
+      p.b = b.p;
+      p.ldb = b.ld;
+    } else {
+      pack(a);
+      pack(b);
+      p.a = a.packed;
+      p.lda = a.packed_ld;
+      p.b = b.packed;
+      p.ldb = b.packed_ld;
+      p.a_width = padded(a.width);
+      p.b_width = padded(b.width);
+      if (layout != kLayoutWeight) p.depth = padded(p.depth);  // deep rows are read to the end of their last chunk
+      if (layout == kLayoutForward) p.depth_b = p.depth;
+    }
     const int64_t kept = scratch.used;
     // The large tile leaves the sums to a pass of their own: their few adds per
     // product cost its loop 85 us of 325 (8192 x 4096 -> 4096 bf16), the pass 20.
     if (sums_out && layout == kLayoutWeight && tile == kTileLarge) {
-      typed([&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        column_sums<T>(static_cast<const T*>(p.a), p.lda, p.depth, p.m, sums_out, sums_dtype);
-      });
+      column_sums_of(a, p.m, sums_out, sums_dtype);
       sums_out = nullptr;
     }
+    const bool sums_left = sums_out && slope && splits > 1;  // the joining launch does not sum dz
+    if (sums_left) sums_out = nullptr;
     if (sums_out) {  // the planes: of the contraction's parts, or of the tile rows
       const int64_t planes = layout == kLayoutWeight ? splits : p.tiles_m, width = layout == kLayoutWeight ? p.m : columns;
       p.sums = static_cast<float*>(scratch.take(planes * width * 4));
     }
     if (splits == 1) {
-      run(p, layout, tile, epi, 1);
+      run(p, layout, tile, any, epi, 1);
       if (sums_out && layout == kLayoutWeight) column_sums<float>(p.sums, p.m, 1, p.m, sums_out, sums_dtype);
       if (sums_out && layout == kLayoutForward) column_sums<float>(p.sums, columns, p.tiles_m, columns, sums_out, sums_dtype);
     } else {
-      const int64_t ld = ceil_div(p.n, 4) * 4;
+      const int64_t ld = ceil_div(columns, 4) * 4;
       GemmParams q = p;
+      q.n = columns;  // (a gated weight's halves side by side)
       q.out = scratch.take(splits * p.m * ld * 4);
       q.ldo = ld;
-      run(q, layout, tile, kEpiPartial, splits);
+      run(q, layout, tile, any, kEpiPartial, splits);
       if (go())
         typed([&](auto* t) {
           using T = std::remove_pointer_t<decltype(t)>;
-          const int64_t quads = p.m * (ld / 4);
+          const int64_t quads = p.m * ceil_div(p.n, 4);
           const bool lanes = splits > 8 && quads < 64 * 256 * 4;
           const int64_t blocks = ceil_div(quads, lanes ? 16 : 256), sum_blocks = sums_out ? ceil_div(p.m, 16) : 0;
-          const auto kernel = lanes ? join_kernel<T, 16> : join_kernel<T, 1>;
+          const auto kernel = lanes ? join_for<T, 16>(epi) : join_for<T, 1>(epi);
           kernel<<<static_cast<uint32_t>(blocks + sum_blocks), 256, 0, stream>>>(
-              static_cast<const float*>(q.out), splits, p.m, p.n, ld, p, static_cast<int>(blocks),
-              sums_out, sums_dtype);
+              static_cast<const float*>(q.out), splits, p.m, p.n, ld, p, static_cast<int>(blocks), sums_out, sums_dtype);
         });
     }
     most = std::max(most, scratch.used);
     scratch.used = kept;  // the next product may use it again: launches of one stream run in order
+    return !sums_left;
+  }
+
+  // Column sums of an operand's n columns.
+  void column_sums_of(const Operand& o, int64_t n, void* out, int32_t out_dtype) {
+    typed([&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      column_sums<T>(static_cast<const T*>(o.p), o.ld, o.rows, n, out, out_dtype);
+    });
   }
   int64_t most = 0;          // of scratch, over all products
 
-  void run(const GemmParams& p, int layout, int tile, int epi, int splits) {
+  void run(const GemmParams& p, int layout, int tile, bool any, int epi, int splits) {
     if (!go()) return;
     const auto f = dtype == VECTRA_DENSE_F32 ? launch_gemm_f32 : dtype == VECTRA_DENSE_F16 ? launch_gemm_f16 : launch_gemm_bf16;
-    const int st = f(p, layout, tile, epi, splits, stream);
+    const int st = f(p, layout, tile, any, epi, splits, stream);
     if (st != VECTRA_DENSE_OK) status = st;
   }
 
@@ -644,16 +740,11 @@ void forward(const vectra_dense_args& a, Call& c) {
     c.status = f(p, a.gated, c.stream);
     return;
   }
-  const Matrix x = c.operand(a.x, a.x_stride, a.rows, a.width_in);
-  const Matrix w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
+  Operand x{a.x, a.x_stride, a.rows, a.width_in}, w{a.weight, a.weight_stride, n_w, a.width_in};
   GemmParams p{};
-  p.a = x.p;
-  p.lda = x.ld;
-  p.b = w.p;
-  p.ldb = w.ld;
   p.m = a.rows;
   p.n = a.width_out;
-  p.depth = p.depth_b = c.padded(a.width_in);
+  p.depth = a.width_in;
   p.out = a.out;
   p.ldo = a.out_stride;
   p.bias = a.bias;
@@ -661,7 +752,7 @@ void forward(const vectra_dense_args& a, Call& c) {
   p.activation = a.activation;
   p.residual = a.residual;
   p.ldr = a.residual_stride;
-  c.product(p, kLayoutForward, a.gated ? kEpiGated : kEpiStore);
+  c.product(p, x, w, kLayoutForward, a.gated ? kEpiGated : kEpiStore);
 }
 
 int check_backward(const vectra_dense_grad_args* a) {
@@ -704,33 +795,30 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
   const bool want_dx = a.dx && a.rows && a.width_in, want_dw = a.dweight && n_w && a.width_in;
   const bool want_db = a.dbias && n_w;
   if (!want_dx && !want_dw && !want_db) return;
-  const bool use_x = slope || want_dw, use_w = slope || want_dx;
+  const bool use_x = slope || want_dw;
   const bool use_dz = want_dw || want_db;
-  Matrix x{nullptr, 0}, w{nullptr, 0}, dz{nullptr, 0};
-  const int64_t depth = c.padded(a.width_in);
-  const int64_t n_pad = c.padded(n_w);
   const bool any = a.rows && a.width_in && n_w;
+  Operand x{a.x, a.x_stride, a.rows, a.width_in}, w{a.weight, a.weight_stride, n_w, a.width_in};
+  Operand dz{a.grad, a.grad_stride, a.rows, n_w};
   // A layer with a slope whose weight fits LDS: dz and dx in one pass over x and grad.
   const int steps = slope && any ? c.resident_steps(a.rows, a.width_in, a.width_out, a.gated) : 0;
   const bool dx_with_dz = steps > 0 && want_dx && c.esize() == 2 && steps <= kResidentDxSteps;
-  if (use_x && any) {
-    if (a.x) {
-      x = steps > 0 && !want_dw ? Matrix{a.x, a.x_stride} : c.operand(a.x, a.x_stride, a.rows, a.width_in);
-    } else {
-      x = {c.scratch.take(a.rows * depth * c.esize()), depth};
-      if (c.go())
-        c.typed([&](auto* t) {
-          using T = std::remove_pointer_t<decltype(t)>;
-          dequantize<T>(a.codes, a.codes_stride, a.scales, a.scales_stride, a.rows, a.width_in, x.p, depth, depth, c);
-        });
-    }
+  if (use_x && any && !a.x) {
+    const int64_t ld = c.padded(a.width_in);
+    x.p = c.scratch.take(a.rows * ld * c.esize());
+    x.ld = ld;
+    x.zeros_from = ld;  // (dequantize writes the padding's zeros)
+    if (c.go())
+      c.typed([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        dequantize<T>(a.codes, a.codes_stride, a.scales, a.scales_stride, a.rows, a.width_in, x.p, ld, ld, c);
+      });
   }
-  if (use_w && any && (steps == 0 || (want_dx && !dx_with_dz)))
-    w = c.operand(a.weight, a.weight_stride, n_w, a.width_in);
   bool db_done = false;
   if (slope && a.rows && n_w && (use_dz || want_dx)) {
     const bool keep_dz = use_dz || !dx_with_dz;
-    if (keep_dz) dz = {c.scratch.take(a.rows * n_pad * c.esize()), n_pad};
+    const int64_t n_pad = c.padded(n_w);
+    if (keep_dz) dz = Operand{c.scratch.take(a.rows * n_pad * c.esize()), n_pad, a.rows, n_w, n_w};
     if (steps > 0) {
       ResidentParams p{};
       p.x = x.p;
@@ -752,13 +840,9 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       c.resident(p, steps, a.gated ? kEpiGatedSlope : kEpiSlope, dx_with_dz);
     } else {
       GemmParams p{};
-      p.a = x.p;
-      p.lda = x.ld;
-      p.b = w.p;
-      p.ldb = w.ld;
       p.m = a.rows;
       p.n = a.width_out;
-      p.depth = p.depth_b = depth;
+      p.depth = a.width_in;
       p.out = const_cast<void*>(dz.p);
       p.ldo = n_pad;
       p.bias = a.bias;
@@ -766,56 +850,31 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
       p.activation = a.activation;
       p.grad = a.grad;
       p.ldg = a.grad_stride;
-      c.product(p, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope, want_db ? a.dbias : nullptr, a.bias_dtype);
-      db_done = want_db;
+      const bool summed = c.product(p, x, w, kLayoutForward, a.gated ? kEpiGatedSlope : kEpiSlope,
+                                    want_db ? a.dbias : nullptr, a.bias_dtype);
+      db_done = want_db && summed;
     }
-    if (keep_dz && n_pad != n_w && c.go())
-      c.typed([&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        zero_tail_kernel<T><<<static_cast<uint32_t>(ceil_div(a.rows * (n_pad - n_w), 256)), 256, 0, c.stream>>>(
-            static_cast<T*>(const_cast<void*>(dz.p)), a.rows, n_w, n_pad);
-      });
-  } else if (want_dx || want_dw) {
-    dz = c.operand(a.grad, a.grad_stride, a.rows, n_w);
-  } else {
-    dz = {a.grad, a.grad_stride};
   }
   // db, where the product that made dz has not summed it: with dW where that is
   // formed too (the sums of its first operand).
-  if (want_db && !db_done && !want_dw)
-    c.typed([&](auto* t) {
-      using T = std::remove_pointer_t<decltype(t)>;
-      c.column_sums<T>(static_cast<const T*>(dz.p), dz.ld, a.rows, n_w, a.dbias, a.bias_dtype);
-    });
+  if (want_db && !db_done && !want_dw) c.column_sums_of(dz, n_w, a.dbias, a.bias_dtype);
   if (want_dx && !dx_with_dz) {
     GemmParams p{};
-    p.a = dz.p;
-    p.lda = dz.ld;
-    p.b = w.p;
-    p.ldb = w.ld;
-    p.b_width = depth;
     p.m = a.rows;
     p.n = a.width_in;
-    p.depth = n_pad;
-    p.depth_b = n_w;
+    p.depth = n_w;
     p.out = a.dx;
     p.ldo = a.dx_stride;
-    c.product(p, kLayoutInput, kEpiStore);
+    c.product(p, dz, w, kLayoutInput, kEpiStore);
   }
   if (want_dw) {
     GemmParams p{};
-    p.a = dz.p;
-    p.lda = dz.ld;
-    p.a_width = n_pad;
-    p.b = x.p;
-    p.ldb = x.ld;
-    p.b_width = depth;
     p.m = n_w;
     p.n = a.width_in;
-    p.depth = p.depth_b = a.rows;
+    p.depth = a.rows;
     p.out = a.dweight;
     p.ldo = a.dweight_stride;
-    c.product(p, kLayoutWeight, kEpiStore, want_db && !db_done ? a.dbias : nullptr, a.bias_dtype);
+    c.product(p, dz, x, kLayoutWeight, kEpiStore, want_db && !db_done ? a.dbias : nullptr, a.bias_dtype);
   }
 }
 

@@ -48,10 +48,11 @@ enum { kTileLarge = 0, kTileMedium = 1, kTileSmall = 2, kTileCount = 3 };
 constexpr int kTileSize[kTileCount] = {256, 128, 64};  // square
 
 // Launches the product with the given layout, tile and epilogue on `splits`
-// contraction parts.  One definition per element type.
-int launch_gemm_bf16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
-int launch_gemm_f16(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
-int launch_gemm_f32(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream);
+// contraction parts; `any`: operands of any alignment (not on the large tile),
+// for which depth, depth_b and the widths are the true sizes.  One definition per element type.
+int launch_gemm_bf16(const GemmParams& p, int layout, int tile, bool any, int epi, int splits, hipStream_t stream);
+int launch_gemm_f16(const GemmParams& p, int layout, int tile, bool any, int epi, int splits, hipStream_t stream);
+int launch_gemm_f32(const GemmParams& p, int layout, int tile, bool any, int epi, int splits, hipStream_t stream);
 
 // A product with a weight that stays in LDS (resident_impl.h).
 struct ResidentParams {

@@ -22,8 +22,10 @@
 // to the global address each lane loads: LDS chunk p of a row holds the row's
 // chunk p ^ f(row).  Buffer bounds turn rows past the operand into zeros;
 // chunks past the contraction's end are sent out of bounds on the last tile.
-// Operands have 16-byte aligned rows of whole chunks (others are copied into
-// the workspace first, zero padded).
+// This wants operands with 16-byte aligned rows of whole chunks.  Others are
+// copied first, zero padded, for the large tile, whose products dwarf the copy;
+// on the other tiles they pass through registers (kAny), full chunks as
+// unaligned 16-byte loads, a row's last partial chunk element by element.
 //
 // LDS reads: deep 16-bit and 32-bit operands read 16 bytes per lane.  Wide
 // 16-bit operands are read with the transposing LDS read (rbf_mfma_ops.h
@@ -40,6 +42,11 @@ namespace vectra_dense {
 
 typedef short lds_v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
+
+template <bool kFlag>
+struct Flag {
+  static constexpr bool value = kFlag;
+};
 
 template <typename T>
 struct Mma;
@@ -268,7 +275,7 @@ __device__ __forceinline__ void stage(lds_char* tile, const T* base, const uint3
 }
 
 template <typename T, int kBM_, int kBN_, int kWM_, int kWN_, bool kWideA_, bool kWideB_, int kEpi_,
-          bool kPhased_ = false>
+          bool kPhased_ = false, bool kAny_ = false>
 struct GemmConfig {
   static constexpr int kBM = kBM_, kBN = kBN_, kWM = kWM_, kWN = kWN_, kEpi = kEpi_;
   static constexpr bool kWideA = kWideA_, kWideB = kWideB_;
@@ -278,23 +285,19 @@ struct GemmConfig {
   static constexpr bool kGated = kEpi == kEpiGated || kEpi == kEpiGatedSlope;
   // The weight's gradient, and with it the bias's: where the registers have
   // room for it (the large tile has none).
-  static constexpr bool kSums = kWideA && kWideB && kTM * kTN <= 16;
+  static constexpr bool kSums = kWideA && kWideB && kTM * kTN <= 16 && (kPhased_ || kAny_);
   using A = Tile<T, kWideA, kBM, kDeep, kThreads>;
   using B = Tile<T, kWideB, kBN, kDeep, kThreads>;
   static constexpr int kStageBytes = A::kBytes + B::kBytes;
   static constexpr int kMmas = sizeof(T) == 2 ? 1 : 4;  // matrix instructions per fragment pair
   static constexpr bool kPhased = kPhased_;
+  static constexpr bool kAny = kAny_;  // operands of any alignment, staged through registers
   static constexpr bool kOpaque = kPhased && sizeof(T) == 2 && (kWideA || kWideB);
   static constexpr int kBandTiles = kTM < 4 ? kTM : 4;  // 16-row tiles per epilogue band
   static constexpr int kBandStride = kTN * 16 + 4;      // rows 16 bytes apart in the banks
   static constexpr int kBandBytes = kEpi == kEpiPartial ? 0 : kWM * kWN * kBandTiles * 16 * kBandStride * 4;
   static constexpr int kLdsBytes = 2 * kStageBytes > kBandBytes ? 2 * kStageBytes : kBandBytes;
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
-};
-
-template <bool kFlag>
-struct Flag {
-  static constexpr bool value = kFlag;
 };
 
 template <typename T, typename C>
@@ -316,6 +319,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
   const int k_last = min(k_first + p.k_tiles_per_split, p.k_tiles);
 
   // ---- per-lane load offsets (bytes from the tile's base) and base pointers
+  // (kAny: row pointers, below)
   const T* a = static_cast<const T*>(p.a);
   const T* b = static_cast<const T*>(p.b);
   uint32_t a_off[A::kSlots], b_off[B::kSlots], a_chunk[A::kSlots], b_chunk[B::kSlots];
@@ -370,6 +374,75 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
       }
     }
   }
+  // kAny: the row of each slot (deep operands: of the output dimension, fixed;
+  // wide ones: of the contraction, a tile further each time), NULL past the
+  // operand's rows, and the loads of one tile into registers.
+  const T* a_row[C::kAny ? A::kSlots : 1];
+  const T* b_row[C::kAny ? B::kSlots : 1];
+  Frag a_next[C::kAny ? A::kSlots : 1], b_next[C::kAny ? B::kSlots : 1];
+  if constexpr (C::kAny) {
+#pragma unroll
+    for (int s = 0; s < A::kSlots; ++s) {
+      int row, chunk;
+      A::slot(s, tid, row, chunk);
+      if constexpr (C::kWideA)
+        a_row[s] = static_cast<const T*>(p.a) + (static_cast<int64_t>(k_first) * C::kDeep + row) * p.lda;
+      else
+        a_row[s] = m0 + row < p.m ? static_cast<const T*>(p.a) + (m0 + row) * p.lda : nullptr;
+    }
+#pragma unroll
+    for (int s = 0; s < B::kSlots; ++s) {
+      int row, chunk;
+      B::slot(s, tid, row, chunk);
+      if constexpr (C::kWideB) {
+        b_row[s] = static_cast<const T*>(p.b) + (static_cast<int64_t>(k_first) * C::kDeep + row) * p.ldb;
+      } else if constexpr (C::kGated) {
+        constexpr int kSeg = C::kTN * 16, kHalf = kSeg / 2;
+        const int in = row % kSeg;
+        const int64_t out = n0 + row / kSeg * kHalf + in % kHalf;
+        b_row[s] = out < p.n ? static_cast<const T*>(p.b) + (out + (in >= kHalf ? p.n : 0)) * p.ldb : nullptr;
+      } else {
+        b_row[s] = n0 + row < p.n ? static_cast<const T*>(p.b) + (n0 + row) * p.ldb : nullptr;
+      }
+    }
+  }
+  const auto fetch = [&](int kt) {
+    const int64_t k0 = static_cast<int64_t>(kt) * C::kDeep;
+    const auto one = [&](auto wide, const T*& at, int row, int chunk, int64_t ld, int64_t first, int64_t width) {
+      Frag f;
+      f.w = u32x4{0, 0, 0, 0};
+      if constexpr (decltype(wide)::value) {
+        if (k0 + row < p.depth && first < width) f = load_row_chunk<T>(at, width, first);
+        at += C::kDeep * ld;
+      } else {
+        const int64_t k = k0 + chunk * A::kPer;
+        if (at && k < p.depth) f = load_row_chunk<T>(at, p.depth, k);
+      }
+      return f;
+    };
+#pragma unroll
+    for (int s = 0; s < (C::kAny ? A::kSlots : 0); ++s) {
+      int row, chunk;
+      A::slot(s, tid, row, chunk);
+      a_next[s] = one(Flag<C::kWideA>{}, a_row[s], row, chunk, p.lda, m0 + chunk * A::kPer, p.m);
+    }
+#pragma unroll
+    for (int s = 0; s < (C::kAny ? B::kSlots : 0); ++s) {
+      int row, chunk;
+      B::slot(s, tid, row, chunk);
+      b_next[s] = one(Flag<C::kWideB>{}, b_row[s], row, chunk, p.ldb, n0 + chunk * B::kPer, p.n);
+    }
+  };
+  const auto put = [&](int buf) {
+    lds_char* const at = smem + buf * C::kStageBytes;
+#pragma unroll
+    for (int s = 0; s < (C::kAny ? A::kSlots : 0); ++s)
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(at + (s * C::kThreads + tid) * 16) = a_next[s].w;
+#pragma unroll
+    for (int s = 0; s < (C::kAny ? B::kSlots : 0); ++s)
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(at + A::kBytes + (s * C::kThreads + tid) * 16) =
+          b_next[s].w;
+  };
   // (The chunks of a tile that hold contraction elements: all but on the last.)
   const int depth_chunks = static_cast<int>((p.depth + A::kPer - 1) / A::kPer);
   const auto load = [&](int kt, int buf) {
@@ -449,6 +522,25 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
       if (!with_sums)
         for (int kt = k_first; kt < k_last; ++kt) one(kt, Flag<false>{});
       wait_all();  // nothing is on its way into LDS when it is used again
+    }
+  } else if constexpr (C::kAny) {
+    // Registers hold the next tile while this one is multiplied; one barrier
+    // per tile (the buffer written is the one read two tiles ago).
+    if (k_first < k_last) fetch(k_first);
+    for (int kt = k_first; kt < k_last; ++kt) {
+      const int buf = (kt - k_first) & 1;
+      put(buf);
+      __syncthreads();
+      if (kt + 1 < k_last) fetch(kt + 1);
+#pragma unroll
+      for (int step = 0; step < C::kDeep / A::kStep; ++step) {
+        Frag fa[C::kTM], fb[C::kTN];
+        read(fa, fb, buf, step);
+        multiply(fa, fb);
+        if constexpr (C::kSums) {
+          if (p.sums && tn == 0) add_sums(fa);
+        }
+      }
     }
   } else {
     static_assert(!C::kSums);

@@ -13,7 +13,7 @@ int launch_one(const GemmParams& p, int splits, hipStream_t stream) {
 }
 
 template <typename T, bool kWideA, bool kWideB, int kEpi>
-int launch_tile(const GemmParams& p, int tile, int splits, hipStream_t stream) {
+int launch_tile(const GemmParams& p, int tile, bool any, int splits, hipStream_t stream) {
   // One or two workgroups per CU need the phased loop; so do the transposing
   // reads of wide operands at any tile (10007 x 1000 -> 5464 bf16 weight
   // gradient on medium tiles: 174 us with the plain loop, 123 phased).
@@ -25,28 +25,30 @@ int launch_tile(const GemmParams& p, int tile, int splits, hipStream_t stream) {
     case kTileLarge:
       return launch_one<T, GemmConfig<T, 256, 256, 2, 4, kWideA, kWideB, kEpi, true>>(p, splits, stream);
     case kTileMedium:
+      if (any) return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi, false, true>>(p, splits, stream);
       return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi, kWide>>(p, splits, stream);
     default:
+      if (any) return launch_one<T, GemmConfig<T, 64, 64, 2, 2, kWideA, kWideB, kEpi, false, true>>(p, splits, stream);
       return launch_one<T, GemmConfig<T, 64, 64, 2, 2, kWideA, kWideB, kEpi, kWide>>(p, splits, stream);
   }
 }
 
 template <typename T>
-int launch_gemm(const GemmParams& p, int layout, int tile, int epi, int splits, hipStream_t stream) {
+int launch_gemm(const GemmParams& p, int layout, int tile, bool any, int epi, int splits, hipStream_t stream) {
   if (layout == kLayoutForward) {
     switch (epi) {
-      case kEpiStore: return launch_tile<T, false, false, kEpiStore>(p, tile, splits, stream);
-      case kEpiPartial: return launch_tile<T, false, false, kEpiPartial>(p, tile, splits, stream);
-      case kEpiGated: return launch_tile<T, false, false, kEpiGated>(p, tile, splits, stream);
-      case kEpiSlope: return launch_tile<T, false, false, kEpiSlope>(p, tile, splits, stream);
-      default: return launch_tile<T, false, false, kEpiGatedSlope>(p, tile, splits, stream);
+      case kEpiStore: return launch_tile<T, false, false, kEpiStore>(p, tile, any, splits, stream);
+      case kEpiPartial: return launch_tile<T, false, false, kEpiPartial>(p, tile, any, splits, stream);
+      case kEpiGated: return launch_tile<T, false, false, kEpiGated>(p, tile, any, splits, stream);
+      case kEpiSlope: return launch_tile<T, false, false, kEpiSlope>(p, tile, any, splits, stream);
+      default: return launch_tile<T, false, false, kEpiGatedSlope>(p, tile, any, splits, stream);
     }
   }
   if (layout == kLayoutInput)
-    return epi == kEpiStore ? launch_tile<T, false, true, kEpiStore>(p, tile, splits, stream)
-                            : launch_tile<T, false, true, kEpiPartial>(p, tile, splits, stream);
-  return epi == kEpiStore ? launch_tile<T, true, true, kEpiStore>(p, tile, splits, stream)
-                          : launch_tile<T, true, true, kEpiPartial>(p, tile, splits, stream);
+    return epi == kEpiStore ? launch_tile<T, false, true, kEpiStore>(p, tile, any, splits, stream)
+                            : launch_tile<T, false, true, kEpiPartial>(p, tile, any, splits, stream);
+  return epi == kEpiStore ? launch_tile<T, true, true, kEpiStore>(p, tile, any, splits, stream)
+                          : launch_tile<T, true, true, kEpiPartial>(p, tile, any, splits, stream);
 }
 
 }  // namespace vectra_dense
