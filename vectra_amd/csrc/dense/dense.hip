@@ -404,6 +404,11 @@ struct Call {
 
   bool whole(const Operand& o) const { return o.rows == 0 || o.width == 0 || o.zeros_from >= 0 || whole_chunks(o.p, o.ld, o.width); }
 
+  // Estimated time of the copy that pack() would make.
+  double copy_time(const Operand& o) const {
+    return o.packed || whole(o) ? 0.0 : 4e-6 + 2.0 * o.rows * o.width * esize() / 4.5e12;
+  }
+
   // Makes `o` readable in whole chunks: as it is, with its padding zeroed, or
   // by a copy that later products of this call use too.
   void pack(Operand& o) {
@@ -431,32 +436,33 @@ struct Call {
   }
 
   // The tile and the number of contraction parts with the least estimated
-  // time.  Measured, 16 bits, 8192 x K -> 4096 (the slope over K, and what a
-  // workgroup costs besides its products, stores above all):
-  //   tile 256: 1.5 PFLOP/s and 9.5 us, one workgroup per CU (LDS)
-  //   tile 128: 1.14 PFLOP/s (1.0 with a wide operand) and 2.2 us per two
-  //   workgroups of a CU
-  //   tile 64: 0.79 PFLOP/s and 2.2 us per five
-  // and 12, 5 and 5 us where the epilogue evaluates activations.  fp32
-  // products run at 0.12 PFLOP/s on any of them.  A CU holding fewer
-  // workgroups than it could runs at a part of its rate (kPart).  The tiles'
-  // operands pass from L2 to LDS at 16 TB/s.  A split costs its fp32 planes,
-  // written and read at 5 TB/s, and the joining launch.
+  // time, and that time.  Measured, 16 bits, 8192 x K -> 4096, as a line in K:
+  //   slope      tile 256: 1.5 PFLOP/s; tile 128: 1.14 (1.0 with a wide
+  //              operand); tile 64: 0.79; fp32: 0.12 on any of them
+  //   intercept  what the epilogue moves at 4.5 TB/s, and 0.42 ps per result
+  //              where it evaluates activations; a part of it (kShown) is not
+  //              hidden behind other workgroups' products: all of it with one
+  //              workgroup per CU (tile 256, by LDS), 0.8 of it with 2 or 5
+  // A CU holding fewer workgroups than it could runs at a part of its rate
+  // (kPart).  The tiles' operands pass from L2 to LDS at 16 TB/s.  A split
+  // costs its fp32 planes, written and read at 5 TB/s, and the joining launch.
   //   chosen / other tiles, us: 8192 x 1024 -> 4096 bf16 62 on 256 (73 on 128);
   //   2051 x 2048 -> 2 x 5632 fp16 gated 97 on 128 (102 on 256); 10007 x 1000
   //   -> 2 x 2730 bf16 gated 123 on 256 (144 on 128); 300 x 1024 -> 1024 10 on
   //   64 (14 on 128); 66560 x 128 -> 256 weight gradient 18 on 64 in 64 parts
   //   (20 on 128 in 128).
-  void choose(const GemmParams& p, int64_t columns, int layout, int epi, int& tile, int& splits) const {
+  double choose(const GemmParams& p, int64_t columns, int layout, int epi, int& tile, int& splits) const {
     static constexpr double kRate16[kTileCount] = {1.5e15, 1.14e15, 0.79e15}, kRate32 = 0.12e15;
-    static constexpr double kBatch[2][kTileCount] = {{9.5e-6, 2.2e-6, 2.2e-6}, {12e-6, 5e-6, 5e-6}};
-    const bool busy = epi > kEpiPartial || p.activation != VECTRA_DENSE_NONE;
     static constexpr int kResident[kTileCount] = {1, 2, 5};
     static constexpr double kPart[kTileCount][5] = {{1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
+    static constexpr double kShown[kTileCount] = {1.0, 0.8, 0.85}, kBatch[kTileCount] = {2e-6, 0.5e-6, 0.5e-6};
+    const bool busy = epi > kEpiPartial || p.activation != VECTRA_DENSE_NONE;
+    const int moved = 1 + (p.residual || p.grad ? 1 : 0) + (epi == kEpiGatedSlope ? 1 : 0);  // values per result
+    const double finish = static_cast<double>(p.m) * p.n * (moved * esize() / 4.5e12 + (busy ? 0.42e-12 : 0));
+    const int most_splits = std::min(256, p.k_tiles / 2);
     double best = 1e30;
     splits = 1;
     tile = kTileCount - 1;
-    const int most_splits = std::min(256, p.k_tiles / 2);
     for (int t = 0; t < kTileCount; ++t) {
       const int64_t tiles = ceil_div(p.m, kTileSize[t]) * ceil_div(columns, kTileSize[t]);
       const double rate16 = t == kTileMedium && layout != kLayoutForward ? 1.0e15 : kRate16[t];
@@ -468,7 +474,7 @@ struct Call {
         const double products = per_cu * 2.0 * kTileSize[t] * kTileSize[t] * depth / (rate * kPart[t][together - 1]);
         const double traffic = tiles * k * 2.0 * kTileSize[t] * depth * esize() / 16e12;
         const double join = k > 1 ? 8.0 * k * p.m * columns / 5e12 + 6e-6 : 0;
-        const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[busy][t] + join;
+        const double time = std::max(products, traffic) + kShown[t] * finish + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
         if (time < best * 0.98) {
           best = time;
           tile = t;
@@ -476,6 +482,7 @@ struct Call {
         }
       }
     }
+    return best;
   }
 
   // One product: A [p.m or contraction rows], B, the contraction p.depth, all in
@@ -490,12 +497,15 @@ struct Call {
     const int deep = static_cast<int>(128 / esize());
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
     int tile, splits;
-    choose(p, columns, layout, epi, tile, splits);
+    const double time = choose(p, columns, layout, epi, tile, splits);
     p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileSize[tile]));
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileSize[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
     splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
-    const bool any = tile != kTileLarge && !(whole(a) && whole(b));
+    // Unaligned operands through registers run at about 0.6 of the rate
+    // (80981 x 728 -> 327 bf16 with an odd W: 136 us, 81 with W copied): that
+    // is taken where copying them would cost more.
+    const bool any = tile != kTileLarge && copy_time(a) + copy_time(b) > 0.6 * time;
     p.depth_b = p.depth;
     if (any) {
       p.a = a.p;
