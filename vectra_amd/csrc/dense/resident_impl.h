@@ -28,6 +28,12 @@
 // contraction along its rows, is read from the same LDS copy by transposing
 // reads of the same four rows per group.
 //
+// Units that are left when the others came out even over all waves are shared:
+// their pairs of output tiles go to several waves of a workgroup (66560 rows
+// are 16.25 units per CU: 256 -> 128 fp16 with a residual 18.6 -> 17.1 us).  Not
+// with dx, whose sums would have to be joined: that took registers the kernel
+// does not have (36 -> 42 us).
+//
 // Rows need no alignment: full chunks are loaded as 16 unaligned bytes, a
 // row's last partial chunk element by element.
 #pragma once
@@ -70,11 +76,22 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, i = lane & 15;
   const int64_t units = (p.rows + 15) / 16;
-  const int64_t hop = static_cast<int64_t>(gridDim.x) * kResidentWaves;
+  const int64_t hop = static_cast<int64_t>(gridDim.x) * kResidentWaves, rounds = units / hop;
   const int pairs = p.n_pad / 32;
   const T* const x = static_cast<const T*>(p.x);
 
-  for (int64_t unit = static_cast<int64_t>(wave) * gridDim.x + blockIdx.x; unit < units; unit += hop) {
+  // After the rounds of whole units, at most `last` units are left for this
+  // workgroup: `share` waves each.
+  const int last = static_cast<int>((units - rounds * hop + gridDim.x - 1) / gridDim.x);
+  int share = 1;
+  if constexpr (!C::kDx)
+    while (2 * share * last <= kResidentWaves && 2 * share <= pairs) share *= 2;
+
+  for (int64_t round = 0; round <= rounds; ++round) {
+    const int waves = round == rounds ? share : 1;
+    const int first_pair = wave % waves;
+    const int64_t unit = round * hop + static_cast<int64_t>(wave / waves) * gridDim.x + blockIdx.x;
+    if (unit >= units) break;
     const int64_t row = unit * 16 + i;
     const bool live = row < p.rows;
     const int64_t row_read = live ? row : p.rows - 1;
@@ -128,7 +145,7 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
       }
     };
 
-    for (int pair = 0; pair < pairs; ++pair) {
+    for (int pair = first_pair; pair < pairs; pair += waves) {
       const int n = pair * 32 + 8 * g;
       const int left = static_cast<int>(p.n - n);
       f32x4 za = product(pair * 32), zb = product(pair * 32 + 16);
