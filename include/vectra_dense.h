@@ -30,7 +30,7 @@
  * Contract (as vectra_rbf.h):
  *  - Plain pointers, sizes and strides; matrices are row-major with unit element
  *    stride and a row stride in ELEMENTS (codes and scales: in bytes, contiguous rows
- *    need not be adjacent).
+ *    need not be adjacent) of at least a row; that of a single row is not read.
  *  - Every buffer is owned by the caller.  Calls that need scratch memory take a
  *    workspace whose size the _workspace_bytes function tells; it needs no set-up,
  *    holds nothing between calls, and must not be shared by calls that can overlap.
@@ -99,7 +99,8 @@ typedef struct vectra_dense_args {
 typedef struct vectra_dense_grad_args {
   int64_t struct_size; /* sizeof(vectra_dense_grad_args) */
 
-  const void* x;      /* the input, or NULL where codes and scales give it in 8 bits */
+  const void* x;      /* the input, or NULL where codes and scales give it in 8 bits; neither is
+                         read, and all may be NULL, for dx and db of an ungated layer without activation */
   const void* codes;
   const void* scales;
   const void* weight;

@@ -152,6 +152,16 @@ def test_nothing_to_do_is_no_error():
     assert lib.vectra_dense_backward(ctypes.byref(args), None, 0, None) == capi.OK
 
 
+def test_an_input_that_no_gradient_reads_may_be_missing():
+    lib = _native.dense_library()
+    need = lib.vectra_dense_backward_workspace_bytes
+    plain = dict(x=None, x_stride=0, activation=capi.ACTIVATIONS['none'], bias=None)
+    assert need(ctypes.byref(grad_args(**plain, dweight=None))) >= 0
+    assert need(ctypes.byref(grad_args(**plain))) == -capi.ERR_NULL_ARGUMENT
+    plain['activation'] = capi.ACTIVATIONS['relu']
+    assert need(ctypes.byref(grad_args(**plain, dweight=None))) == -capi.ERR_NULL_ARGUMENT
+
+
 def test_row_refusals():
     lib = _native.dense_library()
 

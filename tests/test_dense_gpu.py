@@ -251,10 +251,113 @@ def test_a_nan_stays_in_its_row():
     assert torch.equal(y[rows], clean[rows]) and bool(y[17].isnan().all())
 
 
-def test_the_residual_may_be_the_output():
-    x, w = integers(65, 64, most=2, seed=1), integers(128, 64, most=2, seed=2)
-    out = integers(65, 128, most=5, seed=3)
-    want = x @ w.t() + out
+@pytest.mark.parametrize('size', [(300, 96, 100), (16400, 96, 33), (16400, 128, 72)], ids=str)
+@pytest.mark.parametrize('gated', [False, True])
+def test_an_infinity_of_the_input_stays_out_of_the_inputs_gradient(size, gated):
+    """z = +inf where x is and W > 0, and relu's slope there is 1: dx is that of
+    a large finite x, at widths that end inside a tile too.  (Gated: the up half
+    has zeros for that element, and x of -inf in the gate's place: slope 0.)"""
+    rows, width_in, width_out = size
+    for dtype in (torch.bfloat16, torch.float32):
+        x = integers(rows, width_in, most=2, seed=1, dtype=dtype)
+        w = integers(width_out, width_in, most=2, seed=2, dtype=dtype)
+        dy = integers(rows, width_out, most=3, seed=3, dtype=dtype)
+        w[:, 5] = 1
+        if gated:
+            up = integers(width_out, width_in, most=2, seed=4, dtype=dtype)
+            up[:, 5] = 0
+            w = torch.cat((w, up))
+        x[7, 5] = x[rows - 1, 5] = 30000  # z > 0 whatever the rest is, and exact in fp32
+        if gated:
+            x[7, 5] = x[rows - 1, 5] = -30000
+        wanted = [True, False, False]
+        want, = ops.linear_backward(dy, x, None, w, None, 'relu', gated, wanted)
+        x[7, 5] = x[rows - 1, 5] = float('-inf' if gated else 'inf')
+        got, = ops.linear_backward(dy, x, None, w, None, 'relu', gated, wanted)
+        live = torch.ones(rows, dtype=torch.bool)
+        if gated:  # up = ... + inf * 0 is NaN in those rows, by the formula
+            live[[7, rows - 1]] = False
+        assert torch.equal(got[live], want[live])
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_a_single_row_may_have_any_stride(dtype):
+    """Of x, dy and W: its stride is not a distance to another row."""
+    for width_in, width_out in ((64, 48), (33, 8), (4104, 264)):
+        x, dy = integers(1, width_in, most=2, seed=1, dtype=dtype), integers(1, width_out, most=3, seed=2, dtype=dtype)
+        w = integers(width_out, width_in, most=2, seed=3, dtype=dtype)
+        x0, dy0 = x.as_strided(x.shape, (0, 1)), dy.as_strided(dy.shape, (0, 1))
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        db = torch.empty(width_out, dtype=dtype, device='cuda')
+        capi.backward(dy0, x0, w, dx=dx, dweight=dw, dbias=db)
+        assert torch.equal(dx, (dy.double() @ w.double()).to(dtype))
+        assert torch.equal(dw, (dy.double().t() @ x.double()).to(dtype)) and torch.equal(db, dy[0])
+        rows = integers(70, width_in, most=2, seed=4, dtype=dtype)
+        dz, w0 = integers(70, 1, most=3, seed=5, dtype=dtype), x.as_strided(x.shape, (0, 1))
+        dx = torch.empty_like(rows)
+        capi.backward(dz, rows, w0, dx=dx)
+        assert torch.equal(dx, (dz.double() @ x.double()).to(dtype))
+
+
+def test_rows_far_apart_are_copied():
+    for dtype, stride in ((torch.bfloat16, (1 << 22) + 8), (torch.float32, (1 << 21) + 4)):
+        store = torch.zeros(stride * 40 + 64, dtype=dtype, device='cuda')
+        x = store.as_strided((40, 64), (stride, 1))
+        x.copy_(integers(40, 64, most=2, seed=1, dtype=dtype))
+        w, dy = integers(48, 64, most=2, seed=2, dtype=dtype), integers(40, 48, most=3, seed=3, dtype=dtype)
+        assert torch.equal(dense.linear(x, w), (x.double() @ w.double().t()).to(dtype))
+        dw, = ops.linear_backward(dy, x, None, w, None, 'none', False, [False, True, False])
+        assert torch.equal(dw, (dy.double().t() @ x.double()).to(dtype))
+
+
+# rows, width_in, width_out: an operand or a result of more than 2^32 bytes on
+# the products' tiles, on the kernel of resident weights, and on both sides.
+@pytest.mark.parametrize('size', [(1100007, 2048, 64), (1100007, 64, 2048), (17000003, 136, 128)], ids=str)
+def test_offsets_past_32_bits(size):
+    """Rows of zeros but for a few, the last ones among them: exact integers."""
+    rows, width_in, width_out = size
+    dtype = torch.bfloat16
+    at = torch.tensor([0, 1, rows // 2, rows - 130, rows - 2, rows - 1], device='cuda')
+    x = torch.zeros(rows, width_in, dtype=dtype, device='cuda')
+    dy = torch.zeros(rows, width_out, dtype=dtype, device='cuda')
+    x[at], dy[at] = (integers(len(at), n, most=2, seed=n, dtype=dtype) for n in (width_in, width_out))
+    w = integers(width_out, width_in, most=2, seed=3, dtype=dtype)
+    xd, wd, dyd = x[at].double(), w.double(), dy[at].double()
+    y = dense.linear(x, w, activation='relu')
+    assert torch.equal(y[at], (xd @ wd.t()).clamp_min(0).to(dtype))
+    assert int(torch.count_nonzero(y)) == int(torch.count_nonzero(y[at]))
+    del y
+    dz = dyd * (xd @ wd.t() > 0)
+    dx, dw, db = ops.linear_backward(dy, x, None, w, None, 'relu', False, [True, True, True])
+    assert torch.equal(dw, (dz.t() @ xd).to(dtype)) and torch.equal(db, dz.sum(0).to(dtype))
+    assert torch.equal(dx[at], (dz @ wd).to(dtype))
+    assert int(torch.count_nonzero(dx)) == int(torch.count_nonzero(dx[at]))
+
+
+def test_8_bit_rows_past_32_bits():
+    rows, width = 2200003, 2048  # 4.5e9 codes
+    at = torch.tensor([0, rows // 2, rows - 1], device='cuda')
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device='cuda')
+    x[at] = normal(3, width, seed=1, dtype=torch.bfloat16)
+    codes, scales = dense.quantize_rows(x)
+    want = dense.quantize_rows(x[at])
+    for got, few in zip((codes, scales), want):
+        assert torch.equal(got[at].view(torch.uint8), few.view(torch.uint8))
+    assert int(torch.count_nonzero(codes.view(torch.uint8))) == int(torch.count_nonzero(want[0].view(torch.uint8)))
+    back = dense.dequantize_rows(codes, scales, torch.bfloat16)
+    assert torch.equal(back[at], dense.dequantize_rows(*want, torch.bfloat16))
+    assert int(torch.count_nonzero(back)) == int(torch.count_nonzero(back[at]))
+
+
+# On a few rows, a small, a medium and a large tile, in parts, and by resident weights.
+@pytest.mark.parametrize('size', [(1, 300, 40), (65, 64, 128), (300, 4096, 520), (1100, 1024, 2100), (4096, 512, 4104),
+                                  (16400, 128, 100)], ids=str)
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_the_residual_may_be_the_output(size, dtype):
+    rows, width_in, width_out = size
+    x, w = integers(rows, width_in, most=2, seed=1, dtype=dtype), integers(width_out, width_in, most=2, seed=2, dtype=dtype)
+    out = integers(rows, width_out, most=5, seed=3, dtype=dtype)
+    want = (x.float() @ w.float().t() + out.float()).to(dtype)
     capi.forward(x, w, None, out, out=out)
     assert torch.equal(out, want)
 

@@ -370,6 +370,12 @@ struct Operand {
   int64_t packed_ld = 0;
 };
 
+// A caller's matrix.  One row may come with any stride, which the products'
+// bounds, (rows - 1) strides and a row, must not take for another's.
+Operand operand(const void* p, int64_t stride, int64_t rows, int64_t width) {
+  return Operand{p, rows > 1 ? stride : width, rows, width};
+}
+
 // One call: the element type, the scratch and whether kernels are launched.
 struct Call {
   int32_t dtype;
@@ -542,7 +548,9 @@ struct Call {
       if (sums_out && layout == kLayoutWeight) column_sums<float>(p.sums, p.m, 1, p.m, sums_out, sums_dtype);
       if (sums_out && layout == kLayoutForward) column_sums<float>(p.sums, columns, p.tiles_m, columns, sums_out, sums_dtype);
     } else {
-      const int64_t ld = ceil_div(columns, 4) * 4;
+      // Rows of four-column pieces; the join reads such pieces of the up half
+      // from column n on.
+      const int64_t ld = ceil_div(gated ? p.n + ceil_div(p.n, 4) * 4 : columns, 4) * 4;
       GemmParams q = p;
       q.n = columns;  // (a gated weight's halves side by side)
       q.out = scratch.take(splits * p.m * ld * 4);
@@ -674,12 +682,12 @@ int check_sizes(int64_t rows, int64_t width_in, int64_t width_out, int gated) {
   return VECTRA_DENSE_OK;
 }
 
-// A row stride covers the row, and 256 rows (a gated weight's tile: a whole
-// half and 256 rows) span less than 2^31 bytes.
+// A row stride covers the row, and 256 rows of it, or of a copy in whole chunks
+// (a gated weight's tile: a whole half and 256 rows), span less than 2^31 bytes.
 int check_stride(int64_t stride, int64_t width, int64_t rows, int64_t span_rows, int64_t esize) {
   if (rows > 1 && stride < width) return VECTRA_DENSE_ERR_BAD_SHAPE;
   if (stride < 0) return VECTRA_DENSE_ERR_BAD_SHAPE;
-  if (stride > (int64_t{1} << 40) || span_rows * std::max<int64_t>(stride, 64) * esize >= (int64_t{1} << 31))
+  if (stride > (int64_t{1} << 40) || span_rows * std::max<int64_t>({stride, width + 8, 64}) * esize >= (int64_t{1} << 31))
     return VECTRA_DENSE_ERR_TOO_LARGE;
   return VECTRA_DENSE_OK;
 }
@@ -750,7 +758,7 @@ void forward(const vectra_dense_args& a, Call& c) {
     c.status = f(p, a.gated, c.stream);
     return;
   }
-  Operand x{a.x, a.x_stride, a.rows, a.width_in}, w{a.weight, a.weight_stride, n_w, a.width_in};
+  Operand x = operand(a.x, a.x_stride, a.rows, a.width_in), w = operand(a.weight, a.weight_stride, n_w, a.width_in);
   GemmParams p{};
   p.m = a.rows;
   p.n = a.width_out;
@@ -777,13 +785,15 @@ int check_backward(const vectra_dense_grad_args* a) {
   if (int st = check_sizes(a->rows, a->width_in, a->width_out, a->gated)) return st;
   const int64_t n_w = a->width_out * (1 + a->gated);
   const bool any = a->rows && a->width_out;
+  const bool use_x = a->gated || a->activation != VECTRA_DENSE_NONE || a->dweight;
   if (any && !a->grad) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
   if (any && a->width_in) {
     if (!a->weight) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
-    if (!a->x && !(a->codes && a->scales)) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
+    if (use_x && !a->x && !(a->codes && a->scales)) return VECTRA_DENSE_ERR_NULL_ARGUMENT;
   }
   if (any) {
-    if (a->x) {
+    if (!use_x) {
+    } else if (a->x) {
       if (int st = check_stride(a->x_stride, a->width_in, a->rows, 256, es)) return st;
     } else {
       if (int st = check_stride(a->codes_stride, a->width_in, a->rows, 1, 1)) return st;
@@ -808,8 +818,8 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
   const bool use_x = slope || want_dw;
   const bool use_dz = want_dw || want_db;
   const bool any = a.rows && a.width_in && n_w;
-  Operand x{a.x, a.x_stride, a.rows, a.width_in}, w{a.weight, a.weight_stride, n_w, a.width_in};
-  Operand dz{a.grad, a.grad_stride, a.rows, n_w};
+  Operand x = operand(a.x, a.x_stride, a.rows, a.width_in), w = operand(a.weight, a.weight_stride, n_w, a.width_in);
+  Operand dz = operand(a.grad, a.grad_stride, a.rows, n_w);
   // A layer with a slope whose weight fits LDS: dz and dx in one pass over x and grad.
   const int steps = slope && any ? c.resident_steps(a.rows, a.width_in, a.width_out, a.gated) : 0;
   const bool dx_with_dz = steps > 0 && want_dx && c.esize() == 2 && steps <= kResidentDxSteps;

@@ -186,7 +186,7 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         f32x4 ga = {0.f, 0.f, 0.f, 0.f}, gb = {0.f, 0.f, 0.f, 0.f};
         if (live && left > 0)
           load8(static_cast<const T*>(p.grad) + row * p.ldg + n, left, ga, gb);
-        f32x4 da, db, ea, eb;
+        f32x4 da, db, ea = {}, eb = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float value, slope;
@@ -207,8 +207,14 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
           asm volatile("" : "+v"(da), "+v"(db));
           if constexpr (C::kGated) asm volatile("" : "+v"(ea), "+v"(eb));
         }
-        // Outputs past n have weights and biases of zero in LDS, and g = 0
-        // there: dz is zero (act' is finite at 0).
+        // Outputs past n have weights and biases of zero in LDS, so z and dz are
+        // zero there, but for an x that is not finite (inf * 0): dx adds them up.
+        if (left < 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (e >= left) da[e] = ea[e] = 0.f;
+            if (e + 4 >= left) db[e] = eb[e] = 0.f;
+          }
         gradient(pair * 32, da, db);
         if constexpr (C::kGated) gradient(p.n_pad + pair * 32, ea, eb);
         if (p.out && live && left > 0) {

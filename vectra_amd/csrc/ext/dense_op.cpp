@@ -107,8 +107,8 @@ int64_t rows_of(const Tensor& x) {
 }
 
 // A matrix the C ABI can read: rows with unit element stride, one row stride
-// of at least a row.  A view that has none (a transposed or an expanded one)
-// is copied.
+// of at least a row, 256 rows within 2^31 bytes.  A view that has none (a
+// transposed or an expanded one, or one of rows very far apart) is copied.
 struct Rows {
   Tensor t;
   int64_t stride = 0;
@@ -123,7 +123,8 @@ Rows as_rows(const Tensor& x) {
   } else {
     r.t = x.reshape({rows, width});
   }
-  if ((width > 1 && r.t.stride(1) != 1) || (rows > 1 && r.t.stride(0) < width)) r.t = r.t.contiguous();
+  const bool near = rows <= 1 || (r.t.stride(0) >= width && r.t.stride(0) < (int64_t{1} << 23) / x.element_size());
+  if ((width > 1 && r.t.stride(1) != 1) || !near) r.t = r.t.contiguous();
   r.stride = rows > 1 ? r.t.stride(0) : std::max<int64_t>(width, 1);
   return r;
 }
@@ -235,7 +236,7 @@ std::vector<Tensor> linear_backward_hip(const Tensor& grad, const Tensor& x, con
     a.scales = sr.t.data_ptr();
     a.codes_stride = xr.stride;
     a.scales_stride = sr.stride;
-  } else {
+  } else if (gated || act != VECTRA_DENSE_NONE || wanted[1]) {  // (else x's values are not read)
     xr = as_rows(x);
     a.x = xr.t.data_ptr();
     a.x_stride = xr.stride;
