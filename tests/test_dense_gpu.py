@@ -75,7 +75,8 @@ def test_integers_are_exact(size, dtype):
 # Products of many large tiles, with rows, columns and contractions that end
 # inside one: forward, dx and dW each take them at one of these.
 LARGE = [(1100, 4104, 4104), (8200, 264, 4104), (8200, 4104, 264), (2051, 1000, 2056), (4096, 4096, 1024),
-         (4090, 2056, 4090), (8190, 1543, 4090)]
+         (4090, 2056, 4090), (8190, 1543, 4090),
+         (2995, 1032, 4090), (9990, 1000, 5460)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)

@@ -443,25 +443,26 @@ struct Call {
 
   // The tile and the number of contraction parts with the least estimated
   // time, and that time.  Measured, 16 bits, 8192 x K -> 4096, as a line in K:
-  //   slope      tile 256: 1.5 PFLOP/s; tile 128: 1.14 (1.0 with a wide
-  //              operand); tile 64: 0.79; fp32: 0.12 on any of them
+  //   slope      tile 256 x 256: 1.5 PFLOP/s; 192 x 256: 1.42; 128: 1.14 (1.0 with
+  //              a wide operand); 64: 0.79; fp32: 0.12 on any of them
   //   intercept  what the epilogue moves at 4.5 TB/s, and 0.42 ps per result
   //              where it evaluates activations; a part of it (kShown) is not
   //              hidden behind other workgroups' products: all of it with one
-  //              workgroup per CU (tile 256, by LDS), 0.8 of it with 2 or 5
+  //              workgroup per CU (the big tiles, by LDS), 0.8 of it with 2 or 5
   // A CU holding fewer workgroups than it could runs at a part of its rate
   // (kPart).  The tiles' operands pass from L2 to LDS at 16 TB/s.  A split
   // costs its fp32 planes, written and read at 5 TB/s, and the joining launch.
-  //   chosen / other tiles, us: 8192 x 1024 -> 4096 bf16 62 on 256 (73 on 128);
-  //   2051 x 2048 -> 2 x 5632 fp16 gated 97 on 128 (102 on 256); 10007 x 1000
-  //   -> 2 x 2730 bf16 gated 123 on 256 (144 on 128); 300 x 1024 -> 1024 10 on
-  //   64 (14 on 128); 66560 x 128 -> 256 weight gradient 18 on 64 in 64 parts
-  //   (20 on 128 in 128).
+  //   chosen / other tiles, us: 8192 x 4096 -> 4096 bf16 200 on 256 (225 on 192,
+  //   237 on 128); 9216 x 4096 -> 4096 241 on 192 (275 on 256, whose 576 tiles
+  //   are 2.25 per CU; 272 on 128); 2051 x 2048 -> 2 x 5632 fp16 gated 84 on 192
+  //   (98 on 256, 95 on 128); dx of 10007 x 1000 -> 2 x 2730 bf16 109 on 192
+  //   (130 on 256, 154 on 128); 300 x 1024 -> 1024 10 on 64 (14 on 128);
+  //   66560 x 128 -> 256 weight gradient 18 on 64 in 64 parts (20 on 128 in 128).
   double choose(const GemmParams& p, int64_t columns, int layout, int epi, int& tile, int& splits) const {
-    static constexpr double kRate16[kTileCount] = {1.5e15, 1.14e15, 0.79e15}, kRate32 = 0.12e15;
-    static constexpr int kResident[kTileCount] = {1, 2, 5};
-    static constexpr double kPart[kTileCount][5] = {{1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
-    static constexpr double kShown[kTileCount] = {1.0, 0.8, 0.85}, kBatch[kTileCount] = {2e-6, 0.5e-6, 0.5e-6};
+    static constexpr double kRate16[kTileCount] = {1.5e15, 1.42e15, 1.14e15, 0.79e15}, kRate32 = 0.12e15;
+    static constexpr int kResident[kTileCount] = {1, 1, 2, 5};
+    static constexpr double kPart[kTileCount][5] = {{1.0}, {1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
+    static constexpr double kShown[kTileCount] = {1.0, 1.0, 0.8, 0.85}, kBatch[kTileCount] = {2e-6, 2e-6, 0.5e-6, 0.5e-6};
     const bool busy = epi > kEpiPartial || p.activation != VECTRA_DENSE_NONE;
     const int moved = 1 + (p.residual || p.grad ? 1 : 0) + (epi == kEpiGatedSlope ? 1 : 0);  // values per result
     const double finish = static_cast<double>(p.m) * p.n * (moved * esize() / 4.5e12 + (busy ? 0.42e-12 : 0));
@@ -470,15 +471,16 @@ struct Call {
     splits = 1;
     tile = kTileCount - 1;
     for (int t = 0; t < kTileCount; ++t) {
-      const int64_t tiles = ceil_div(p.m, kTileSize[t]) * ceil_div(columns, kTileSize[t]);
+      if (t == kTileTall && dtype == VECTRA_DENSE_F32) continue;
+      const int64_t tiles = ceil_div(p.m, kTileRows[t]) * ceil_div(columns, kTileColumns[t]);
       const double rate16 = t == kTileMedium && layout != kLayoutForward ? 1.0e15 : kRate16[t];
       const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : rate16) / 256;  // of a full CU
       for (int k = 1; k <= std::max(1, most_splits); k *= 2) {
         const int64_t depth = ceil_div(p.k_tiles, k) * (128 / esize());
         const int64_t per_cu = ceil_div(tiles * k, cus);
         const int together = static_cast<int>(std::min<int64_t>(per_cu, kResident[t]));
-        const double products = per_cu * 2.0 * kTileSize[t] * kTileSize[t] * depth / (rate * kPart[t][together - 1]);
-        const double traffic = tiles * k * 2.0 * kTileSize[t] * depth * esize() / 16e12;
+        const double products = per_cu * 2.0 * kTileRows[t] * kTileColumns[t] * depth / (rate * kPart[t][together - 1]);
+        const double traffic = tiles * k * static_cast<double>(kTileRows[t] + kTileColumns[t]) * depth * esize() / 16e12;
         const double join = k > 1 ? 8.0 * k * p.m * columns / 5e12 + 6e-6 : 0;
         const double time = std::max(products, traffic) + kShown[t] * finish + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
         if (time < best * 0.98) {
@@ -504,14 +506,14 @@ struct Call {
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
     int tile, splits;
     const double time = choose(p, columns, layout, epi, tile, splits);
-    p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileSize[tile]));
-    p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileSize[tile]));
+    p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileRows[tile]));
+    p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileColumns[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
     splits = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_split)));
     // Unaligned operands through registers run at about 0.6 of the rate
     // (80981 x 728 -> 327 bf16 with an odd W: 136 us, 81 with W copied): that
     // is taken where copying them would cost more.
-    const bool any = tile != kTileLarge && copy_time(a) + copy_time(b) > 0.6 * time;
+    const bool any = !kTileBig[tile] && copy_time(a) + copy_time(b) > 0.6 * time;
     p.depth_b = p.depth;
     if (any) {
       p.a = a.p;
@@ -531,9 +533,9 @@ struct Call {
       if (layout == kLayoutForward) p.depth_b = p.depth;
     }
     const int64_t kept = scratch.used;
-    // The large tile leaves the sums to a pass of their own: their few adds per
+    // The big tiles leave the sums to a pass of their own: their few adds per
     // product cost its loop 85 us of 325 (8192 x 4096 -> 4096 bf16), the pass 20.
-    if (sums_out && layout == kLayoutWeight && tile == kTileLarge) {
+    if (sums_out && layout == kLayoutWeight && kTileBig[tile]) {
       column_sums_of(a, p.m, sums_out, sums_dtype);
       sums_out = nullptr;
     }

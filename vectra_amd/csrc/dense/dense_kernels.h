@@ -36,7 +36,7 @@ struct GemmParams {
   int64_t ldg;
   // Slope epilogues: column sums of dz, fp32 [tiles_m, columns], to be added up.
   // Weight layout: sums of A over the contraction (the bias's gradient), fp32
-  // [parts, m], to be added up; NULL: not wanted (always on the large tile).
+  // [parts, m], to be added up; NULL: not wanted (always on the big tiles).
   float* sums;
   int32_t bias_dtype;
   int32_t activation;
@@ -44,11 +44,14 @@ struct GemmParams {
 
 // The shapes of one tiled product's kernels.
 enum { kLayoutForward = 0, kLayoutInput = 1, kLayoutWeight = 2 };
-enum { kTileLarge = 0, kTileMedium = 1, kTileSmall = 2, kTileCount = 3 };
-constexpr int kTileSize[kTileCount] = {256, 128, 64};  // square
+enum { kTileLarge = 0, kTileTall = 1, kTileMedium = 2, kTileSmall = 3, kTileCount = 4 };
+constexpr int kTileRows[kTileCount] = {256, 192, 128, 64}, kTileColumns[kTileCount] = {256, 256, 128, 64};
+// The small ones take operands of any alignment and sum the bias's gradient
+// beside the weight's; the tall one is for 16-bit types.
+constexpr bool kTileBig[kTileCount] = {true, true, false, false};
 
 // Launches the product with the given layout, tile and epilogue on `splits`
-// contraction parts; `any`: operands of any alignment (not on the large tile),
+// contraction parts; `any`: operands of any alignment (not on the big tiles),
 // for which depth, depth_b and the widths are the true sizes.  One definition per element type.
 int launch_gemm_bf16(const GemmParams& p, int layout, int tile, bool any, int epi, int splits, hipStream_t stream);
 int launch_gemm_f16(const GemmParams& p, int layout, int tile, bool any, int epi, int splits, hipStream_t stream);

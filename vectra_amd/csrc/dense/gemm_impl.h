@@ -23,9 +23,9 @@
 // chunk p ^ f(row).  Buffer bounds turn rows past the operand into zeros;
 // chunks past the contraction's end are sent out of bounds on the last tile.
 // This wants operands with 16-byte aligned rows of whole chunks.  Others are
-// copied first, zero padded, for the large tile, whose products dwarf the copy;
-// on the other tiles they pass through registers (kAny), full chunks as
-// unaligned 16-byte loads, a row's last partial chunk element by element.
+// copied first, zero padded, or, on the tiles of 128 and 64 rows and where the
+// copy would cost more, pass through registers (kAny): full chunks as unaligned
+// 16-byte loads, a row's last partial chunk element by element.
 //
 // LDS reads: deep 16-bit and 32-bit operands read 16 bytes per lane.  Wide
 // 16-bit operands are read with the transposing LDS read (rbf_mfma_ops.h
@@ -125,13 +125,13 @@ struct Tile {
   //  deep, 64-byte rows: four rows share a line; (r >> 2) & 3 likewise.
   //  wide, 16-bit: a transposing read takes 32-byte pieces of rows {0..3} and
   //    {8..11} (then {4..7}, {12..15}) at once: piece index ^ f, f from row
-  //    bits 0, 1 and 3 (a 128-byte row holds two of those bits by parity).
+  //    bits 0, 1 and 3 (rows of 128 or 384 bytes hold bit 0 by their address).
   //  wide, fp32: 64-byte pieces of the rows 4g + j, g = 0..3: piece ^ g.
   static __device__ __forceinline__ int swizzle(int row) {
     if constexpr (!kWide) {
       return kChunks == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
     } else if constexpr (sizeof(T) == 2) {
-      if constexpr (kRowBytes >= 256) return ((row & 3) | ((row >> 1) & 4)) << 1;
+      if constexpr (kRowBytes % 256 == 0) return ((row & 3) | ((row >> 1) & 4)) << 1;
       return (((row >> 1) & 1) | ((row >> 2) & 2)) << 1;
     } else {
       return kRowBytes >= 256 ? ((row >> 2) & 3) << 2 : ((row >> 3) & 1) << 2;
@@ -284,7 +284,7 @@ struct GemmConfig {
   static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
   static constexpr bool kGated = kEpi == kEpiGated || kEpi == kEpiGatedSlope;
   // The weight's gradient, and with it the bias's: where the registers have
-  // room for it (the large tile has none).
+  // room for it (the big tiles have none).
   static constexpr bool kSums = kWideA && kWideB && kTM * kTN <= 16 && (kPhased_ || kAny_);
   using A = Tile<T, kWideA, kBM, kDeep, kThreads>;
   using B = Tile<T, kWideB, kBN, kDeep, kThreads>;
@@ -293,7 +293,7 @@ struct GemmConfig {
   static constexpr bool kPhased = kPhased_;
   static constexpr bool kAny = kAny_;  // operands of any alignment, staged through registers
   static constexpr bool kOpaque = kPhased && sizeof(T) == 2 && (kWideA || kWideB);
-  static constexpr int kBandTiles = kTM < 4 ? kTM : 4;  // 16-row tiles per epilogue band
+  static constexpr int kBandTiles = kTM % 4 == 0 ? 4 : kTM % 3 == 0 ? 3 : kTM;  // 16-row tiles per epilogue band
   static constexpr int kBandStride = kTN * 16 + 4;      // rows 16 bytes apart in the banks
   static constexpr int kBandBytes = kEpi == kEpiPartial ? 0 : kWM * kWN * kBandTiles * 16 * kBandStride * 4;
   static constexpr int kLdsBytes = 2 * kStageBytes > kBandBytes ? 2 * kStageBytes : kBandBytes;

@@ -24,6 +24,11 @@ int launch_tile(const GemmParams& p, int tile, bool any, int splits, hipStream_t
   switch (tile) {
     case kTileLarge:
       return launch_one<T, GemmConfig<T, 256, 256, 2, 4, kWideA, kWideB, kEpi, true>>(p, splits, stream);
+    case kTileTall:
+      // (fp32 does not choose it: its rate is the same on any tile.)
+      if constexpr (sizeof(T) == 2)
+        return launch_one<T, GemmConfig<T, 192, 256, 2, 4, kWideA, kWideB, kEpi, true>>(p, splits, stream);
+      return VECTRA_DENSE_ERR_LAUNCH;
     case kTileMedium:
       if (any) return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi, false, true>>(p, splits, stream);
       return launch_one<T, GemmConfig<T, 128, 128, 2, 2, kWideA, kWideB, kEpi, kWide>>(p, splits, stream);
