@@ -45,14 +45,6 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* x, int64_t stride, i
   *reinterpret_cast<u32x4*>(out + at * kPer) = w;
 }
 
-// Zeros columns [from, stride) of a matrix.
-template <typename T>
-__global__ __launch_bounds__(256) void zero_tail_kernel(T* x, int64_t rows, int64_t from, int64_t stride) {
-  const int64_t n = stride - from;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (at < rows * n) x[at / n * stride + from + at % n] = static_cast<T>(0.f);
-}
-
 // Adds up the planes of a split product in a fixed order and finishes it with
 // the product's epilogue.  A thread adds every kLanes-th plane of four columns
 // (a gated layer: of both halves), four planes in flight; the kLanes threads of
@@ -74,7 +66,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
     float s = 0.f;
     if (at < m) {
 #pragma unroll 4
-      for (int k = lane; k < splits; k += 16) s += p.sums[k * m + at];
+      for (int k = lane; k < splits; k += 16) s += static_cast<const float*>(p.sums)[k * m + at];
     }
     sum_part[lane][c] = s;
     __syncthreads();
@@ -155,6 +147,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
     }
     store4(out, s[0], left);
     if constexpr (kGated) store4(out + n, up, left);
+    if (col + 4 >= n) zero_padding(static_cast<T*>(p.out) + row * p.ldo, n * kHalves, p.ldo);
   }
 }
 
@@ -365,7 +358,7 @@ struct Scratch {
 struct Operand {
   const void* p = nullptr;
   int64_t ld = 0, rows = 0, width = 0;
-  int64_t zeros_from = -1;  // a padded matrix of this call's own: columns to be zeroed before they are read, or -1
+  bool padded = false;  // a matrix of this call's own: rows of whole chunks, the padding zeros
   const void* packed = nullptr;
   int64_t packed_ld = 0;
 };
@@ -408,26 +401,19 @@ struct Call {
 
   int64_t padded(int64_t width) const { return ceil_div(width, per()) * per(); }
 
-  bool whole(const Operand& o) const { return o.rows == 0 || o.width == 0 || o.zeros_from >= 0 || whole_chunks(o.p, o.ld, o.width); }
+  bool whole(const Operand& o) const { return o.rows == 0 || o.width == 0 || o.padded || whole_chunks(o.p, o.ld, o.width); }
 
   // Estimated time of the copy that pack() would make.
   double copy_time(const Operand& o) const {
     return o.packed || whole(o) ? 0.0 : 4e-6 + 2.0 * o.rows * o.width * esize() / 4.5e12;
   }
 
-  // Makes `o` readable in whole chunks: as it is, with its padding zeroed, or
-  // by a copy that later products of this call use too.
+  // Makes `o` readable in whole chunks: as it is, or by a copy that later
+  // products of this call use too.
   void pack(Operand& o) {
     if (o.packed) return;
     o.packed = o.p;
     o.packed_ld = o.ld;
-    if (o.zeros_from >= 0 && o.zeros_from < o.ld && go())
-      typed([&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        const int64_t n = o.rows * (o.ld - o.zeros_from);
-        zero_tail_kernel<T><<<static_cast<uint32_t>(ceil_div(n, 256)), 256, 0, stream>>>(
-            const_cast<T*>(static_cast<const T*>(o.p)), o.rows, o.zeros_from, o.ld);
-      });
     if (whole(o)) return;
     o.packed_ld = padded(o.width);
     const int64_t chunks = o.packed_ld / per();
@@ -541,14 +527,16 @@ struct Call {
     }
     const bool sums_left = sums_out && slope && splits > 1;  // the joining launch does not sum dz
     if (sums_left) sums_out = nullptr;
-    if (sums_out) {  // the planes: of the contraction's parts, or of the tile rows
-      const int64_t planes = layout == kLayoutWeight ? splits : p.tiles_m, width = layout == kLayoutWeight ? p.m : columns;
-      p.sums = static_cast<float*>(scratch.take(planes * width * 4));
+    // The sums' planes: of the contraction's parts, or of the tile rows.
+    const int64_t planes = layout == kLayoutWeight ? splits : p.tiles_m, sum_width = layout == kLayoutWeight ? p.m : columns;
+    if (sums_out) {
+      p.sums = planes == 1 ? sums_out : scratch.take(planes * sum_width * 4);
+      p.sums_dtype = planes == 1 ? sums_dtype : VECTRA_DENSE_F32;
     }
     if (splits == 1) {
       run(p, layout, tile, any, epi, 1);
-      if (sums_out && layout == kLayoutWeight) column_sums<float>(p.sums, p.m, 1, p.m, sums_out, sums_dtype);
-      if (sums_out && layout == kLayoutForward) column_sums<float>(p.sums, columns, p.tiles_m, columns, sums_out, sums_dtype);
+      if (sums_out && planes > 1)
+        column_sums<float>(static_cast<const float*>(p.sums), sum_width, planes, sum_width, sums_out, sums_dtype);
     } else {
       // Rows of four-column pieces; the join reads such pieces of the up half
       // from column n on.
@@ -829,7 +817,7 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
     const int64_t ld = c.padded(a.width_in);
     x.p = c.scratch.take(a.rows * ld * c.esize());
     x.ld = ld;
-    x.zeros_from = ld;  // (dequantize writes the padding's zeros)
+    x.padded = true;
     if (c.go())
       c.typed([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -840,7 +828,7 @@ void backward(const vectra_dense_grad_args& a, Call& c) {
   if (slope && a.rows && n_w && (use_dz || want_dx)) {
     const bool keep_dz = use_dz || !dx_with_dz;
     const int64_t n_pad = c.padded(n_w);
-    if (keep_dz) dz = Operand{c.scratch.take(a.rows * n_pad * c.esize()), n_pad, a.rows, n_w, n_w};
+    if (keep_dz) dz = Operand{c.scratch.take(a.rows * n_pad * c.esize()), n_pad, a.rows, n_w, true};
     if (steps > 0) {
       ResidentParams p{};
       p.x = x.p;

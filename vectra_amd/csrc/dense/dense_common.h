@@ -178,6 +178,15 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int left) {
   }
 }
 
+// Zeros behind a row's `columns` elements up to its stride, at most seven: dz,
+// whose rows are padded to whole 16-byte chunks for the products that read it.
+template <typename T>
+__device__ __forceinline__ void zero_padding(T* row, int64_t columns, int64_t stride) {
+#pragma unroll
+  for (int e = 0; e < 7; ++e)
+    if (columns + e < stride) row[columns + e] = static_cast<T>(0.f);
+}
+
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int left, f32x4& a, f32x4& b) {
   if constexpr (sizeof(T) == 2) {

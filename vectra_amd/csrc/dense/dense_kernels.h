@@ -34,10 +34,12 @@ struct GemmParams {
   int64_t ldr;
   const void* grad;
   int64_t ldg;
-  // Slope epilogues: column sums of dz, fp32 [tiles_m, columns], to be added up.
-  // Weight layout: sums of A over the contraction (the bias's gradient), fp32
-  // [parts, m], to be added up; NULL: not wanted (always on the big tiles).
-  float* sums;
+  // Slope epilogues: column sums of dz, [tiles_m, columns].  Weight layout: sums
+  // of A over the contraction (the bias's gradient), [parts, m].  Several rows
+  // are fp32, to be added up; a single one is the result itself.  NULL: not
+  // wanted (always on the big tiles' weight products).
+  void* sums;
+  int32_t sums_dtype;
   int32_t bias_dtype;
   int32_t activation;
 };

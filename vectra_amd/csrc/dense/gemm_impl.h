@@ -650,6 +650,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
             T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
             store8(out, z[0], z[1], left);
             if constexpr (C::kGated) store8(out + p.n, up[0], up[1], left);
+            if (n + 8 >= p.n) zero_padding(static_cast<T*>(p.out) + m * p.ldo, p.n * (C::kGated ? 2 : 1), p.ldo);
             if constexpr (kSlope) {
               column[0] += z[0];
               column[1] += z[1];
@@ -687,7 +688,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
           float v = 0.f;
 #pragma unroll
           for (int w = 0; w < C::kWM; ++w) v += sums_lds[(w * (C::kGated ? 2 : 1) + half) * kSumCols + at % kSumCols];
-          p.sums[static_cast<int64_t>(tm) * (C::kGated ? 2 * p.n : p.n) + half * p.n + to] = v;
+          store_as(p.sums, static_cast<int64_t>(tm) * (C::kGated ? 2 * p.n : p.n) + half * p.n + to, p.sums_dtype, v);
         }
       }
     }
@@ -703,7 +704,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         const int64_t m = m0 + (wm * C::kTM + t) * 16 + i;
-        if (g == 0 && m < p.m) p.sums[static_cast<int64_t>(part) * p.m + m] = s;
+        if (g == 0 && m < p.m) store_as(p.sums, static_cast<int64_t>(part) * p.m + m, p.sums_dtype, s);
       }
     }
   }

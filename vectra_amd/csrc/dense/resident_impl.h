@@ -224,6 +224,10 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         }
       }
     }
+    if constexpr (C::kSlope) {
+      if (p.out && live && g == 0 && first_pair == 0)
+        zero_padding(static_cast<T*>(p.out) + row * p.ldo, p.n * (C::kGated ? 2 : 1), p.ldo);
+    }
     if constexpr (C::kDx) {
       if (live && p.dx) {
         T* const out = static_cast<T*>(p.dx) + row * p.lddx;
