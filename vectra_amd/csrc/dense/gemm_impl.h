@@ -599,19 +599,30 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
     constexpr bool kSlope = C::kEpi == kEpiSlope || C::kEpi == kEpiGatedSlope;
     f32x4 column[kSlope ? (C::kGated ? 4 : 2) : 1] = {};
     __syncthreads();  // all waves are done with the tiles
+    // The residual's or the gradient's rows, kAhead of them on their way.
+    constexpr int kTurns = kBandTiles * 16 / kRows;
+    constexpr int kAhead = kTurns % 2 == 0 ? 2 : 1;
+    Eight<T> ahead[kAhead];
+    const T* const beside = static_cast<const T*>(kSlope ? p.grad : C::kEpi == kEpiStore ? p.residual : nullptr);
+    const int64_t ld_beside = kSlope ? p.ldg : p.ldr;
+    const auto fetch_beside = [&](int64_t m, int slot) {
+      if (beside && m < p.m && left > 0) ahead[slot] = load_eight<T>(beside + m * ld_beside, p.n, n);
+    };
 #pragma unroll
     for (int first = 0; first < C::kTM; first += kBandTiles) {
+      const int64_t m_band = m0 + (wm * C::kTM + first) * 16 + lane / kLanes;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) fetch_beside(m_band + j * kRows, j);
 #pragma unroll
       for (int t = 0; t < kBandTiles; ++t)
 #pragma unroll
         for (int u = 0; u < C::kTN; ++u)
           *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(band + (t * 16 + i) * kStride + u * 16 + 4 * g) =
               acc[u][first + t];
-      const int64_t m_band = m0 + (wm * C::kTM + first) * 16 + lane / kLanes;
       with_activation(p.activation, [&](auto act) {
         constexpr int kAct = decltype(act)::value;
-#pragma unroll 2
-        for (int r = 0; r < kBandTiles * 16; r += kRows) {
+        // Rows r .. of the band; `near`: the residual's or the gradient's.
+        const auto finish = [&](int r, const f32x4(&near)[2], auto with) {
           const int64_t m = m_band + r;
           const __attribute__((address_space(3))) f32x4* const from =
               (const __attribute__((address_space(3))) f32x4*)(band + (r + lane / kLanes) * kStride + col);
@@ -620,31 +631,28 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
             u[0] = from[kOut / 4] + bias_up[0];
             u[1] = from[kOut / 4 + 1] + bias_up[1];
           }
-          if (m >= p.m || left <= 0) continue;
+          if (m >= p.m || left <= 0) return;
           if constexpr (C::kEpi == kEpiStore || C::kEpi == kEpiGated) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               z[e / 4][e % 4] = act_value(z[e / 4][e % 4], kAct);
               if constexpr (C::kGated) z[e / 4][e % 4] *= u[e / 4][e % 4];
             }
-            if (C::kEpi == kEpiStore && p.residual) {
-              f32x4 ra, rb;
-              load8(static_cast<const T*>(p.residual) + m * p.ldr + n, left, ra, rb);
-              z[0] += ra;
-              z[1] += rb;
+            if constexpr (decltype(with)::value) {
+              z[0] += near[0];
+              z[1] += near[1];
             }
             store8(static_cast<T*>(p.out) + m * p.ldo + n, z[0], z[1], left);
           } else {
-            f32x4 dy[2], up[2];
-            load8(static_cast<const T*>(p.grad) + m * p.ldg + n, left, dy[0], dy[1]);
+            f32x4 up[2];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               float value, slope;
               act_slope(z[e / 4][e % 4], kAct, value, slope);
-              z[e / 4][e % 4] = dy[e / 4][e % 4] * slope;
+              z[e / 4][e % 4] = near[e / 4][e % 4] * slope;
               if constexpr (C::kGated) {
                 z[e / 4][e % 4] *= u[e / 4][e % 4];
-                up[e / 4][e % 4] = dy[e / 4][e % 4] * value;
+                up[e / 4][e % 4] = near[e / 4][e % 4] * value;
               }
             }
             T* const out = static_cast<T*>(p.out) + m * p.ldo + n;
@@ -660,6 +668,27 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
               }
             }
           }
+        };
+        // (Two loops: a branch around the loads would wait for them in its own
+        // block, one loop without it costs the plain store 10%.)
+        if (kSlope || (C::kEpi == kEpiStore && beside)) {
+          if constexpr (kSlope || C::kEpi == kEpiStore) {
+#pragma unroll 1
+            for (int turn = 0; turn < kTurns; turn += kAhead) {
+#pragma unroll
+              for (int j = 0; j < kAhead; ++j) {
+                const int r = (turn + j) * kRows;
+                f32x4 near[2];
+                widen_eight(ahead[j], near[0], near[1]);
+                if (turn + kAhead < kTurns) fetch_beside(m_band + r + kAhead * kRows, j);
+                finish(r, near, Flag<true>{});
+              }
+            }
+          }
+        } else {
+          const f32x4 none[2] = {};
+#pragma unroll 2
+          for (int r = 0; r < kTurns * kRows; r += kRows) finish(r, none, Flag<false>{});
         }
       });
     }
