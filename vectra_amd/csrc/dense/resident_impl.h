@@ -126,16 +126,20 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         const uint2 hi = __builtin_bit_cast(uint2, __builtin_convertvector(b, T4));
         Frag fz;
         fz.w = u32x4{lo.x, lo.y, hi.x, hi.y};
+        // Row 4 g + i / 4, chunk (i % 4) / 2 of pair t = 0; rows are powers of
+        // two apart, so pair t is an XOR away.  Opaque: as loop invariants the
+        // addresses of all t are more than the registers hold.
+        const int r = 4 * g + i / 4;
+        int at = r * C::kRowBytes + ((((i % 4) / 2) ^ resident_swizzle<C::kChunks>(r)) * 16) + (i & 1) * 8;
+        asm volatile("" : "+v"(at));
 #pragma unroll
         for (int t = 0; t < C::kDeep / 16; ++t) {
           Frag fw;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int r = first + 16 * j + 4 * g + i / 4;
-            const int chunk = (2 * t + (i % 4) / 2) ^ resident_swizzle<C::kChunks>(4 * g + i / 4);
             const lds_v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) lds_v4s*)(const_cast<lds_char*>(w_lds) + r * C::kRowBytes +
-                                                             chunk * 16 + (i & 1) * 8));
+                (__attribute__((address_space(3))) lds_v4s*)(const_cast<lds_char*>(w_lds) + first * C::kRowBytes + (at ^ (t * 32)) +
+                                                             16 * j * C::kRowBytes));
             const uint2 u = __builtin_bit_cast(uint2, v);
             fw.w[2 * j] = u.x;
             fw.w[2 * j + 1] = u.y;
