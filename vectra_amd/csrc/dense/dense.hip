@@ -238,7 +238,8 @@ __device__ __forceinline__ f32x4 from_e4m3x4(uint32_t w) {
 // Both kernels move eight elements per thread and turn, 16 bytes of a 16-bit
 // row, and turn their work's index into a row and a column by 32-bit division
 // (Index) where the counts allow: a 64-bit one costs more than the rest of a
-// turn (66560 x 256 bf16: 16.6 us with it and four elements per thread).
+// turn (66560 x 256 bf16: 16.6 us with it and four elements per thread; now 22
+// us for both kernels, 103 MB).
 
 // Four lanes per block of 32.
 template <typename T, typename Index>
@@ -579,9 +580,8 @@ struct Call {
   }
 
   // Contraction steps of the resident kernel that serves these sizes, or 0.
-  // Its workgroups copy the whole weight first, so it needs rows enough that
-  // every CU's 8 waves have a unit of 32 rows at least (a quarter of them
-  // still pays).
+  // Its workgroups copy the whole weight first, so it needs rows enough for
+  // the 16 waves of a quarter of the CUs, a unit of 16 rows each.
   int resident_steps(int64_t rows, int64_t width, int64_t n, bool gated) const {
     if (rows < 16 * 16 * cus / 4) return 0;
     const int64_t bytes = width * esize(), n_pad = ceil_div(n, 32) * 32 * (1 + gated);

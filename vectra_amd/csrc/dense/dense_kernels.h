@@ -65,7 +65,6 @@ struct ResidentParams {
   int64_t ldx, rows, width;  // width: contraction
   const void* w;
   int64_t ldw;
-  int32_t w_wide;    // 0: W [n, width]; 1: W [width, n]
   int32_t n, n_pad;  // outputs (gated: of a half), and rounded up to 32
   const void* bias;
   int32_t bias_dtype, activation;

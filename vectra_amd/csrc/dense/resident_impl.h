@@ -13,8 +13,16 @@
 // second operand (lane l: row l % 16, 16-byte chunk l / 16 of each step), W
 // fragments come from LDS, and the result leaves in the layout it has.  While
 // some waves of a SIMD wait for rows, others evaluate activations, which is
-// what the vector units are busy with: a GELU takes about 25 issue slots of
-// four cycles per 64 elements, 10 us for 17 million elements on 256 CUs.
+// what the vector units are busy with: a GELU takes about 26 issue slots of
+// four cycles per 64 elements, 11 us for 17 million elements on 256 CUs.
+//
+// Measured, 66560 rows, 128 -> 256 bf16: forward with a GELU 21 us (51 MB; the
+// vector units are busy 78% of it, the matrix cores 10%), dz and dx 31 us;
+// gated with SiLU 22 and 49 us; 65536 rows, 141 -> 256 fp32 with a GELU 56 us
+// (matrix cores 59% busy, 31 us of work).  One unit of 16 rows per wave and 16
+// waves are the fastest of what was tried: two units per wave, or 8 and 12
+// waves with more registers each, were 5-20% slower, loads one pair ahead the
+// same.
 //
 // W's rows are stored in an order that gives a lane eight consecutive outputs
 // of its row: LDS row 32 p + 16 j + i holds output 32 p + 8 (i / 4) + 4 j + i % 4,
@@ -30,7 +38,7 @@
 //
 // Units that are left when the others came out even over all waves are shared:
 // their pairs of output tiles go to several waves of a workgroup (66560 rows
-// are 16.25 units per CU: 256 -> 128 fp16 with a residual 18.6 -> 17.1 us).  Not
+// are 16.25 units per CU: 256 -> 128 bf16 with a residual 18.6 -> 17.1 us).  Not
 // with dx, whose sums would have to be joined: that took registers the kernel
 // does not have (36 -> 42 us).
 //
@@ -255,8 +263,7 @@ __global__ __launch_bounds__(64 * kResidentWaves) void resident_kernel(const Res
   // output given above; outputs past n are zeros.
   const T* const w = static_cast<const T*>(p.w);
   for (int at = threadIdx.x; at < rows_lds * C::kChunks; at += 64 * kResidentWaves) {
-    // Neighbouring threads read neighbouring elements of either form of W.
-    const int r = p.w_wide ? at % rows_lds : at / C::kChunks, chunk = p.w_wide ? at / rows_lds : at % C::kChunks;
+    const int r = at / C::kChunks, chunk = at % C::kChunks;
     const bool up = C::kGated && r >= p.n_pad;
     const int in = up ? r - p.n_pad : r;
     const int n = (in & ~31) + 8 * ((in >> 2) & 3) + 4 * ((in >> 4) & 1) + (in & 3);
@@ -264,17 +271,7 @@ __global__ __launch_bounds__(64 * kResidentWaves) void resident_kernel(const Res
     f.w = u32x4{0, 0, 0, 0};
     if (n < p.n) {
       const int64_t w_row = n + (up ? p.n : 0);
-      if (p.w_wide) {  // contraction along W's rows: element (n, k) at k ldw + n
-        T v[C::kPer];
-#pragma unroll
-        for (int e = 0; e < C::kPer; ++e) {
-          const int64_t k = chunk * C::kPer + e;
-          v[e] = k < p.width ? w[k * p.ldw + w_row] : static_cast<T>(0.f);
-        }
-        __builtin_memcpy(&f.w, v, 16);
-      } else {
-        f = load_row_chunk<T>(w + w_row * p.ldw, p.width, chunk * C::kPer);
-      }
+      f = load_row_chunk<T>(w + w_row * p.ldw, p.width, chunk * C::kPer);
     }
     const int to = C::kPowerOfTwo ? chunk ^ resident_swizzle<C::kChunks>(r & 15) : chunk;
     *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(w_lds + r * C::kRowBytes + to * 16) = f.w;
