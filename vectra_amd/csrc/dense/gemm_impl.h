@@ -30,7 +30,7 @@
 // Measured, 8192 x 4096 -> 4096 bf16: forward 200 us, dx 205, dW 206, 1.34 to 1.37
 // PFLOP/s where the library's products reach 1.36 (in turn with them: forward
 // 1.35 against 1.55, dx 1.28 against 1.35, dW 1.26 against 1.22).  The matrix
-// cores are busy 57 to 63% of the launch: what a tile of 256 x 256 leaves idle
+// cores are busy 61 to 62% of the launch: what a tile of 256 x 256 leaves idle
 // is its first loads and its epilogue, with one workgroup per CU, and the clock
 // falls under full load.
 //
