@@ -1,4 +1,4 @@
-"""Checker of the dense operators: the layers, their gradients and the 8-bit
+"""Oracle of the dense operators: the layers, their gradients and the 8-bit
 rows from their definitions in 64 bits, and bounds on how far a computation in
 fp32 sums with stated roundings may be from them.
 
