@@ -350,6 +350,39 @@ def test_8_bit_rows_past_32_bits():
     assert int(torch.count_nonzero(back)) == int(torch.count_nonzero(back[at]))
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('size', [(0, 40, 24), (5, 0, 24), (5, 40, 0), (0, 0, 0), (0, 512, 4104), (300, 0, 600)], ids=str)
+@pytest.mark.parametrize('gated', [False, True])
+def test_empty_sizes(size, gated, dtype):
+    """No rows: gradients of the weight and the bias are zero.  No inputs: z = b."""
+    rows, width_in, width_out = size
+    n = width_out * (1 + gated)
+    x, w = integers(rows, width_in, most=2, seed=1, dtype=dtype), integers(n, width_in, most=2, seed=2, dtype=dtype)
+    b, dy = integers(n, most=3, seed=3, dtype=dtype), integers(rows, width_out, most=3, seed=4, dtype=dtype)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = dense.gated_linear(*leaves, 'relu') if gated else dense.linear(*leaves, None, 'relu')
+    got = torch.autograd.grad(y, leaves, dy)
+    z = b.double().expand(rows, n)
+    if gated:
+        gate, up = z.chunk(2, 1)
+        want_y, dz = gate.clamp_min(0) * up, torch.cat([dy * up * (gate > 0), dy * gate.clamp_min(0)], 1)
+    else:
+        want_y, dz = z.clamp_min(0), dy.double() * (z > 0)
+    assert torch.equal(y, want_y.to(dtype))
+    assert got[0].shape == x.shape and got[1].shape == w.shape
+    assert not got[0].any() and not got[1].any() and torch.equal(got[2], dz.sum(0).to(dtype))
+
+
+@pytest.mark.parametrize('checkpoint', dense.CHECKPOINTS)
+def test_a_broadcast_gradient_is_read_as_its_rows(checkpoint):
+    """y.sum() gives a gradient of stride zero, as an expanded x has."""
+    x = integers(1, 72, most=2, seed=1, dtype=torch.bfloat16).expand(130, 72).requires_grad_()
+    w = integers(40, 72, most=2, seed=2, dtype=torch.bfloat16).requires_grad_()
+    dx, dw = torch.autograd.grad(dense.linear(x, w, checkpoint=checkpoint).sum(), (x, w))
+    assert torch.equal(dx, w.double().sum(0).to(dx.dtype).expand(130, 72))
+    assert torch.equal(dw, (130 * x[0].double()).to(dw.dtype).expand(40, 72))
+
+
 # On a few rows, a small, a medium and a large tile, in parts, and by resident weights.
 @pytest.mark.parametrize('size', [(1, 300, 40), (65, 64, 128), (300, 4096, 520), (1100, 1024, 2100), (4096, 512, 4104),
                                   (16400, 128, 100)], ids=str)
