@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const FewRowsP
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    z[e] = act_value(z[e], p.activation);
+    z[e] = act_value<T>(z[e], p.activation);
     if constexpr (kGated) z[e] *= u[e];
   }
   if (!kGated && p.residual) z += load4(static_cast<const T*>(p.residual) + m * p.ldr + n, left);

@@ -13,8 +13,8 @@
 // second operand (lane l: row l % 16, 16-byte chunk l / 16 of each step), W
 // fragments come from LDS, and the result leaves in the layout it has.  While
 // some waves of a SIMD wait for rows, others evaluate activations, which is
-// what the vector units are busy with: a GELU takes about 26 issue slots of
-// four cycles per 64 elements, 11 us for 17 million elements on 256 CUs.
+// what the vector units are busy with: a GELU takes about 24 issue slots of
+// four cycles per 64 elements, 10 us for 17 million elements on 256 CUs.
 //
 // Measured, 66560 rows, 128 -> 256 bf16: forward with a GELU 21 us (51 MB; the
 // vector units are busy 78% of it, the matrix cores 10%), dz and dx 34 us;
@@ -178,8 +178,8 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
         f32x4 ya, yb;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          ya[e] = act_value(za[e], kAct);
-          yb[e] = act_value(zb[e], kAct);
+          ya[e] = act_value<T>(za[e], kAct);
+          yb[e] = act_value<T>(zb[e], kAct);
           if constexpr (C::kGated) {
             ya[e] *= ua[e];
             yb[e] *= ub[e];
@@ -202,13 +202,13 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float value, slope;
-          act_slope(za[e], kAct, value, slope);
+          act_slope<T>(za[e], kAct, value, slope);
           da[e] = ga[e] * slope;
           if constexpr (C::kGated) {
             da[e] *= ua[e];
             ea[e] = ga[e] * value;
           }
-          act_slope(zb[e], kAct, value, slope);
+          act_slope<T>(zb[e], kAct, value, slope);
           db[e] = gb[e] * slope;
           if constexpr (C::kGated) {
             db[e] *= ub[e];
