@@ -525,6 +525,16 @@ class Layer : public torch::autograd::Function<Layer> {
   }
 };
 
+// The layers have no forward-mode derivative: below autograd a tangent would be
+// dropped without a word.
+void refuse_tangents(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                     const char* op) {
+  const auto dual = [](const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(!dual(x) && !dual(weight) && !(has(bias) && dual(*bias)) &&
+                                  !(has(residual) && dual(*residual)),
+                              op, ": forward-mode derivatives are not supported (an argument carries a tangent)");
+}
+
 bool any_requires_grad(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual) {
   return at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() ||
                                         (has(bias) && bias->requires_grad()) ||
@@ -533,6 +543,7 @@ bool any_requires_grad(const Tensor& x, const Tensor& weight, const OptTensor& b
 
 Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                        c10::string_view activation, c10::string_view checkpoint) {
+  refuse_tangents(x, weight, bias, residual, "vectra::linear");
   if (!any_requires_grad(x, weight, bias, residual)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_linear(x, weight, bias, residual, activation, checkpoint);
@@ -542,6 +553,7 @@ Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& b
 
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, c10::string_view activation,
                              c10::string_view checkpoint) {
+  refuse_tangents(x, weight, bias, std::nullopt, "vectra::gated_linear");
   if (!any_requires_grad(x, weight, bias, std::nullopt)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_gated(x, weight, bias, activation, checkpoint);

@@ -29,7 +29,8 @@ code; codes are float8_e4m3fn [..., width], scales float8_e8m0fnu
 dz, the gradient before the layer's products, is rounded once to x's type (a
 16-bit matrix product reads 16-bit operands); dx = dz @ weight and dW = dz.T @ x
 are formed from that in fp32 sums, db = dz.sum(0) from dz before or after that
-rounding.  Gradients of gradients are refused.
+rounding.  Gradients of gradients and forward-mode derivatives (an argument
+that carries a tangent) are refused.
 
 A backward pass may be captured into a HIP graph through
 torch.ops.vectra.linear_backward, which autograd calls.  (Capturing
