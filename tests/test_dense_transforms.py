@@ -1,5 +1,5 @@
-"""What the dense operators do under forward-mode differentiation: nothing that
-drops a derivative without a word."""
+"""The dense operators where they have no derivative (forward mode, through the
+8-bit rows, a second time): an error, never a derivative that is dropped."""
 
 import pytest
 import torch
@@ -73,3 +73,39 @@ def test_jvp_of_the_price_model_is_that_of_its_plain_layers_or_refused():
     model.set_dense_kernels()
     with pytest.raises(NotImplementedError, match='forward-mode'):
         torch.func.jvp(price, (inputs[0],), tangents)
+
+
+# The operators without a derivative, as a function of one tensor.
+def eight_bits(x):
+    return dense.dequantize_rows(*dense.quantize_rows(x), torch.float32)
+
+
+def second(x):
+    w = randn(4, 8, seed=2, device=x.device)
+    dy = randn(3, 4, seed=3, device=x.device)
+    return torch.ops.vectra.linear_backward(dy, x, None, w, None, 'gelu', False, [True, False, False])[0]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('f', [eight_bits, second])
+def test_a_gradient_through_an_operator_without_one_is_refused(f, device):
+    x = randn(3, 8, seed=1, device=device)
+    want = f(x)
+    leaf = x.clone().requires_grad_()
+    y = f(leaf)
+    assert torch.equal(y, want) and y.requires_grad
+    with pytest.raises(RuntimeError, match='not implemented'):
+        torch.autograd.grad((y * leaf).sum(), leaf)
+    with torch.no_grad():
+        assert not f(leaf).requires_grad
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match='forward AD'):
+        f(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+def test_8_bit_rows_are_well_formed_where_a_gradient_is_asked_for():
+    x = randn(3, 40, seed=1).requires_grad_()
+    torch.library.opcheck(torch.ops.vectra.quantize_rows.default, (x,),
+                          test_utils=('test_schema', 'test_faketensor', 'test_autograd_registration'))
+    codes, scales = dense.quantize_rows(x.detach())
+    torch.library.opcheck(torch.ops.vectra.dequantize_rows.default, (codes, scales, torch.float32),
+                          test_utils=('test_faketensor',))

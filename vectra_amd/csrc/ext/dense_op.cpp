@@ -8,8 +8,9 @@
 //                                      on the caller's current HIP stream, with
 //                                      scratch memory from torch's allocator
 //   CPU key                         -> the same formulas in fp32 tensors
-//   Autograd key                    -> saves the input (or its 8-bit form), calls
-//                                      linear_backward
+//   Autograd key                    -> the layers: saves the input (or its 8-bit
+//                                      form), calls linear_backward; the others:
+//                                      no derivative, refused
 //   fake/meta                       -> registered from Python
 // There is no CPU fallback for device tensors: if the HIP library cannot be
 // loaded this extension does not load either.
@@ -18,6 +19,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -596,4 +598,9 @@ TORCH_LIBRARY_IMPL(vectra, CPU, m) {
 TORCH_LIBRARY_IMPL(vectra, Autograd, m) {
   m.impl("linear", linear_autograd);
   m.impl("gated_linear", gated_linear_autograd);
+  // No derivatives: a backward pass that reaches one of these raises, and so
+  // does a tangent.
+  m.impl("linear_backward", torch::autograd::autogradNotImplementedFallback());
+  m.impl("quantize_rows", torch::autograd::autogradNotImplementedFallback());
+  m.impl("dequantize_rows", torch::autograd::autogradNotImplementedFallback());
 }

@@ -17,7 +17,9 @@ copied), bias in that type or float32.  activation is 'none', 'relu', 'gelu'
 (the exact one), 'gelu_tanh' or 'silu'.  Products are accumulated in fp32 and
 the result is rounded once.
 
-Both layers have gradients for every tensor argument.  Nothing but their inputs
+Both layers have gradients for every tensor argument; the 8-bit rows and
+linear_backward have none, and a backward pass through them raises (quantise
+x.detach(), or under no_grad, what is kept beside a graph).  Nothing but their inputs
 is kept for the backward pass: the pre-activation is computed again.  With
 ``checkpoint='e4m3'`` the input too is given up: its 8-bit form is kept (33
 bytes for 32 elements), and the gradients are those of the layer at the values
