@@ -443,7 +443,11 @@ struct Call {
   //   (98 on 256, 95 on 128); dx of 10007 x 1000 -> 2 x 2730 bf16 109 on 192
   //   (130 on 256, 154 on 128); 300 x 1024 -> 1024 10 on 64 (14 on 128);
   //   66560 x 128 -> 256 weight gradient 18 on 64 in 64 parts (20 on 128 in 128).
-  double choose(const GemmParams& p, int64_t columns, int layout, int epi, int& tile, int& splits) const {
+  //
+  // a_row_bytes: of a deep row operand, whose tile the kernels address with 31
+  // bits (dz of a gated layer in fp32 has rows of up to 16 MB, twice those of
+  // the gradient that the caller's stride was checked for); 0 for a wide one.
+  double choose(const GemmParams& p, int64_t columns, int layout, int epi, int64_t a_row_bytes, int& tile, int& splits) const {
     static constexpr double kRate16[kTileCount] = {1.5e15, 1.42e15, 1.14e15, 0.79e15}, kRate32 = 0.12e15;
     static constexpr int kResident[kTileCount] = {1, 1, 2, 5};
     static constexpr double kPart[kTileCount][5] = {{1.0}, {1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
@@ -457,6 +461,7 @@ struct Call {
     tile = kTileCount - 1;
     for (int t = 0; t < kTileCount; ++t) {
       if (t == kTileTall && dtype == VECTRA_DENSE_F32) continue;
+      if (kTileRows[t] * a_row_bytes >= int64_t{1} << 31) continue;  // (the small tile's 64 rows always fit)
       const int64_t tiles = ceil_div(p.m, kTileRows[t]) * ceil_div(columns, kTileColumns[t]);
       const double rate16 = t == kTileMedium && layout != kLayoutForward ? 1.0e15 : kRate16[t];
       const double rate = (dtype == VECTRA_DENSE_F32 ? kRate32 : rate16) / 256;  // of a full CU
@@ -490,7 +495,8 @@ struct Call {
     const int deep = static_cast<int>(128 / esize());
     p.k_tiles = static_cast<int32_t>(ceil_div(p.depth, deep));
     int tile, splits;
-    const double time = choose(p, columns, layout, epi, tile, splits);
+    const int64_t a_row_bytes = layout == kLayoutWeight ? 0 : std::max(a.ld, padded(a.width)) * esize();
+    const double time = choose(p, columns, layout, epi, a_row_bytes, tile, splits);
     p.tiles_m = static_cast<int32_t>(ceil_div(p.m, kTileRows[tile]));
     p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTileColumns[tile]));
     p.k_tiles_per_split = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, splits)));
@@ -660,7 +666,8 @@ constexpr int64_t kMostWidth = int64_t{1} << 21;
 
 bool known_dtype(int32_t t) { return t == VECTRA_DENSE_F32 || t == VECTRA_DENSE_F16 || t == VECTRA_DENSE_BF16; }
 
-// Sizes that the kernels' 32-bit offsets within a tile and their grids cover.
+// Sizes that the kernels' grids cover (offsets within a tile: check_stride, and
+// for dz of a gated layer Call::choose).
 int check_sizes(int64_t rows, int64_t width_in, int64_t width_out, int gated) {
   if (rows < 0 || width_in < 0 || width_out < 0) return VECTRA_DENSE_ERR_BAD_SHAPE;
   if (rows > kMostRows || width_in > kMostWidth || width_out > kMostWidth) return VECTRA_DENSE_ERR_TOO_LARGE;
