@@ -1,13 +1,98 @@
-"""The dense operators' kernels for large sizes: rows whose tile spans more than
-2^31 bytes."""
+"""The dense operators' kernels for many rows and for large tiles: ordinary
+values against the 64-bit oracle with every activation, results that do not
+depend on the run, and rows whose tile spans more than 2^31 bytes.
+
+The 64-bit side runs on the GPU (matrix products of doubles).
+"""
 
 import pytest
 import torch
 
-from vectra_amd.kernels import dense  # noqa: F401  (registers the operators)
+from oracle import dense as oracle
+from vectra_amd.kernels import dense
 
 pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 ops = torch.ops.vectra
+
+
+def normal(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    return (torch.randn(*shape, generator=gen, device='cuda') * scale).to(dtype)
+
+
+def within(got, want, bound, name):
+    off = (got.detach().double() - want).abs()
+    bad = ~(off <= bound)
+    assert not bool(bad.any()), (
+        f'{name}: {int(bad.sum())} of {bad.numel()} outside; worst {float((off / bound).max()):.3g} times the bound, '
+        f'first at {torch.nonzero(bad)[0].tolist()}')
+
+
+def arguments(rows, width_in, width_out, dtype, gated, bias_dtype=None):
+    n = width_out * (1 + gated)
+    return dict(x=normal(rows, width_in, seed=1, dtype=dtype).requires_grad_(),
+                w=normal(n, width_in, seed=2, scale=width_in ** -0.5, dtype=dtype).requires_grad_(),
+                b=normal(n, seed=3, scale=0.2, dtype=bias_dtype or dtype).requires_grad_(),
+                r=None if gated else normal(rows, width_out, seed=4, dtype=dtype),
+                dy=normal(rows, width_out, seed=5, dtype=dtype))
+
+
+def call(t, activation, gated, checkpoint='none'):
+    if gated:
+        return dense.gated_linear(t['x'], t['w'], t['b'], activation, checkpoint)
+    return dense.linear(t['x'], t['w'], t['b'], t['r'], activation, checkpoint)
+
+
+def check(t, activation, gated):
+    y = call(t, activation, gated)
+    grads = torch.autograd.grad(y, (t['x'], t['w'], t['b']), t['dy'])
+    wide = [None if t[k] is None else t[k].detach().double() for k in ('x', 'w', 'b', 'r')]
+    layer = oracle.Layer(*wide, activation, gated)
+    dtype = t['x'].dtype
+    within(y, *layer.forward(dtype), 'y')
+    # (The oracle's own backward() brings the gradient to the CPU.)
+    on_host = oracle.Layer(*[None if v is None else v.cpu() for v in wide], activation, gated)
+    for g, (name, (want, bound)) in zip(grads, on_host.backward(t['dy'], dtype, t['b'].dtype).items()):
+        within(g, want.cuda(), bound.cuda(), name)
+
+
+SMOOTH = ['gelu', 'gelu_tanh', 'silu']
+
+
+# Many rows by a weight that stays in LDS: contractions of every length that
+# such a kernel exists for, widths inside and at the end of a tile, a last unit
+# of 16 rows that is short, rows that leave waves unequal.
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('activation', SMOOTH)
+@pytest.mark.parametrize('gated', [False, True])
+@pytest.mark.parametrize('size', [(16391, 60, 70), (16640, 128, 256), (16400, 141, 100), (17003, 250, 128)], ids=str)
+def test_many_rows_stay_in_their_bounds(size, gated, activation, dtype):
+    t = arguments(*size, dtype, gated, torch.float32 if activation == 'gelu' else dtype)
+    check(t, activation, gated)
+
+
+# Tiles of 256 and 192 rows in the forward product, dx and dW, whole and not.
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('gated,activation', [(False, a) for a in SMOOTH] + [(True, a) for a in SMOOTH])
+@pytest.mark.parametrize('size', [(2048, 1024, 4096), (2051, 1000, 4090)], ids=str)
+def test_large_tiles_stay_in_their_bounds(size, gated, activation, dtype):
+    t = arguments(*size, dtype, gated, torch.float32 if activation == 'gelu' else dtype)
+    check(t, activation, gated)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('gated', [False, True])
+@pytest.mark.parametrize('checkpoint', dense.CHECKPOINTS)
+@pytest.mark.parametrize('size', [(16640, 128, 256), (3001, 1000, 2730), (300, 2048, 520), (40, 512, 96)], ids=str)
+def test_a_step_gives_the_same_bits_every_time(size, checkpoint, gated, dtype):
+    t = arguments(*size, dtype, gated)
+    first = None
+    for _ in range(4):
+        y = call(t, 'silu', gated, checkpoint)
+        now = (y.detach(), *torch.autograd.grad(y, (t['x'], t['w'], t['b']), t['dy']))
+        first = first or now
+        assert all(torch.equal(a, c) for a, c in zip(first, now))
 
 
 def test_gated_gradients_whose_tile_spans_more_than_31_bits():
