@@ -11,11 +11,14 @@
 //   Autograd key                    -> the layers: saves the input (or its 8-bit
 //                                      form), calls linear_backward; the others:
 //                                      no derivative, refused
+//   Autocast keys                   -> the layers in autocast's type, as
+//                                      torch's own linear layers are
 //   fake/meta                       -> registered from Python
 // There is no CPU fallback for device tensors: if the HIP library cannot be
 // loaded this extension does not load either.
 
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -66,6 +69,12 @@ bool eight_bit(std::string_view checkpoint, const char* op) {
   return checkpoint == "e4m3";
 }
 
+void check_residual_shape(const Tensor& x, const Tensor& weight, const Tensor& residual, const char* op) {
+  bool same = residual.dim() == x.dim() && residual.size(-1) == weight.size(0);
+  for (int64_t d = 0; same && d + 1 < x.dim(); ++d) same = residual.size(d) == x.size(d);
+  TORCH_CHECK(same, op, ": residual must have the output's shape; got ", residual.sizes());
+}
+
 void check_layer(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, bool gated,
                  const char* op) {
   TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2, op, ": x must be [..., width_in] and weight [width, width_in]; got ",
@@ -86,9 +95,7 @@ void check_layer(const Tensor& x, const Tensor& weight, const OptTensor& bias, c
     TORCH_CHECK(bias->device() == x.device(), op, ": bias must be on ", x.device(), "; got ", bias->device());
   }
   if (has(residual)) {
-    bool same = residual->dim() == x.dim() && residual->size(-1) == weight.size(0);
-    for (int64_t d = 0; same && d + 1 < x.dim(); ++d) same = residual->size(d) == x.size(d);
-    TORCH_CHECK(same, op, ": residual must have the output's shape; got ", residual->sizes());
+    check_residual_shape(x, weight, *residual, op);
     TORCH_CHECK(residual->scalar_type() == x.scalar_type(), op, ": residual must have x's dtype; got ",
                 residual->scalar_type());
     TORCH_CHECK(residual->device() == x.device(), op, ": residual must be on ", x.device(), "; got ",
@@ -563,6 +570,44 @@ Tensor gated_linear_autograd(const Tensor& x, const Tensor& weight, const OptTen
   return Layer::apply(x, weight, bias, std::nullopt, std::string(activation), std::string(checkpoint), true);
 }
 
+// ---------------------------------------------------------------- autocast
+//
+// x and weight in autocast's type.  A bias of fp32 stays as it is: it joins the
+// product's fp32 sums.  So does a residual of another type, the fp32 stream that
+// blocks under autocast add their 16-bit branches to: it is added to the layer's
+// output by torch's own rules, and the result has the wider type.
+
+Tensor cast_to(at::ScalarType type, const Tensor& t, c10::DeviceType device) {
+  return at::autocast::cached_cast(type, t, device);
+}
+
+OptTensor cast_bias(at::ScalarType type, const OptTensor& bias, c10::DeviceType device) {
+  return has(bias) && bias->scalar_type() != at::kFloat ? OptTensor(cast_to(type, *bias, device)) : bias;
+}
+
+template <c10::DeviceType kDevice, c10::DispatchKey kKey>
+Tensor linear_autocast(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                       c10::string_view activation, c10::string_view checkpoint) {
+  c10::impl::ExcludeDispatchKeyGuard no_autocast(kKey);
+  const at::ScalarType type = at::autocast::get_autocast_dtype(kDevice);
+  const Tensor xc = cast_to(type, x, kDevice), wc = cast_to(type, weight, kDevice);
+  const OptTensor bc = cast_bias(type, bias, kDevice);
+  if (!has(residual) || residual->scalar_type() == xc.scalar_type())
+    return call_linear(xc, wc, bc, residual, activation, checkpoint);
+  const Tensor y = call_linear(xc, wc, bc, std::nullopt, activation, checkpoint);
+  check_residual_shape(x, weight, *residual, "vectra::linear");
+  return at::add(*residual, y);
+}
+
+template <c10::DeviceType kDevice, c10::DispatchKey kKey>
+Tensor gated_linear_autocast(const Tensor& x, const Tensor& weight, const OptTensor& bias, c10::string_view activation,
+                             c10::string_view checkpoint) {
+  c10::impl::ExcludeDispatchKeyGuard no_autocast(kKey);
+  const at::ScalarType type = at::autocast::get_autocast_dtype(kDevice);
+  return call_gated(cast_to(type, x, kDevice), cast_to(type, weight, kDevice), cast_bias(type, bias, kDevice), activation,
+                    checkpoint);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(vectra, m) {
@@ -603,4 +648,15 @@ TORCH_LIBRARY_IMPL(vectra, Autograd, m) {
   m.impl("linear_backward", torch::autograd::autogradNotImplementedFallback());
   m.impl("quantize_rows", torch::autograd::autogradNotImplementedFallback());
   m.impl("dequantize_rows", torch::autograd::autogradNotImplementedFallback());
+}
+
+// (Autocast is the key of GPU tensors.)
+TORCH_LIBRARY_IMPL(vectra, Autocast, m) {
+  m.impl("linear", TORCH_FN((linear_autocast<at::kCUDA, c10::DispatchKey::Autocast>)));
+  m.impl("gated_linear", TORCH_FN((gated_linear_autocast<at::kCUDA, c10::DispatchKey::Autocast>)));
+}
+
+TORCH_LIBRARY_IMPL(vectra, AutocastCPU, m) {
+  m.impl("linear", TORCH_FN((linear_autocast<at::kCPU, c10::DispatchKey::AutocastCPU>)));
+  m.impl("gated_linear", TORCH_FN((gated_linear_autocast<at::kCPU, c10::DispatchKey::AutocastCPU>)));
 }

@@ -17,6 +17,10 @@ copied), bias in that type or float32.  activation is 'none', 'relu', 'gelu'
 (the exact one), 'gelu_tanh' or 'silu'.  Products are accumulated in fp32 and
 the result is rounded once.
 
+Under torch.autocast the layers run in autocast's type, as torch's own linear
+layers do; a float32 bias stays float32, and a residual of another type is added
+to the layer's output by torch's rules (a float32 residual stream stays one).
+
 Both layers have gradients for every tensor argument; the 8-bit rows and
 linear_backward have none, and a backward pass through them raises (quantise
 x.detach(), or under no_grad, what is kept beside a graph).  Nothing but their inputs
