@@ -1,0 +1,149 @@
+"""set_dense_kernels beside what users put on a model's layers: hooks, wrappers
+and replacements run as they do on the plain model (host only)."""
+
+import copy
+
+import pytest
+import torch
+from torch import nn
+
+from vectra_amd.price_transformer import model as model_lib
+from vectra_amd.price_transformer import plain_modules
+
+
+def build(gate=False):
+    torch.manual_seed(0)
+    config = model_lib.ModelConfig(d_model=32, num_heads=2, num_layers=2, ffn_dim=48, num_candidates=6,
+                                   embedding_dim=8, attribute_dim=3, ffn_gate=gate)
+    model = model_lib.PriceTransformer(config).eval()
+    return model, model_lib.example_inputs(config, 3, 'cpu', seed=1)
+
+
+def relative(a, b):
+    return float((a - b).norm() / b.norm())
+
+
+def calls(model, inputs, register):
+    """Names of the modules whose hook ran, in order, and the output."""
+    seen = []
+    handles = [getattr(m, register)(lambda *args, name=name: seen.append(name)) for name, m in model.named_modules()]
+    out = model(*inputs)
+    if 'backward' in register:
+        out.sum().backward()
+    for h in handles:
+        h.remove()
+    return seen, out.detach()
+
+
+@pytest.mark.parametrize('gate', [False, True])
+@pytest.mark.parametrize('register', ['register_forward_hook', 'register_forward_pre_hook',
+                                      'register_full_backward_hook', 'register_full_backward_pre_hook'])
+def test_every_hook_runs_as_on_the_plain_model(register, gate):
+    model, inputs = build(gate)
+    want, want_y = calls(model, inputs, register)
+    got, y = calls(copy.deepcopy(model).set_dense_kernels(), inputs, register)
+    assert got == want and len(want) > 20
+    assert relative(y, want_y) < 1e-5
+
+
+@pytest.mark.parametrize('gate', [False, True])
+def test_a_hook_may_change_what_a_layer_gives(gate):
+    model, inputs = build(gate)
+    names = [name for name, m in model.named_modules() if name and not isinstance(m, nn.ModuleList)]
+    for name in names:
+        pair = [copy.deepcopy(model), copy.deepcopy(model).set_dense_kernels()]
+        for m in pair:
+            m.get_submodule(name).register_forward_hook(lambda module, args, out: out * 1.5)
+        with torch.no_grad():
+            want, got = (m(*inputs) for m in pair)
+            assert not torch.equal(want, model(*inputs)), name
+        assert relative(got, want) < 1e-5, name
+
+
+def test_a_global_hook_sees_every_layer():
+    model, inputs = build()
+    seen = {}
+    for kind in ('plain', 'dense'):
+        m = copy.deepcopy(model).set_dense_kernels(kind == 'dense')
+        handle = torch.nn.modules.module.register_module_forward_hook(
+            lambda module, args, out, kind=kind: seen.setdefault(kind, []).append(type(module).__name__))
+        m(*inputs)
+        handle.remove()
+    assert seen['plain'] == seen['dense'] and 'Linear' in seen['plain']
+
+
+class LowRank(nn.Linear):
+    """A fine-tuning layer: its forward is not that of its weight alone."""
+
+    def forward(self, x):
+        return super().forward(x) + 0.3 * x.roll(1, -1) @ self.weight.t()
+
+
+class Wrapped(nn.Module):
+    """A layer without a weight of its own."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, *args, **kwargs):
+        return 2.0 * self.inner(*args, **kwargs)
+
+
+def low_rank(m):
+    new = LowRank(m.in_features, m.out_features)
+    new.load_state_dict(m.state_dict())
+    return new
+
+
+def patched(m):
+    before = m.forward
+    m.forward = lambda *args, **kwargs: 2.0 * before(*args, **kwargs)
+    return m
+
+
+def parametrised(m):
+    return nn.utils.parametrizations.weight_norm(m)
+
+
+LAYERS = ['query_encoder.mlp.0', 'candidate_encoder.mlp.2', 'blocks.0.attention.qkv', 'blocks.1.attention.out',
+          'blocks.0.ffn.0', 'blocks.1.ffn.2']
+OTHERS = ['query_encoder.mlp', 'blocks.0.ffn', 'blocks.0.ffn.1', 'blocks.1.attention']
+
+
+@pytest.mark.parametrize('name,change', [(n, c) for n in LAYERS for c in (low_rank, Wrapped, patched, parametrised)]
+                         + [(n, c) for n in OTHERS for c in (Wrapped, patched)]
+                         + [('blocks.0.ffn.1', lambda m: nn.ReLU()), ('candidate_encoder.mlp.1', lambda m: nn.GELU('tanh'))])
+def test_replaced_layers_run_as_they_are(name, change):
+    model, inputs = build()
+    with torch.no_grad():
+        before = model(*inputs)
+    model.set_submodule(name, change(model.get_submodule(name)))
+    with torch.no_grad():
+        want = model(*inputs)
+        got = model.set_dense_kernels()(*inputs)
+    if change is not parametrised:
+        assert relative(want, before) > 1e-6
+    assert relative(got, want) < 1e-5
+
+
+def test_which_modules_are_plain():
+    layer = nn.Linear(2, 3)
+    assert plain_modules.is_plain(layer, nn.Linear)
+    handle = layer.register_forward_hook(lambda *args: None)
+    assert not plain_modules.is_plain(layer, nn.Linear)
+    handle.remove()
+    assert plain_modules.is_plain(layer, nn.Linear)
+    assert not plain_modules.is_plain(LowRank(2, 3), nn.Linear)
+    assert plain_modules.is_plain_mlp(nn.Sequential(nn.Linear(2, 3), nn.GELU(), nn.Linear(3, 2)))
+    assert not plain_modules.is_plain_mlp(nn.Sequential(nn.Linear(2, 3), nn.GELU('tanh'), nn.Linear(3, 2)))
+    assert not plain_modules.is_plain_mlp(nn.Sequential(nn.Linear(2, 3), nn.GELU(), nn.Linear(3, 2), nn.Dropout(0.5)))
+
+
+def test_the_operators_still_serve_an_untouched_model():
+    model, inputs = build()
+    model.set_dense_kernels()
+    with torch.no_grad(), torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        model(*inputs)
+    count = sum(e.count for e in prof.key_averages() if e.key == 'vectra::linear')
+    assert count == 2 * 2 + 4 * len(model.blocks)

@@ -9,6 +9,8 @@ since sale, radius-scaled offsets and distance, and the cell flags).
 import torch
 from torch import nn
 
+from vectra_amd.price_transformer import plain_modules
+
 LOG_PRICE_CENTER = 13.12  # log of $500,000
 LOG_PRICE_SCALE = 0.6
 DAYS_PER_YEAR = 365.25
@@ -21,7 +23,7 @@ def _mlp(n_in: int, hidden: int, n_out: int) -> nn.Sequential:
 
 def _run_mlp(mlp: nn.Sequential, x: torch.Tensor, dense_kernels: bool) -> torch.Tensor:
     """The MLP, layer by layer or on torch.ops.vectra.linear."""
-    if not dense_kernels:
+    if not dense_kernels or not plain_modules.is_plain_mlp(mlp):
         return mlp(x)
     first, _, second = mlp
     hidden = torch.ops.vectra.linear(x, first.weight, first.bias, None, 'gelu')

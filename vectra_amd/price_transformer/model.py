@@ -21,6 +21,7 @@ from torch import nn
 
 from vectra_amd.price_transformer import candidate_encoder
 from vectra_amd.price_transformer import microhood
+from vectra_amd.price_transformer import plain_modules
 from vectra_amd.price_transformer import spatial_attention
 
 
@@ -106,6 +107,8 @@ class GatedFeedForward(nn.Module):
 class Block(nn.Module):
     """Pre-norm Transformer block with spatial attention."""
 
+    dense_checkpoint: str | None = None  # as SpatialAttention's
+
     def __init__(self, config: ModelConfig):
         super().__init__()
         self.norm1 = nn.LayerNorm(config.d_model)
@@ -121,20 +124,27 @@ class Block(nn.Module):
             )
 
     def forward(self, x, key_bias):
-        if self.attention.dense_checkpoint is None:
+        if self.dense_checkpoint is None:
             x = x + self.attention(self.norm1(x), key_bias)
             return x + self.ffn(self.norm2(x))
-        x = self.attention(self.norm1(x), key_bias, residual=x)
-        return self._feed_forward(self.norm2(x), x, self.attention.dense_checkpoint)
+        if plain_modules.is_plain(self.attention, spatial_attention.SpatialAttention):
+            x = self.attention(self.norm1(x), key_bias, residual=x)
+        else:
+            x = x + self.attention(self.norm1(x), key_bias)
+        return self._feed_forward(self.norm2(x), x, self.dense_checkpoint)
 
     def _feed_forward(self, x, residual, checkpoint):
         """The feed-forward block on the dense operators, onto the residual."""
-        if isinstance(self.ffn, GatedFeedForward):
-            first, second = self.ffn.gate_up, self.ffn.down
+        ffn = self.ffn
+        if (plain_modules.is_plain(ffn, GatedFeedForward) and plain_modules.is_plain(ffn.gate_up, nn.Linear)
+                and plain_modules.is_plain(ffn.down, nn.Linear)):
+            first, second = ffn.gate_up, ffn.down
             hidden = torch.ops.vectra.gated_linear(x, first.weight, first.bias, 'silu', checkpoint)
-        else:
-            first, second = self.ffn[0], self.ffn[2]
+        elif plain_modules.is_plain_mlp(ffn):
+            first, second = ffn[0], ffn[2]
             hidden = torch.ops.vectra.linear(x, first.weight, first.bias, None, 'gelu', checkpoint)
+        else:
+            return residual + ffn(x)
         return torch.ops.vectra.linear(hidden, second.weight, second.bias, residual, 'none', checkpoint)
 
 
@@ -166,14 +176,18 @@ class PriceTransformer(nn.Module):
         in the product's epilogue, for training with the operators' own
         gradients.  `checkpoint='e4m3'`: the blocks keep their layers' inputs
         in 8 bits for the backward pass (the encoders' inputs, prices and
-        distances, stay as they are).  The parameters are the same either way."""
+        distances, stay as they are).  The parameters are the same either way.
+        Layers that carry hooks, and ones that were wrapped or replaced, are
+        called as they are (plain_modules.py)."""
         if enabled:
             from vectra_amd.kernels import dense  # pylint: disable=import-outside-toplevel
 
             if checkpoint not in dense.CHECKPOINTS:
                 raise ValueError(f'checkpoint must be one of {dense.CHECKPOINTS}, not {checkpoint!r}')
         for block in self.blocks:
-            block.attention.dense_checkpoint = checkpoint if enabled else None
+            block.dense_checkpoint = checkpoint if enabled else None
+            if isinstance(block.attention, spatial_attention.SpatialAttention):
+                block.attention.dense_checkpoint = block.dense_checkpoint
         self.query_encoder.dense_kernels = self.candidate_encoder.dense_kernels = enabled
         return self
 

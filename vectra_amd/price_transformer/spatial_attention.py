@@ -17,6 +17,8 @@ import math
 import torch
 from torch import nn
 
+from vectra_amd.price_transformer import plain_modules
+
 
 class SpatialAttention(nn.Module):
     def __init__(self, d_model: int, num_heads: int):
@@ -36,7 +38,7 @@ class SpatialAttention(nn.Module):
         self.dense_checkpoint: str | None = None
 
     def _project(self, layer: nn.Linear, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
-        if self.dense_checkpoint is None:
+        if self.dense_checkpoint is None or not plain_modules.is_plain(layer, nn.Linear):
             return layer(x) if residual is None else residual + layer(x)
         return torch.ops.vectra.linear(x, layer.weight, layer.bias, residual, 'none', self.dense_checkpoint)
 
