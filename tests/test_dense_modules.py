@@ -7,8 +7,10 @@ import pytest
 import torch
 from torch import nn
 
+from vectra_amd.price_transformer import candidate_encoder
 from vectra_amd.price_transformer import model as model_lib
 from vectra_amd.price_transformer import plain_modules
+from vectra_amd.price_transformer import spatial_attention
 
 
 def build(gate=False):
@@ -147,3 +149,15 @@ def test_the_operators_still_serve_an_untouched_model():
         model(*inputs)
     count = sum(e.count for e in prof.key_averages() if e.key == 'vectra::linear')
     assert count == 2 * 2 + 4 * len(model.blocks)
+
+
+@pytest.mark.parametrize('kind', [spatial_attention.SpatialAttention, candidate_encoder.QueryEncoder,
+                                  candidate_encoder.CandidateEncoder, model_lib.Block])
+def test_modules_restored_without_the_switch_run_plain(kind):
+    """A module pickled before the switch existed holds no attribute of it."""
+    model, inputs = build()
+    for m in model.modules():
+        if isinstance(m, kind):
+            m.__dict__.pop('dense_checkpoint', None)
+            m.__dict__.pop('dense_kernels', None)
+    model(*inputs)

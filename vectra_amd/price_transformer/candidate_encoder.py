@@ -33,11 +33,12 @@ def _run_mlp(mlp: nn.Sequential, x: torch.Tensor, dense_kernels: bool) -> torch.
 class QueryEncoder(nn.Module):
     """[B, E], [B, A] -> [B, d_model]."""
 
+    dense_kernels = False
+
     def __init__(self, embedding_dim: int, attribute_dim: int, d_model: int):
         super().__init__()
         self.mlp = _mlp(embedding_dim + attribute_dim, 2 * d_model, d_model)
         self.role = nn.Parameter(torch.zeros(d_model))
-        self.dense_kernels = False
 
     def forward(self, embedding, attributes):
         return _run_mlp(self.mlp, torch.cat([embedding, attributes], dim=-1), self.dense_kernels) + self.role
@@ -46,10 +47,11 @@ class QueryEncoder(nn.Module):
 class CandidateEncoder(nn.Module):
     """[B, K, ...] comparable features -> [B, K, d_model]."""
 
+    dense_kernels = False
+
     def __init__(self, embedding_dim: int, attribute_dim: int, d_model: int):
         super().__init__()
         self.mlp = _mlp(embedding_dim + attribute_dim + _EXTRA_FEATURES, 2 * d_model, d_model)
-        self.dense_kernels = False
 
     def forward(self, embedding, attributes, log_price, sale_age_days, offsets_km, distance_km,
                 radius_km, cell_flags):

@@ -21,6 +21,10 @@ from vectra_amd.price_transformer import plain_modules
 
 
 class SpatialAttention(nn.Module):
+    # None: nn.Linear's own forward; else the form in which
+    # torch.ops.vectra.linear keeps its input for the backward pass.
+    dense_checkpoint: str | None = None
+
     def __init__(self, d_model: int, num_heads: int):
         super().__init__()
         if d_model % num_heads:
@@ -33,9 +37,6 @@ class SpatialAttention(nn.Module):
         self.log_sigma = nn.Parameter(
             torch.full((1, num_heads, 1, 1), 0.5 * math.log(self.head_dim))
         )
-        # None: nn.Linear's own forward; else the form in which
-        # torch.ops.vectra.linear keeps its input for the backward pass.
-        self.dense_checkpoint: str | None = None
 
     def _project(self, layer: nn.Linear, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         if self.dense_checkpoint is None or not plain_modules.is_plain(layer, nn.Linear):
