@@ -27,8 +27,11 @@ __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcp
 //   Phi(-a) = exp(-a^2 / 2) t P(t),  t = 1 / (1 + c a),
 // the form of Abramowitz and Stegun 26.2.17 with polynomials of this file's own
 // (least squares at Chebyshev nodes, weighted towards the least largest relative
-// error over a in [0, 14]): degree 8 for fp32 (1.7e-8), degree 6 where the
-// result is rounded to 16 bits (8e-7, a 300th of fp16's half step).  It has no
+// error over a in [0, 14]): degree 8 for fp32 (3.0e-8, half of fp32's half step;
+// its coefficients were rounded one after the other, the rest fitted again each
+// time), degree 6 where the result is rounded to 16 bits (8.2e-7, a 600th of
+// fp16's half step).  These are the errors of the constants as they stand,
+// evaluated exactly; the fp32 evaluation adds its own roundings.  It has no
 // cancellation on either side: for z < 0 the tail is the value, for z > 0 it is
 // subtracted from 1.  About 20 instructions (18), where erff's branches take
 // about 60: at 17 million elements on 256 CUs that is 9 us of vector issue
@@ -39,15 +42,15 @@ __device__ __forceinline__ void normal_tail(float a, float& tail, float& gauss) 
   float t, p;
   if constexpr (sizeof(T) == 4) {
     t = rcp_fast(__builtin_fmaf(0.21f, a, 1.f));
-    p = -0.07165610045194626f;
-    p = __builtin_fmaf(p, t, 0.2835877239704132f);
-    p = __builtin_fmaf(p, t, -0.33025193214416504f);
-    p = __builtin_fmaf(p, t, 0.3493996560573578f);
-    p = __builtin_fmaf(p, t, -0.09392443299293518f);
-    p = __builtin_fmaf(p, t, 0.12487246096134186f);
-    p = __builtin_fmaf(p, t, 0.06919222325086594f);
-    p = __builtin_fmaf(p, t, 0.08506885170936584f);
-    p = __builtin_fmaf(p, t, 0.08371157944202423f);
+    p = -0.07165627926588058f;
+    p = __builtin_fmaf(p, t, 0.2835884094238281f);
+    p = __builtin_fmaf(p, t, -0.3302529752254486f);
+    p = __builtin_fmaf(p, t, 0.34940046072006226f);
+    p = __builtin_fmaf(p, t, -0.09392476826906204f);
+    p = __builtin_fmaf(p, t, 0.12487250566482544f);
+    p = __builtin_fmaf(p, t, 0.06919223815202713f);
+    p = __builtin_fmaf(p, t, 0.08506884425878525f);
+    p = __builtin_fmaf(p, t, 0.08371157199144363f);
   } else {
     t = rcp_fast(__builtin_fmaf(0.3625f, a, 1.f));
     p = 0.04806305468082428f;
