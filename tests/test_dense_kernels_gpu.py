@@ -5,10 +5,12 @@ depend on the run, and rows whose tile spans more than 2^31 bytes.
 The 64-bit side runs on the GPU (matrix products of doubles).
 """
 
+import numpy as np
 import pytest
 import torch
 
 from oracle import dense as oracle
+from tests import test_dense_activations
 from vectra_amd.kernels import dense
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +124,30 @@ def test_gated_gradients_whose_tile_spans_more_than_31_bits():
     assert len(wrong) == 0, f'{len(wrong)} rows of dx are wrong, the first ones {wrong[:4].tolist()}'
     assert torch.equal(dw[at], (da.t() @ xd).float()) and torch.equal(dw[width_out + at], (du.t() @ xd).float())
     assert int(torch.count_nonzero(dw)) == int(torch.count_nonzero(dw[at])) + int(torch.count_nonzero(dw[width_out + at]))
+
+
+@pytest.mark.parametrize('dtype', DTYPES[:2], ids=str)
+def test_a_fp32_bias_gradient_has_fp32_slopes(dtype):
+    """x = 0, so z is the fp32 bias itself, and the only row of dy that is not
+    zero is ones: db is gelu'(z), of which nothing is rounded to 16 bits.  Its
+    error holds none of the error of the polynomial that serves 16-bit results
+    (e6, up to 8e-7 of the tail): projected on e6 it is near 0, where it would
+    be 1; roundings, of 1 / 7 of e6's size and uncorrelated with it, leave less
+    than a half."""
+    rows, width_in, n = 40, 64, 4096
+    b = torch.linspace(-4, 4, n, device='cuda')
+    dy = torch.zeros(rows, n, dtype=dtype, device='cuda')
+    dy[7] = 1
+    x = torch.zeros(rows, width_in, dtype=dtype, device='cuda')
+    db, = ops.linear_backward(dy, x, None, normal(n, width_in, dtype=dtype), b, 'gelu', False, [False, False, True])
+    assert db.dtype == torch.float32
+    z = b.double().cpu()
+    error = db.double().cpu() - oracle.activation(z, 'gelu')[1]
+    assert float(error.abs().max()) < 32 * oracle.U
+    # e6: the tail by degree 6 less the tail, with the sign that the slope takes it with.
+    c, powers = test_dense_activations.constants(1)
+    t = 1 / (1 + c * z.abs().numpy())
+    tail = 0.5 * torch.special.erfc(z.abs() / 2 ** 0.5)
+    e6 = torch.exp(-z * z / 2) * torch.from_numpy(np.polyval(powers, t) * t) - tail
+    e6 = torch.where(z < 0, e6, -e6)
+    assert abs(float((error * e6).sum() / (e6 * e6).sum())) < 0.5

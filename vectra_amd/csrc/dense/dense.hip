@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* parts, int split
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float value, slope;
-      act_slope<T>(s[0][e], p.activation, value, slope);
+      act_slope(s[0][e], p.activation, value, slope);
       s[0][e] = dy[e] * slope;
       if constexpr (kGated) {
         s[0][e] *= s[1][e];

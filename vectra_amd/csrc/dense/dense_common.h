@@ -29,7 +29,7 @@ __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcp
 // (least squares at Chebyshev nodes, weighted towards the least largest relative
 // error over a in [0, 14]): degree 8 for fp32 (3.0e-8, half of fp32's half step;
 // its coefficients were rounded one after the other, the rest fitted again each
-// time), degree 6 where the result is rounded to 16 bits (8.2e-7, a 600th of
+// time), degree 6 for values that are rounded to 16 bits (8.2e-7, a 600th of
 // fp16's half step).  These are the errors of the constants as they stand,
 // evaluated exactly; the fp32 evaluation adds its own roundings.  It has no
 // cancellation on either side: for z < 0 the tail is the value, for z > 0 it is
@@ -100,8 +100,9 @@ __device__ __forceinline__ float act_value(float z, int act) {
   }
 }
 
-// act(z) and act'(z).
-template <typename T>
+// act(z) and act'(z), for dz.  With fp32's polynomial whatever the operands' type:
+// a bias's gradient may be fp32 beside 16-bit operands, and is summed from dz
+// before its rounding.
 __device__ __forceinline__ void act_slope(float z, int act, float& value, float& slope) {
   switch (act) {
     case VECTRA_DENSE_RELU:
@@ -110,7 +111,7 @@ __device__ __forceinline__ void act_slope(float z, int act, float& value, float&
       return;
     case VECTRA_DENSE_GELU: {
       float tail, gauss;
-      normal_tail<T>(__builtin_fabsf(z), tail, gauss);
+      normal_tail<float>(__builtin_fabsf(z), tail, gauss);
       const float cdf = z < 0.f ? tail : 1.f - tail;
       value = z * cdf;
       slope = __builtin_fmaf(z, gauss * 0.3989422804014327f, cdf);

@@ -655,7 +655,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void gemm_kernel(const GemmParams p
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               float value, slope;
-              act_slope<T>(z[e / 4][e % 4], kAct, value, slope);
+              act_slope(z[e / 4][e % 4], kAct, value, slope);
               z[e / 4][e % 4] = near[e / 4][e % 4] * slope;
               if constexpr (C::kGated) {
                 z[e / 4][e % 4] *= u[e / 4][e % 4];

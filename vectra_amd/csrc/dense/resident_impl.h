@@ -202,13 +202,13 @@ __device__ __forceinline__ void resident_body(const ResidentParams& p, const lds
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float value, slope;
-          act_slope<T>(za[e], kAct, value, slope);
+          act_slope(za[e], kAct, value, slope);
           da[e] = ga[e] * slope;
           if constexpr (C::kGated) {
             da[e] *= ua[e];
             ea[e] = ga[e] * value;
           }
-          act_slope<T>(zb[e], kAct, value, slope);
+          act_slope(zb[e], kAct, value, slope);
           db[e] = gb[e] * slope;
           if constexpr (C::kGated) {
             db[e] *= ub[e];
