@@ -121,7 +121,8 @@ __device__ __forceinline__ void act_slope(float z, int act, float& value, float&
       float s, rest;
       sigmoid_pair(2.f * kTanhC * __builtin_fmaf(kTanhK * z * z, z, z), s, rest);
       value = z * s;
-      slope = __builtin_fmaf(value * rest, 2.f * kTanhC * __builtin_fmaf(3.f * kTanhK * z, z, 1.f), s);
+      // (z^2 held finite: past |z| = 1.8e19 it would be inf beside a rest or value of 0.)
+      slope = __builtin_fmaf(value * rest, 2.f * kTanhC * __builtin_fmaf(3.f * kTanhK, __builtin_fminf(z * z, 1e30f), 1.f), s);
       return;
     }
     case VECTRA_DENSE_SILU: {

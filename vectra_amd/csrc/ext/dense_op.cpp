@@ -337,7 +337,8 @@ std::pair<Tensor, Tensor> activation_cpu(const Tensor& z, int32_t act) {
     case VECTRA_DENSE_GELU_TANH: {
       const double c = std::sqrt(2.0 / M_PI), k = 0.044715;
       const Tensor y = (z + z * z * z * k) * (2 * c), s = at::sigmoid(y);
-      return {z * s, s + z * s * at::sigmoid(-y) * (z * z * (3 * k) + 1) * (2 * c)};
+      // (z^2 held finite, as on the GPU.)
+      return {z * s, s + z * s * at::sigmoid(-y) * ((z * z).clamp_max(1e30) * (3 * k) + 1) * (2 * c)};
     }
     case VECTRA_DENSE_SILU: {
       const Tensor s = at::sigmoid(z);
