@@ -138,6 +138,11 @@ Rows as_rows(const Tensor& x) {
   return r;
 }
 
+// Scales [..., ceil(width / 32)] beside codes [..., width].
+bool scales_fit(const Tensor& codes, const Tensor& scales) {
+  return codes.dim() >= 1 && scales.sizes() == at::IntArrayRef(with_last(codes, (codes.size(-1) + kBlock - 1) / kBlock));
+}
+
 void check_status(int status, const char* op) {
   TORCH_CHECK(status == VECTRA_DENSE_OK, op, ": ", vectra_dense_status_string(status));
 }
@@ -207,9 +212,8 @@ void check_backward(const Tensor& grad, const Tensor& x, const OptTensor& scales
     TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && scales->scalar_type() == at::kFloat8_e8m0fnu, op,
                 ": an input given with scales must be float8_e4m3fn codes and float8_e8m0fnu scales; got ",
                 x.scalar_type(), " and ", scales->scalar_type());
-    TORCH_CHECK(scales->dim() == x.dim() && rows_of(*scales) == rows_of(x) &&
-                    scales->size(-1) == (x.size(-1) + kBlock - 1) / kBlock,
-                op, ": scales must be [..., ceil(width_in / 32)]; got ", scales->sizes(), " for codes ", x.sizes());
+    TORCH_CHECK(scales_fit(x, *scales), op, ": scales must be [..., ceil(width_in / 32)]; got ", scales->sizes(),
+                " for codes ", x.sizes());
     TORCH_CHECK(scales->device() == x.device(), op, ": scales must be on ", x.device());
     check_layer(grad.new_empty({0, x.size(-1)}, x.options().dtype(weight.scalar_type())), weight, bias, std::nullopt,
                 gated, op);
@@ -302,9 +306,8 @@ void check_codes(const Tensor& codes, const Tensor& scales, at::ScalarType dtype
   TORCH_CHECK(codes.scalar_type() == at::kFloat8_e4m3fn && scales.scalar_type() == at::kFloat8_e8m0fnu, op,
               ": codes must be float8_e4m3fn and scales float8_e8m0fnu; got ", codes.scalar_type(), " and ",
               scales.scalar_type());
-  TORCH_CHECK(codes.dim() >= 1 && scales.dim() == codes.dim() && rows_of(scales) == rows_of(codes) &&
-                  scales.size(-1) == (codes.size(-1) + kBlock - 1) / kBlock,
-              op, ": scales must be [..., ceil(width / 32)]; got ", scales.sizes(), " for codes ", codes.sizes());
+  TORCH_CHECK(scales_fit(codes, scales), op, ": scales must be [..., ceil(width / 32)]; got ", scales.sizes(),
+              " for codes ", codes.sizes());
   TORCH_CHECK(scales.device() == codes.device(), op, ": scales must be on ", codes.device());
   TORCH_CHECK(dense_dtype(dtype) >= 0, op, ": dtype must be float32, float16 or bfloat16; got ", dtype);
 }
