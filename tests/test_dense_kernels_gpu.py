@@ -151,3 +151,23 @@ def test_a_fp32_bias_gradient_has_fp32_slopes(dtype):
     e6 = torch.exp(-z * z / 2) * torch.from_numpy(np.polyval(powers, t) * t) - tail
     e6 = torch.where(z < 0, e6, -e6)
     assert abs(float((error * e6).sum() / (e6 * e6).sum())) < 0.5
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('size', [(2051, 1000, 2056), (4096, 4096, 1024)], ids=str)
+def test_large_operands_that_start_anywhere(size, dtype):
+    """Rows of whole chunks whose first element is not 16-byte aligned, of x, W
+    and dy: copied first, exact integers, NaN around them."""
+    rows, width_in, width_out = size
+    gen = torch.Generator(device='cuda').manual_seed(1)
+
+    def shifted(r, c, most):
+        wide = torch.full((r, c + 16), float('nan'), dtype=dtype, device='cuda')
+        wide[:, 1:c + 1] = torch.randint(-most, most + 1, (r, c), generator=gen, device='cuda').to(dtype)
+        return wide[:, 1:c + 1]
+
+    x, w, dy = shifted(rows, width_in, 2), shifted(width_out, width_in, 1), shifted(rows, width_out, 3)
+    assert torch.equal(dense.linear(x, w), (x.double() @ w.double().t()).to(dtype))
+    dx, dw = ops.linear_backward(dy, x, None, w, None, 'none', False, [True, True, False])
+    assert torch.equal(dx, (dy.double() @ w.double()).to(dtype))
+    assert torch.equal(dw, (dy.double().t().contiguous() @ x.double()).to(dtype))
