@@ -121,15 +121,18 @@ def make_grad_args(grad, x, weight, bias, dx, dweight, dbias, activation='none',
 
 def _call(name, a, device, workspace, stream):
     lib = _native.dense_library()
-    need = getattr(lib, name + '_workspace_bytes')(ctypes.byref(a))
-    if need < 0:
-        raise DenseError(-need)
-    if workspace is None and need > 0:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    if stream is None:
-        stream = torch.cuda.current_stream(device).cuda_stream
-    status = getattr(lib, name)(ctypes.byref(a), _pointer(workspace), 0 if workspace is None else workspace.numel(),
-                                stream)
+    with torch.cuda.device(device):
+        need = getattr(lib, name + '_workspace_bytes')(ctypes.byref(a))
+        if need < 0:
+            raise DenseError(-need)
+        own = torch.cuda.current_stream() if stream is None else torch.cuda.ExternalStream(stream)
+        if workspace is None and need > 0:
+            # Memory of the stream that uses it: the allocator may hand it on once
+            # this call returns, but only to what that stream runs afterwards.
+            with torch.cuda.stream(own):
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        status = getattr(lib, name)(ctypes.byref(a), _pointer(workspace),
+                                    0 if workspace is None else workspace.numel(), own.cuda_stream)
     if status != OK:
         raise DenseError(status)
 
