@@ -129,7 +129,8 @@ int vectra_dense_forward(const vectra_dense_args* args, void* workspace, int64_t
  * negative: -status. */
 int64_t vectra_dense_forward_workspace_bytes(const vectra_dense_args* args);
 
-/* dx, dW and db, those that are wanted.  rows == 0 sets dW and db to zero. */
+/* dx, dW and db, those that are wanted.  rows == 0 sets dW and db to zero.  No
+ * output may overlap an input or another output. */
 int vectra_dense_backward(const vectra_dense_grad_args* args, void* workspace, int64_t workspace_bytes,
                           vectra_dense_stream_t stream);
 int64_t vectra_dense_backward_workspace_bytes(const vectra_dense_grad_args* args);

@@ -27,11 +27,11 @@
 // copy would cost more, pass through registers (kAny): full chunks as unaligned
 // 16-byte loads, a row's last partial chunk element by element.
 //
-// Measured, 8192 x 4096 -> 4096 bf16: forward 200 us, dx 205, dW 206, 1.34 to 1.37
-// PFLOP/s where the library's products reach 1.36 (in turn with them: forward
-// 1.35 against 1.55, dx 1.28 against 1.35, dW 1.26 against 1.22).  The matrix
-// cores are busy 61 to 62% of the launch: what a tile of 256 x 256 leaves idle
-// is its first loads and its epilogue, with one workgroup per CU, and the clock
+// Measured, 8192 x 4096 -> 4096 bf16, four sets of operands, in turn with the
+// library's products: forward 215 us against 179 (1.28 and 1.53 PFLOP/s), dx 221
+// against 208 (1.25 and 1.32), dW 221 against 243 (1.25 and 1.13).  The matrix
+// cores are busy 61 to 62% of the launch: what a tile of 256 x 256 leaves idle is
+// its first loads and its epilogue, with one workgroup per CU, and the clock
 // falls under full load.
 //
 // LDS reads: deep 16-bit and 32-bit operands read 16 bytes per lane.  Wide
