@@ -9,13 +9,12 @@ wrapper or a parametrised layer has a forward of its own) that carries no hooks.
 import torch
 from torch import nn
 
-_HOOKS = ('_forward_hooks', '_forward_pre_hooks', '_backward_hooks', '_backward_pre_hooks')
-
 
 def is_plain(module: nn.Module, kind: type) -> bool:
     """Whether calling `module` runs `kind`'s forward and nothing besides."""
     return (type(module) is kind and 'forward' not in module.__dict__
-            and not any(getattr(module, name) for name in _HOOKS)
+            and not (module._forward_hooks or module._forward_pre_hooks  # pylint: disable=protected-access
+                     or module._backward_hooks or module._backward_pre_hooks)
             and not torch.nn.modules.module._has_any_global_hook())  # pylint: disable=protected-access
 
 
