@@ -17,7 +17,7 @@
 // four cycles per 64 elements, 10 us for 17 million elements on 256 CUs.
 //
 // Measured, 66560 rows, 128 -> 256 bf16: forward with a GELU 21 us (51 MB; the
-// vector units are busy 78% of it, the matrix cores 10%), dz and dx 34 us;
+// vector units are busy 77% of it, the matrix cores 11%), dz and dx 35 us;
 // gated with SiLU 22 and 46 us; 65536 rows, 141 -> 256 fp32 with a GELU 56 us
 // (matrix cores 59% busy, 31 us of work).  One unit of 16 rows per wave and 16
 // waves are the fastest of what was tried: two units per wave, or 8 and 12
