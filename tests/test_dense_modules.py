@@ -161,3 +161,44 @@ def test_modules_restored_without_the_switch_run_plain(kind):
             m.__dict__.pop('dense_checkpoint', None)
             m.__dict__.pop('dense_kernels', None)
     model(*inputs)
+
+
+class Forwarding(nn.Module):
+    """A wrapper that hands on its inner module's attributes, as those for
+    recomputation and sharding do."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, *args, **kwargs):
+        return self.inner(*args, **kwargs)
+
+    def __getattr__(self, name):
+        try:
+            return super().__getattr__(name)
+        except AttributeError:
+            return getattr(super().__getattr__('inner'), name)
+
+
+def count_linears(model, inputs):
+    with torch.no_grad(), torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        model(*inputs)
+    return sum(e.count for e in prof.key_averages() if e.key == 'vectra::linear')
+
+
+@pytest.mark.parametrize('wrapper', [Forwarding, Wrapped])
+@pytest.mark.parametrize('name,fused', [('blocks.0', 0), ('query_encoder', 0), ('blocks.1.attention', 0), ('blocks.0.ffn', 2)])
+def test_the_switch_reaches_modules_inside_wrappers(name, fused, wrapper):
+    """On and off; only a layer whose own call is wrapped stays as it is (`fused`
+    of them: a feed-forward block's layers are fused from outside it)."""
+    model, inputs = build()
+    with torch.no_grad():
+        model.set_dense_kernels()
+        whole = count_linears(model, inputs)
+        model.set_submodule(name, wrapper(model.get_submodule(name)))
+        assert count_linears(model, inputs) == whole - fused
+        model.set_dense_kernels(False)
+        assert count_linears(model, inputs) == 0
+        model.set_dense_kernels()
+        assert count_linears(model, inputs) == whole - fused

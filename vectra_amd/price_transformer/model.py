@@ -184,11 +184,11 @@ class PriceTransformer(nn.Module):
 
             if checkpoint not in dense.CHECKPOINTS:
                 raise ValueError(f'checkpoint must be one of {dense.CHECKPOINTS}, not {checkpoint!r}')
-        for block in self.blocks:
-            block.dense_checkpoint = checkpoint if enabled else None
-            if isinstance(block.attention, spatial_attention.SpatialAttention):
-                block.attention.dense_checkpoint = block.dense_checkpoint
-        self.query_encoder.dense_kernels = self.candidate_encoder.dense_kernels = enabled
+        for module in self.modules():  # (those inside wrappers too)
+            if isinstance(module, (Block, spatial_attention.SpatialAttention)):
+                module.dense_checkpoint = checkpoint if enabled else None
+            elif isinstance(module, (candidate_encoder.QueryEncoder, candidate_encoder.CandidateEncoder)):
+                module.dense_kernels = enabled
         return self
 
     def forward(self, query_embedding, query_attributes, query_location, query_cell6,
