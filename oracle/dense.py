@@ -109,6 +109,8 @@ class Layer:
             (a, b), (da, db) = self._halves(z), self._halves(dz_err)
             value, slope = activation(a, self.activation)
             dv, ds = steep * da + ACT_ERROR * (1 + a.abs()), bend * da + ACT_ERROR * (1 + a.abs())
+            if self.activation == 'relu':  # as below: within its error of 0 the gate's slope is 0 or 1
+                ds = torch.where(a.abs() <= da, torch.ones_like(ds), ds)
             first, second = g * b * slope, g * value
             err = torch.cat([g.abs() * (ds * (b.abs() + db) + slope.abs() * db) + 3 * U * first.abs(),
                              g.abs() * dv + 2 * U * second.abs()], 1)

@@ -64,3 +64,14 @@ def test_far_from_zero_an_activation_is_the_identity_or_zero(gated, activation, 
                       (dx[:, 0], keeps.to(dtype))):
         assert got.isfinite().all(), got
         assert ((got - want).abs().float() <= 1e-11 + 4 * oracle.U * want.abs().float()).all(), got
+
+
+def test_the_oracle_allows_either_slope_where_a_gate_is_within_its_error_of_zero():
+    """a = x W of one term is exact but for the order of its rounding with the
+    bias: z = 1 - 1 = 0 here, where relu's slope may be taken as 0 or 1."""
+    x, w = torch.ones(1, 1), torch.tensor([[1.0], [1.0]])
+    layer = oracle.Layer.of(x, w, torch.tensor([-1.0, 0.0]), None, 'relu', True)
+    want, bound = layer.backward(torch.ones(1, 1), torch.float32, torch.float32)['x']
+    assert float(want) == 0 and float(bound) >= 1
+    far = oracle.Layer.of(x, w, torch.tensor([-0.5, 0.0]), None, 'relu', True)
+    assert float(far.backward(torch.ones(1, 1), torch.float32, torch.float32)['x'][1]) < 1e-4
