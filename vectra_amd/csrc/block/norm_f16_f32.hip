@@ -1,0 +1,9 @@
+// Norms of a _Float16 branch on a float stream.
+#include "norm_impl.h"
+
+namespace vectra_block {
+int launch_norm_f16_f32(const NormParams& p, int cus, hipStream_t stream) { return launch_norm<_Float16, float>(p, cus, stream); }
+int launch_norm_grad_f16_f32(const NormGradParams& p, int workgroups, hipStream_t stream) {
+  return launch_norm_grad<_Float16, float>(p, workgroups, stream);
+}
+}  // namespace vectra_block

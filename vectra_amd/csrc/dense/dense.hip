@@ -17,6 +17,7 @@
 
 #include "dense_common.h"
 #include "dense_kernels.h"
+#include "eight_bit.h"
 #include "row_chunk.h"
 
 namespace vectra_dense {
@@ -203,35 +204,6 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const In* x, int64_t s
 
 // ------------------------------------------------------------- 8-bit rows
 
-// The exponent byte of a block whose largest finite magnitude is `largest`:
-// the smallest e with largest <= 448 * 2^e, at least `lowest`, plus 127.
-// largest = f * 2^x with f in [1, 2): 448 = 1.75 * 2^8.
-__device__ __forceinline__ int block_exponent(float largest, int lowest) {
-  const uint32_t bits = __float_as_uint(largest);
-  int e;
-  if (bits < 0x00800000u) {
-    e = lowest;  // zero or an fp32 subnormal: far below the lowest exponent
-  } else {
-    e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x007fffffu) > 0x00600000u ? 1 : 0);
-  }
-  return max(e, lowest) + 127;
-}
-
-// 2^e as fp32 for e in [-126, 127].
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
-
-// fp32 in [-448, 448] to e4m3, ties to even (v_cvt_pk_fp8_f32); NaN to NaN.
-__device__ __forceinline__ uint32_t to_e4m3x4(f32x4 v) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true));
-}
-
-__device__ __forceinline__ f32x4 from_e4m3x4(uint32_t w) {
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
-  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
-  return f32x4{lo[0], lo[1], hi[0], hi[1]};
-}
-
 // Both kernels move eight elements per thread and turn, 16 bytes of a 16-bit
 // row, and turn their work's index into a row and a column by 32-bit division
 // (Index) where the counts allow: a 64-bit one costs more than the rest of a
@@ -252,40 +224,18 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t rows,
   const int left = live ? static_cast<int>(most(least(width - col, 8), 0)) : 0;
   f32x4 v[2] = {};
   if (left > 0) load8(x + row * stride + col, left, v[0], v[1]);
-  float largest = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float a = __builtin_fabsf(v[k / 4][k % 4]);
-    if (a <= 3.4028234663852886e38f) {
-      largest = a > largest ? a : largest;
-    } else {
-      v[k / 4][k % 4] = __builtin_nanf("");
-    }
-  }
+  float largest = largest_finite(v, 0.f);
 #pragma unroll
   for (int d = 1; d < 4; d <<= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
   const int byte = block_exponent(largest, kLowest);
-  const int e = byte - 127;
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    v[h] *= power_of_two(-e);  // e in [-117, 120]
-    // The type's largest value, 255.9 * 2^8 (fp16) or 2^120, would round to
-    // 256 times that, which the type lacks: at its exponent, magnitudes of
-    // 248 and more take the code below, 240.
-    if (e == kHighest)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (__builtin_fabsf(v[h][k]) >= 248.f) v[h][k] = __builtin_copysignf(240.f, v[h][k]);
-    w[h] = to_e4m3x4(v[h]);
-  }
+  const uint2 w = to_codes(v, byte - 127, kHighest);
   uint8_t* const out = codes + row * codes_stride + col;
   if (left == 8) {
-    __builtin_memcpy(out, w, 8);
+    __builtin_memcpy(out, &w, 8);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (k < left) out[k] = static_cast<uint8_t>(w[k / 4] >> (8 * (k % 4)));
+      if (k < left) out[k] = static_cast<uint8_t>((k < 4 ? w.x : w.y) >> (8 * (k % 4)));
   }
   if (live && (threadIdx.x & 3) == 0) scales[row * scales_stride + block] = static_cast<uint8_t>(byte);
 }

@@ -33,35 +33,14 @@
 #include <string_view>
 #include <vector>
 
+#include "op_common.h"
 #include "vectra_dense.h"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
+using namespace vectra_ops;
 
 constexpr int64_t kBlock = 32;  // elements of a row that share a power of two
-
-bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-int32_t dense_dtype(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return VECTRA_DENSE_F32;
-    case at::kHalf: return VECTRA_DENSE_F16;
-    case at::kBFloat16: return VECTRA_DENSE_BF16;
-    default: return -1;
-  }
-}
-
-int32_t activation_of(std::string_view name, const char* op) {
-  if (name == "none") return VECTRA_DENSE_NONE;
-  if (name == "relu") return VECTRA_DENSE_RELU;
-  if (name == "gelu") return VECTRA_DENSE_GELU;
-  if (name == "gelu_tanh") return VECTRA_DENSE_GELU_TANH;
-  if (name == "silu") return VECTRA_DENSE_SILU;
-  TORCH_CHECK_VALUE(false, op, ": activation must be 'none', 'relu', 'gelu', 'gelu_tanh' or 'silu'; got '",
-                    std::string(name), "'");
-}
 
 bool eight_bit(std::string_view checkpoint, const char* op) {
   TORCH_CHECK_VALUE(checkpoint == "none" || checkpoint == "e4m3", op, ": checkpoint must be 'none' or 'e4m3'; got '",
@@ -101,41 +80,6 @@ void check_layer(const Tensor& x, const Tensor& weight, const OptTensor& bias, c
     TORCH_CHECK(residual->device() == x.device(), op, ": residual must be on ", x.device(), "; got ",
                 residual->device());
   }
-}
-
-std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
-  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
-  sizes.back() = last;
-  return sizes;
-}
-
-int64_t rows_of(const Tensor& x) {
-  int64_t rows = 1;
-  for (int64_t d = 0; d + 1 < x.dim(); ++d) rows *= x.size(d);
-  return rows;
-}
-
-// A matrix the C ABI can read: rows with unit element stride, one row stride
-// of at least a row, 256 rows within 2^31 bytes.  A view that has none (a
-// transposed or an expanded one, or one of rows very far apart) is copied.
-struct Rows {
-  Tensor t;
-  int64_t stride = 0;
-};
-
-Rows as_rows(const Tensor& x) {
-  const int64_t width = x.size(-1);
-  const int64_t rows = rows_of(x);
-  Rows r;
-  if (x.dim() == 2) {
-    r.t = x;
-  } else {
-    r.t = x.reshape({rows, width});
-  }
-  const bool near = rows <= 1 || (r.t.stride(0) >= width && r.t.stride(0) < (int64_t{1} << 23) / x.element_size());
-  if ((width > 1 && r.t.stride(1) != 1) || !near) r.t = r.t.contiguous();
-  r.stride = rows > 1 ? r.t.stride(0) : std::max<int64_t>(width, 1);
-  return r;
 }
 
 // Scales [..., ceil(width / 32)] beside codes [..., width].
@@ -328,28 +272,6 @@ Tensor dequantize_rows_hip(const Tensor& codes, const Tensor& scales, at::Scalar
 // ------------------------------------------------------------------- host
 //
 // The operators off the GPU: the same formulas on fp32 tensors.
-
-// act(z) and act'(z).
-std::pair<Tensor, Tensor> activation_cpu(const Tensor& z, int32_t act) {
-  switch (act) {
-    case VECTRA_DENSE_RELU: return {z.clamp_min(0), z.gt(0).to(z.scalar_type())};
-    case VECTRA_DENSE_GELU: {
-      const Tensor cdf = at::erfc(z * -std::sqrt(0.5)) * 0.5;
-      return {z * cdf, cdf + z * at::exp(z * z * -0.5) * (1.0 / std::sqrt(2.0 * M_PI))};
-    }
-    case VECTRA_DENSE_GELU_TANH: {
-      const double c = std::sqrt(2.0 / M_PI), k = 0.044715;
-      const Tensor y = (z + z * z * z * k) * (2 * c), s = at::sigmoid(y);
-      // (z^2 held finite, as on the GPU.)
-      return {z * s, s + z * s * at::sigmoid(-y) * ((z * z).clamp_max(1e30) * (3 * k) + 1) * (2 * c)};
-    }
-    case VECTRA_DENSE_SILU: {
-      const Tensor s = at::sigmoid(z);
-      return {z * s, s + z * s * at::sigmoid(-z)};
-    }
-    default: return {z, at::ones_like(z)};
-  }
-}
 
 Tensor project_cpu(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
   Tensor z = at::matmul(x.to(at::kFloat), weight.to(at::kFloat).t());

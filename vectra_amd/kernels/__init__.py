@@ -7,5 +7,6 @@ vectra_kernels.custom_ops does in the reference
 (torch.ops.vectra.linear and its relatives) are registered with it.
 """
 
+from vectra_amd.kernels import block  # noqa: F401  (registers the fakes of what stands between them)
 from vectra_amd.kernels import custom_ops  # noqa: F401  (registers the op)
 from vectra_amd.kernels import dense  # noqa: F401  (registers the dense operators' fakes)
