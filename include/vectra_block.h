@@ -43,6 +43,7 @@
  * Contract (as vectra_dense.h):
  *  - Plain pointers, sizes and strides; matrices are row-major with unit element stride
  *    and a row stride in ELEMENTS of at least a row; that of a single row is not read.
+ *    Codes begin at a multiple of 16 bytes, scales of 4.
  *  - Every buffer is owned by the caller.  Calls that need scratch memory take a workspace
  *    whose size the _workspace_bytes function tells; it needs no set-up, holds nothing
  *    between calls, and must not be shared by calls that can overlap.
@@ -80,7 +81,7 @@ enum {
   VECTRA_BLOCK_OK = 0,
   VECTRA_BLOCK_ERR_NULL_ARGUMENT = 1,
   VECTRA_BLOCK_ERR_BAD_DTYPE = 2,
-  VECTRA_BLOCK_ERR_BAD_SHAPE = 3,  /* negative sizes, strides smaller than a row */
+  VECTRA_BLOCK_ERR_BAD_SHAPE = 3,  /* negative sizes, strides smaller than a row, unaligned codes */
   VECTRA_BLOCK_ERR_BAD_STRUCT = 4, /* struct_size does not match this build      */
   VECTRA_BLOCK_ERR_TOO_LARGE = 5,  /* a size exceeds the kernels' range          */
   VECTRA_BLOCK_ERR_LAUNCH = 6,     /* the HIP launch itself failed               */

@@ -262,3 +262,44 @@ def values(codes, scales, high, width):
     e = scales.astype(np.int64)[:, :codes.shape[1] // BLOCK] - 127
     e = np.repeat(np.repeat(e, high, 0)[:codes.shape[0]], BLOCK, 1)
     return torch.from_numpy(np.where(e == 128, np.nan, np.ldexp(value, e))[:, :width])
+
+
+# --------------------------------------------------------------- 8-bit products
+
+
+def layer(x, weight, bias=None, residual=None, activation='none', gated=False, dtype=torch.float32, cores=False):
+    """(y, bound) of a layer on float64 values x [rows, width] and weight [n_w, width].
+
+    Exact products in fp32 sums, or with `cores` the 8-bit matrix cores': products p of a group are aligned to
+    the largest one's power of two, 2^q, and lose what lies below g = 2^(q - 13).  A product of two e4m3 values
+    has at most eight significant bits, so one of at least 2^(q - 6) loses nothing and a smaller one at most
+    min(|p|, g); the sums that pass through a group's alignment lose at most g each, four times per block of 128.
+    The group is bounded by its block."""
+    z = x @ weight.t()
+    size = x.abs() @ weight.abs().t()
+    err = (x.shape[1] + 2) * U * 1.01 * size
+    if cores:
+        for k in range(0, x.shape[1], BLOCK):
+            p = (x[:, None, k:k + BLOCK] * weight[None, :, k:k + BLOCK]).abs()
+            largest = p.amax(-1, keepdim=True)
+            q = torch.floor(torch.log2(largest.clamp_min(1e-300)))
+            g = torch.exp2(q - 13)
+            err = err + (torch.where(p < torch.exp2(q - 6), torch.minimum(p, g), torch.zeros_like(p)).sum(-1) + 4 * g[..., 0])
+    if bias is not None:
+        z = z + bias
+        err = err + U * z.abs() + U * bias.abs()
+    steep = dense.MOST_SLOPE[activation]
+    if gated:
+        n = z.shape[1] // 2
+        a, b, da, db = z[:, :n], z[:, n:], err[:, :n], err[:, n:]
+        value, _ = dense.activation(a, activation)
+        dv = steep * da + dense.ACT_ERROR * (1 + a.abs())
+        y = value * b
+        e = dv * (b.abs() + db) + value.abs() * db + 2 * U * y.abs()
+    else:
+        y, _ = dense.activation(z, activation)
+        e = steep * err + (dense.ACT_ERROR * (1 + z.abs()) if activation != 'none' else 0)
+    if residual is not None:
+        y = y + residual
+        e = e + 2 * U * (y.abs() + residual.abs())
+    return y, e * 1.01 + rounding(y, e, dtype)

@@ -1,0 +1,362 @@
+"""torch.ops.vectra.quantize_blocks, linear_8bit and gated_linear_8bit on the CPU and
+the GPU: codes bit for bit, integers bit for bit, ordinary values within bounds that
+the oracle derives, layouts and refusals."""
+
+import itertools
+
+import pytest
+import torch
+
+from oracle import block as oracle
+from vectra_amd.kernels import block
+from vectra_amd.kernels import dense
+
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+FEW = 64  # rows up to which results are exact products in fp32 sums
+
+
+def normal(*shape, seed=0, scale=1.0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale
+
+
+def integers(*shape, most, seed=0):
+    return torch.randint(-most, most + 1, shape, generator=torch.Generator().manual_seed(seed)).float()
+
+
+def as_bytes(t):
+    """Bytes on the CPU; codes with e4m3's NaN, which has no sign of its own, as 0x7F."""
+    b = t.view(torch.uint8).cpu()
+    return torch.where(b == 0xFF, 0x7F, b) if t.dtype == torch.float8_e4m3fn else b
+
+
+# ----------------------------------------------------------------------- codes
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('shape', [(1, 1), (3, 127), (2, 128), (5, 129), (130, 300), (7, 512), (2, 513), (257, 1000)], ids=str)
+def test_codes(shape, dtype, device):
+    x = (normal(*shape, seed=3) * torch.exp(3 * normal(*shape, seed=4))).to(dtype).to(device)
+    for tiles in (False, True):
+        codes, scales = block.quantize_blocks(x, tiles)
+        want = oracle.quantize(x, 128 if tiles else 1)
+        assert codes.dtype == torch.float8_e4m3fn and scales.dtype == torch.float8_e8m0fnu
+        assert torch.equal(as_bytes(codes), want[0]) and torch.equal(as_bytes(scales), want[1])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_codes_of_edges(device):
+    """Zeros, the block maxima around 448 * 2^e, ties, fp32's ends, infinities and NaN."""
+    edges = torch.tensor([0.0, -0.0, 448.0, 448.0 * (1 + 2.0 ** -23), 449.0, 464.0, 464.0001, 1e-45, 2.0 ** -126, 2.0 ** -140, 3.4e38,
+                          3.4028234663852886e38, float('inf'), float('-inf'), float('nan'), 17.0, 19.0, 1.0625, 1.1875, 2.0 ** -10,
+                          3 * 2.0 ** -10, 2.0 ** 119, 2.0 ** 127])
+    x = torch.zeros(len(edges) * 4, 160)
+    for i, e in enumerate(edges):
+        x[4 * i, 5] = e
+        x[4 * i + 1, 0], x[4 * i + 1, 127] = e, 448.0
+        x[4 * i + 2, 128], x[4 * i + 2, 0] = -e, 1.0
+        x[4 * i + 3, 3], x[4 * i + 3, 4] = e, 3.4e38
+    for tiles in (False, True):
+        codes, scales = block.quantize_blocks(x.to(device), tiles)
+        want = oracle.quantize(x, 128 if tiles else 1)
+        assert torch.equal(as_bytes(codes), want[0]) and torch.equal(as_bytes(scales), want[1])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_codes_of_views_and_of_nothing(device):
+    x = normal(6, 40, 50, seed=1).to(device)
+    for view in (x[:, 3:30, 7:41], x.transpose(1, 2), x[::2, :, ::3], x[:, :1].expand(6, 7, 50)):
+        got, want = block.quantize_blocks(view), block.quantize_blocks(view.contiguous())
+        assert all(torch.equal(as_bytes(a), as_bytes(b)) for a, b in zip(got, want))
+        assert got[0].shape == (*view.shape[:-1], 128) and got[1].shape == (*view.shape[:-1], 4)
+    for shape in ((0, 5), (3, 0), (2, 0, 9)):
+        codes, scales = block.quantize_blocks(torch.zeros(shape, device=device))
+        assert codes.shape[:-1] == scales.shape[:-1] == shape[:-1]
+
+
+# ---------------------------------------------------------------------- layers
+
+
+def run(x, weight, bias, residual, activation, gated, as_codes, dtype):
+    codes, scales = block.quantize_blocks(weight, tiles=True)
+    given = {}
+    if as_codes:
+        x, given['scales'] = block.quantize_blocks(x)
+        given['dtype'] = dtype
+    if gated:
+        return block.gated_linear_8bit(x, codes, scales, bias, activation, **given)
+    return block.linear_8bit(x, codes, scales, bias, residual, activation, **given)
+
+
+def check(rows, width, n, dtype, device, *, gated=False, activation='none', bias=True, residual=False, as_codes=False, exact=False,
+          seed=0):
+    n_w = 2 * n if gated else n
+    if exact:  # integers: codes, products and sums are exact, and so is the result where it fits its type
+        x, w = integers(rows, width, most=4, seed=seed), integers(n_w, width, most=2, seed=seed + 1)
+        b, r = integers(n_w, most=3, seed=seed + 2), integers(rows, n, most=9, seed=seed + 3)
+    else:
+        x, w = normal(rows, width, seed=seed), normal(n_w, width, seed=seed + 1, scale=max(width, 1) ** -0.5)
+        b, r = normal(n_w, seed=seed + 2, scale=0.3), normal(rows, n, seed=seed + 3)
+    x, b, r = (t.to(dtype).to(device) for t in (x, b, r))
+    w = w.to(device)
+    y = run(x, w, b if bias else None, r if residual else None, activation, gated, as_codes, dtype)
+    assert y.dtype == dtype and y.shape == (rows, n) and y.is_contiguous()
+    xs = oracle.values(*block.quantize_blocks(x), 1, width)
+    ws = oracle.values(*block.quantize_blocks(w, True), 128, width)
+    if exact:
+        assert torch.equal(xs, x.double().cpu()) and torch.equal(ws, w.double().cpu())
+    want, bound = oracle.layer(xs, ws, b.double().cpu() if bias else None, r.double().cpu() if residual else None, activation, gated,
+                               dtype, cores=not exact and device != 'cpu' and dtype != F32 and rows > FEW)
+    if exact and activation in ('none', 'relu'):
+        assert torch.equal(y.cpu(), want.to(dtype)), (rows, width, n)
+    else:
+        oracle.assert_within(y, want, bound)
+
+
+SIZES = [(1, 1, 1), (1, 128, 16), (2, 129, 17), (16, 300, 130), (17, 1000, 33), (31, 512, 40), (33, 640, 300), (64, 257, 65),
+         (65, 128, 64), (65, 1, 300), (100, 700, 131), (128, 128, 128), (129, 513, 257), (300, 1100, 129)]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('rows,width,n', SIZES)
+def test_integers(rows, width, n, dtype, device):
+    for i, (gated, as_codes) in enumerate(itertools.product((False, True), (False, True))):
+        check(rows, width, n, dtype, device, gated=gated, as_codes=as_codes, residual=not gated, activation='none', exact=True, seed=i)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('rows,width,n', [(1, 4096, 48), (5, 1000, 100), (40, 520, 200), (70, 300, 150), (200, 1000, 70)])
+def test_ordinary_values(rows, width, n, dtype, device):
+    for i, activation in enumerate(dense.ACTIVATIONS):
+        check(rows, width, n, dtype, device, activation=activation, residual=i % 2 == 0, bias=i % 3 != 1, as_codes=i % 2 == 1, seed=i)
+        check(rows, width, n, dtype, device, activation=activation, gated=True, bias=i % 2 == 0, seed=i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('rows,width,n', [(2049, 1300, 2100), (1024, 4096, 512), (300, 8200, 384), (4100, 260, 1030), (70, 16384, 64),
+                                          (66, 2048, 24000)])
+def test_large_integers(rows, width, n, dtype):
+    """Every tile, split and tail, bit for bit (on the GPU the products' own reference: fp32 sums of integers)."""
+    for gated in (False, True):
+        n_half = n // 2 if gated else n
+        x, w = integers(rows, width, most=2, seed=1).cuda(), integers(n_half * (2 if gated else 1), width, most=1, seed=2).cuda()
+        b = integers(w.shape[0], most=3, seed=3).cuda()
+        z = x @ w.t() + b  # below 2^24: exact in any order
+        assert float(z.abs().max()) < 2 ** 24
+        if gated:
+            want = torch.relu(z[:, :n_half]) * z[:, n_half:]
+            assert float(want.abs().max()) < 2 ** 24
+        else:
+            want = torch.relu(z) + 5
+        y = run(x.to(dtype), w, b, None if gated else torch.full_like(want, 5).to(dtype), 'relu', gated, False, dtype)
+        assert torch.equal(y, want.to(dtype)), gated
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F16, BF16])
+def test_the_8_bit_cores_are_as_near_as_documented(dtype):
+    """Normal operands: 1.6e-5 of the result by its 2-norm before the rounding, so a result is within
+    (half a step / sqrt(3) = the rounding's own 2-norm) + 3e-5."""
+    x, w = normal(512, 4096, seed=1).to(dtype).cuda(), normal(512, 4096, seed=2).cuda()
+    y = run(x, w, None, None, 'none', False, False, dtype).double().cpu()
+    want = oracle.values(*block.quantize_blocks(x), 1, 4096) @ oracle.values(*block.quantize_blocks(w, True), 128, 4096).t()
+    assert float((y - want).norm() / want.norm()) < torch.finfo(dtype).eps / 2 / 3 ** 0.5 + 3e-5
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_strides_and_alignment(device):
+    w = normal(70, 300, seed=1).to(device)
+    codes, scales = block.quantize_blocks(w, True)
+    for rows in (5, 90):
+        wide = normal(rows, 2, 340, seed=2).to(device).half()
+        x, r = wide[:, 1, 7:307], normal(rows, 140, seed=3).to(device).half()[:, ::2]
+        want = block.linear_8bit(x.contiguous(), codes, scales, None, r.contiguous())
+        assert torch.equal(block.linear_8bit(x, codes, scales, None, r), want)
+        turned = x.t().contiguous().t()
+        assert torch.equal(block.linear_8bit(turned, codes, scales, None, r), want)
+        # Codes and scales that begin anywhere, and with rows apart.
+        flat = torch.zeros(codes.numel() + 3, dtype=torch.uint8, device=device)
+        flat[3:] = codes.view(torch.uint8).view(-1)
+        moved = flat[3:].view(70, 384).view(torch.float8_e4m3fn)
+        apart = torch.zeros(70, 400, dtype=torch.uint8, device=device)
+        apart[:, 8:392] = codes.view(torch.uint8)
+        odd = torch.zeros(5, dtype=torch.uint8, device=device)
+        odd[1:] = scales.view(torch.uint8).view(-1)
+        for other in (moved, apart[:, 8:392].view(torch.float8_e4m3fn)):
+            assert torch.equal(block.linear_8bit(x, other, scales, None, r), want)
+        assert torch.equal(block.linear_8bit(x, codes, odd[1:].view(1, 4).view(torch.float8_e8m0fnu), None, r), want)
+        xc, xs = block.quantize_blocks(x)
+        assert torch.equal(block.linear_8bit(xc, codes, scales, None, r, scales=xs, dtype=torch.float16), want)
+        batched = block.linear_8bit(x.reshape(rows, 1, 1, 300), codes, scales, None, r.reshape(rows, 1, 1, 70))
+        assert torch.equal(batched.reshape(rows, 70), want)
+    vector = normal(300, seed=4).to(device)
+    assert torch.equal(block.linear_8bit(vector, codes, scales), block.linear_8bit(vector[None], codes, scales)[0])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_empty(device):
+    w, s = block.quantize_blocks(normal(6, 40).to(device), True)
+    assert block.linear_8bit(torch.zeros(0, 40, device=device), w, s).shape == (0, 6)
+    assert block.gated_linear_8bit(torch.zeros(2, 0, 40, device=device), w, s).shape == (2, 0, 3)
+    none, scales = block.quantize_blocks(torch.zeros(0, 40, device=device), True)
+    assert block.linear_8bit(torch.zeros(5, 40, device=device), none, scales).shape == (5, 0)
+    for rows in (3, 80):
+        w, s = block.quantize_blocks(torch.zeros(6, 0, device=device), True)
+        b, r = normal(6).to(device), normal(rows, 6, seed=1).to(device)
+        y = block.linear_8bit(torch.zeros(rows, 0, device=device), w, s, b, r, 'relu')
+        assert torch.equal(y, b.clamp_min(0) + r)
+        gated = block.gated_linear_8bit(torch.zeros(rows, 0, device=device), w, s, b, 'relu')
+        assert torch.equal(gated, (b[:3].clamp_min(0) * b[3:]).expand(rows, 3))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows', [5, 40, 130])
+def test_rows_with_nan_and_infinity_stay_alone(rows, dtype, device):
+    x, w = normal(rows, 300, seed=1).to(dtype).to(device), normal(90, 300, seed=2).to(device)
+    codes, scales = block.quantize_blocks(w, True)
+    want = block.linear_8bit(x, codes, scales)
+    x[1, 5], x[4, 299] = float('nan'), float('inf')
+    y = block.linear_8bit(x, codes, scales)
+    others = [r for r in range(rows) if r not in (1, 4)]
+    assert torch.equal(y[others], want[others]) and bool(torch.isnan(y[[1, 4]]).all())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_wide_ranges_of_scales(device):
+    """Blocks whose powers of two lie far apart: each block's scale reaches its own products."""
+    for rows, dtype in ((4, F32), (4, BF16), (100, F32), (100, BF16)):
+        e = (torch.arange(1100) // 128 * 7 - 30).float()
+        x = integers(rows, 1100, most=2, seed=5) * torch.exp2(e)
+        w = integers(200, 1100, most=1, seed=6) * torch.exp2(-e)
+        x, w = x.to(dtype).to(device), w.to(device)
+        y = run(x, w, None, None, 'none', False, False, dtype)
+        assert torch.equal(y.cpu().double(), (x.double().cpu() @ w.double().cpu().t()).to(dtype).double())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_refusals(device):
+    w = normal(6, 40).to(device)
+    codes, scales = block.quantize_blocks(w, True)
+    x = normal(3, 40, seed=1).to(device)
+    xc, xs = block.quantize_blocks(x)
+
+    def refuse(match, *args, error=RuntimeError, **kwargs):
+        for f in (block.linear_8bit, block.gated_linear_8bit):
+            with pytest.raises(error, match=match):
+                f(*args, **kwargs)
+
+    refuse('x must be float32', x.double(), codes, scales)
+    refuse('codes with their scales', xc, codes, scales)
+    refuse('weight must be float8', x, w, scales)
+    refuse('weight must be float8', x, codes, scales.view(torch.uint8))
+    refuse('tiles of 128 x 128', x[:, :39], codes[:, :64], scales)
+    refuse('tiles of 128 x 128', normal(3, 129).to(device), codes, scales)
+    refuse('tiles of 128 x 128', x, codes, scales[:, :1])
+    refuse('tiles of 128 x 128', x, codes, scales.repeat(2, 1))
+    refuse('bias must be', x, codes, scales, torch.zeros(5, device=device))
+    refuse("bias must have x's dtype", x, codes, scales, torch.zeros(6, device=device).half())
+    refuse('needs dtype', xc, codes, scales, scales=xs)
+    refuse('dtype must be float32', xc, codes, scales, scales=xs, dtype=torch.float64)
+    refuse("dtype must be x's", x, codes, scales, dtype=BF16)
+    refuse('must be float8_e4m3fn codes', x, codes, scales, scales=xs)
+    refuse('whole blocks', xc, codes, scales, scales=xs[:, :1], dtype=F32)
+    refuse('whole blocks', xc[:, :40], codes, scales, scales=xs, dtype=F32)
+    refuse('activation must be', x, codes, scales, activation='tanh', error=ValueError)
+    with pytest.raises(RuntimeError, match='residual must have'):
+        block.linear_8bit(x, codes, scales, None, torch.zeros(3, 5, device=device))
+    with pytest.raises(RuntimeError, match='residual must be'):
+        block.linear_8bit(x, codes, scales, None, torch.zeros(3, 6, device=device).half())
+    odd, odd_scales = block.quantize_blocks(normal(5, 40).to(device), True)
+    with pytest.raises(RuntimeError, match='as many rows of the up'):
+        block.gated_linear_8bit(x, odd, odd_scales)
+    with pytest.raises(RuntimeError, match='a matrix for tiles'):
+        block.quantize_blocks(x[None], True)
+    with pytest.raises(RuntimeError, match='x must be float32'):
+        block.quantize_blocks(x.double())
+    for f in (lambda t: block.linear_8bit(t, codes, scales), lambda t: block.gated_linear_8bit(t, codes, scales),
+              lambda t: block.quantize_blocks(t)[0].float()):
+        leaf = x.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match='not implemented'):
+            (f(leaf).float().sum() + leaf.sum()).backward()
+
+
+@pytest.mark.gpu
+def test_devices_are_refused():
+    w, s = block.quantize_blocks(normal(6, 40).cuda(), True)
+    x = normal(3, 40)
+    with pytest.raises(RuntimeError, match='must be on'):
+        block.linear_8bit(x.cuda(), w.cpu(), s)
+    with pytest.raises(RuntimeError, match='must be on'):
+        block.linear_8bit(x.cuda(), w, s, torch.zeros(6))
+
+
+def test_opcheck():
+    w = normal(300, 600)
+    for tiles in (False, True):
+        torch.library.opcheck(torch.ops.vectra.quantize_blocks.default, (w, tiles), test_utils=('test_schema', 'test_faketensor'))
+    utils = ('test_faketensor',)  # (test_schema multiplies its arguments, which torch's CPU cannot do with e4m3 ones)
+    codes, scales = block.quantize_blocks(w, True)
+    x, r = normal(2, 3, 600).half(), normal(2, 3, 300).half()
+    torch.library.opcheck(torch.ops.vectra.linear_8bit.default, (x, codes, scales, normal(300), r, 'gelu'), test_utils=utils)
+    torch.library.opcheck(torch.ops.vectra.gated_linear_8bit.default, (x, codes, scales, normal(300), 'silu'), test_utils=utils)
+    xc, xs = block.quantize_blocks(x)
+    torch.library.opcheck(torch.ops.vectra.linear_8bit.default, (xc, codes, scales), {'scales': xs, 'dtype': BF16}, test_utils=utils)
+
+
+@pytest.mark.gpu
+def test_streams_and_captured_graphs():
+    """Workspaces of two captured calls are their own; replays follow the inputs."""
+    w = normal(512, 1024, seed=1).cuda()
+    codes, scales = block.quantize_blocks(w, True)
+    graphs = []
+    for rows in (4, 40, 100, 900):
+        x = normal(rows, 1024, seed=rows).cuda().half()
+        block.linear_8bit(x, codes, scales)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = block.linear_8bit(x, codes, scales, None, None, 'gelu')
+            z = block.gated_linear_8bit(x, codes, scales)
+        graphs.append((graph, x, y, z))
+    for _ in range(3):
+        for _, x, *_ in graphs:
+            x.normal_()
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, x, y, z in graphs:
+            assert torch.equal(y, block.linear_8bit(x, codes, scales, None, None, 'gelu'))
+            assert torch.equal(z, block.gated_linear_8bit(x, codes, scales))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [block.linear_8bit(x, codes, scales, None, None, 'gelu') for _, x, *_ in graphs]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, y) for a, (_, _, y, _) in zip(again, graphs))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_norm_into_the_product(device):
+    """A block's way in serving: the branch onto the stream, its norm in 8 bits, the next layer; as the calls one by one."""
+    x, r = normal(90, 700, seed=1).to(device).bfloat16(), normal(90, 700, seed=2).to(device)
+    weight = 1 + 0.1 * normal(700, seed=3).to(device)
+    w1, s1 = block.quantize_blocks(normal(512, 700, seed=4).to(device), True)
+    w2, s2 = block.quantize_blocks(normal(700, 256, seed=5).to(device), True)
+    h, codes, scales = block.residual_norm_8bit(x, r, weight, norm='layer')
+    hidden = block.gated_linear_8bit(codes, w1, s1, scales=scales, dtype=BF16)
+    out = block.linear_8bit(hidden, w2, s2)
+    h2, n = block.residual_norm(x.float(), r, weight, norm='layer')
+    assert torch.equal(h, h2)
+    c2, sc2 = block.quantize_blocks(n)
+    assert torch.equal(as_bytes(codes), as_bytes(c2)) and torch.equal(as_bytes(scales), as_bytes(sc2))
+    xs = oracle.values(c2, sc2, 1, 700)
+    want, bound = oracle.layer(xs, oracle.values(w1, s1, 128, 700), activation='silu', gated=True, dtype=BF16, cores=device != 'cpu')
+    oracle.assert_within(hidden, want, bound)
+    want, bound = oracle.layer(oracle.values(*block.quantize_blocks(hidden), 1, 256), oracle.values(w2, s2, 128, 256), dtype=BF16,
+                               cores=device != 'cpu')
+    oracle.assert_within(out, want, bound)

@@ -7,6 +7,7 @@
 
 #include "block_common.h"
 #include "block_kernels.h"
+#include "product8_kernels.h"
 
 namespace vectra_block {
 namespace {
@@ -157,6 +158,42 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(const T* x, int64_t
       *reinterpret_cast<uint2*>(codes + (row0 + j * 16) * depth + column) = vectra_dense::to_codes(v[j], byte - 127, kHighestExponent);
 }
 
+// Adds up a split product's planes in a fixed order and finishes it with the layer's
+// epilogue: a thread per four columns (a gated layer: of both halves).
+template <typename T, bool kGated>
+__global__ __launch_bounds__(256) void join8_kernel(const float* planes, int parts, int64_t plane_stride, Product8Params p) {
+  constexpr int kHalves = kGated ? 2 : 1;
+  const int64_t quads = (p.n + 3) / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= p.rows * quads) return;
+  const int64_t row = at / quads, column = (at - row * quads) * 4;
+  const int left = static_cast<int>(least(p.n - column, 4));
+  f32x4 z[kHalves];
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    const float* const from = planes + row * plane_stride + h * p.n + column;
+    z[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      f32x4 v;  // (the up half starts at any column; its rows are long enough)
+      __builtin_memcpy(&v, from + k * p.rows * plane_stride, 16);
+      z[h] += v;
+    }
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) z[h][e] += vectra_dense::load_bias(p.bias, h * p.n + column + e, p.bias_dtype);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    z[0][e] = vectra_dense::act_value<T>(z[0][e], p.activation);
+    if constexpr (kGated) z[0][e] *= z[1][e];
+  }
+  if (!kGated && p.residual) z[0] += vectra_dense::load4(static_cast<const T*>(p.residual) + row * p.residual_stride + column, left);
+  vectra_dense::store4(static_cast<T*>(p.out) + row * p.out_stride + column, z[0], left);
+}
+
 // -------------------------------------------------------------------- host
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -204,6 +241,8 @@ int check_stride(int64_t stride, int64_t width, int64_t rows) {
   if (rows > 1 && stride > (int64_t{1} << 40)) return VECTRA_BLOCK_ERR_TOO_LARGE;
   return VECTRA_BLOCK_OK;
 }
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 bool known_threshold(int32_t t) { return t >= 0 && t <= 65535; }
 
@@ -261,6 +300,7 @@ int check_forward(const vectra_norm_args* a) {
   if (a->rows == 0 || a->width == 0) return VECTRA_BLOCK_OK;
   if (!a->x || !a->residual || !a->h || (!a->n && (!a->codes || !a->scales))) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
   if (a->threshold && !a->rng) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
+  if (!a->n && !aligned(a->codes, 16)) return VECTRA_BLOCK_ERR_BAD_SHAPE;
   if (int st = check_stride(a->x_stride, a->width, a->rows)) return st;
   if (int st = check_stride(a->residual_stride, a->width, a->rows)) return st;
   if (int st = check_stride(a->h_stride, a->width, a->rows)) return st;
@@ -454,6 +494,135 @@ int backward(const vectra_norm_grad_args& a, Scratch& scratch, bool launch, int 
   return launched();
 }
 
+// ------------------------------------------------------------- products in 8 bits
+
+int check_linear8(const vectra_linear8_args* a) {
+  if (!a) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
+  if (a->struct_size != static_cast<int64_t>(sizeof(vectra_linear8_args))) return VECTRA_BLOCK_ERR_BAD_STRUCT;
+  if (!known_dtype(a->dtype)) return VECTRA_BLOCK_ERR_BAD_DTYPE;
+  if (!vector_dtype(a->bias, a->bias_dtype, a->dtype)) return VECTRA_BLOCK_ERR_BAD_DTYPE;
+  if (a->activation < VECTRA_DENSE_NONE || a->activation > VECTRA_DENSE_SILU) return VECTRA_BLOCK_ERR_BAD_OPTION;
+  if ((a->gated != 0 && a->gated != 1) || (a->gated && a->residual)) return VECTRA_BLOCK_ERR_BAD_SHAPE;
+  if (int st = check_sizes(a->rows, a->width)) return st;
+  if (int st = check_sizes(a->rows, a->width_out * (1 + a->gated))) return st;
+  if (a->rows == 0 || a->width_out == 0) return VECTRA_BLOCK_OK;
+  if (!a->out || (a->width && (!a->weight || !a->weight_scales || (!a->x && (!a->codes || !a->scales)))))
+    return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
+  if (a->width) {
+    if (!aligned(a->weight, 16) || !aligned(a->weight_scales, 4)) return VECTRA_BLOCK_ERR_BAD_SHAPE;
+    if (!a->x && (!aligned(a->codes, 16) || !aligned(a->scales, 4))) return VECTRA_BLOCK_ERR_BAD_SHAPE;
+  }
+  // Offsets within a tile's operands, and from a gate's row to its up row, have 31 bits.
+  const int64_t depth = ceil_div(a->width, 128) * 128;
+  if ((a->gated * a->width_out + 256) * depth >= int64_t{1} << 31) return VECTRA_BLOCK_ERR_TOO_LARGE;
+  if (a->x)
+    if (int st = check_stride(a->x_stride, a->width, a->rows)) return st;
+  if (a->residual)
+    if (int st = check_stride(a->residual_stride, a->width_out, a->rows)) return st;
+  return check_stride(a->out_stride, a->width_out, a->rows);
+}
+
+// The tile and the number of contraction parts with the least estimated time.
+//   kRate      of all CUs, full, by tile (16-bit results; fp32's)
+//   kResident  workgroups that a CU holds; one that holds fewer runs at kPart of the rate
+//   kBatch     a workgroup's first loads and its epilogue
+// Tiles' operands pass from L2 to LDS at 16 TB/s.  A split costs its fp32 planes,
+// written and read at 5 TB/s, and the joining launch.
+void choose8(const Product8Params& p, int64_t columns, int32_t dtype, int cus, int& tile, int& parts) {
+  static constexpr double kRate16[kTiles8] = {2.4e15, 1.7e15, 1.0e15}, kRate32[kTiles8] = {0, 0.9e15, 0.6e15};
+  static constexpr int kResident[kTiles8] = {1, 2, 5};
+  static constexpr double kPart[kTiles8][5] = {{1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
+  static constexpr double kBatch[kTiles8] = {4e-6, 2e-6, 1.5e-6};
+  const bool precise = dtype == VECTRA_BLOCK_F32;
+  double best = 1e30;
+  tile = kSmall8;
+  parts = 1;
+  for (int t = precise ? kMedium8 : kLarge8; t < kTiles8; ++t) {
+    const int64_t tiles = ceil_div(p.rows, kTile8[t]) * ceil_div(columns, kTile8[t]);
+    const double rate = (precise ? kRate32[t] : kRate16[t]) / 256;
+    for (int k = 1; k <= std::max(1, std::min(16, p.k_tiles / 2)); k *= 2) {
+      const int64_t depth = ceil_div(p.k_tiles, k) * 128;
+      const int64_t per_cu = ceil_div(tiles * k, cus);
+      const int together = static_cast<int>(std::min<int64_t>(per_cu, kResident[t]));
+      const double products = per_cu * 2.0 * kTile8[t] * kTile8[t] * depth / (rate * kPart[t][together - 1]);
+      const double traffic = tiles * k * 2.0 * kTile8[t] * depth / 16e12;
+      const double join = k > 1 ? 8.0 * k * p.rows * columns / 5e12 + 4e-6 : 0;
+      const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
+      if (time < best * 0.98) {
+        best = time;
+        tile = t;
+        parts = k;
+      }
+    }
+  }
+}
+
+int linear8(const vectra_linear8_args& a, Scratch& scratch, bool launch, int cus, hipStream_t stream) {
+  if (a.rows == 0 || a.width_out == 0) return VECTRA_BLOCK_OK;
+  Product8Params p{};
+  p.rows = a.rows;
+  p.n = a.width_out;
+  p.width = a.width;
+  p.depth = ceil_div(a.width, 128) * 128;
+  p.scale_stride = ceil_div(a.width, 512) * 4;
+  p.weight = static_cast<const uint8_t*>(a.weight);
+  p.weight_scales = static_cast<const uint8_t*>(a.weight_scales);
+  p.codes = static_cast<const uint8_t*>(a.codes);
+  p.scales = static_cast<const uint8_t*>(a.scales);
+  p.bias = a.bias;
+  p.bias_dtype = a.bias_dtype;
+  p.activation = a.activation;
+  p.residual = a.residual;
+  p.residual_stride = a.residual_stride;
+  p.out = a.out;
+  p.out_stride = a.out_stride;
+  if (launch) (void)hipGetLastError();  // an error left by other work is not this call's
+  if (a.x && a.rows <= kFewRaw8) {
+    p.x = a.x;
+    p.x_stride = a.x_stride;
+  } else if (a.x) {
+    uint8_t* const codes = static_cast<uint8_t*>(scratch.take(a.rows * p.depth));
+    uint8_t* const scales = static_cast<uint8_t*>(scratch.take(a.rows * p.scale_stride));
+    p.codes = codes;
+    p.scales = scales;
+    if (launch && a.width)
+      if (int st = quantize(a.x, a.dtype, a.rows, a.width, a.x_stride, false, codes, scales, stream)) return st;
+  }
+  if (a.rows <= kFewRows8) {
+    if (!launch) return VECTRA_BLOCK_OK;
+    const auto f = a.dtype == VECTRA_BLOCK_F32 ? launch_few8_f32 : a.dtype == VECTRA_BLOCK_F16 ? launch_few8_f16 : launch_few8_bf16;
+    return f(p, a.gated, stream);
+  }
+  const int64_t columns = a.gated ? 2 * p.n : p.n;
+  p.k_tiles = static_cast<int32_t>(p.depth / 128);
+  int tile, parts;
+  choose8(p, columns, a.dtype, cus, tile, parts);
+  p.tiles_m = static_cast<int32_t>(ceil_div(p.rows, kTile8[tile]));
+  p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTile8[tile]));
+  p.k_tiles_per_part = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, parts)));
+  parts = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_part)));
+  const auto f = a.dtype == VECTRA_BLOCK_F32   ? launch_product8_f32
+                 : a.dtype == VECTRA_BLOCK_F16 ? launch_product8_f16
+                                               : launch_product8_bf16;
+  if (parts == 1) return launch ? f(p, tile, a.gated ? kGated8 : kStore8, 1, stream) : VECTRA_BLOCK_OK;
+  // Planes of four-column pieces; the join reads such pieces of the up half from
+  // column n on.
+  const int64_t ld = ceil_div(a.gated ? p.n + ceil_div(p.n, 4) * 4 : columns, 4) * 4;
+  Product8Params q = p;
+  q.n = columns;
+  q.out = scratch.take(parts * p.rows * ld * 4);
+  q.out_stride = ld;
+  if (!launch) return VECTRA_BLOCK_OK;
+  if (int st = f(q, tile, kPartial8, parts, stream)) return st;
+  typed(a.dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    const auto kernel = a.gated ? join8_kernel<T, true> : join8_kernel<T, false>;
+    kernel<<<static_cast<uint32_t>(ceil_div(p.rows * ceil_div(p.n, 4), 256)), 256, 0, stream>>>(
+        static_cast<const float*>(q.out), parts, ld, p);
+  });
+  return launched();
+}
+
 }  // namespace
 }  // namespace vectra_block
 
@@ -517,9 +686,29 @@ int vectra_blocks_quantize(const void* x, int32_t dtype, int64_t rows, int64_t w
   if (int st = check_sizes(rows, width)) return st;
   if (rows == 0 || width == 0) return VECTRA_BLOCK_OK;
   if (!x || !codes || !scales) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
+  if (!aligned(codes, 16)) return VECTRA_BLOCK_ERR_BAD_SHAPE;
   if (int st = check_stride(x_stride, width, rows)) return st;
   (void)hipGetLastError();
   return quantize(x, dtype, rows, width, x_stride, tiles, codes, scales, reinterpret_cast<hipStream_t>(stream));
+}
+
+int vectra_linear8_forward(const vectra_linear8_args* args, void* workspace, int64_t workspace_bytes,
+                           vectra_block_stream_t stream) {
+  if (int st = check_linear8(args)) return st;
+  const int cus = compute_units();
+  Scratch sized{nullptr, 0};
+  if (int st = linear8(*args, sized, false, cus, nullptr)) return st;
+  if (sized.used > 0 && (!workspace || workspace_bytes < sized.used || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return VECTRA_BLOCK_ERR_WORKSPACE;
+  Scratch scratch{static_cast<char*>(workspace), 0};
+  return linear8(*args, scratch, true, cus, reinterpret_cast<hipStream_t>(stream));
+}
+
+int64_t vectra_linear8_workspace_bytes(const vectra_linear8_args* args) {
+  if (int st = check_linear8(args)) return -st;
+  Scratch sized{nullptr, 0};
+  if (int st = linear8(*args, sized, false, compute_units(), nullptr)) return -st;
+  return sized.used;
 }
 
 const char* vectra_block_status_string(int status) {

@@ -3,6 +3,10 @@
 //   residual_norm           a branch onto the residual stream, and the stream's norm
 //   residual_norm_8bit      the same with the norm in 8-bit rows
 //   residual_norm_backward  residual_norm's gradients
+//   quantize_blocks         a matrix in 8 bits: rows of 128, or tiles of 128 x 128, that
+//                           share a power of two
+//   linear_8bit             act(x^ W^T + b) + residual on such codes
+//   gated_linear_8bit       act(x^ G^T + b_g) * (x^ U^T + b_u)
 //
 //   CUDA key (HIP tensors on ROCm)  -> libvectra_block.so (include/vectra_block.h),
 //                                      on the caller's current HIP stream, with
@@ -598,6 +602,187 @@ std::vector<Tensor> residual_norm_backward_cpu(const OptTensor& grad_h, const Op
   return out;
 }
 
+// ------------------------------------------------------------- products in 8 bits
+
+std::tuple<Tensor, Tensor> check_quantised(const Tensor& x, bool tiles) {
+  constexpr const char* op = "vectra::quantize_blocks";
+  TORCH_CHECK(x.dim() >= 1 && (!tiles || x.dim() == 2), op, ": x must be ", tiles ? "a matrix for tiles" : "[..., width]",
+              "; got ", x.sizes());
+  TORCH_CHECK(is_float(x.scalar_type()), op, ": x must be float32, float16 or bfloat16; got ", x.scalar_type());
+  std::vector<int64_t> sizes = scales_sizes(x);
+  if (tiles) sizes[0] = (sizes[0] + 127) / 128;
+  return {at::empty(codes_sizes(x), x.options().dtype(at::kFloat8_e4m3fn)),
+          at::empty(sizes, x.options().dtype(at::kFloat8_e8m0fnu))};
+}
+
+std::tuple<Tensor, Tensor> quantize_blocks_hip(const Tensor& x, bool tiles) {
+  c10::DeviceGuard guard(x.device());
+  auto [codes, scales] = check_quantised(x, tiles);
+  const Rows xr = as_rows(x);
+  check_status(vectra_blocks_quantize(xr.t.data_ptr(), dense_dtype(x.scalar_type()), rows_of(x), x.size(-1), xr.stride, tiles,
+                                      codes.data_ptr(), scales.data_ptr(), stream_of(x)),
+               "vectra::quantize_blocks");
+  return {codes, scales};
+}
+
+std::tuple<Tensor, Tensor> quantize_blocks_cpu(const Tensor& x, bool tiles) {
+  auto [codes, scales] = check_quantised(x, tiles);
+  const auto [c, s] = quantize_cpu(wide(x).reshape({rows_of(x), x.size(-1)}), tiles ? 128 : 1);
+  return {c.reshape(codes.sizes()), s.reshape(scales.sizes())};
+}
+
+// A layer's arguments: the result's type and the contraction's width.
+struct Layer8 {
+  at::ScalarType dtype;
+  int64_t width, n_w;
+};
+
+Layer8 check_layer8(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
+                    const OptTensor& residual, const OptTensor& scales, std::optional<at::ScalarType> dtype, bool gated,
+                    const char* op) {
+  TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && weight_scales.dim() == 2, op,
+              ": x must be [..., width], weight and weight_scales matrices; got ", x.sizes(), ", ", weight.sizes(), " and ",
+              weight_scales.sizes());
+  TORCH_CHECK(weight.scalar_type() == at::kFloat8_e4m3fn && weight_scales.scalar_type() == at::kFloat8_e8m0fnu, op,
+              ": weight must be float8_e4m3fn codes with float8_e8m0fnu scales; got ", weight.scalar_type(), " and ",
+              weight_scales.scalar_type());
+  Layer8 l{x.scalar_type(), x.size(-1), weight.size(0)};
+  if (has(scales)) {
+    TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && scales->scalar_type() == at::kFloat8_e8m0fnu, op,
+                ": an input given with scales must be float8_e4m3fn codes and float8_e8m0fnu scales; got ", x.scalar_type(),
+                " and ", scales->scalar_type());
+    TORCH_CHECK(l.width % 128 == 0 && scales->sizes() == at::IntArrayRef(scales_sizes(x)), op,
+                ": codes must be whole blocks of 128 and scales [..., 4 ceil(width / 512)]; got ", x.sizes(), " and ",
+                scales->sizes());
+    TORCH_CHECK(dtype.has_value(), op, ": an input in 8 bits needs dtype, the result's");
+    TORCH_CHECK(is_float(*dtype), op, ": dtype must be float32, float16 or bfloat16; got ", *dtype);
+    TORCH_CHECK(scales->device() == x.device(), op, ": scales must be on ", x.device(), "; got ", scales->device());
+    l.dtype = *dtype;
+  } else {
+    TORCH_CHECK(is_float(l.dtype), op, ": x must be float32, float16 or bfloat16, or codes with their scales; got ", l.dtype);
+    TORCH_CHECK(!dtype.has_value() || *dtype == l.dtype, op, ": dtype must be x's, ", l.dtype, "; got ", *dtype);
+  }
+  TORCH_CHECK(weight.size(1) == (l.width + 127) / 128 * 128 && weight_scales.size(0) == (l.n_w + 127) / 128 &&
+                  weight_scales.size(1) == (l.width + 511) / 512 * 4,
+              op, ": weight must be [width_out, width] in tiles of 128 x 128, as quantize_blocks makes it; got ",
+              weight.sizes(), " with scales ", weight_scales.sizes(), " for x ", x.sizes());
+  TORCH_CHECK(!gated || l.n_w % 2 == 0, op, ": weight must hold the gate's rows and as many rows of the up projection; got ",
+              weight.sizes());
+  TORCH_CHECK(weight.device() == x.device() && weight_scales.device() == x.device(), op, ": weight and weight_scales must be on ",
+              x.device(), "; got ", weight.device(), " and ", weight_scales.device());
+  if (has(bias)) check_vector(bias, l.n_w, l.dtype, x.device(), "bias", op);
+  if (has(residual)) {
+    TORCH_CHECK(residual->sizes() == at::IntArrayRef(with_last(x, l.n_w)), op, ": residual must have the output's shape; got ",
+                residual->sizes());
+    TORCH_CHECK(residual->scalar_type() == l.dtype && residual->device() == x.device(), op, ": residual must be ", l.dtype, " on ",
+                x.device(), "; got ", residual->scalar_type(), " on ", residual->device());
+  }
+  return l;
+}
+
+// Bytes that lie one row after the other, from a multiple of 16 bytes on.
+Tensor packed(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone() : c;
+}
+
+Tensor layer8_hip(const Tensor& x, const Tensor& weight_in, const Tensor& weight_scales_in, const OptTensor& bias_in,
+                  const OptTensor& residual, c10::string_view activation, const OptTensor& scales_in,
+                  std::optional<at::ScalarType> dtype, bool gated, const char* op) {
+  const Layer8 l = check_layer8(x, weight_in, weight_scales_in, bias_in, residual, scales_in, dtype, gated, op);
+  const int32_t act = activation_of(activation, op);
+  c10::DeviceGuard guard(x.device());
+  const int64_t n = gated ? l.n_w / 2 : l.n_w;
+  Tensor out = at::empty(with_last(x, n), x.options().dtype(l.dtype));
+  const Tensor weight = packed(weight_in), weight_scales = packed(weight_scales_in);
+  const Tensor bias = has(bias_in) ? bias_in->contiguous() : Tensor();
+  Rows xr, rr;
+  Tensor codes, scales;
+  vectra_linear8_args a{};
+  a.struct_size = sizeof(a);
+  if (has(scales_in)) {
+    codes = packed(x);
+    scales = packed(*scales_in);
+    a.codes = codes.data_ptr();
+    a.scales = scales.data_ptr();
+  } else {
+    xr = as_rows(x);
+    a.x = xr.t.data_ptr();
+  }
+  if (has(residual)) rr = as_rows(*residual);
+  a.weight = weight.data_ptr();
+  a.weight_scales = weight_scales.data_ptr();
+  a.bias = bias.defined() ? bias.data_ptr() : nullptr;
+  a.residual = rr.t.defined() ? rr.t.data_ptr() : nullptr;
+  a.out = out.data_ptr();
+  a.dtype = dense_dtype(l.dtype);
+  a.bias_dtype = bias.defined() ? dense_dtype(bias.scalar_type()) : a.dtype;
+  a.activation = act;
+  a.gated = gated;
+  a.rows = rows_of(x);
+  a.width = l.width;
+  a.width_out = n;
+  a.x_stride = xr.stride;
+  a.residual_stride = rr.stride;
+  a.out_stride = std::max<int64_t>(n, 1);
+  const int64_t need = vectra_linear8_workspace_bytes(&a);
+  if (need < 0) check_status(static_cast<int>(-need), op);
+  Tensor workspace;
+  if (need > 0) workspace = at::empty({need}, x.options().dtype(at::kByte));
+  check_status(vectra_linear8_forward(&a, need > 0 ? workspace.data_ptr() : nullptr, need, stream_of(x)), op);
+  return out;
+}
+
+// What codes and scales stand for, in fp32 [rows, depth].
+Tensor values_cpu(const Tensor& codes_in, const Tensor& scales_in, int64_t high) {
+  const Tensor codes = codes_in.reshape({-1, codes_in.size(-1)});
+  const Tensor e = scales_in.contiguous().view(at::kByte).reshape({-1, scales_in.size(-1)}).to(at::kInt) - 127;
+  const Tensor each = e.narrow(1, 0, codes.size(1) / 128).repeat_interleave(high, 0).narrow(0, 0, codes.size(0)).repeat_interleave(128, 1);
+  const Tensor value = at::ldexp(codes.to(at::kDouble), each);
+  return at::where(each == 128, at::full_like(value, std::nan("")), value).to(at::kFloat);
+}
+
+Tensor layer8_cpu(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
+                  const OptTensor& residual, c10::string_view activation, const OptTensor& scales,
+                  std::optional<at::ScalarType> dtype, bool gated, const char* op) {
+  const Layer8 l = check_layer8(x, weight, weight_scales, bias, residual, scales, dtype, gated, op);
+  const int32_t act = activation_of(activation, op);
+  const int64_t rows = rows_of(x), n = gated ? l.n_w / 2 : l.n_w;
+  if (rows == 0 || n == 0) return at::empty(with_last(x, n), x.options().dtype(l.dtype));
+  Tensor z;
+  if (l.width == 0) {
+    z = at::zeros({rows, l.n_w}, x.options().dtype(at::kFloat));
+  } else {
+    const auto [c, s] = has(scales) ? std::tuple<Tensor, Tensor>(x, *scales) : quantize_cpu(wide(x).reshape({rows, l.width}), 1);
+    z = at::matmul(values_cpu(c, s, 1), values_cpu(weight, weight_scales, 128).t());
+  }
+  if (has(bias)) z = z + wide(*bias);
+  Tensor y;
+  if (gated) {
+    const auto halves = z.chunk(2, -1);
+    y = activation_cpu(halves[0], act).first * halves[1];
+  } else {
+    y = act == VECTRA_DENSE_NONE ? z : activation_cpu(z, act).first;
+  }
+  if (has(residual)) y = y + wide(*residual).reshape({rows, n});
+  return y.to(l.dtype).reshape(with_last(x, n)).contiguous();
+}
+
+template <Tensor (*kLayer)(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::string_view,
+                           const OptTensor&, std::optional<at::ScalarType>, bool, const char*)>
+Tensor linear_8bit(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
+                   const OptTensor& residual, c10::string_view activation, const OptTensor& scales,
+                   std::optional<at::ScalarType> dtype) {
+  return kLayer(x, weight, weight_scales, bias, residual, activation, scales, dtype, false, "vectra::linear_8bit");
+}
+
+template <Tensor (*kLayer)(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::string_view,
+                           const OptTensor&, std::optional<at::ScalarType>, bool, const char*)>
+Tensor gated_linear_8bit(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
+                         c10::string_view activation, const OptTensor& scales, std::optional<at::ScalarType> dtype) {
+  return kLayer(x, weight, weight_scales, bias, std::nullopt, activation, scales, dtype, true, "vectra::gated_linear_8bit");
+}
+
 // --------------------------------------------------------------- gradients
 
 Tensor call_dropout(const Tensor& x, double p, const Tensor& rng, int64_t stream) {
@@ -769,6 +954,13 @@ TORCH_LIBRARY_FRAGMENT(vectra, m) {
       "residual_norm_backward(Tensor? grad_h, Tensor? grad_n, Tensor? h, Tensor? x, Tensor? residual, Tensor? weight, "
       "Tensor? bias, Tensor? gate, Tensor? post_weight, Tensor? post_bias, str norm, str post, float eps, "
       "float residual_scale, float p, Tensor? rng, int stream, ScalarType dtype, bool[7] wanted) -> Tensor[]");
+  m.def("quantize_blocks(Tensor x, bool tiles=False) -> (Tensor, Tensor)");
+  m.def(
+      "linear_8bit(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None, Tensor? residual=None, "
+      "str activation='none', *, Tensor? scales=None, ScalarType? dtype=None) -> Tensor");
+  m.def(
+      "gated_linear_8bit(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None, str activation='silu', *, "
+      "Tensor? scales=None, ScalarType? dtype=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(vectra, CUDA, m) {
@@ -776,6 +968,9 @@ TORCH_LIBRARY_IMPL(vectra, CUDA, m) {
   m.impl("residual_norm", residual_norm_hip);
   m.impl("residual_norm_8bit", residual_norm_8bit_hip);
   m.impl("residual_norm_backward", residual_norm_backward_hip);
+  m.impl("quantize_blocks", quantize_blocks_hip);
+  m.impl("linear_8bit", linear_8bit<layer8_hip>);
+  m.impl("gated_linear_8bit", gated_linear_8bit<layer8_hip>);
 }
 
 TORCH_LIBRARY_IMPL(vectra, CPU, m) {
@@ -783,6 +978,9 @@ TORCH_LIBRARY_IMPL(vectra, CPU, m) {
   m.impl("residual_norm", residual_norm_cpu);
   m.impl("residual_norm_8bit", residual_norm_8bit_cpu);
   m.impl("residual_norm_backward", residual_norm_backward_cpu);
+  m.impl("quantize_blocks", quantize_blocks_cpu);
+  m.impl("linear_8bit", linear_8bit<layer8_cpu>);
+  m.impl("gated_linear_8bit", gated_linear_8bit<layer8_cpu>);
 }
 
 TORCH_LIBRARY_IMPL(vectra, Autograd, m) {
@@ -792,4 +990,7 @@ TORCH_LIBRARY_IMPL(vectra, Autograd, m) {
   // does a tangent.
   m.impl("residual_norm_8bit", torch::autograd::autogradNotImplementedFallback());
   m.impl("residual_norm_backward", torch::autograd::autogradNotImplementedFallback());
+  m.impl("quantize_blocks", torch::autograd::autogradNotImplementedFallback());
+  m.impl("linear_8bit", torch::autograd::autogradNotImplementedFallback());
+  m.impl("gated_linear_8bit", torch::autograd::autogradNotImplementedFallback());
 }

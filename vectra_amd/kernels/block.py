@@ -1,5 +1,5 @@
 """What stands between the dense operators of a Transformer block on MI355X:
-dropout, and the residual stream with its norms.
+dropout, and the residual stream with its norms; and those operators in 8 bits.
 
   y = torch.ops.vectra.dropout(x, p, rng, stream=0)
   h, n = torch.ops.vectra.residual_norm(
@@ -11,8 +11,15 @@ dropout, and the residual stream with its norms.
       next branch reads, in one pass
   h, codes, scales = torch.ops.vectra.residual_norm_8bit(...the same...)
       n in 8-bit rows, as torch.ops.vectra.linear_8bit reads them
+  codes, scales = torch.ops.vectra.quantize_blocks(x, tiles=False)
+  y = torch.ops.vectra.linear_8bit(x, weight, weight_scales, bias=None,
+      residual=None, activation='none', *, scales=None, dtype=None)
+      act(x @ weight.T + bias) + residual, x and weight in 8 bits
+  y = torch.ops.vectra.gated_linear_8bit(x, weight, weight_scales, bias=None,
+      activation='silu', *, scales=None, dtype=None)
+      act(x @ gate.T + b_g) * (x @ up.T + b_u), weight = cat([gate, up])
 
-x [..., width] is float32, float16 or bfloat16 (any strides; views without unit
+Dropout and norms.  x [..., width] is float32, float16 or bfloat16 (any strides; views without unit
 element stride are copied); the residual, of x's shape, has x's type or float32
 (a stream wider than its branches), and h has the residual's, n x's.  Rows of a
 norm have at most 16,384 elements.  norm is 'rms' or 'layer', post 'none', 'rms'
@@ -45,7 +52,26 @@ norm, else h.  Gradients of gradients (of residual_norm) and forward-mode
 derivatives are refused, and so is any derivative of residual_norm_8bit, a serving
 form.  The gradients of the vectors are summed in fp32 in a fixed order.
 
-A backward pass may be captured into a HIP graph through
+Products in 8 bits, for serving.  quantize_blocks brings a matrix into e4m3 codes
+whose blocks share a power of two, the smallest that no element exceeds 448 times:
+128 consecutive elements of a row, for inputs, or with tiles=True tiles of 128 x 128,
+for weights, once when a model is loaded.  codes are float8_e4m3fn [..., width
+rounded up to 128] (zeros behind the width), scales float8_e8m0fnu
+[..., 4 ceil(width / 512)] (a tile's: [ceil(rows / 128), ...]; those past
+ceil(width / 128) are not used).  A layer takes float32, float16 or bfloat16 inputs,
+which it brings into 8 bits itself, and returns their type; or codes with `scales`
+(residual_norm_8bit's, or quantize_blocks'), and returns `dtype`.  bias is the
+result's type or float32, the residual the result's type.
+
+float32 results, and those of at most 64 rows, are exact products of the 8-bit values
+in fp32 sums, rounded once.  float16 and bfloat16 results of more rows come from the
+8-bit matrix cores, which drop, of the 16 products that they add at a time, what lies
+below 2^-13 of the largest one's power of two: with normal operands 1.6e-5 of a
+result, where the rounding to bfloat16 is 1.7e-3 and to float16 2.1e-4.  They have no
+derivative: a backward pass through them raises.  Under torch.autocast they run in
+their input's type.
+
+Gradients.  A backward pass may be captured into a HIP graph through
 torch.ops.vectra.residual_norm_backward, which autograd calls, and through
 torch.ops.vectra.dropout on the gradient.  (Capturing torch.autograd.grad itself
 while an eager graph over the same leaves is alive fails in autograd's own stream
@@ -107,6 +133,26 @@ def _residual_norm_backward_fake(grad_h, grad_n, h, x, residual, weight, bias, g
     return [make() for make, want in zip(made, wanted) if want]
 
 
+@torch.library.register_fake('vectra::quantize_blocks')
+def _quantize_blocks_fake(x, tiles=False):
+    scales = list(_scales_shape(x.shape))
+    if tiles:
+        scales[0] = (scales[0] + BLOCK - 1) // BLOCK
+    return (x.new_empty(_codes_shape(x.shape), dtype=torch.float8_e4m3fn), x.new_empty(scales, dtype=torch.float8_e8m0fnu))
+
+
+@torch.library.register_fake('vectra::linear_8bit')
+def _linear_8bit_fake(x, weight, weight_scales, bias=None, residual=None, activation='none', *, scales=None, dtype=None):
+    del weight_scales, bias, residual, activation, scales
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dtype)
+
+
+@torch.library.register_fake('vectra::gated_linear_8bit')
+def _gated_linear_8bit_fake(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None):
+    del weight_scales, bias, activation, scales
+    return x.new_empty((*x.shape[:-1], weight.shape[0] // 2), dtype=dtype)
+
+
 def dropout(x, p, rng, stream=0):
     """x with elements dropped and the others scaled (torch.ops.vectra.dropout)."""
     return torch.ops.vectra.dropout(x, p, rng, stream)
@@ -120,3 +166,18 @@ def residual_norm(x, residual, weight=None, bias=None, gate=None, post_weight=No
 def residual_norm_8bit(x, residual, weight=None, bias=None, gate=None, post_weight=None, post_bias=None, **options):
     """residual_norm with n in 8-bit rows: (h, codes, scales) (torch.ops.vectra.residual_norm_8bit)."""
     return torch.ops.vectra.residual_norm_8bit(x, residual, weight, bias, gate, post_weight, post_bias, **options)
+
+
+def quantize_blocks(x, tiles=False):
+    """x in 8 bits: (codes, scales) (torch.ops.vectra.quantize_blocks)."""
+    return torch.ops.vectra.quantize_blocks(x, tiles)
+
+
+def linear_8bit(x, weight, weight_scales, bias=None, residual=None, activation='none', *, scales=None, dtype=None):
+    """act(x @ weight.T + bias) + residual in 8 bits (torch.ops.vectra.linear_8bit)."""
+    return torch.ops.vectra.linear_8bit(x, weight, weight_scales, bias, residual, activation, scales=scales, dtype=dtype)
+
+
+def gated_linear_8bit(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None):
+    """act(x @ gate.T + b_g) * (x @ up.T + b_u) in 8 bits (torch.ops.vectra.gated_linear_8bit)."""
+    return torch.ops.vectra.gated_linear_8bit(x, weight, weight_scales, bias, activation, scales=scales, dtype=dtype)
