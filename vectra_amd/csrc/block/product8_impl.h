@@ -123,28 +123,30 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
     b_bytes -= 128;
   };
 
-  // ---- the scales of this lane's rows (clamped: those past the end are not stored)
-  const uint32_t* a_scale[C::kTM];
-  const uint32_t* b_scale[C::kTN];
+  // ---- the scales of this lane's rows (clamped: those past the end are not stored),
+  // as offsets in words from the tile's first
+  const uint32_t* const a_scales = reinterpret_cast<const uint32_t*>(p.scales + m0 * p.scale_stride);
+  const uint32_t* const b_scales = reinterpret_cast<const uint32_t*>(p.weight_scales);
+  const int words = static_cast<int>(p.scale_stride / 4);
+  uint32_t a_scale[C::kTM], b_scale[C::kTN];
 #pragma unroll
   for (int t = 0; t < C::kTM; ++t)
-    a_scale[t] = reinterpret_cast<const uint32_t*>(p.scales + least(m0 + (wm * C::kTM + t) * 32 + i, p.rows - 1) * p.scale_stride);
+    a_scale[t] = static_cast<uint32_t>(least((wm * C::kTM + t) * 32 + i, p.rows - 1 - m0)) * words;
 #pragma unroll
   for (int t = 0; t < C::kTN; ++t) {
     bool there;
     const int64_t row = weight_row((wn * C::kTN + t) * 32 + i, there);
-    b_scale[t] = reinterpret_cast<const uint32_t*>(p.weight_scales + (there ? row / 128 : 0) * p.scale_stride);
+    b_scale[t] = static_cast<uint32_t>(there ? row / 128 : 0) * words;
   }
-  const int words = static_cast<int>(p.scale_stride / 4);
   struct Scales {
     uint32_t a[C::kTM], b[C::kTN];
-  } now, next;
+  } now;
   const auto load_scales = [&](Scales& s, int word) {
     const int at = min(word, words - 1);
 #pragma unroll
-    for (int t = 0; t < C::kTM; ++t) s.a[t] = a_scale[t][at];
+    for (int t = 0; t < C::kTM; ++t) s.a[t] = a_scales[a_scale[t] + at];
 #pragma unroll
-    for (int t = 0; t < C::kTN; ++t) s.b[t] = b_scale[t][at];
+    for (int t = 0; t < C::kTN; ++t) s.b[t] = b_scales[b_scale[t] + at];
   };
 
   f32x16 acc[C::kTN][C::kTM];
@@ -164,32 +166,37 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
           tile + row * 128 + (((step * 4 + 2 * j + half) ^ A::swizzle(i)) * 16));
     return f;
   };
-  const auto read = [&](Frag8(&fa)[C::kTM], Frag8(&fb)[C::kTN], int buf, int step) {
-    const lds_char* const ta = smem + buf * C::kStageBytes;
-    const lds_char* const tb = ta + A::kBytes;
+  // The products of a step, and the fragments of the step after it: W's first, x's
+  // each into the registers of the one just used, so that little more than one step's
+  // are held at a time.
+  Frag8 fa[C::kTM], fb[C::kTN];
+  const auto read_b = [&](Frag8(&f)[C::kTN], int buf, int step) {
+    const lds_char* const tb = smem + buf * C::kStageBytes + A::kBytes;
 #pragma unroll
-    for (int t = 0; t < C::kTN; ++t) fb[t] = read_one(tb, (wn * C::kTN + t) * 32, step);
-#pragma unroll
-    for (int t = 0; t < C::kTM; ++t) fa[t] = read_one(ta, (wm * C::kTM + t) * 32, step);
+    for (int u = 0; u < C::kTN; ++u) f[u] = read_one(tb, (wn * C::kTN + u) * 32, step);
   };
-  const auto multiply = [&](const Frag8(&fa)[C::kTM], const Frag8(&fb)[C::kTN], int shift) {
+  const auto read_a = [&](int t, int buf, int step) {
+    return read_one(smem + buf * C::kStageBytes, (wm * C::kTM + t) * 32, step);
+  };
+  const auto step = [&](int shift, int buf, int next_step) {
+    Frag8 fb_next[C::kTN];
+    read_b(fb_next, buf, next_step);
     if constexpr (C::kPrecise) {
-      float sa[C::kTM], sb[C::kTN];
-#pragma unroll
-      for (int t = 0; t < C::kTM; ++t) sa[t] = scale_of(now.a[t] >> shift & 255);
+      float sb[C::kTN];
 #pragma unroll
       for (int u = 0; u < C::kTN; ++u) sb[u] = scale_of(now.b[u] >> shift & 255);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 xa[C::kTM];
+      for (int t = 0; t < C::kTM; ++t) {
+        const float sa = scale_of(now.a[t] >> shift & 255);
 #pragma unroll
-        for (int t = 0; t < C::kTM; ++t) xa[t] = decode(fa[t].w[j / 2][j % 2 * 2], fa[t].w[j / 2][j % 2 * 2 + 1], sa[t]);
+        for (int j = 0; j < 4; ++j) {
+          const bf16x8 xa = decode(fa[t].w[j / 2][j % 2 * 2], fa[t].w[j / 2][j % 2 * 2 + 1], sa);
 #pragma unroll
-        for (int u = 0; u < C::kTN; ++u) {
-          const bf16x8 xb = decode(fb[u].w[j / 2][j % 2 * 2], fb[u].w[j / 2][j % 2 * 2 + 1], sb[u]);
-#pragma unroll
-          for (int t = 0; t < C::kTM; ++t) acc[u][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[t], acc[u][t], 0, 0, 0);
+          for (int u = 0; u < C::kTN; ++u)
+            acc[u][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                decode(fb[u].w[j / 2][j % 2 * 2], fb[u].w[j / 2][j % 2 * 2 + 1], sb[u]), xa, acc[u][t], 0, 0, 0);
         }
+        fa[t] = read_a(t, buf, next_step);
       }
     } else {
       const auto codes = [](const Frag8& f) {
@@ -198,43 +205,53 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
                      static_cast<int>(f.w[1][2]), static_cast<int>(f.w[1][3])};
       };
 #pragma unroll
-      for (int t = 0; t < C::kTM; ++t)
+      for (int t = 0; t < C::kTM; ++t) {
 #pragma unroll
         for (int u = 0; u < C::kTN; ++u)
           acc[u][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes(fb[u]), codes(fa[t]), acc[u][t], 0, 0, 0,
                                                                       static_cast<int>(now.b[u] >> shift), 0,
                                                                       static_cast<int>(now.a[t] >> shift));
+        fa[t] = read_a(t, buf, next_step);
+      }
+      // (The order above, which the scheduler would otherwise undo: LDS reads first.)
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * C::kTN, 0);
+#pragma unroll
+      for (int t = 0; t < C::kTM; ++t) {
+        __builtin_amdgcn_sched_group_barrier(0x008, C::kTN, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, (A::kSlots + B::kSlots + C::kTM - 1) / C::kTM, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < C::kTN; ++u) fb[u] = fb_next[u];
   };
 
-  // Two tiles in LDS, two steps per tile, the fragments of one step ahead in
-  // registers.  While the products of step 0 run, step 1 is read; then one barrier,
-  // after which nobody reads this tile any more and the next one is there; while the
-  // products of step 1 run, the tile after next is loaded over this one and step 0 of
-  // the next is read.  Loads past the last tile go out of bounds (zeros, never
-  // multiplied).
+  // Two tiles in LDS, two steps per tile, the fragments of one step ahead.  While the
+  // products of step 0 run, step 1 is read; then one barrier, after which nobody reads
+  // this tile any more and the next one is there; while the products of step 1 run, the
+  // tile after next is loaded over this one and step 0 of the next is read.  Loads past
+  // the last tile go out of bounds (zeros, never multiplied).
   if (k_first < k_last) {
-    Frag8 fa0[C::kTM], fb0[C::kTN], fa1[C::kTM], fb1[C::kTN];
     load_scales(now, k_first / 4);
-    load_scales(next, k_first / 4 + 1);
     load(k_first, 0);
     vectra_dense::wait_loads();
     __builtin_amdgcn_s_barrier();
     load(k_first + 1, 1);
-    read(fa0, fb0, 0, 0);
+    read_b(fb, 0, 0);
+#pragma unroll
+    for (int t = 0; t < C::kTM; ++t) fa[t] = read_a(t, 0, 0);
     for (int kt = k_first; kt < k_last; ++kt) {
       const int buf = (kt - k_first) & 1, shift = (kt & 3) * 8;
-      read(fa1, fb1, buf, 1);
-      multiply(fa0, fb0, shift);
+      Scales next;  // (each tile's own load of the word: a branch every fourth would part the products from their reads)
+      load_scales(next, (kt + 1) / 4);
+      step(shift, buf, 1);
       vectra_dense::wait_all();
       __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
       load(kt + 2, buf);
-      read(fa0, fb0, buf ^ 1, 0);
-      multiply(fa1, fb1, shift);
-      if ((kt & 3) == 3) {
-        now = next;
-        load_scales(next, kt / 4 + 2);
-      }
+      step(shift, buf ^ 1, 0);
+      now = next;
+      __builtin_amdgcn_sched_barrier(0);
     }
     vectra_dense::wait_all();  // nothing is on its way into LDS when it is used again
   }
