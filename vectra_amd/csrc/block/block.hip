@@ -523,16 +523,21 @@ int check_linear8(const vectra_linear8_args* a) {
 }
 
 // The tile and the number of contraction parts with the least estimated time.
-//   kRate      of all CUs, full, by tile (16-bit results; fp32's)
+//   kRate      of all CUs, full, by tile (16-bit results; fp32's), as a line in the
+//              contraction: 8192 x K -> 16384 takes 1.45, 0.69 and 0.28 us per block and
+//              tile on 256, 128 and 64
 //   kResident  workgroups that a CU holds; one that holds fewer runs at kPart of the rate
-//   kBatch     a workgroup's first loads and its epilogue
-// Tiles' operands pass from L2 to LDS at 16 TB/s.  A split costs its fp32 planes,
-// written and read at 5 TB/s, and the joining launch.
+//   kBatch     a CU's first loads and epilogues: the line's intercept, 10.4, 2.1 and 0.5
+//              us per tile
+// A split costs its fp32 planes, written and read at 5 TB/s, and the joining launch.
+//   chosen / others, bf16, us: 4096 x 4096 -> 4096 65 on 256 (91 on 128); 1024 x 4096 ->
+//   4096 25 on 128 (49 on 256, 43 on 64); 128 x 4096 -> 4096 9.5 and a join on 64 in 4
+//   parts (15 in one, 10.3 on 128 in 4)
 void choose8(const Product8Params& p, int64_t columns, int32_t dtype, int cus, int& tile, int& parts) {
-  static constexpr double kRate16[kTiles8] = {2.4e15, 1.7e15, 1.0e15}, kRate32[kTiles8] = {0, 0.9e15, 0.6e15};
+  static constexpr double kRate16[kTiles8] = {2.9e15, 1.55e15, 0.95e15}, kRate32[kTiles8] = {0, 0.72e15, 0.55e15};
   static constexpr int kResident[kTiles8] = {1, 2, 5};
-  static constexpr double kPart[kTiles8][5] = {{1.0}, {0.65, 1.0}, {0.35, 0.6, 0.8, 0.9, 1.0}};
-  static constexpr double kBatch[kTiles8] = {4e-6, 2e-6, 1.5e-6};
+  static constexpr double kPart[kTiles8][5] = {{1.0}, {0.95, 1.0}, {0.63, 0.75, 0.8, 0.86, 1.0}};
+  static constexpr double kBatch[kTiles8] = {10.4e-6, 4.2e-6, 2.6e-6};
   const bool precise = dtype == VECTRA_BLOCK_F32;
   double best = 1e30;
   tile = kSmall8;
@@ -540,14 +545,13 @@ void choose8(const Product8Params& p, int64_t columns, int32_t dtype, int cus, i
   for (int t = precise ? kMedium8 : kLarge8; t < kTiles8; ++t) {
     const int64_t tiles = ceil_div(p.rows, kTile8[t]) * ceil_div(columns, kTile8[t]);
     const double rate = (precise ? kRate32[t] : kRate16[t]) / 256;
-    for (int k = 1; k <= std::max(1, std::min(16, p.k_tiles / 2)); k *= 2) {
+    for (int k = 1; k <= std::max(1, std::min(16, p.k_tiles / 4)); k *= 2) {
       const int64_t depth = ceil_div(p.k_tiles, k) * 128;
       const int64_t per_cu = ceil_div(tiles * k, cus);
       const int together = static_cast<int>(std::min<int64_t>(per_cu, kResident[t]));
       const double products = per_cu * 2.0 * kTile8[t] * kTile8[t] * depth / (rate * kPart[t][together - 1]);
-      const double traffic = tiles * k * 2.0 * kTile8[t] * depth / 16e12;
       const double join = k > 1 ? 8.0 * k * p.rows * columns / 5e12 + 4e-6 : 0;
-      const double time = std::max(products, traffic) + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
+      const double time = products + ceil_div(per_cu, kResident[t]) * kBatch[t] + join;
       if (time < best * 0.98) {
         best = time;
         tile = t;
@@ -599,7 +603,8 @@ int linear8(const vectra_linear8_args& a, Scratch& scratch, bool launch, int cus
   choose8(p, columns, a.dtype, cus, tile, parts);
   p.tiles_m = static_cast<int32_t>(ceil_div(p.rows, kTile8[tile]));
   p.tiles_n = static_cast<int32_t>(ceil_div(columns, kTile8[tile]));
-  p.k_tiles_per_part = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(p.k_tiles, parts)));
+  // (A part begins with a word of scales.)
+  p.k_tiles_per_part = static_cast<int32_t>(std::max<int64_t>(1, parts == 1 ? p.k_tiles : ceil_div(ceil_div(p.k_tiles, parts), 4) * 4));
   parts = static_cast<int>(std::max<int64_t>(1, ceil_div(p.k_tiles, p.k_tiles_per_part)));
   const auto f = a.dtype == VECTRA_BLOCK_F32   ? launch_product8_f32
                  : a.dtype == VECTRA_BLOCK_F16 ? launch_product8_f16

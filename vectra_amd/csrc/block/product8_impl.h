@@ -41,20 +41,52 @@ struct Frag8 {
   u32x4 w[2];
 };
 
-template <int kBM_, int kBN_, int kWM_, int kWN_, int kEpi_, bool kPrecise_>
+template <int kByte>
+struct Byte {
+  static constexpr int value = kByte;
+};
+
+// kDeep: of the contraction per stage, 64 or 128.  In LDS: four stages of 64, or three
+// of x and two of W of 128.
+template <int kBM_, int kBN_, int kWM_, int kWN_, int kDeep_, int kEpi_, bool kPrecise_>
 struct Config8 {
   static constexpr int kBM = kBM_, kBN = kBN_, kWM = kWM_, kWN = kWN_, kEpi = kEpi_;
   static constexpr bool kPrecise = kPrecise_, kGated = kEpi == kGated8;
   static constexpr int kThreads = 64 * kWM * kWN;
   static constexpr int kTM = kBM / kWM / 32, kTN = kBN / kWN / 32;
-  using A = vectra_dense::Tile<uint8_t, false, kBM, 128, kThreads>;
-  using B = vectra_dense::Tile<uint8_t, false, kBN, 128, kThreads>;
-  static constexpr int kStageBytes = A::kBytes + B::kBytes;
+  static constexpr int kDeep = kDeep_, kStagesA = kDeep == 64 ? 4 : 3, kStagesB = kDeep == 64 ? 4 : 2;
+  using A = vectra_dense::Tile<uint8_t, false, kBM, kDeep, kThreads>;
+  using B = vectra_dense::Tile<uint8_t, false, kBN, kDeep, kThreads>;
+  static constexpr int kLoads = A::kSlots + B::kSlots;  // of a thread, for a stage
   static constexpr int kBandStride = kTN * 32 + 4;  // rows 16 bytes apart in the banks
   static constexpr int kBandBytes = kEpi == kPartial8 ? 0 : kWM * kWN * 32 * kBandStride * 4;
-  static constexpr int kLdsBytes = 2 * kStageBytes > kBandBytes ? 2 * kStageBytes : kBandBytes;
+  static constexpr int kStageBytes = kStagesA * A::kBytes + kStagesB * B::kBytes;
+  static constexpr int kLdsBytes = kStageBytes > kBandBytes ? kStageBytes : kBandBytes;
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
 };
+
+// Waits until at most `kLeft` of this wave's vector memory operations are on their way
+// (kReads: and no LDS reads).
+template <int kLeft, bool kReads = false>
+__device__ __forceinline__ void wait_but() {
+  static_assert(kLeft < 64);
+  __builtin_amdgcn_s_waitcnt((kReads ? 0x0070 : 0x0f70) | (kLeft & 15) | (kLeft >> 4) << 14);
+}
+
+// Loads a stage of one operand into LDS, 16 bytes per lane and slot: `offset` from
+// `base` (out of bounds: zeros), `at` further along the contraction.
+__device__ __forceinline__ void load8_to_lds(__amdgpu_buffer_rsrc_t rsrc, lds_char* to, uint32_t offset, int at) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)to, 16, offset, at, 0, 0);
+}
+
+template <typename TileT, int kThreads>
+__device__ __forceinline__ void stage8(lds_char* stage, const uint8_t* base, int64_t bytes,
+                                       const uint32_t (&offset)[TileT::kSlots], int at, int wave) {
+#pragma unroll
+  for (int s = 0; s < TileT::kSlots; ++s)
+    load8_to_lds(vectra::plane_rsrc(base, static_cast<uint32_t>(least(bytes, 0x7fffffff))),
+                 stage + (s * kThreads + wave * 64) * 16, offset[s], at);
+}
 
 template <typename T, typename C>
 __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8Params p) {
@@ -89,18 +121,14 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
     }
   };
 
-  // ---- per-lane load offsets (bytes from the tile's base)
-  const uint8_t* a = p.codes + m0 * p.depth + static_cast<int64_t>(k_first) * 128;
-  const uint8_t* b = p.weight + n0 * p.depth + static_cast<int64_t>(k_first) * 128;
-  int64_t a_bytes = least(p.rows - m0, C::kBM) * p.depth - static_cast<int64_t>(k_first) * 128;
-  int64_t b_bytes = ((C::kGated ? p.n : 0) + least(p.n - n0, kOutN)) * p.depth - static_cast<int64_t>(k_first) * 128;
-  uint32_t a_off[A::kSlots], b_off[B::kSlots], a_chunk[A::kSlots], b_chunk[B::kSlots];
+  // ---- per-lane load offsets (bytes from the tile's first row; rows past the operand's
+  // end out of bounds).  The contraction's offset is the loads' scalar one.
+  uint32_t a_off[A::kSlots], b_off[B::kSlots];
 #pragma unroll
   for (int s = 0; s < A::kSlots; ++s) {
     int row, chunk;
     A::slot(s, tid, row, chunk);
     a_off[s] = m0 + row < p.rows ? static_cast<uint32_t>(row * p.depth) + chunk * 16 : vectra_dense::kOutside;
-    a_chunk[s] = 0;  // (whole blocks: every chunk of a tile exists)
   }
 #pragma unroll
   for (int s = 0; s < B::kSlots; ++s) {
@@ -109,18 +137,19 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
     bool there;
     const int64_t w_row = weight_row(row, there);
     b_off[s] = there ? static_cast<uint32_t>((w_row - n0) * p.depth) + chunk * 16 : vectra_dense::kOutside;
-    b_chunk[s] = 0;
   }
-  const auto load = [&](int kt, int buf) {
-    lds_char* const at = smem + buf * C::kStageBytes;
-    const bool there = kt < k_last;
-    vectra_dense::stage<A, uint8_t, false, C::kThreads, false>(at, a, a_off, there ? least(a_bytes, 0x7fffffff) : 0, 1, a_chunk, wave);
-    vectra_dense::stage<B, uint8_t, false, C::kThreads, false>(at + A::kBytes, b, b_off, there ? least(b_bytes, 0x7fffffff) : 0, 1,
-                                                               b_chunk, wave);
-    a += 128;
-    b += 128;
-    a_bytes -= 128;
-    b_bytes -= 128;
+  const uint8_t* const a_base = p.codes + m0 * p.depth;
+  const uint8_t* const b_base = p.weight + n0 * p.depth;
+  const int64_t a_bytes = least(p.rows - m0, C::kBM) * p.depth;
+  const int64_t b_bytes = ((C::kGated ? p.n : 0) + least(p.n - n0, kOutN)) * p.depth;
+  const int last_stage = k_last * (128 / C::kDeep) - 1;
+  // (Past the last stage: that one again, into a buffer that nobody reads.)
+  const auto load_a = [&](int stage, int buf) {
+    stage8<A, C::kThreads>(smem + buf * A::kBytes, a_base, a_bytes, a_off, min(stage, last_stage) * C::kDeep, wave);
+  };
+  const auto load_b = [&](int stage, int buf) {
+    stage8<B, C::kThreads>(smem + C::kStagesA * A::kBytes + buf * B::kBytes, b_base, b_bytes, b_off,
+                           min(stage, last_stage) * C::kDeep, wave);
   };
 
   // ---- the scales of this lane's rows (clamped: those past the end are not stored),
@@ -140,7 +169,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
   }
   struct Scales {
     uint32_t a[C::kTM], b[C::kTN];
-  } now;
+  } now, next;
   const auto load_scales = [&](Scales& s, int word) {
     const int at = min(word, words - 1);
 #pragma unroll
@@ -157,37 +186,44 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[u][t][e] = 0.f;
 
-  const auto read_one = [&](const lds_char* tile, int row0, int step) {
+  // LDS holds the stages of x, then those of W.  A lane's address within one, but for
+  // the row block and the step: a fragment's chunks are three bits of it at most, so
+  // they are this with constants XORed in.  (Opaque in each step: hoisted out of the
+  // loop, every step's addresses would be registers of their own, and the large tile
+  // has none left.)
+  const uint32_t in_block = i * C::kDeep + ((half ^ A::swizzle(i)) * 16);
+  const uint32_t a_at = wm * C::kTM * 32 * C::kDeep + in_block;
+  const uint32_t b_at = C::kStagesA * A::kBytes + wn * C::kTN * 32 * C::kDeep + in_block;
+  const auto read_one = [&](uint32_t at, int offset, int step) {
     Frag8 f;
-    const int row = row0 + i;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      f.w[j] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
-          tile + row * 128 + (((step * 4 + 2 * j + half) ^ A::swizzle(i)) * 16));
+      f.w[j] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(smem + (at ^ ((step * 4 + 2 * j) * 16)) + offset);
     return f;
   };
+
   // The products of a step, and the fragments of the step after it: W's first, x's
   // each into the registers of the one just used, so that little more than one step's
   // are held at a time.
   Frag8 fa[C::kTM], fb[C::kTN];
-  const auto read_b = [&](Frag8(&f)[C::kTN], int buf, int step) {
-    const lds_char* const tb = smem + buf * C::kStageBytes + A::kBytes;
+  const auto read_b = [&](Frag8(&f)[C::kTN], uint32_t at, int buf, int step) {
 #pragma unroll
-    for (int u = 0; u < C::kTN; ++u) f[u] = read_one(tb, (wn * C::kTN + u) * 32, step);
+    for (int u = 0; u < C::kTN; ++u) f[u] = read_one(at, buf * B::kBytes + u * 32 * C::kDeep, step);
   };
-  const auto read_a = [&](int t, int buf, int step) {
-    return read_one(smem + buf * C::kStageBytes, (wm * C::kTM + t) * 32, step);
-  };
-  const auto step = [&](int shift, int buf, int next_step) {
+  const auto read_a = [&](int t, uint32_t at, int step) { return read_one(at, t * 32 * C::kDeep, step); };
+  const auto multiply = [&](auto which, int next_a, int next_b, int next_step) {
+    constexpr int kByte = decltype(which)::value;
+    uint32_t from_a = a_at + next_a * A::kBytes, from_b = b_at;
+    if constexpr (C::kDeep == 128) asm volatile("" : "+v"(from_a), "+v"(from_b));
     Frag8 fb_next[C::kTN];
-    read_b(fb_next, buf, next_step);
+    read_b(fb_next, from_b, next_b, next_step);
     if constexpr (C::kPrecise) {
       float sb[C::kTN];
 #pragma unroll
-      for (int u = 0; u < C::kTN; ++u) sb[u] = scale_of(now.b[u] >> shift & 255);
+      for (int u = 0; u < C::kTN; ++u) sb[u] = scale_of(now.b[u] >> (8 * kByte) & 255);
 #pragma unroll
       for (int t = 0; t < C::kTM; ++t) {
-        const float sa = scale_of(now.a[t] >> shift & 255);
+        const float sa = scale_of(now.a[t] >> (8 * kByte) & 255);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const bf16x8 xa = decode(fa[t].w[j / 2][j % 2 * 2], fa[t].w[j / 2][j % 2 * 2 + 1], sa);
@@ -196,7 +232,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
             acc[u][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 decode(fb[u].w[j / 2][j % 2 * 2], fb[u].w[j / 2][j % 2 * 2 + 1], sb[u]), xa, acc[u][t], 0, 0, 0);
         }
-        fa[t] = read_a(t, buf, next_step);
+        fa[t] = read_a(t, from_a, next_step);
       }
     } else {
       const auto codes = [](const Frag8& f) {
@@ -208,17 +244,17 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
       for (int t = 0; t < C::kTM; ++t) {
 #pragma unroll
         for (int u = 0; u < C::kTN; ++u)
-          acc[u][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes(fb[u]), codes(fa[t]), acc[u][t], 0, 0, 0,
-                                                                      static_cast<int>(now.b[u] >> shift), 0,
-                                                                      static_cast<int>(now.a[t] >> shift));
-        fa[t] = read_a(t, buf, next_step);
+          acc[u][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes(fb[u]), codes(fa[t]), acc[u][t], 0, 0, kByte,
+                                                                      static_cast<int>(now.b[u]), kByte,
+                                                                      static_cast<int>(now.a[t]));
+        fa[t] = read_a(t, from_a, next_step);
       }
       // (The order above, which the scheduler would otherwise undo: LDS reads first.)
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * C::kTN, 0);
 #pragma unroll
       for (int t = 0; t < C::kTM; ++t) {
         __builtin_amdgcn_sched_group_barrier(0x008, C::kTN, 0);
-        __builtin_amdgcn_sched_group_barrier(0x020, (A::kSlots + B::kSlots + C::kTM - 1) / C::kTM, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, (C::kLoads + C::kTM - 1) / C::kTM, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
     }
@@ -226,32 +262,98 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
     for (int u = 0; u < C::kTN; ++u) fb[u] = fb_next[u];
   };
 
-  // Two tiles in LDS, two steps per tile, the fragments of one step ahead.  While the
-  // products of step 0 run, step 1 is read; then one barrier, after which nobody reads
-  // this tile any more and the next one is there; while the products of step 1 run, the
-  // tile after next is loaded over this one and step 0 of the next is read.  Loads past
-  // the last tile go out of bounds (zeros, never multiplied).
+  // The fragments of one step of 64 ahead in registers; a word holds a row's scales of
+  // four blocks, the byte is the matrix instruction's own selection, so four blocks are
+  // a turn, and the next word, loaded in the first, has the others' time to arrive.
+  const auto turns = [&](auto&& block) {
+    for (int kt = k_first;; kt += 4) {
+      block(kt, Byte<0>{});
+      if (kt + 1 >= k_last) break;
+      block(kt + 1, Byte<1>{});
+      if (kt + 2 >= k_last) break;
+      block(kt + 2, Byte<2>{});
+      if (kt + 3 >= k_last) break;
+      block(kt + 3, Byte<3>{});
+      if (kt + 4 >= k_last) break;
+    }
+  };
+  const auto read_first = [&] {
+    read_b(fb, b_at, 0, 0);
+#pragma unroll
+    for (int t = 0; t < C::kTM; ++t) fa[t] = read_a(t, a_at, 0);
+  };
   if (k_first < k_last) {
     load_scales(now, k_first / 4);
-    load(k_first, 0);
-    vectra_dense::wait_loads();
-    __builtin_amdgcn_s_barrier();
-    load(k_first + 1, 1);
-    read_b(fb, 0, 0);
-#pragma unroll
-    for (int t = 0; t < C::kTM; ++t) fa[t] = read_a(t, 0, 0);
-    for (int kt = k_first; kt < k_last; ++kt) {
-      const int buf = (kt - k_first) & 1, shift = (kt & 3) * 8;
-      Scales next;  // (each tile's own load of the word: a branch every fourth would part the products from their reads)
-      load_scales(next, (kt + 1) / 4);
-      step(shift, buf, 1);
-      vectra_dense::wait_all();
+    if constexpr (C::kDeep == 128) {
+      // A stage is a block, two steps.  While the products of step 0 run, step 1 is
+      // read; then one barrier, after which nobody reads this stage any more and the
+      // next one is there; while the products of step 1 run, step 0 of the next is
+      // read, and W's block after next and x's third from here are loaded over this
+      // one: as much on its way as LDS holds.
+      load_b(k_first, 0);
+      load_a(k_first, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      load_a(k_first + 1, 1);
+      load_b(k_first + 1, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      load_a(k_first + 2, 2);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_but<2 * A::kSlots + B::kSlots>();
       __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-      load(kt + 2, buf);
-      step(shift, buf ^ 1, 0);
-      now = next;
-      __builtin_amdgcn_sched_barrier(0);
+      read_first();
+      int buf_a = 0;
+      turns([&](int kt, auto which) {
+        constexpr int kByte = decltype(which)::value, kBuf = kByte & 1;
+        multiply(which, buf_a, kBuf, 1);
+        // (x's block after next stays on its way; a word of scales issued with it is
+        // waited for.)
+        wait_but<A::kSlots, true>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kByte == 0) load_scales(next, kt / 4 + 1);
+        load_b(kt + 2, kBuf);
+        __builtin_amdgcn_sched_barrier(0x0007);  // (arithmetic may pass: the loads' order is what the wait counts on)
+        load_a(kt + 3, buf_a);
+        buf_a = buf_a == 2 ? 0 : buf_a + 1;
+        multiply(which, buf_a, kBuf ^ 1, 0);
+        if constexpr (kByte == 3) now = next;
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    } else {
+      constexpr int kStages = C::kStagesA;
+      // kStages steps in LDS or on their way there.  A step: wait for the next one's
+      // loads, of this wave, then at the barrier of all; nobody reads the stage before
+      // this one any more, and the step kStages - 1 ahead is loaded over it; the next
+      // step is read while this one is multiplied.
+#pragma unroll
+      for (int s = 0; s < kStages - 1; ++s) {
+        load_a(2 * k_first + s, s);
+        load_b(2 * k_first + s, s);
+      }
+      wait_but<(kStages - 2) * C::kLoads>();
+      __builtin_amdgcn_s_barrier();
+      read_first();
+      const auto step = [&](int at, auto which) {
+        constexpr int kStep = decltype(which)::value, kAhead = kStages - 1;
+        // Younger than the next step's loads: those of the steps behind it, and the
+        // scales' while they are (not counted where both were issued in one step, in an
+        // order that is the compiler's).
+        constexpr int kScales = kStep >= 1 && kStep < kAhead - 1 ? C::kTM + C::kTN : 0;
+        wait_but<(kStages - 3) * C::kLoads + kScales>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        load_a(at + kAhead, (kStep + kAhead) % kStages);
+        load_b(at + kAhead, (kStep + kAhead) % kStages);
+        if constexpr (kStep == 0) load_scales(next, at / 8 + 1);
+        multiply(Byte<kStep / 2>{}, (kStep + 1) % kStages, (kStep + 1) % kStages, 0);
+        if constexpr (kStep == 7) now = next;
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      turns([&](int kt, auto which) {
+        constexpr int kByte = decltype(which)::value;
+        step(2 * kt, Byte<2 * kByte>{});
+        step(2 * kt + 1, Byte<2 * kByte + 1>{});
+      });
     }
     vectra_dense::wait_all();  // nothing is on its way into LDS when it is used again
   }
@@ -349,14 +451,14 @@ int launch_tile8(const Product8Params& p, int tile, int parts, hipStream_t strea
   switch (tile) {
     case kLarge8:
       // (fp32 does not choose it: the decoded operands would not fit its registers.)
-      if constexpr (!kPrecise) return launch_one8<T, Config8<256, 256, 2, 4, kEpi, false>>(p, parts, stream);
+      if constexpr (!kPrecise) return launch_one8<T, Config8<256, 256, 2, 4, 128, kEpi, false>>(p, parts, stream);
       return VECTRA_BLOCK_ERR_LAUNCH;
     case kMedium8:
-      return launch_one8<T, Config8<128, 128, 2, 2, kEpi, kPrecise>>(p, parts, stream);
+      return launch_one8<T, Config8<128, 128, 2, 2, 64, kEpi, kPrecise>>(p, parts, stream);
     default:
       // (A wave of 32 columns holds no gate and up half: two waves side by side in m.)
-      if constexpr (kEpi == kGated8) return launch_one8<T, Config8<64, 64, 2, 1, kEpi, kPrecise>>(p, parts, stream);
-      return launch_one8<T, Config8<64, 64, 2, 2, kEpi, kPrecise>>(p, parts, stream);
+      if constexpr (kEpi == kGated8) return launch_one8<T, Config8<64, 64, 2, 1, 64, kEpi, kPrecise>>(p, parts, stream);
+      return launch_one8<T, Config8<64, 64, 2, 2, 64, kEpi, kPrecise>>(p, parts, stream);
   }
 }
 

@@ -22,7 +22,7 @@ struct Product8Params {
   int64_t residual_stride;
   void* out;  // kPartial: fp32 planes [parts, rows, out_stride]
   int64_t out_stride;
-  int32_t tiles_m, tiles_n, k_tiles, k_tiles_per_part;
+  int32_t tiles_m, tiles_n, k_tiles, k_tiles_per_part;  // (of several parts: a multiple of 4)
 };
 
 enum { kStore8 = 0, kGated8 = 1, kPartial8 = 2 };
