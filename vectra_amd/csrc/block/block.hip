@@ -581,7 +581,7 @@ int linear8(const vectra_linear8_args& a, Scratch& scratch, bool launch, int cus
   p.out = a.out;
   p.out_stride = a.out_stride;
   if (launch) (void)hipGetLastError();  // an error left by other work is not this call's
-  if (a.x && a.rows <= kFewRaw8) {
+  if (a.x && a.rows <= kFewRaw8 && a.rows * p.depth <= kRawBytes) {
     p.x = a.x;
     p.x_stride = a.x_stride;
   } else if (a.x) {

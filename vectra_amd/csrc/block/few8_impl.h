@@ -1,4 +1,4 @@
-// Products in 8 bits of a few rows (one token to 64) with a weight that is read once:
+// Products in 8 bits of a few rows (one token to 32) with a weight that is read once:
 // the kernel template, instantiated per type in product8_<type>.hip.
 //
 //   y = act(x^ W^T + b) + r,  or the gated product
@@ -13,9 +13,9 @@
 // The order of the contraction within a block is the matrix instruction's own
 // affair: both operands use the same.
 //
-// Up to 16 rows a wave brings its own blocks of x into 8 bits, from registers to
-// registers: four lanes share a row's block.  There is no second launch and nothing
-// in the workspace.  More rows come as codes.
+// A few rows that are short enough are brought into 8 bits by each workgroup for
+// itself, in LDS, while its first rows of W are on their way: no second launch and
+// nothing in the workspace.  More come as codes.
 #pragma once
 
 #include "block_common.h"
@@ -27,25 +27,17 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// 2^(byte - 127) as fp32: the exponent's own bits, but for byte 0 (2^-127, an fp32
-// subnormal) and 255 (NaN).
-__device__ __forceinline__ float scale_of(uint32_t byte) {
-  const uint32_t bits = byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23;
-  return __uint_as_float(bits);
-}
+// 2^(byte - 127) as the conversions below take it: in the exponent's bits.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Eight codes times a power of two as bf16: four bits of significand, exact (past
-// bf16's range: infinity, or a subnormal).
+// Eight codes times a power of two as bf16, by gfx950's scaled conversion of pairs:
+// four bits of significand, exact (past bf16's range: infinity, or a subnormal).
 __device__ __forceinline__ bf16x8 decode(uint32_t lo, uint32_t hi, float scale) {
-  bf16x8 r;
-  const uint32_t words[2] = {lo, hi};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4 v = vectra_dense::from_e4m3x4(words[h]) * scale;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[4 * h + e] = static_cast<__bf16>(v[e]);
-  }
-  return r;
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // One lane's 32 codes of a block, decoded: the operands of four matrix instructions.
@@ -55,39 +47,14 @@ struct Block8 {
   __device__ __forceinline__ bf16x8 part(int j) const { return decode(w[j / 2][j % 2 * 2], w[j / 2][j % 2 * 2 + 1], scale); }
 };
 
-// A lane's 32 elements of a row's block, zeros past the row's end, in 8 bits.  The
-// four lanes (g = 0 .. 3) of row i find the block's largest together.
-template <typename T>
-__device__ __forceinline__ Block8 quantise_block(const T* row, int64_t width, int64_t first) {
-  f32x4 v[4][2];
-  float largest = 0.f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int left = static_cast<int>(most(least(row ? width - first - 8 * j : 0, 8), 0));
-    v[j][0] = v[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (left > 0) vectra_dense::load8(row + first + 8 * j, left, v[j][0], v[j][1]);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) largest = vectra_dense::largest_finite(v[j], largest);
-  largest = vectra::allreduce_bit16(largest, vectra::OpMax{});
-  largest = vectra::allreduce_bit32(largest, vectra::OpMax{});
-  const int e = vectra_dense::block_exponent(largest, kLowestExponent) - 127;
-  Block8 b;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint2 c = vectra_dense::to_codes(v[j], e, kHighestExponent);
-    b.w[j / 2][j % 2 * 2] = c.x;
-    b.w[j / 2][j % 2 * 2 + 1] = c.y;
-  }
-  b.scale = vectra_dense::power_of_two(e);
-  return b;
-}
-
 template <typename T, int kRowTiles, bool kGated, bool kRaw, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params p) {
   constexpr int kHalves = kGated ? 2 : 1;
   constexpr int kBatch = 2;  // blocks of W on their way
   __shared__ f32x4 part[kWaves][kHalves][kRowTiles][64];
+  // x in 8 bits: rows 32 bytes apart in the banks.
+  __shared__ __attribute__((aligned(16))) uint8_t x_codes[kRaw ? kRawBytes + kFewRaw8 * 32 : 16];
+  __shared__ uint8_t x_bytes[kRaw ? kRawBytes / 128 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, i = lane & 15;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
@@ -109,50 +76,84 @@ __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params 
 #pragma unroll
     for (int t = 0; t < kRowTiles; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int first = wave; first < blocks; first += kWaves * kBatch) {
-    Block8 w[kBatch][kHalves];
-    uint32_t byte[kBatch][kHalves];
+  Block8 w[kBatch][kHalves];
+  uint32_t w_byte[kBatch][kHalves];
+  const auto load_w = [&](int first) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int at = first + b * kWaves;
       if (at >= blocks) continue;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
-        const u32x4* const from = reinterpret_cast<const u32x4*>(w_row[h] + at * 128);
-        w[b][h].w[0] = from[0];
-        w[b][h].w[1] = from[1];
-        byte[b][h] = w_scale[h][at];
+        w[b][h].w[0] = *reinterpret_cast<const u32x4*>(w_row[h] + at * 128);
+        w[b][h].w[1] = *reinterpret_cast<const u32x4*>(w_row[h] + at * 128 + 16);
+        w_byte[b][h] = w_scale[h][at];
       }
     }
+  };
+  if constexpr (kRaw) load_w(wave);
+  const int x_stride = static_cast<int>(p.depth) + 32;
+  if constexpr (kRaw) {
+    // A block of a row by 16 lanes, eight elements each.
+    const int eights = static_cast<int>(p.depth / 8), total = static_cast<int>(p.rows) * eights;
+    for (int base = wave * 64; base < total; base += 64 * kWaves) {
+      const int at = base + lane;
+      const bool live = at < total;  // (a block's 16 lanes alike)
+      const int row = live ? at / eights : 0, column = live ? (at - row * eights) * 8 : 0;
+      f32x4 v[2] = {};
+      const int left = live ? static_cast<int>(most(least(p.width - column, 8), 0)) : 0;
+      if (left > 0) vectra_dense::load8(static_cast<const T*>(p.x) + row * p.x_stride + column, left, v[0], v[1]);
+      const float largest = vectra::reduce_low<16>(vectra_dense::largest_finite(v, 0.f), vectra::OpMax{});
+      const int byte = vectra_dense::block_exponent(largest, kLowestExponent);
+      const uint2 c = vectra_dense::to_codes(v, byte - 127, kHighestExponent);
+      if (!live) continue;
+      *reinterpret_cast<uint2*>(x_codes + row * x_stride + column) = c;
+      if (lane % 16 == 0) x_bytes[row * blocks + column / 128] = static_cast<uint8_t>(byte);
+    }
+    __syncthreads();
+  }
+  for (int first = wave; first < blocks; first += kWaves * kBatch) {
+    // A batch's loads, all of them before the first is used: W's blocks and, from L2
+    // after the first workgroups, x's.
+    if (!kRaw || first != wave) load_w(first);
+    Block8 x[kBatch][kRowTiles];
+    uint32_t x_byte[kBatch][kRowTiles];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int at = first + b * kWaves;
       if (at >= blocks) continue;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) w[b][h].scale = scale_of(byte[b][h]);
-#pragma unroll
       for (int t = 0; t < kRowTiles; ++t) {
         const int row = t * 16 + i;
-        Block8 x;
-        if constexpr (kRaw) {
-          x = quantise_block<T>(row < p.rows ? static_cast<const T*>(p.x) + row * p.x_stride : nullptr, p.width,
-                                static_cast<int64_t>(at) * 128 + g * 32);
-        } else {
-          x.w[0] = x.w[1] = u32x4{0, 0, 0, 0};
-          x.scale = 0.f;
-          if (row < p.rows) {
-            const u32x4* const from = reinterpret_cast<const u32x4*>(p.codes + row * p.depth + static_cast<int64_t>(at) * 128 + g * 32);
-            x.w[0] = from[0];
-            x.w[1] = from[1];
-            x.scale = scale_of(p.scales[row * p.scale_stride + at]);
-          }
+        x[b][t].w[0] = x[b][t].w[1] = u32x4{0, 0, 0, 0};
+        x_byte[b][t] = 127;
+        if (row < p.rows) {
+          const uint8_t* const from = kRaw ? x_codes + row * x_stride + at * 128 + g * 32
+                                           : p.codes + row * p.depth + static_cast<int64_t>(at) * 128 + g * 32;
+          x[b][t].w[0] = *reinterpret_cast<const u32x4*>(from);
+          x[b][t].w[1] = *reinterpret_cast<const u32x4*>(from + 16);
+          x_byte[b][t] = kRaw ? x_bytes[row * blocks + at] : p.scales[row * p.scale_stride + at];
         }
+      }
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bf16x8 xj = x.part(j);
+    for (int b = 0; b < kBatch; ++b) {
+      if (first + b * kWaves >= blocks) continue;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) w[b][h].scale = scale_of(w_byte[b][h]);
+#pragma unroll
+      for (int t = 0; t < kRowTiles; ++t) x[b][t].scale = scale_of(x_byte[b][t]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bf16x8 wj[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) wj[h] = w[b][h].part(j);
+#pragma unroll
+        for (int t = 0; t < kRowTiles; ++t) {
+          const bf16x8 xj = x[b][t].part(j);
 #pragma unroll
           for (int h = 0; h < kHalves; ++h)
-            acc[h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[b][h].part(j), xj, acc[h][t], 0, 0, 0);
+            acc[h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wj[h], xj, acc[h][t], 0, 0, 0);
         }
       }
     }
@@ -194,9 +195,7 @@ __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params 
 template <typename T, bool kGated, int kWaves>
 auto few8_for(int64_t rows, bool raw) {
   if (raw) return few8_kernel<T, 1, kGated, true, kWaves>;
-  return rows <= 16   ? few8_kernel<T, 1, kGated, false, kWaves>
-         : rows <= 32 ? few8_kernel<T, 2, kGated, false, kWaves>
-                      : few8_kernel<T, 4, kGated, false, kWaves>;
+  return rows <= 16 ? few8_kernel<T, 1, kGated, false, kWaves> : few8_kernel<T, 2, kGated, false, kWaves>;
 }
 
 template <typename T>

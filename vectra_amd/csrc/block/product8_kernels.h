@@ -29,9 +29,9 @@ enum { kStore8 = 0, kGated8 = 1, kPartial8 = 2 };
 enum { kLarge8 = 0, kMedium8 = 1, kSmall8 = 2, kTiles8 = 3 };
 constexpr int kTile8[kTiles8] = {256, 128, 64};  // rows and columns
 
-// Rows up to which a product reads the weight straight into registers, and up to
-// which it also brings its input into 8 bits itself.
-constexpr int kFewRows8 = 64, kFewRaw8 = 16;
+// Rows up to which a product reads the weight straight into registers, and rows and
+// bytes of them up to which its workgroups bring the input into 8 bits themselves.
+constexpr int kFewRows8 = 32, kFewRaw8 = 16, kRawBytes = 16384;
 
 // One definition per type of result.
 int launch_product8_f32(const Product8Params& p, int tile, int epilogue, int parts, hipStream_t stream);

@@ -63,7 +63,7 @@ which it brings into 8 bits itself, and returns their type; or codes with `scale
 (residual_norm_8bit's, or quantize_blocks'), and returns `dtype`.  bias is the
 result's type or float32, the residual the result's type.
 
-float32 results, and those of at most 64 rows, are exact products of the 8-bit values
+float32 results, and those of at most 32 rows, are exact products of the 8-bit values
 in fp32 sums, rounded once.  float16 and bfloat16 results of more rows come from the
 8-bit matrix cores, which drop, of the 16 products that they add at a time, what lies
 below 2^-13 of the largest one's power of two: with normal operands 1.6e-5 of a
