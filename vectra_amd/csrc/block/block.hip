@@ -38,9 +38,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, int64_t rows, 
     f32x4 v[2];
     widen_eight(in[j], v[0], v[1]);
     if (d.threshold) {
-      f32x4 k[2];
-      dropout_factors(d, key, at[j], k);
-      drop(v, k);
+      drop(v, dropout_kept(d, key, at[j]), d.scale);
     }
     store8(y + static_cast<int64_t>(row[j]) * y_stride + column, v[0], v[1], static_cast<int>(least(width - column, 8)));
   }
@@ -441,13 +439,18 @@ int backward(const vectra_norm_grad_args& a, Scratch& scratch, bool launch, int 
   p.dresidual_stride = a.dresidual_stride;
   p.dgate_stride = a.dgate_stride;
 
-  // Units: the rows, or a gate's groups of rows, in parts, as many as fill the card
-  // and no more than leave each slot of a workgroup a row.
-  const int lanes = norm_lanes(a.width), threads = std::max(lanes, 256), slots = threads / lanes;
-  const int64_t wanted = static_cast<int64_t>(cus) * (1024 / threads);
+  // Units: the rows, or a gate's groups of rows, in parts: as many as the registers let
+  // the card hold at once (2 waves per SIMD with a gate and a post norm, 3 with one of
+  // them, 4 with neither), and where there are rows enough for the card no more than
+  // leave a workgroup's slots eight each, beside which its sums, 8 bytes a column written
+  // and read, are little.
+  const NormShape shape = norm_shape(a.width);
+  const int threads = a.gate ? (a.post ? 512 : 768) : a.post ? 768 : 1024;  // of a CU
+  const int64_t wanted = static_cast<int64_t>(cus) * std::max(1, threads / shape.threads);
   p.unit_rows = gate_full ? a.rows : gate_rows;
   const int64_t groups = a.rows ? ceil_div(a.rows, p.unit_rows) : 0;
-  int64_t parts = groups ? std::min(ceil_div(wanted, groups), ceil_div(p.unit_rows, slots)) : 1;
+  const int64_t each = std::max<int64_t>(1, std::min<int64_t>(8, a.rows / (2 * shape.rows * cus)));
+  const int64_t parts = groups ? std::min(ceil_div(wanted, groups), ceil_div(p.unit_rows, each * shape.rows)) : 1;
   p.rows_per_part = std::max<int64_t>(1, ceil_div(p.unit_rows, parts));
   p.parts = static_cast<int32_t>(ceil_div(p.unit_rows, p.rows_per_part));
   if (a.rows == 0) p.parts = 0;

@@ -47,12 +47,12 @@ __device__ __forceinline__ DropoutKey dropout_key(const Dropout& d) {
   return DropoutKey{static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32), static_cast<uint32_t>(d.rng[1])};
 }
 
-// The factors, scale or 0, of the eight elements of a group: Philox 4x32, ten
+// Which of the eight elements of a group are kept, a bit each: Philox 4x32, ten
 // rounds (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3;
 // SC 2011).  16 bits per element: with 32 the twenty wide multiplications, at a
 // quarter of the vector rate, would be shared by four elements instead of eight,
 // and dropout of 16-bit elements would be bound by them rather than by memory.
-__device__ __forceinline__ void dropout_factors(const Dropout& d, const DropoutKey& key, uint64_t group, f32x4 (&k)[2]) {
+__device__ __forceinline__ uint32_t dropout_kept(const Dropout& d, const DropoutKey& key, uint64_t group) {
   uint32_t a = static_cast<uint32_t>(group), b = static_cast<uint32_t>(group >> 32), c = d.stream, e = key.offset;
   uint32_t k0 = key.k0, k1 = key.k1;
 #pragma unroll
@@ -66,17 +66,19 @@ __device__ __forceinline__ void dropout_factors(const Dropout& d, const DropoutK
     k1 += 0xBB67AE85u;
   }
   const uint32_t words[4] = {a, b, c, e}, t = static_cast<uint32_t>(d.threshold);
+  uint32_t kept = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    k[j / 2][2 * j % 4] = (words[j] & 0xffffu) >= t ? d.scale : 0.f;
-    k[j / 2][2 * j % 4 + 1] = (words[j] >> 16) >= t ? d.scale : 0.f;
+    kept |= (words[j] & 0xffffu) >= t ? 1u << 2 * j : 0u;
+    kept |= (words[j] >> 16) >= t ? 2u << 2 * j : 0u;
   }
+  return kept;
 }
 
-// x * k, with 0 for a dropped element whatever x holds.
-__device__ __forceinline__ void drop(f32x4 (&x)[2], const f32x4 (&k)[2]) {
+// The elements scaled, with 0 for a dropped one whatever it holds.
+__device__ __forceinline__ void drop(f32x4 (&x)[2], uint32_t kept, float scale) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = k[i / 4][i % 4] == 0.f ? 0.f : x[i / 4][i % 4] * k[i / 4][i % 4];
+  for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = kept >> i & 1 ? x[i / 4][i % 4] * scale : 0.f;
 }
 
 // -------------------------------------------------------------------- 8 bits

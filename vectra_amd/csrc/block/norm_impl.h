@@ -3,13 +3,18 @@
 //
 //   h = s r + gate * k * post(x),  n = norm(h)
 //
-// A row of `width` elements is held in registers by 16 to 1024 lanes, eight
-// consecutive columns each (two such chunks past 8192 columns): 16 bytes of a
-// 16-bit row per lane and access.  Everything between the loads and the stores of
-// a row happens there, so each tensor is moved once; the per-column vectors are
-// loaded once per workgroup, and the next row's loads are issued before a row is
-// worked on.  What bounds it is HBM; the sums of a row cross lanes by DPP moves and
-// lane swaps, and waves through LDS with one barrier each.
+// A row of `width` elements is held in registers by 16, 32 or 64 lanes or by up to 8
+// waves, eight consecutive columns per lane (past 4096 columns two or four such
+// chunks): 16 bytes of a 16-bit row per lane and access.  Everything between the loads
+// and the stores of a row happens there, so each tensor is moved once; the per-column
+// vectors are loaded once per workgroup, and the next row's loads are issued before a
+// row is worked on.  The sums of a row cross lanes by DPP moves and lane swaps, and
+// waves through LDS with one barrier each.  What bounds it is HBM: 8192 x 4096 bf16 on
+// an fp32 stream, rms norms on both sides and a gate over all rows, 81 us forward
+// (5.0 TB/s) and 148 backward (4.1); 66560 x 128 bf16, layer norm and dropout, 17.5 us
+// and 30 (3.9, 2.9 TB/s).  Past 4096 columns, and with a post norm past 8192 above all,
+// the registers do not hold a row's sums and gradients: 4096 x 8192, both norms and a
+// gate, 139 us and 405; 2048 x 16384 184 us and 1740.
 //
 // Layer norm's variance is the mean of (x - mean)^2, not a difference of squares:
 // within a wave from the wave's own mean, the waves' joined by
@@ -30,58 +35,70 @@ namespace vectra_block {
 using vectra::OpMax;
 using vectra::OpSum;
 using vectra::reduce_low;
+using vectra_dense::u32x4;
 
-// Threads of the workgroup that holds rows of so many lanes.
-constexpr int row_threads(int lanes) { return lanes > 64 ? lanes : 256; }
+// How a row's last chunk is read.  Whole: rows are whole chunks.  Ragged: as the row's
+// last eight elements, moved into place afterwards; read element by element, it would
+// be waited for before the next load (6000 x 1001 bf16 backward 46 -> 36 us).  Narrow:
+// rows of fewer than eight elements, by those.  (Kinds of their own, because a branch
+// among the loads of the row ahead waits for them where its sides meet: 8192 x 4096
+// forward 77 us, with such a branch 112.)
+enum { kWhole = 0, kRagged = 1, kNarrow = 2 };
 
-template <int kLanes_, int kChunks_>
+// kLanes: of a row, or 0: all of the workgroup's (kMany).
+constexpr int kMany = 0;
+constexpr int kMostLanes = 512;
+constexpr int row_threads(int lanes) { return lanes == kMany ? kMostLanes : 256; }  // at most
+
+template <int kLanes, int kChunks_, int kKind>
 struct Row {
-  static constexpr int kLanes = kLanes_, kChunks = kChunks_;
-  static constexpr bool kMany = kLanes > 64;  // several waves per row, one row per workgroup
-  static constexpr int kThreads = row_threads(kLanes);
-  static constexpr int kRows = kThreads / kLanes;
-  static constexpr int kWaves = kMany ? kLanes / 64 : 1;
+  static constexpr int kChunks = kChunks_;
+  static constexpr bool kWaves = kLanes == kMany;  // several waves per row, one row per workgroup
+  static constexpr int kRows = kWaves ? 1 : 256 / kLanes;
+  static constexpr int kLds = kWaves ? 2 * kMostLanes / 64 : 1;
 
   typedef f32x4 Values[kChunks][2];  // a lane's part of a row; 0 past the row's end
 
-  int lane, slot;
+  int lane, slot, lanes, waves;
   int64_t width;
-  int64_t column[kChunks];
+  int32_t column[kChunks];
   int left[kChunks];  // elements of the chunk that exist
-  f32x4* lds;         // 2 kWaves of them
+  f32x4* lds;         // kLds of them
   int turn = 0;
 
   __device__ __forceinline__ Row(int64_t width_, f32x4* lds_) : width(width_), lds(lds_) {
-    lane = threadIdx.x % kLanes;
-    slot = threadIdx.x / kLanes;
+    lanes = kWaves ? static_cast<int>(blockDim.x) : kLanes;
+    waves = lanes / 64;
+    lane = kWaves ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % kLanes;
+    slot = kWaves ? 0 : static_cast<int>(threadIdx.x) / kLanes;
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-      column[j] = (static_cast<int64_t>(j) * kLanes + lane) * 8;
-      left[j] = static_cast<int>(most(least(width - column[j], 8), 0));
+      column[j] = (j * lanes + lane) * 8;
+      left[j] = max(min(static_cast<int>(width) - column[j], 8), 0);
     }
   }
 
   // What each wave of the row holds, for all of them to read.  Two buffers: a wave
   // may write the next while another still reads this one, and no further.
   __device__ __forceinline__ const f32x4* share(f32x4 mine) {
-    f32x4* const at = lds + turn * kWaves;
-    turn ^= 1;
+    f32x4* const at = lds + turn;
+    turn ^= kMostLanes / 64;
     if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = mine;
     __syncthreads();
     return at;
   }
 
-  static __device__ __forceinline__ float wave_sum(float v) { return reduce_low<kLanes < 64 ? kLanes : 64>(v, OpSum{}); }
+  static __device__ __forceinline__ float wave_sum(float v) { return reduce_low<kWaves ? 64 : kLanes>(v, OpSum{}); }
 
   // Sums of two quantities over the row's lanes.
   __device__ __forceinline__ void sum(float& a, float& b) {
     a = wave_sum(a);
     b = wave_sum(b);
-    if constexpr (kMany) {
+    if constexpr (kWaves) {
       const f32x4* const at = share(f32x4{a, b, 0.f, 0.f});
       a = b = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+#pragma unroll 2
+      for (int w = 0; w < waves; ++w) {
         const f32x4 v = at[w];
         a += v[0];
         b += v[1];
@@ -115,10 +132,10 @@ struct Row {
       for (int i = 0; i < 8; ++i) s += v[j][i / 4][i % 4];
     s = wave_sum(s);
     float mean = s * inverse_width, count = 0.f;
-    if constexpr (kMany) {  // of this wave's elements first
+    if constexpr (kWaves) {  // of this wave's elements first
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
-        count += static_cast<float>(most(least(width - (column[j] - (lane & 63) * 8), 512), 0));
+        count += static_cast<float>(max(min(static_cast<int>(width) - (column[j] - (lane & 63) * 8), 512), 0));
       mean = count > 0.f ? s / count : 0.f;
     }
     float m2 = 0.f;
@@ -130,14 +147,14 @@ struct Row {
         m2 = __builtin_fmaf(d, d, m2);
       }
     m2 = wave_sum(m2);
-    if constexpr (kMany) {
+    if constexpr (kWaves) {
       const f32x4* const at = share(f32x4{s, m2, count, mean});
       s = m2 = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) s += at[w][0];
+#pragma unroll 2
+      for (int w = 0; w < waves; ++w) s += at[w][0];
       mean = s * inverse_width;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+#pragma unroll 2
+      for (int w = 0; w < waves; ++w) {
         const f32x4 u = at[w];
         const float d = u[3] - mean;
         m2 += __builtin_fmaf(u[2] * d, d, u[1]);
@@ -175,24 +192,111 @@ struct Row {
       for (int h = 0; h < 2; ++h) g[j][h] = (g[j][h] - hat[j][h] * along - total) * r;
   }
 
-  __device__ __forceinline__ void load_vector_of(const Vector& v, int64_t at, float missing, Values& out) const {
-#pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      const void* const row =
-          v.p ? static_cast<const char*>(v.p) + at * (v.dtype == VECTRA_BLOCK_F32 ? 4 : 2) : nullptr;
-      load_vector(row, v.dtype, column[j], left[j], missing, out[j]);
+  // A vector over the columns, from element `at` of it on: held in registers, or with
+  // more than one chunk per lane, whose registers are full, read where it is used (from
+  // L1 and L2: every row reads the same).
+  struct Held {
+    Vector from;
+    int64_t at;
+    float missing;
+    f32x4 value[kChunks == 1 ? 2 : 1];
+  };
+  __device__ __forceinline__ void load_chunk(const Held& v, int j, f32x4(&out)[2]) const {
+    const void* const row =
+        v.from.p ? static_cast<const char*>(v.from.p) + v.at * (v.from.dtype == VECTRA_BLOCK_F32 ? 4 : 2) : nullptr;
+    load_vector(row, v.from.dtype, column[j], left[j], v.missing, out);
+  }
+  __device__ __forceinline__ void hold(const Vector& from, int64_t at, float missing, Held& v) const {
+    v.from = from;
+    v.at = at;
+    v.missing = missing;
+    if constexpr (kChunks == 1) load_chunk(v, 0, v.value);
+  }
+  __device__ __forceinline__ void use(const Held& v, int j, f32x4(&out)[2]) const {
+    if constexpr (kChunks == 1) {
+      out[0] = v.value[0];
+      out[1] = v.value[1];
+    } else {
+      load_chunk(v, j, out);
     }
   }
+  // The same in two steps, the loads and the conversion: a gate's row on its way while
+  // the row before is worked on.
+  struct Coming {
+    u32x4 w[2];
+  };
+  __device__ __forceinline__ void fetch(const Held& v, Coming& c) const {
+    if (v.from.dtype == VECTRA_BLOCK_F32) {
+      const Eight<float> e = load_chunk_of(static_cast<const float*>(v.from.p) + v.at, 0);
+      c.w[0] = e.part[0].w;
+      c.w[1] = e.part[1].w;
+    } else {
+      c.w[0] = load_chunk_of(static_cast<const _Float16*>(v.from.p) + v.at, 0).part[0].w;
+    }
+  }
+  __device__ __forceinline__ void take(const Coming& c, Held& v) const {
+    if (v.from.dtype == VECTRA_BLOCK_F32) {
+      Eight<float> e;
+      e.part[0].w = c.w[0];
+      e.part[1].w = c.w[1];
+      widen_chunk(e, 0, v.value);
+    } else if (v.from.dtype == VECTRA_BLOCK_F16) {
+      Eight<_Float16> e;
+      e.part[0].w = c.w[0];
+      widen_chunk(e, 0, v.value);
+    } else {
+      Eight<__bf16> e;
+      e.part[0].w = c.w[0];
+      widen_chunk(e, 0, v.value);
+    }
+  }
+  // x * weight + bias in place.
+  __device__ __forceinline__ void affine(f32x4(&x)[2], const Held& weight, const Held& bias, int j) const {
+    f32x4 w[2], b[2];
+    use(weight, j, w);
+    use(bias, j, b);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x[e] = x[e] * w[e] + b[e];
+  }
 
+  // Chunk j of a row as it is in memory.
+  template <typename T>
+  __device__ __forceinline__ Eight<T> load_chunk_of(const T* row, int j) const {
+    Eight<T> e{};
+    if (left[j] > 0) {
+      if constexpr (kKind == kNarrow) {
+        e = load_eight<T>(row, width, column[j]);
+      } else {
+        const T* const from = row + (kKind == kRagged ? min(column[j], static_cast<int>(width) - 8) : column[j]);
+        __builtin_memcpy(&e, from, sizeof(e));  // unaligned
+      }
+    }
+    return e;
+  }
   template <typename T>
   __device__ __forceinline__ void load(const void* p, int64_t row, int64_t stride, Eight<T> (&out)[kChunks]) const {
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      if (left[j] > 0)
-        out[j] = load_eight<T>(static_cast<const T*>(p) + row * stride, width, column[j]);
-      else
-        out[j] = Eight<T>{};
-    }
+    for (int j = 0; j < kChunks; ++j) out[j] = load_chunk_of(static_cast<const T*>(p) + row * stride, j);
+  }
+  __device__ __forceinline__ void settle_chunk(f32x4(&v)[2], int j) const {
+    const int shift = left[j] > 0 ? 8 - left[j] : 0;
+#pragma unroll
+    for (int by = 1; by < 8; by *= 2)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float from = i + by < 8 ? v[(i + by) / 4 % 2][(i + by) % 4] : 0.f;
+        v[i / 4][i % 4] = shift & by ? from : v[i / 4][i % 4];
+      }
+  }
+  template <typename T>
+  __device__ __forceinline__ void widen_chunk(const Eight<T>& in, int j, f32x4(&out)[2]) const {
+    widen_eight(in, out[0], out[1]);
+    if constexpr (kKind == kRagged) settle_chunk(out, j);
+  }
+  template <typename T>
+  __device__ __forceinline__ void widen(const Eight<T> (&in)[kChunks], Values& out) const {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) widen_chunk(in[j], j, out[j]);
   }
 
   template <typename T>
@@ -203,27 +307,21 @@ struct Row {
   }
 };
 
-template <typename T, int kChunks>
-__device__ __forceinline__ void widen_row(const Eight<T> (&in)[kChunks], f32x4 (&out)[kChunks][2]) {
-#pragma unroll
-  for (int j = 0; j < kChunks; ++j) widen_eight(in[j], out[j][0], out[j][1]);
-}
-
 // -------------------------------------------------------------------- forward
 
-template <typename T, typename R, int kLanes, int kChunks>
+template <typename T, typename R, int kLanes, int kChunks, int kKind>
 __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormParams p) {
-  using Row = Row<kLanes, kChunks>;
+  using Row = Row<kLanes, kChunks, kKind>;
   typedef typename Row::Values Values;
-  __shared__ f32x4 lds[2 * Row::kWaves];
+  __shared__ f32x4 lds[Row::kLds];
   Row row(p.width, lds);
-  Values weight, bias, gate, post_weight, post_bias;
-  row.load_vector_of(p.weight, 0, 1.f, weight);
-  row.load_vector_of(p.bias, 0, 0.f, bias);
-  row.load_vector_of(p.post_weight, 0, 1.f, post_weight);
-  row.load_vector_of(p.post_bias, 0, 0.f, post_bias);
+  typename Row::Held weight, bias, gate, post_weight, post_bias;
+  row.hold(p.weight, 0, 1.f, weight);
+  row.hold(p.bias, 0, 0.f, bias);
+  row.hold(p.post_weight, 0, 1.f, post_weight);
+  row.hold(p.post_bias, 0, 0.f, post_bias);
   const bool gate_each = p.gate.p && p.gate_rows < p.rows;
-  row.load_vector_of(p.gate, 0, 1.f, gate);
+  row.hold(p.gate, 0, 1.f, gate);
   const Dropout dropout{p.rng, p.threshold, p.stream_id, p.drop_scale};
   const DropoutKey key = dropout_key(dropout);
   const uint32_t groups = static_cast<uint32_t>((p.width + 7) / 8);
@@ -231,47 +329,53 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormPar
   const int64_t step = static_cast<int64_t>(gridDim.x) * Row::kRows;
   Eight<T> x_next[kChunks];
   Eight<R> r_next[kChunks];
+  typename Row::Coming gate_next;
   const auto fetch = [&](int64_t base) {
     const int64_t at = least(base + row.slot, p.rows - 1);  // (rows past the end repeat the last; they are not stored)
     row.load(p.x, at, p.x_stride, x_next);
     row.load(p.residual, at, p.residual_stride, r_next);
+    if (gate_each) {
+      gate.at = static_cast<uint32_t>(at) / static_cast<uint32_t>(p.gate_rows) * p.gate_stride;
+      if constexpr (kChunks == 1) row.fetch(gate, gate_next);
+    }
   };
   int64_t base = static_cast<int64_t>(blockIdx.x) * Row::kRows;
-  if (base < p.rows) fetch(base);
+  if constexpr (kChunks == 1) {  // (the registers of more have no room for a row ahead)
+    if (base < p.rows) fetch(base);
+  }
   for (; base < p.rows; base += step) {
     const bool live = base + row.slot < p.rows;
     const int64_t at = live ? base + row.slot : p.rows - 1;
     Values v, h;
-    widen_row(x_next, v);
-    widen_row(r_next, h);
-    if (base + step < p.rows) fetch(base + step);
-    if (gate_each)
-      row.load_vector_of(p.gate, static_cast<uint32_t>(at) / static_cast<uint32_t>(p.gate_rows) * p.gate_stride, 1.f, gate);
+    if constexpr (kChunks > 1) fetch(base);
+    row.widen(x_next, v);
+    row.widen(r_next, h);
+    if constexpr (kChunks == 1) {
+      if (gate_each) row.take(gate_next, gate);
+      if (base + step < p.rows) fetch(base + step);
+    }
     if (p.post != VECTRA_BLOCK_NO_NORM) {
       row.normalise(v, p.post, p.inverse_width, p.eps);
 #pragma unroll
-      for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) v[j][e] = v[j][e] * post_weight[j][e] + post_bias[j][e];
+      for (int j = 0; j < kChunks; ++j) row.affine(v[j], post_weight, post_bias, j);
     }
     if (p.threshold) {
 #pragma unroll
       for (int j = 0; j < kChunks; ++j) {
-        f32x4 k[2];
-        dropout_factors(dropout, key, static_cast<uint64_t>(at) * groups + (row.column[j] >> 3), k);
-        drop(v[j], k);
+        drop(v[j], dropout_kept(dropout, key, static_cast<uint64_t>(at) * groups + (row.column[j] >> 3)), p.drop_scale);
       }
     }
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j)
+    for (int j = 0; j < kChunks; ++j) {
+      f32x4 k[2];
+      row.use(gate, j, k);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) h[j][e] = h[j][e] * p.residual_scale + v[j][e] * gate[j][e];
+      for (int e = 0; e < 2; ++e) h[j][e] = h[j][e] * p.residual_scale + v[j][e] * k[e];
+    }
     if (live) row.template store<R>(p.h, at, p.h_stride, h);
     row.normalise(h, p.norm, p.inverse_width, p.eps);
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) h[j][e] = h[j][e] * weight[j][e] + bias[j][e];
+    for (int j = 0; j < kChunks; ++j) row.affine(h[j], weight, bias, j);
     if (p.n) {
       if (live) row.template store<T>(p.n, at, p.n_stride, h);
     } else {
@@ -286,29 +390,29 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormPar
         if (row.lane % 16 == 0) p.scales[at * p.scale_stride + row.column[j] / 128] = static_cast<uint8_t>(byte);
       }
       if (live)
-        for (int64_t k = p.depth / 128 + row.lane; k < p.scale_stride; k += kLanes) p.scales[at * p.scale_stride + k] = 0;
+        for (int64_t k = p.depth / 128 + row.lane; k < p.scale_stride; k += row.lanes) p.scales[at * p.scale_stride + k] = 0;
     }
   }
 }
 
 // ------------------------------------------------------------------- backward
 
-// kBranch: the branch's output matters, by a gate or a post norm; x and r are read,
-// else h.
-template <typename T, typename R, int kLanes, int kChunks, bool kBranch>
+// With a gate or a post norm the branch's output matters: x and r are read, else h.
+template <typename T, typename R, int kLanes, int kChunks, int kKind, bool kGate, bool kPost>
 __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const NormGradParams p) {
-  using Row = Row<kLanes, kChunks>;
+  constexpr bool kBranch = kGate || kPost;
+  using Row = Row<kLanes, kChunks, kKind>;
   typedef typename Row::Values Values;
-  __shared__ f32x4 lds[2 * Row::kWaves];
-  __shared__ float slots[Row::kMany ? 1 : Row::kRows][Row::kMany ? 1 : kLanes * 8 + 4];
+  __shared__ f32x4 lds[Row::kLds];
+  __shared__ float slots[Row::kRows][Row::kWaves ? 1 : kLanes * 8 + 4];
   Row row(p.width, lds);
-  Values weight, gate, post_weight, post_bias;
-  row.load_vector_of(p.weight, 0, 1.f, weight);
-  if constexpr (kBranch) {
-    row.load_vector_of(p.post_weight, 0, 1.f, post_weight);
-    row.load_vector_of(p.post_bias, 0, 0.f, post_bias);
-    row.load_vector_of(p.gate, 0, 1.f, gate);
+  typename Row::Held weight, gate, post_weight, post_bias;
+  row.hold(p.weight, 0, 1.f, weight);
+  if constexpr (kPost) {
+    row.hold(p.post_weight, 0, 1.f, post_weight);
+    row.hold(p.post_bias, 0, 0.f, post_bias);
   }
+  if constexpr (kGate) row.hold(p.gate, 0, 1.f, gate);
   const bool gate_full = p.gate.p && p.gate_rows == 1;  // a gate row, and its gradient, for each row
   const bool gate_each = p.gate.p && p.unit_rows == p.gate_rows;
   const Dropout dropout{p.rng, p.threshold, p.stream_id, p.drop_scale};
@@ -320,19 +424,17 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
   // The sum over the workgroup's slots of what each holds of a vector's gradient.
   // To all threads' d of slot 0; a workgroup with one slot has it already.
   const auto over_slots = [&](Values& d) {
-    if constexpr (!Row::kMany) {
+    if constexpr (!Row::kWaves) {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 8; ++e) slots[row.slot][row.lane * 8 + e] = d[0][e / 4][e % 4];
       __syncthreads();
       if (row.slot == 0) {
+        d[0][0] = d[0][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+        for (int k = 0; k < Row::kRows; ++k)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float s = 0.f;
-#pragma unroll
-          for (int k = 0; k < Row::kRows; ++k) s += slots[k][row.lane * 8 + e];
-          d[0][e / 4][e % 4] = s;
-        }
+          for (int e = 0; e < 8; ++e) d[0][e / 4][e % 4] += slots[k][row.lane * 8 + e];
       }
     }
   };
@@ -366,56 +468,69 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
     const int64_t group = unit / p.parts, part = unit - group * p.parts;
     const int64_t first = group * p.unit_rows + part * p.rows_per_part;
     const int64_t last = least(least(first + p.rows_per_part, (group + 1) * p.unit_rows), p.rows);
-    if constexpr (kBranch) {
-      if (gate_each && !gate_full) row.load_vector_of(p.gate, group * p.gate_stride, 1.f, gate);
+    if constexpr (kGate) {
+      if (gate_each && !gate_full) row.hold(p.gate, group * p.gate_stride, 1.f, gate);
     }
-    if (first < last) fetch(least(first + row.slot, last - 1));
+    if constexpr (kChunks == 1) {
+      if (first < last) fetch(least(first + row.slot, last - 1));
+    }
     for (int64_t base = first; base < last; base += Row::kRows) {
       const bool live = base + row.slot < last;
       const int64_t at = live ? base + row.slot : last - 1;
+      if constexpr (kChunks > 1) fetch(at);
       Values g, gt, x, h;
-      widen_row(g_next, g);
-      widen_row(gh_next, gt);
-      widen_row(r_next, h);
-      if constexpr (kBranch) {
-        widen_row(x_next, x);
-        if (gate_full) row.load_vector_of(p.gate, at * p.gate_stride, 1.f, gate);
+      row.widen(g_next, g);
+      row.widen(gh_next, gt);
+      row.widen(r_next, h);
+      if constexpr (kBranch) row.widen(x_next, x);
+      if constexpr (kGate) {
+        if (gate_full) row.hold(p.gate, at * p.gate_stride, 1.f, gate);
       }
-      if (base + Row::kRows < last) fetch(least(base + Row::kRows + row.slot, last - 1));
+      if constexpr (kChunks == 1) {
+        if (base + Row::kRows < last) fetch(least(base + Row::kRows + row.slot, last - 1));
+      }
       if (!live) {  // (a row of another slot: it must not be summed twice)
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) g[j][0] = g[j][1] = gt[j][0] = gt[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      f32x4 k[kChunks][2];
+      uint32_t kept[kChunks];
       if (p.threshold) {
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
-          dropout_factors(dropout, key, static_cast<uint64_t>(at) * groups + (row.column[j] >> 3), k[j]);
+          kept[j] = dropout_kept(dropout, key, static_cast<uint64_t>(at) * groups + (row.column[j] >> 3));
       }
+      // The branch before its gate, of chunk j: from the normalised x where it has a norm.
+      const auto branch = [&](int j, f32x4(&v)[2]) {
+        v[0] = x[j][0];
+        v[1] = x[j][1];
+        if constexpr (kPost) row.affine(v, post_weight, post_bias, j);
+        if (p.threshold) drop(v, kept[j], p.drop_scale);
+      };
       float post_r = 1.f;
-      Values v;  // the branch before its gate
+      if constexpr (kPost) post_r = row.normalise(x, p.post, p.inverse_width, p.eps);
       if constexpr (kBranch) {
-        if (p.post != VECTRA_BLOCK_NO_NORM) post_r = row.normalise(x, p.post, p.inverse_width, p.eps);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
+          f32x4 v[2], k[2];
+          branch(j, v);
+          if constexpr (kGate) row.use(gate, j, k);
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            v[j][e] = p.post != VECTRA_BLOCK_NO_NORM ? x[j][e] * post_weight[j][e] + post_bias[j][e] : x[j][e];
-          if (p.threshold) drop(v[j], k[j]);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) h[j][e] = h[j][e] * p.residual_scale + v[j][e] * gate[j][e];
+          for (int e = 0; e < 2; ++e) h[j][e] = h[j][e] * p.residual_scale + (kGate ? v[e] * k[e] : v[e]);
         }
       }
       if (p.grad_n) {
         const float r = row.normalise(h, p.norm, p.inverse_width, p.eps);
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j)
+        for (int j = 0; j < kChunks; ++j) {
+          f32x4 w[2];
+          row.use(weight, j, w);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             d_weight[j][e] += g[j][e] * h[j][e];
             d_bias[j][e] += g[j][e];
-            g[j][e] *= weight[j][e];
+            g[j][e] *= w[e];
           }
+        }
         row.transpose(g, h, r, p.norm, p.inverse_width);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
@@ -430,43 +545,44 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
           for (int e = 0; e < 2; ++e) d[j][e] = gt[j][e] * p.residual_scale;
         row.template store<R>(p.dresidual, at, p.dresidual_stride, d);
       }
-      if constexpr (kBranch) {
-        Values own;
+      if constexpr (kGate) {
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j)
+        for (int j = 0; j < kChunks; ++j) {
+          f32x4 v[2], k[2];
+          branch(j, v);
+          row.use(gate, j, k);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            own[j][e] = gt[j][e] * v[j][e];
-            d_gate[j][e] += own[j][e];
-            gt[j][e] *= gate[j][e];
+            v[e] *= gt[j][e];
+            d_gate[j][e] += v[e];
+            gt[j][e] *= k[e];
           }
-        if (p.dgate && gate_full && live) {
-#pragma unroll
-          for (int j = 0; j < kChunks; ++j)
+          if (p.dgate && gate_full && live)
             store_vector(static_cast<char*>(p.dgate) + at * p.dgate_stride * (p.dgate_dtype == VECTRA_BLOCK_F32 ? 4 : 2),
-                         p.dgate_dtype, row.column[j], row.left[j], own[j]);
+                         p.dgate_dtype, row.column[j], row.left[j], v);
         }
       }
       if (p.threshold) {
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) drop(gt[j], k[j]);
+        for (int j = 0; j < kChunks; ++j) drop(gt[j], kept[j], p.drop_scale);
       }
-      if constexpr (kBranch) {
-        if (p.post != VECTRA_BLOCK_NO_NORM) {
+      if constexpr (kPost) {
 #pragma unroll
-          for (int j = 0; j < kChunks; ++j)
+        for (int j = 0; j < kChunks; ++j) {
+          f32x4 w[2];
+          row.use(post_weight, j, w);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              d_post_weight[j][e] += gt[j][e] * x[j][e];
-              d_post_bias[j][e] += gt[j][e];
-              gt[j][e] *= post_weight[j][e];
-            }
-          row.transpose(gt, x, post_r, p.post, p.inverse_width);
+          for (int e = 0; e < 2; ++e) {
+            d_post_weight[j][e] += gt[j][e] * x[j][e];
+            d_post_bias[j][e] += gt[j][e];
+            gt[j][e] *= w[e];
+          }
         }
+        row.transpose(gt, x, post_r, p.post, p.inverse_width);
       }
       if (p.dx && live) row.template store<T>(p.dx, at, p.dx_stride, gt);
     }
-    if constexpr (kBranch) {
+    if constexpr (kGate) {
       if (p.gate_sums || (p.dgate && !gate_full)) {
         over_slots(d_gate);
         if (row.slot == 0) {
@@ -487,7 +603,7 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
   const int64_t plane = static_cast<int64_t>(blockIdx.x) * p.width;
   if (p.weight_sums) write_sums(d_weight, p.weight_sums + plane);
   if (p.bias_sums) write_sums(d_bias, p.bias_sums + plane);
-  if constexpr (kBranch) {
+  if constexpr (kPost) {
     if (p.post_weight_sums) write_sums(d_post_weight, p.post_weight_sums + plane);
     if (p.post_bias_sums) write_sums(d_post_bias, p.post_bias_sums + plane);
   }
@@ -495,45 +611,54 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
 
 // ----------------------------------------------------------------------- host
 
-template <int kLanes_, int kChunks_>
+template <int kLanes_, int kChunks_, int kKind_>
 struct Shape {
-  static constexpr int kLanes = kLanes_, kChunks = kChunks_;
+  static constexpr int kLanes = kLanes_, kChunks = kChunks_, kKind = kKind_;
 };
 
-template <typename F>
-void with_shape(int64_t width, F&& f) {
-  switch (norm_lanes(width)) {
-    case 16: return f(Shape<16, 1>{});
-    case 32: return f(Shape<32, 1>{});
-    case 64: return f(Shape<64, 1>{});
-    case 128: return f(Shape<128, 1>{});
-    case 256: return f(Shape<256, 1>{});
-    case 512: return f(Shape<512, 1>{});
-    default: return width <= 8192 ? f(Shape<1024, 1>{}) : f(Shape<1024, 2>{});
+template <int kKind, typename F>
+void with_kind(const NormShape& shape, F&& f) {
+  switch (shape.lanes) {
+    case 16: return f(Shape<16, 1, kKind>{});
+    case 32: return f(Shape<32, 1, kKind>{});
+    case 64: return f(Shape<64, 1, kKind>{});
+    default:
+      return shape.chunks == 1   ? f(Shape<kMany, 1, kKind>{})
+             : shape.chunks == 2 ? f(Shape<kMany, 2, kKind>{})
+                                 : f(Shape<kMany, 4, kKind>{});
   }
+}
+
+template <typename F>
+void with_shape(const NormShape& shape, int64_t width, F&& f) {
+  if (width < 8) return f(Shape<16, 1, kNarrow>{});
+  return width % 8 ? with_kind<kRagged>(shape, f) : with_kind<kWhole>(shape, f);
 }
 
 template <typename T, typename R>
 int launch_norm(const NormParams& p, int cus, hipStream_t stream) {
-  with_shape(p.width, [&](auto shape) {
-    using S = decltype(shape);
-    using Geometry = Row<S::kLanes, S::kChunks>;
-    const int64_t blocks = (p.rows + Geometry::kRows - 1) / Geometry::kRows;
-    const int64_t most_blocks = static_cast<int64_t>(cus) * (2048 / Geometry::kThreads);
-    norm_kernel<T, R, S::kLanes, S::kChunks>
-        <<<static_cast<uint32_t>(blocks < most_blocks ? blocks : most_blocks), Geometry::kThreads, 0, stream>>>(p);
+  const NormShape shape = norm_shape(p.width);
+  const int64_t blocks = (p.rows + shape.rows - 1) / shape.rows;
+  const int64_t most_blocks = static_cast<int64_t>(cus) * (2048 / shape.threads);
+  with_shape(shape, p.width, [&](auto s) {
+    using S = decltype(s);
+    norm_kernel<T, R, S::kLanes, S::kChunks, S::kKind>
+        <<<static_cast<uint32_t>(blocks < most_blocks ? blocks : most_blocks), shape.threads, 0, stream>>>(p);
   });
   return hipGetLastError() == hipSuccess ? VECTRA_BLOCK_OK : VECTRA_BLOCK_ERR_LAUNCH;
 }
 
 template <typename T, typename R>
 int launch_norm_grad(const NormGradParams& p, int workgroups, hipStream_t stream) {
-  with_shape(p.width, [&](auto shape) {
-    using S = decltype(shape);
-    constexpr int kThreads = Row<S::kLanes, S::kChunks>::kThreads;
-    const auto kernel = p.x ? norm_grad_kernel<T, R, S::kLanes, S::kChunks, true>
-                            : norm_grad_kernel<T, R, S::kLanes, S::kChunks, false>;
-    kernel<<<static_cast<uint32_t>(workgroups), kThreads, 0, stream>>>(p);
+  const NormShape shape = norm_shape(p.width);
+  with_shape(shape, p.width, [&](auto s) {
+    using S = decltype(s);
+    const bool post = p.post != VECTRA_BLOCK_NO_NORM;
+    const auto kernel = p.gate.p ? (post ? norm_grad_kernel<T, R, S::kLanes, S::kChunks, S::kKind, true, true>
+                                         : norm_grad_kernel<T, R, S::kLanes, S::kChunks, S::kKind, true, false>)
+                                 : (post ? norm_grad_kernel<T, R, S::kLanes, S::kChunks, S::kKind, false, true>
+                                         : norm_grad_kernel<T, R, S::kLanes, S::kChunks, S::kKind, false, false>);
+    kernel<<<static_cast<uint32_t>(workgroups), shape.threads, 0, stream>>>(p);
   });
   return hipGetLastError() == hipSuccess ? VECTRA_BLOCK_OK : VECTRA_BLOCK_ERR_LAUNCH;
 }
