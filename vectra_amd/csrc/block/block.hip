@@ -507,6 +507,7 @@ int check_linear8(const vectra_linear8_args* a) {
   if (a->activation < VECTRA_DENSE_NONE || a->activation > VECTRA_DENSE_SILU) return VECTRA_BLOCK_ERR_BAD_OPTION;
   if ((a->gated != 0 && a->gated != 1) || (a->gated && a->residual)) return VECTRA_BLOCK_ERR_BAD_SHAPE;
   if (int st = check_sizes(a->rows, a->width)) return st;
+  if (int st = check_sizes(a->rows, a->width_out)) return st;
   if (int st = check_sizes(a->rows, a->width_out * (1 + a->gated))) return st;
   if (a->rows == 0 || a->width_out == 0) return VECTRA_BLOCK_OK;
   if (!a->out || (a->width && (!a->weight || !a->weight_scales || (!a->x && (!a->codes || !a->scales)))))

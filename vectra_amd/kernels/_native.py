@@ -2,8 +2,11 @@
 
 * ``libvectra_rbf.so``   -- the C-ABI HIP library (include/vectra_rbf.h);
 * ``libvectra_dense.so`` -- the C-ABI dense operators (include/vectra_dense.h);
+* ``libvectra_block.so`` -- the C-ABI operators between a block's dense products,
+  and those products in 8 bits (include/vectra_block.h);
 * ``libvectra_torch.so`` -- the torch.library extension that registers
-  ``vectra::rbf_attention`` and the dense operators and links the first two;
+  ``vectra::rbf_attention``, the dense and the block operators and links the
+  first three;
 * ``libvectra_scan.so``  -- the C-ABI distance scans (include/vectra_scan.h),
   used by vectra_amd.index.
 
@@ -25,6 +28,7 @@ LIB_DIR = os.environ.get('VECTRA_LIB_DIR') or os.path.join(
 HIP_LIBRARY = os.path.join(LIB_DIR, 'libvectra_rbf.so')
 TORCH_LIBRARY = os.path.join(LIB_DIR, 'libvectra_torch.so')
 DENSE_LIBRARY = os.path.join(LIB_DIR, 'libvectra_dense.so')
+BLOCK_LIBRARY = os.path.join(LIB_DIR, 'libvectra_block.so')
 SCAN_LIBRARY = os.path.join(LIB_DIR, 'libvectra_scan.so')
 
 
@@ -100,6 +104,37 @@ def dense_library() -> ctypes.CDLL:
     lib.vectra_dense_status_string.restype = ctypes.c_char_p
     lib.vectra_dense_abi_version.argtypes = []
     lib.vectra_dense_abi_version.restype = ctypes.c_int
+    return lib
+
+
+@functools.cache
+def block_library() -> ctypes.CDLL:
+    """The block-operator library as a ctypes handle (shared with the extension)."""
+    lib = ctypes.CDLL(_require(BLOCK_LIBRARY))
+    lib.vectra_dropout.argtypes = [
+        ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p,
+    ]
+    lib.vectra_dropout.restype = ctypes.c_int
+    lib.vectra_norm_forward.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    lib.vectra_norm_forward.restype = ctypes.c_int
+    lib.vectra_blocks_quantize.argtypes = [
+        ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+    ]
+    lib.vectra_blocks_quantize.restype = ctypes.c_int
+    for name in ('vectra_norm_backward', 'vectra_linear8_forward'):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    for name in ('vectra_norm_backward_workspace_bytes', 'vectra_linear8_workspace_bytes'):
+        size = getattr(lib, name)
+        size.argtypes = [ctypes.c_void_p]
+        size.restype = ctypes.c_int64
+    lib.vectra_block_status_string.argtypes = [ctypes.c_int]
+    lib.vectra_block_status_string.restype = ctypes.c_char_p
+    lib.vectra_block_abi_version.argtypes = []
+    lib.vectra_block_abi_version.restype = ctypes.c_int
     return lib
 
 
