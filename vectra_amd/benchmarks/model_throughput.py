@@ -12,7 +12,8 @@ whole price model at the serving batch (config 5: d_model 128, 8 heads, 3 or
 Modes: `eager` (the baseline), `inductor` (torch.compile without the rewrite,
 which separates Inductor's own fusion from the HIP operator) and `vectra`
 (the deployment compile: every attention site on vectra::rbf_attention).
-`--dense-kernels` puts the model's linear layers on vectra::linear in any mode.
+`--dense-kernels` puts the model's linear layers on vectra::linear in any mode,
+`--norm-kernels` its residual sums and norms on vectra::residual_norm.
 Each run first gates its numerics against the eager model (rtol 1e-3), then
 times `--iters` forward passes after `--warmup` with events, as the median of
 `--trials` trials.  `--compare` checks a candidate against a baseline: same
@@ -59,7 +60,7 @@ def timed(fn, inputs, iters: int, warmup: int, trials: int) -> list[float]:
 
 
 def run(mode: str, batch_size: int, layers: int, block_dtype: str, iters: int, warmup: int,
-        trials: int, dense_kernels: bool = False) -> dict:
+        trials: int, dense_kernels: bool = False, norm_kernels: bool = False) -> dict:
     device = 'cuda'
     spec = compile_entry.ServingSpec(device, batch_size, block_dtype)
     torch.manual_seed(0)
@@ -69,6 +70,8 @@ def run(mode: str, batch_size: int, layers: int, block_dtype: str, iters: int, w
     model = eager
     if dense_kernels:  # the same weights, their linear layers on the dense operators
         model = copy.deepcopy(eager).set_dense_kernels()
+    if norm_kernels:
+        model = copy.deepcopy(model).set_norm_kernels()
     if mode == 'eager':
         fn = model
     elif mode == 'inductor':
@@ -80,7 +83,7 @@ def run(mode: str, batch_size: int, layers: int, block_dtype: str, iters: int, w
     seconds = timed(fn, inputs, iters, warmup, trials)
     per_batch = statistics.median(seconds)
     return {
-        'mode': mode + ('+dense' if dense_kernels else ''),
+        'mode': mode + ('+dense' if dense_kernels else '') + ('+norms' if norm_kernels else ''),
         'device': torch.cuda.get_device_name(device),
         'batch_size': batch_size,
         'block_dtype': block_dtype,
@@ -123,6 +126,8 @@ def main(argv=None) -> int:
     p.add_argument('--trials', type=int, default=5)
     p.add_argument('--dense-kernels', action='store_true',
                    help='run the linear layers through vectra::linear (PriceTransformer.set_dense_kernels)')
+    p.add_argument('--norm-kernels', action='store_true',
+                   help='run residual sums and norms through vectra::residual_norm (PriceTransformer.set_norm_kernels)')
     p.add_argument('--out', default='')
     p.add_argument('--compare', nargs=2, metavar=('BASELINE', 'CANDIDATE'))
     p.add_argument('--min-ratio', type=float, default=3.0)
@@ -142,7 +147,7 @@ def main(argv=None) -> int:
         print('model_throughput needs a GPU', file=sys.stderr)
         return 2
     result = run(args.mode, args.batch_size, args.layers, args.block_dtype, args.iters, args.warmup,
-                 args.trials, args.dense_kernels)
+                 args.trials, args.dense_kernels, args.norm_kernels)
     text = json.dumps(result)
     if args.out:
         os.makedirs(os.path.dirname(args.out) or '.', exist_ok=True)

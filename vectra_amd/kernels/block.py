@@ -89,6 +89,7 @@ from vectra_amd.kernels import _native
 
 NORMS = ('rms', 'layer')
 POST_NORMS = ('none', 'rms', 'layer')
+NORM_WIDTH = 16384  # widest row of a norm
 BLOCK = 128  # elements of a row (and rows of a tile) that share a power of two
 
 _native.load_torch_extension()

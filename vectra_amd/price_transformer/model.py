@@ -36,6 +36,8 @@ class ModelConfig:
     num_candidates: int = 64
     min_candidates: int = 4  # kept when no comparable lies inside the radius
     ffn_gate: bool = False  # a gated (SiLU) feed-forward block; no counterpart in the reference
+    # Of each branch's output before the residual, in training; no counterpart in the reference.
+    dropout: float = 0.0
 
     @classmethod
     def from_dict(cls, values: Mapping[str, typing.Any]) -> 'ModelConfig':
@@ -43,10 +45,12 @@ class ModelConfig:
         return cls(**{k: v for k, v in values.items() if k in names})
 
     def to_dict(self) -> dict[str, typing.Any]:
-        """The fields as the reference writes them; `ffn_gate` only where it is set."""
+        """The fields as the reference writes them; `ffn_gate` and `dropout` only where
+        they are set."""
         values = dataclasses.asdict(self)
-        if not self.ffn_gate:
-            del values['ffn_gate']
+        for own in ('ffn_gate', 'dropout'):
+            if not values[own]:
+                del values[own]
         return values
 
 
@@ -108,9 +112,13 @@ class Block(nn.Module):
     """Pre-norm Transformer block with spatial attention."""
 
     dense_checkpoint: str | None = None  # as SpatialAttention's
+    norm_kernels = False  # residual sums and norms on torch.ops.vectra.residual_norm
+    dropout = 0.0
+    index = 0  # of the block: its two branches draw as streams 2 index and 2 index + 1
 
-    def __init__(self, config: ModelConfig):
+    def __init__(self, config: ModelConfig, index: int = 0):
         super().__init__()
+        self.dropout, self.index = config.dropout, index
         self.norm1 = nn.LayerNorm(config.d_model)
         self.attention = spatial_attention.SpatialAttention(config.d_model, config.num_heads)
         self.norm2 = nn.LayerNorm(config.d_model)
@@ -123,18 +131,46 @@ class Block(nn.Module):
                 nn.Linear(config.ffn_dim, config.d_model),
             )
 
-    def forward(self, x, key_bias):
-        if self.dense_checkpoint is None:
-            x = x + self.attention(self.norm1(x), key_bias)
-            return x + self.ffn(self.norm2(x))
-        if plain_modules.is_plain(self.attention, spatial_attention.SpatialAttention):
-            x = self.attention(self.norm1(x), key_bias, residual=x)
+    def forward(self, x, key_bias, rng=None, normed=None, following=None):
+        """x [B, N, d_model] through both branches.  rng: what dropout draws from (None:
+        none is dropped).  normed: norm1(x), where the caller has it.  following: a norm
+        of the result, which is returned beside it then."""
+        if normed is None:
+            normed = self.norm1(x)
+        joined = self.norm_kernels and plain_modules.is_plain_norm(self.norm2, x.shape[-1])
+        if (self.dense_checkpoint is not None and rng is None and not joined
+                and plain_modules.is_plain(self.attention, spatial_attention.SpatialAttention)):
+            x = self.attention(normed, key_bias, residual=x)
+            normed = self.norm2(x)
         else:
-            x = x + self.attention(self.norm1(x), key_bias)
-        return self._feed_forward(self.norm2(x), x, self.dense_checkpoint)
+            x, normed = self._join(self.attention(normed, key_bias), x, self.norm2, rng, 2 * self.index)
+        if self.dense_checkpoint is None:
+            branch = self.ffn(normed)
+        elif rng is None and following is None:
+            return self._feed_forward(normed, x, self.dense_checkpoint)
+        else:
+            branch = self._feed_forward(normed, None, self.dense_checkpoint)
+        if following is None:
+            return x + self._drop(branch, rng, 2 * self.index + 1)
+        return self._join(branch, x, following, rng, 2 * self.index + 1)
+
+    def _drop(self, branch, rng, stream):
+        return branch if rng is None else torch.ops.vectra.dropout(branch, self.dropout, rng, stream)
+
+    def _join(self, branch, x, norm, rng, stream):
+        """The residual stream with a branch's output, and `norm` of it: in one pass
+        where the norm is a plain one and the types are the operator's (under autocast
+        branches may be narrower than the stream, never wider)."""
+        if (self.norm_kernels and plain_modules.is_plain_norm(norm, x.shape[-1])
+                and x.dtype in (branch.dtype, torch.float32)
+                and (norm.weight is None or norm.weight.dtype in (branch.dtype, torch.float32))):
+            return torch.ops.vectra.residual_norm(branch, x, norm.weight, norm.bias, norm='layer', eps=norm.eps,
+                                                  p=0.0 if rng is None else self.dropout, rng=rng, stream=stream)
+        x = x + self._drop(branch, rng, stream)
+        return x, norm(x)
 
     def _feed_forward(self, x, residual, checkpoint):
-        """The feed-forward block on the dense operators, onto the residual."""
+        """The feed-forward block on the dense operators, onto the residual if there is one."""
         ffn = self.ffn
         if (plain_modules.is_plain(ffn, GatedFeedForward) and plain_modules.is_plain(ffn.gate_up, nn.Linear)
                 and plain_modules.is_plain(ffn.down, nn.Linear)):
@@ -144,7 +180,7 @@ class Block(nn.Module):
             first, second = ffn[0], ffn[2]
             hidden = torch.ops.vectra.linear(x, first.weight, first.bias, None, 'gelu', checkpoint)
         else:
-            return residual + ffn(x)
+            return ffn(x) if residual is None else residual + ffn(x)
         return torch.ops.vectra.linear(hidden, second.weight, second.bias, residual, 'none', checkpoint)
 
 
@@ -158,10 +194,36 @@ class PriceTransformer(nn.Module):
         self.candidate_encoder = candidate_encoder.CandidateEncoder(
             config.embedding_dim, config.attribute_dim, config.d_model
         )
-        self.blocks = nn.ModuleList([Block(config) for _ in range(config.num_layers)])
+        self.blocks = nn.ModuleList([Block(config, i) for i in range(config.num_layers)])
         self.norm = nn.LayerNorm(config.d_model)
         self.head = nn.Linear(config.d_model, 1)
         self._block_dtype = torch.float32
+        if config.dropout:
+            if not 0.0 <= config.dropout < 1.0 - 2 ** -17:  # (in steps of 2^-16)
+                raise ValueError(f'dropout must be at least 0 and at most 1 - 2^-16, not {config.dropout}')
+            # The seed of dropout's generator and the number of training passes so far.
+            # Part of a training run, not of the weights: it is not in the state dict.
+            self.register_buffer('dropout_rng', torch.tensor([torch.initial_seed() % 2**63, 0]), persistent=False)
+
+    def seed_dropout(self, seed: int, passes: int = 0) -> 'PriceTransformer':
+        """Dropout's generator: training pass number `passes` of `seed` comes next.  (Data
+        parallel ranks with equal seeds drop the same elements of their batches.)"""
+        if not self.config.dropout:
+            raise ValueError('the model has no dropout')
+        self.dropout_rng.copy_(torch.tensor([seed, passes]))
+        return self
+
+    def _next_rng(self):
+        """What this pass's dropout draws from; None where nothing is dropped."""
+        if not self.training or not self.config.dropout:
+            return None
+        from vectra_amd.kernels import block as _  # pylint: disable=import-outside-toplevel
+
+        # A copy: the backward pass draws from it again, after later passes too.  Counted
+        # on the device, so that each replay of a captured pass draws anew.
+        rng = self.dropout_rng.clone()
+        self.dropout_rng[1].add_(1)
+        return rng
 
     def set_block_dtype(self, dtype: torch.dtype) -> 'PriceTransformer':
         """Runs the Transformer blocks in `dtype`; encoders, geometry and the
@@ -191,6 +253,31 @@ class PriceTransformer(nn.Module):
                 module.dense_kernels = enabled
         return self
 
+    def set_norm_kernels(self, enabled: bool = True) -> 'PriceTransformer':
+        """Runs the blocks' residual sums and the norms that follow them, dropout
+        between them included, through torch.ops.vectra.residual_norm: one pass over
+        the tokens each, forward and backward, also across blocks.  With
+        set_dense_kernels the residual is added there and not in the products'
+        epilogues.  Norms and blocks that carry hooks, and ones that were wrapped or
+        replaced, are called as they are."""
+        if enabled:
+            from vectra_amd.kernels import block  # pylint: disable=import-outside-toplevel
+
+            if self.config.d_model > block.NORM_WIDTH:
+                raise ValueError(f'd_model {self.config.d_model} exceeds the widest row of a norm, {block.NORM_WIDTH}')
+        for module in self.modules():  # (those inside wrappers too)
+            if isinstance(module, Block):
+                module.norm_kernels = enabled
+        return self
+
+    def _following(self, i: int):
+        """The norm that block i computes with its result: the next block's first, where
+        calls of the two would do nothing besides."""
+        pair = self.blocks[i:i + 2]
+        if len(pair) < 2 or not all(plain_modules.is_plain(b, Block) for b in pair) or not pair[0].norm_kernels:
+            return None
+        return pair[1].norm1 if plain_modules.is_plain_norm(pair[1].norm1, self.config.d_model) else None
+
     def forward(self, query_embedding, query_attributes, query_location, query_cell6,
                 valuation_day, radius_km, cand_embedding, cand_attributes, cand_log_price,
                 cand_sale_day, cand_location, cand_cell6, cand_valid) -> torch.Tensor:
@@ -215,8 +302,15 @@ class PriceTransformer(nn.Module):
         key_bias = torch.zeros_like(token_valid, dtype=tokens.dtype).masked_fill(
             ~token_valid, float('-inf')
         )[:, None, None, :]
-        for block in self.blocks:
-            tokens = block(tokens, key_bias)
+        rng, normed = self._next_rng(), None
+        for i, block in enumerate(self.blocks):
+            following = self._following(i)
+            if following is not None:
+                tokens, normed = block(tokens, key_bias, rng, normed, following)
+            elif normed is not None:
+                tokens, normed = block(tokens, key_bias, rng, normed), None
+            else:  # (a wrapped block need not take more)
+                tokens = block(tokens, key_bias) if rng is None else block(tokens, key_bias, rng)
         weights = valid.to(cand_log_price.dtype)
         baseline = (cand_log_price * weights).sum(-1) / weights.sum(-1).clamp_min(1.0)
         readout = self.head(self.norm(tokens[:, 0].float()))

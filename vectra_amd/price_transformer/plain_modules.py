@@ -1,7 +1,7 @@
 """Which modules an operator may stand in for.
 
-PriceTransformer.set_dense_kernels reads the parameters of linear layers instead
-of calling the layers.  That is the same function only where a call of the module
+PriceTransformer.set_dense_kernels and set_norm_kernels read the parameters of
+linear layers and norms instead of calling them.  That is the same function only where a call of the module
 would do nothing else: for a module of the expected class itself (a subclass, a
 wrapper or a parametrised layer has a forward of its own) that carries no hooks.
 """
@@ -25,3 +25,8 @@ def is_plain_mlp(module: nn.Module) -> bool:
     first, act, second = module
     return (is_plain(first, nn.Linear) and is_plain(act, nn.GELU) and act.approximate == 'none'
             and is_plain(second, nn.Linear))
+
+
+def is_plain_norm(module: nn.Module, width: int) -> bool:
+    """Whether `module` is a plain layer norm over rows of `width`."""
+    return is_plain(module, nn.LayerNorm) and tuple(module.normalized_shape) == (width,)
