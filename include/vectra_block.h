@@ -132,7 +132,7 @@ typedef struct vectra_norm_grad_args {
 
   const void* grad_h; /* NULL: zero */
   const void* grad_n; /* NULL: zero */
-  /* With a gate or a post norm: x and residual.  Else: h as the forward pass rounded it. */
+  /* With a gate, a post norm or a stream of 16 bits: x and residual.  Else h, in fp32. */
   const void* x;
   const void* residual;
   const void* h;

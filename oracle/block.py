@@ -177,7 +177,7 @@ class Stream:
     def backward(self, grad_h=None, grad_n=None):
         """{argument's name: (gradient, bound)}."""
         h, v, post_hat, post_r = self._forward()
-        if self.gate is None and self.post == 'none':  # from h as it was rounded
+        if self.gate is None and self.post == 'none' and self.residual.dtype == torch.float32:  # from h as it was rounded
             h = Bounded(h.v, h.e + rounding(h.v, h.e, self.residual.dtype))
 
         def flat(g):

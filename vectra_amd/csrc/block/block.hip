@@ -284,6 +284,12 @@ int check_norm(const Args& a) {
   return VECTRA_BLOCK_OK;
 }
 
+// Whether the gradients read the branch and the residual, or h: h where it tells all that
+// matters, without a gate and a post norm and as the forward pass had it, in fp32.
+bool reads_branch(const vectra_norm_grad_args& a) {
+  return a.gate || a.post != VECTRA_BLOCK_NO_NORM || a.stream_dtype != VECTRA_BLOCK_F32;
+}
+
 // A vector that is given has the branch's type or fp32.
 bool vector_dtype(const void* p, int32_t dtype, int32_t of) { return !p || dtype == of || dtype == VECTRA_BLOCK_F32; }
 
@@ -363,7 +369,7 @@ int check_backward(const vectra_norm_grad_args* a) {
       !fits(a->post_bias, a->dpost_bias, a->post_bias_dtype))
     return VECTRA_BLOCK_ERR_BAD_DTYPE;
   if (a->width == 0) return VECTRA_BLOCK_OK;
-  const bool branch = a->gate || a->post != VECTRA_BLOCK_NO_NORM;
+  const bool branch = reads_branch(*a);
   if (a->dgate && !a->gate) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
   if ((a->dpost_weight || a->dpost_bias) && a->post == VECTRA_BLOCK_NO_NORM) return VECTRA_BLOCK_ERR_BAD_OPTION;
   if (a->gate && a->gate_rows < 1) return VECTRA_BLOCK_ERR_BAD_SHAPE;
@@ -402,7 +408,7 @@ int backward(const vectra_norm_grad_args& a, Scratch& scratch, bool launch, int 
   const bool sums = a.dweight || a.dbias || a.dpost_weight || a.dpost_bias;
   if (!sums && (a.rows == 0 || (!a.dx && !a.dresidual && !a.dgate))) return VECTRA_BLOCK_OK;
   NormGradParams p{};
-  const bool branch = a.gate || a.post != VECTRA_BLOCK_NO_NORM;
+  const bool branch = reads_branch(a);
   const int64_t gate_rows = a.gate ? std::max<int64_t>(1, std::min(a.gate_rows, a.rows)) : std::max<int64_t>(1, a.rows);
   const bool gate_full = a.gate && gate_rows == 1;
   p.grad_h = a.grad_h;

@@ -10,9 +10,9 @@
 // vectors are loaded once per workgroup, and the next row's loads are issued before a
 // row is worked on.  The sums of a row cross lanes by DPP moves and lane swaps, and
 // waves through LDS with one barrier each.  What bounds it is HBM: 8192 x 4096 bf16 on
-// an fp32 stream, rms norms on both sides and a gate over all rows, 81 us forward
-// (5.0 TB/s) and 148 backward (4.1); 66560 x 128 bf16, layer norm and dropout, 17.5 us
-// and 30 (3.9, 2.9 TB/s).  Past 4096 columns, and with a post norm past 8192 above all,
+// an fp32 stream, rms norms on both sides and a gate over all rows, 80 us forward
+// (5.0 TB/s) and 142 backward (4.3); 66560 x 128 bf16, layer norm and dropout, 17.5 us
+// and 34 (3.9, 3.0 TB/s).  Past 4096 columns, and with a post norm past 8192 above all,
 // the registers do not hold a row's sums and gradients: 4096 x 8192, both norms and a
 // gate, 139 us and 405; 2048 x 16384 184 us and 1740.
 //
@@ -20,9 +20,8 @@
 // within a wave from the wave's own mean, the waves' joined by
 //   sum (x - mean)^2 = sum over waves of [sum (x - mean_w)^2 + count_w (mean_w - mean)^2].
 //
-// The backward pass computes the normalised rows again, from x and r where a gate
-// or a post norm needs them anyway (h is then not read: the same bytes, and in
-// fp32 as the forward pass had it), else from h as it was rounded; statistics are
+// The backward pass computes the normalised rows again, from x and r (h is then not
+// read) or from an fp32 h, in fp32 as the forward pass had them; statistics are
 // not kept.  The vectors' gradients are summed over the rows of a workgroup in
 // registers, then over the workgroups by a second launch in a fixed order.
 #pragma once
@@ -39,7 +38,7 @@ using vectra_dense::u32x4;
 
 // How a row's last chunk is read.  Whole: rows are whole chunks.  Ragged: as the row's
 // last eight elements, moved into place afterwards; read element by element, it would
-// be waited for before the next load (6000 x 1001 bf16 backward 46 -> 36 us).  Narrow:
+// be waited for before the next load (6000 x 1001 bf16 backward 46 -> 36 us, of 5 rows read or written).  Narrow:
 // rows of fewer than eight elements, by those.  (Kinds of their own, because a branch
 // among the loads of the row ahead waits for them where its sides meet: 8192 x 4096
 // forward 77 us, with such a branch 112.)
@@ -397,10 +396,13 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormPar
 
 // ------------------------------------------------------------------- backward
 
-// With a gate or a post norm the branch's output matters: x and r are read, else h.
+// With a gate or a post norm the branch's output matters: x and r are read.  With a
+// stream of 16 bits too, because h as it was rounded is not what the forward pass
+// normalised: the weight's gradient, a sum over the rows, would be off by 1.3e-3 of its
+// norm (a fifth more bytes: 16384 x 2048 bf16 90 us from x and r, 74 from h).
 template <typename T, typename R, int kLanes, int kChunks, int kKind, bool kGate, bool kPost>
 __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const NormGradParams p) {
-  constexpr bool kBranch = kGate || kPost;
+  constexpr bool kBranch = kGate || kPost || sizeof(R) == 2;
   using Row = Row<kLanes, kChunks, kKind>;
   typedef typename Row::Values Values;
   __shared__ f32x4 lds[Row::kLds];

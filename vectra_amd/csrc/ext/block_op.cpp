@@ -316,7 +316,15 @@ std::tuple<Tensor, Tensor, Tensor> residual_norm_8bit_hip(const Tensor& x, const
   return {h, codes, scales};
 }
 
-// The gradients' operands.  h, or x and residual where the branch's output matters.
+// Whether the gradients read x and the residual, or h (of a stream of this type).
+bool reads_branch(at::ScalarType stream_dtype, const OptTensor& gate, std::string_view post) {
+  return has(gate) || post != "none" || stream_dtype != at::kFloat;
+}
+bool reads_branch(const OptTensor& h, const OptTensor& residual, const OptTensor& gate, std::string_view post) {
+  return reads_branch(has(residual) ? residual->scalar_type() : has(h) ? h->scalar_type() : at::kFloat, gate, post);
+}
+
+// The gradients' operands.
 NormOptions check_norm_backward(const OptTensor& grad_h, const OptTensor& grad_n, const OptTensor& h, const OptTensor& x,
                                 const OptTensor& residual, const OptTensor& weight, const OptTensor& bias,
                                 const OptTensor& gate, const OptTensor& post_weight, const OptTensor& post_bias,
@@ -324,9 +332,9 @@ NormOptions check_norm_backward(const OptTensor& grad_h, const OptTensor& grad_n
                                 const OptTensor& rng, int64_t stream, at::ScalarType dtype, at::ArrayRef<bool> wanted) {
   constexpr const char* op = "vectra::residual_norm_backward";
   TORCH_CHECK(wanted.size() == 7, op, ": wanted must name seven gradients (x, residual, weight, bias, gate, post_weight, post_bias)");
-  const bool branch = has(gate) || post != "none";
+  const bool branch = reads_branch(h, residual, gate, post);
   TORCH_CHECK(branch ? has(x) && has(residual) : has(h), op, ": needs ",
-              branch ? "x and residual with a gate or a post norm" : "h, the forward pass's result");
+              branch ? "x and residual with a gate, a post norm or a stream of 16 bits" : "h, the forward pass's result");
   const Tensor& stream_side = branch ? *residual : *h;
   TORCH_CHECK(is_float(dtype), op, ": dtype, x's, must be float32, float16 or bfloat16; got ", dtype);
   TORCH_CHECK(stream_side.dim() >= 1, op, ": h or residual must be [..., width]; got a scalar");
@@ -362,7 +370,7 @@ std::vector<Tensor> residual_norm_backward_hip(const OptTensor& grad_h, const Op
   constexpr const char* op = "vectra::residual_norm_backward";
   const NormOptions o = check_norm_backward(grad_h, grad_n, h, x, residual, weight, bias, gate, post_weight, post_bias, norm,
                                             post, eps, residual_scale, p, rng_in, stream, dtype, wanted);
-  const bool branch = has(gate) || o.post != VECTRA_BLOCK_NO_NORM;
+  const bool branch = reads_branch(h, residual, gate, post);
   const Tensor& side = branch ? *residual : *h;
   c10::DeviceGuard guard(side.device());
   const int64_t width = side.size(-1), rows = rows_of(side);
@@ -566,7 +574,7 @@ std::vector<Tensor> residual_norm_backward_cpu(const OptTensor& grad_h, const Op
                                                int64_t stream, at::ScalarType dtype, std::array<bool, 7> wanted) {
   const NormOptions o = check_norm_backward(grad_h, grad_n, h_in, x, residual, weight, bias, gate, post_weight, post_bias,
                                             norm, post, eps, residual_scale, p, rng, stream, dtype, wanted);
-  const bool with_branch = has(gate) || o.post != VECTRA_BLOCK_NO_NORM;
+  const bool with_branch = reads_branch(h_in, residual, gate, post);
   const Tensor& side = with_branch ? *residual : *h_in;
   const int64_t width = side.size(-1), rows = rows_of(side);
   BranchCpu b;
@@ -867,7 +875,7 @@ Tensor dropout_autograd(const Tensor& x, double p, const Tensor& rng, int64_t st
   return Dropout::apply(x, p, rng, stream);
 }
 
-// Saved: x and the residual where a gate or a post norm reads the branch, else h.
+// Saved: x and the residual, or an fp32 h that tells all that matters.
 class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
@@ -890,7 +898,7 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     ctx->saved_data["p"] = p;
     ctx->saved_data["stream"] = stream;
     ctx->saved_data["dtype"] = static_cast<int64_t>(x.scalar_type());
-    const bool branch = has(gate) || post != "none";
+    const bool branch = reads_branch(residual.scalar_type(), gate, post);
     const auto kept = [](const OptTensor& t) { return has(t) ? *t : Tensor(); };
     ctx->save_for_backward({branch ? Tensor() : h, branch ? x : Tensor(), branch ? residual : Tensor(), kept(weight),
                             kept(bias), kept(gate), kept(post_weight), kept(post_bias), p > 0 ? kept(rng) : Tensor()});

@@ -47,8 +47,8 @@ program that replays a captured graph changes it between replays (rng[1].add_(1)
 and draws anew.
 
 dropout and residual_norm have gradients for every tensor argument but rng;
-residual_norm keeps x and the residual for them where there is a gate or a post
-norm, else h.  Gradients of gradients (of residual_norm) and forward-mode
+residual_norm keeps x and the residual for them where there is a gate, a post
+norm or a residual of 16 bits, else h (in float32: what was normalised).  Gradients of gradients (of residual_norm) and forward-mode
 derivatives are refused, and so is any derivative of residual_norm_8bit, a serving
 form.  The gradients of the vectors are summed in fp32 in a fixed order.
 
@@ -127,8 +127,8 @@ def _residual_norm_8bit_fake(x, residual, weight=None, bias=None, gate=None, pos
 @torch.library.register_fake('vectra::residual_norm_backward')
 def _residual_norm_backward_fake(grad_h, grad_n, h, x, residual, weight, bias, gate, post_weight, post_bias, norm, post,
                                  eps, residual_scale, p, rng, stream, dtype, wanted):
-    del grad_h, grad_n, x, norm, eps, residual_scale, p, rng, stream
-    side = residual if gate is not None or post != 'none' else h
+    del grad_h, grad_n, x, norm, post, eps, residual_scale, p, rng, stream
+    side = residual if residual is not None else h
     made = [lambda: side.new_empty(side.shape, dtype=dtype), lambda: side.new_empty(side.shape)]
     made += [lambda t=t: t.new_empty(t.shape) for t in (weight, bias, gate, post_weight, post_bias)]
     return [make() for make, want in zip(made, wanted) if want]
