@@ -90,6 +90,16 @@ def test_the_widest_rows(width, dtype, stream):
     check(*make((6, width), dtype, stream, norm='rms', device='cuda', seed=width), 'cuda')
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('width', [4097, 8190, 8192, 9001, 16383, 16384])
+@pytest.mark.parametrize('gate,post', [('none', 'none'), ('none', 'layer'), ('vector', 'none'), ('sequence', 'rms'), ('full', 'layer')])
+def test_the_widest_rows_of_several_turns(width, gate, post):
+    """Sums of several rows in a workgroup, with each set of vectors."""
+    shape = (3, 230, width)
+    gate = {'none': None, 'vector': (width,), 'sequence': (3, 1, width), 'full': shape}[gate]
+    check(*make(shape, BF16, F32, norm='layer', post=post, gate=gate, p=0.25 if post == 'layer' else 0.0, device='cuda', seed=width), 'cuda')
+
+
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('dtype,stream', TYPES, ids=str)
 @pytest.mark.parametrize('norm', block.NORMS)

@@ -12,9 +12,12 @@
 // waves through LDS with one barrier each.  What bounds it is HBM: 8192 x 4096 bf16 on
 // an fp32 stream, rms norms on both sides and a gate over all rows, 80 us forward
 // (5.0 TB/s) and 142 backward (4.3); 66560 x 128 bf16, layer norm and dropout, 17.5 us
-// and 34 (3.9, 3.0 TB/s).  Past 4096 columns, and with a post norm past 8192 above all,
-// the registers do not hold a row's sums and gradients: 4096 x 8192, both norms and a
-// gate, 139 us and 405; 2048 x 16384 184 us and 1740.
+// and 34 (3.9, 3.0 TB/s).  Past 4096 columns the registers do not hold a row, its
+// gradients and their sums over the rows: most of the sums are in LDS there, and the
+// vectors over the columns are read again for every row: 4096 x 8192, both norms and a
+// gate, 100 us and 217 (all in registers, spilled: 139 and 405); 2048 x 16384 107 us and
+// 326 (184, 1740).  (A row ahead in registers at two chunks per lane: 96 us with an fp32
+// stream, but 75 instead of 68 with one of 16 bits, so not.)
 //
 // Layer norm's variance is the mean of (x - mean)^2, not a difference of squares:
 // within a wave from the wave's own mean, the waves' joined by
@@ -22,8 +25,7 @@
 //
 // The backward pass computes the normalised rows again, from x and r (h is then not
 // read) or from an fp32 h, in fp32 as the forward pass had them; statistics are
-// not kept.  The vectors' gradients are summed over the rows of a workgroup in
-// registers, then over the workgroups by a second launch in a fixed order.
+// not kept.  The vectors' gradients are summed over the rows of a workgroup, then over the workgroups by a second launch in a fixed order.
 #pragma once
 
 #include "block_common.h"
@@ -200,10 +202,17 @@ struct Row {
     float missing;
     f32x4 value[kChunks == 1 ? 2 : 1];
   };
+  // Chunk j's first column; with several chunks, whose registers are full, known anew at
+  // each use: an address for every vector, chunk and type would be held over the loop.
+  __device__ __forceinline__ int column_of(int j) const {
+    int at = column[j];
+    if constexpr (kChunks > 1) asm volatile("" : "+v"(at));
+    return at;
+  }
   __device__ __forceinline__ void load_chunk(const Held& v, int j, f32x4(&out)[2]) const {
     const void* const row =
         v.from.p ? static_cast<const char*>(v.from.p) + v.at * (v.from.dtype == VECTRA_BLOCK_F32 ? 4 : 2) : nullptr;
-    load_vector(row, v.from.dtype, column[j], left[j], v.missing, out);
+    load_vector(row, v.from.dtype, column_of(j), left[j], v.missing, out);
   }
   __device__ __forceinline__ void hold(const Vector& from, int64_t at, float missing, Held& v) const {
     v.from = from;
@@ -266,7 +275,8 @@ struct Row {
       if constexpr (kKind == kNarrow) {
         e = load_eight<T>(row, width, column[j]);
       } else {
-        const T* const from = row + (kKind == kRagged ? min(column[j], static_cast<int>(width) - 8) : column[j]);
+        const int at = column_of(j);
+        const T* const from = row + (kKind == kRagged ? min(at, static_cast<int>(width) - 8) : at);
         __builtin_memcpy(&e, from, sizeof(e));  // unaligned
       }
     }
@@ -302,7 +312,7 @@ struct Row {
   __device__ __forceinline__ void store(void* p, int64_t row, int64_t stride, const Values& v) const {
 #pragma unroll
     for (int j = 0; j < kChunks; ++j)
-      if (left[j] > 0) store8(static_cast<T*>(p) + row * stride + column[j], v[j][0], v[j][1], left[j]);
+      if (left[j] > 0) store8(static_cast<T*>(p) + row * stride + column_of(j), v[j][0], v[j][1], left[j]);
   }
 };
 
@@ -396,6 +406,28 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormPar
 
 // ------------------------------------------------------------------- backward
 
+// A lane's sums over the rows of a workgroup: in registers, or, past 4096 columns, whose
+// registers are full, in LDS, at kMostLanes vectors apart from `at` on.  A lane's own, which
+// no other reads, so nothing waits for them.
+template <int kChunks, bool kInLds>
+struct Total {
+  f32x4 held[kInLds ? 1 : kChunks * 2];
+  f32x4* at;
+  __device__ __forceinline__ Total(f32x4* mine, int plane) : at(mine + plane * (kChunks * 2 * kMostLanes)) {}
+  __device__ __forceinline__ f32x4& of(int j, int e) { return kInLds ? at[(j * 2 + e) * kMostLanes] : held[kInLds ? 0 : j * 2 + e]; }
+  __device__ __forceinline__ void add(int j, int e, f32x4 v) { of(j, e) += v; }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) of(j, 0) = of(j, 1) = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void get(f32x4 (&out)[kChunks][2]) {
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) out[j][e] = of(j, e);
+  }
+};
+
 // With a gate or a post norm the branch's output matters: x and r are read.  With a
 // stream of 16 bits too, because h as it was rounded is not what the forward pass
 // normalised: the weight's gradient, a sum over the rows, would be off by 1.3e-3 of its
@@ -406,6 +438,10 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
   using Row = Row<kLanes, kChunks, kKind>;
   typedef typename Row::Values Values;
   __shared__ f32x4 lds[Row::kLds];
+  // The vectors' sums that are in LDS, in order: the weight's, the gate's, the post
+  // norm's, the bias's.
+  constexpr int kSums = 2 + kGate + 2 * kPost, kFits = kChunks == 1 ? 0 : 8 / kChunks, kInLds = kFits < kSums ? kFits : kSums;
+  __shared__ f32x4 planes[kInLds ? kInLds * kChunks * 2 * kMostLanes : 1];
   __shared__ float slots[Row::kRows][Row::kWaves ? 1 : kLanes * 8 + 4];
   Row row(p.width, lds);
   typename Row::Held weight, gate, post_weight, post_bias;
@@ -421,7 +457,19 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
   const DropoutKey key = dropout_key(dropout);
   const uint32_t groups = static_cast<uint32_t>((p.width + 7) / 8);
 
-  Values d_weight = {}, d_bias = {}, d_gate = {}, d_post_weight = {}, d_post_bias = {};
+  f32x4* const mine = planes + (kInLds ? threadIdx.x : 0);
+  Total<kChunks, (0 < kInLds)> d_weight(mine, 0);
+  Total<kChunks, (1 < kInLds)> d_gate(mine, 1);
+  Total<kChunks, (1 + kGate < kInLds)> d_post_weight(mine, 1 + kGate);
+  Total<kChunks, (2 + kGate < kInLds)> d_post_bias(mine, 2 + kGate);
+  Total<kChunks, (kSums - 1 < kInLds)> d_bias(mine, kSums - 1);
+  d_weight.clear();
+  d_bias.clear();
+  if constexpr (kGate) d_gate.clear();
+  if constexpr (kPost) {
+    d_post_weight.clear();
+    d_post_bias.clear();
+  }
 
   // The sum over the workgroup's slots of what each holds of a vector's gradient.
   // To all threads' d of slot 0; a workgroup with one slot has it already.
@@ -440,7 +488,9 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
       }
     }
   };
-  const auto write_sums = [&](Values& d, float* to) {
+  const auto write_sums = [&](auto& total, float* to) {
+    Values d;
+    total.get(d);
     over_slots(d);
     if (row.slot == 0)
 #pragma unroll
@@ -449,9 +499,14 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
 
   Eight<T> g_next[kChunks], x_next[kBranch ? kChunks : 1];
   Eight<R> gh_next[kChunks], r_next[kChunks];
+  // With four chunks per lane the gradients are loaded where they are used, that of h
+  // onto what comes from n's: three rows of values in registers instead of four.
+  constexpr bool kLate = kChunks > 2;
   const auto fetch = [&](int64_t at) {
-    if (p.grad_n) row.load(p.grad_n, at, p.grad_n_stride, g_next);
-    if (p.grad_h) row.load(p.grad_h, at, p.grad_h_stride, gh_next);
+    if constexpr (!kLate) {
+      if (p.grad_n) row.load(p.grad_n, at, p.grad_n_stride, g_next);
+      if (p.grad_h) row.load(p.grad_h, at, p.grad_h_stride, gh_next);
+    }
     if constexpr (kBranch) {
       row.load(p.x, at, p.x_stride, x_next);
       row.load(p.residual, at, p.residual_stride, r_next);
@@ -481,8 +536,10 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
       const int64_t at = live ? base + row.slot : last - 1;
       if constexpr (kChunks > 1) fetch(at);
       Values g, gt, x, h;
-      row.widen(g_next, g);
-      row.widen(gh_next, gt);
+      if constexpr (!kLate) {
+        row.widen(g_next, g);
+        row.widen(gh_next, gt);
+      }
       row.widen(r_next, h);
       if constexpr (kBranch) row.widen(x_next, x);
       if constexpr (kGate) {
@@ -491,9 +548,11 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
       if constexpr (kChunks == 1) {
         if (base + Row::kRows < last) fetch(least(base + Row::kRows + row.slot, last - 1));
       }
-      if (!live) {  // (a row of another slot: it must not be summed twice)
+      if constexpr (!Row::kWaves) {
+        if (!live) {  // (a row of another slot: it must not be summed twice)
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) g[j][0] = g[j][1] = gt[j][0] = gt[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int j = 0; j < kChunks; ++j) g[j][0] = g[j][1] = gt[j][0] = gt[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
       }
       uint32_t kept[kChunks];
       if (p.threshold) {
@@ -522,22 +581,38 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
       }
       if (p.grad_n) {
         const float r = row.normalise(h, p.norm, p.inverse_width, p.eps);
+        if constexpr (kLate) {
+          row.load(p.grad_n, at, p.grad_n_stride, g_next);
+          row.widen(g_next, g);
+        }
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
           f32x4 w[2];
           row.use(weight, j, w);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            d_weight[j][e] += g[j][e] * h[j][e];
-            d_bias[j][e] += g[j][e];
+            d_weight.add(j, e, g[j][e] * h[j][e]);
+            d_bias.add(j, e, g[j][e]);
             g[j][e] *= w[e];
           }
         }
         row.transpose(g, h, r, p.norm, p.inverse_width);
+        if constexpr (!kLate) {
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j)
+          for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) gt[j][e] += g[j][e];
+            for (int e = 0; e < 2; ++e) gt[j][e] += g[j][e];
+        }
+      }
+      if constexpr (kLate) {
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+          gt[j][0] = gt[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (p.grad_h) row.widen_chunk(row.load_chunk_of(static_cast<const R*>(p.grad_h) + at * p.grad_h_stride, j), j, gt[j]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (p.grad_n) gt[j][e] += g[j][e];
+        }
       }
       if (p.dresidual && live) {
         Values d;
@@ -556,12 +631,12 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             v[e] *= gt[j][e];
-            d_gate[j][e] += v[e];
+            d_gate.add(j, e, v[e]);
             gt[j][e] *= k[e];
           }
           if (p.dgate && gate_full && live)
             store_vector(static_cast<char*>(p.dgate) + at * p.dgate_stride * (p.dgate_dtype == VECTRA_BLOCK_F32 ? 4 : 2),
-                         p.dgate_dtype, row.column[j], row.left[j], v);
+                         p.dgate_dtype, row.column_of(j), row.left[j], v);
         }
       }
       if (p.threshold) {
@@ -575,8 +650,8 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
           row.use(post_weight, j, w);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            d_post_weight[j][e] += gt[j][e] * x[j][e];
-            d_post_bias[j][e] += gt[j][e];
+            d_post_weight.add(j, e, gt[j][e] * x[j][e]);
+            d_post_bias.add(j, e, gt[j][e]);
             gt[j][e] *= w[e];
           }
         }
@@ -586,19 +661,20 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const No
     }
     if constexpr (kGate) {
       if (p.gate_sums || (p.dgate && !gate_full)) {
-        over_slots(d_gate);
+        Values d;
+        d_gate.get(d);
+        over_slots(d);
         if (row.slot == 0) {
 #pragma unroll
           for (int j = 0; j < kChunks; ++j) {
             if (p.gate_sums)
-              store_vector(p.gate_sums + unit * p.width, VECTRA_BLOCK_F32, row.column[j], row.left[j], d_gate[j]);
+              store_vector(p.gate_sums + unit * p.width, VECTRA_BLOCK_F32, row.column[j], row.left[j], d[j]);
             else
               store_vector(static_cast<char*>(p.dgate) + group * p.dgate_stride * (p.dgate_dtype == VECTRA_BLOCK_F32 ? 4 : 2),
-                           p.dgate_dtype, row.column[j], row.left[j], d_gate[j]);
+                           p.dgate_dtype, row.column[j], row.left[j], d[j]);
           }
         }
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) d_gate[j][0] = d_gate[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        d_gate.clear();
       }
     }
   }
