@@ -416,3 +416,18 @@ def test_captured_graphs_and_eager_calls_between_replays():
         torch.cuda.synchronize()
         for want, (_, out, *_) in zip(wants, graphs):
             assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('width', [40, 1000])
+@pytest.mark.parametrize('norm', block.NORMS)
+def test_rows_whose_mean_square_is_subnormal(width, norm, device):
+    """Without eps.  Elements of 1e-20 to 2e-20 in alternating signs: each square, their
+    mean and its product with 1 / width are off by half of 2^-149 at most, 7e-6 of 1e-40
+    or more, and the root halves relative errors: less than 2^-16 together."""
+    x = torch.rand(3, width, dtype=torch.float64, generator=torch.Generator().manual_seed(width)).add(1).mul(1e-20).float()
+    x[:, ::2].neg_()
+    centred = x.double() - (x.double().mean(-1, keepdim=True) if norm == 'layer' else 0)
+    want = centred / centred.square().mean(-1, keepdim=True).sqrt()
+    _, n = torch.ops.vectra.residual_norm(x.to(device), torch.zeros(3, width, device=device), norm=norm, eps=0.0)
+    assert (n.cpu().double() - want).abs().max() <= 2.0 ** -16 * want.abs().max()

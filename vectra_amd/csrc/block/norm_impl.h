@@ -46,6 +46,12 @@ using vectra_dense::u32x4;
 // forward 77 us, with such a branch 112.)
 enum { kWhole = 0, kRagged = 1, kNarrow = 2 };
 
+// 1 / sqrt(v); the instruction takes subnormals for zero.
+__device__ __forceinline__ float inverse_root(float v) {
+  const bool small = v < 0x1p-126f;
+  return __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v) * (small ? 0x1p32f : 1.f);
+}
+
 // kLanes: of a row, or 0: all of the workgroup's (kMany).
 constexpr int kMany = 0;
 constexpr int kMostLanes = 512;
@@ -115,7 +121,7 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < 8; ++i) s = __builtin_fmaf(v[j][i / 4][i % 4], v[j][i / 4][i % 4], s);
     sum(s, none);
-    const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(s, inverse_width, eps));
+    const float r = inverse_root(__builtin_fmaf(s, inverse_width, eps));
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
       v[j][0] *= r;
@@ -161,7 +167,7 @@ struct Row {
         m2 += __builtin_fmaf(u[2] * d, d, u[1]);
       }
     }
-    const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(m2, inverse_width, eps));
+    const float r = inverse_root(__builtin_fmaf(m2, inverse_width, eps));
 #pragma unroll
     for (int j = 0; j < kChunks; ++j)
 #pragma unroll
