@@ -157,6 +157,19 @@ def test_large_integers(rows, width, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('n', [8191, 8192, 8193, 8207, 8208, 8209, 8224, 10007])
+def test_few_rows_onto_wide_results(n, dtype):
+    """Results around the width from which a workgroup takes two tiles of the weight's rows,
+    and its ends in either of them."""
+    for rows, width in ((1, 300), (16, 1025), (17, 128), (31, 260), (32, 1300), (33, 300)):
+        check(rows, width, n, dtype, 'cuda', exact=True, activation='relu' if n % 2 else 'none', residual=rows != 17, as_codes=rows == 1,
+              seed=rows)
+    check(9, 2000, n, dtype, 'cuda', activation='gelu', residual=True)
+    check(20, 140, n, dtype, 'cuda', gated=True, activation='silu')
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [F16, BF16])
 def test_the_8_bit_cores_are_as_near_as_documented(dtype):
     """Normal operands: 1.6e-5 of the result by its 2-norm before the rounding, so a result is within

@@ -6,7 +6,8 @@
 // Such a call is the weight's bytes, one for each element.  A workgroup of 8 or 16
 // waves takes 16 rows of W (gated: 16 of the gate and the same 16 of the up
 // projection), and its waves share out the blocks of 128 of the contraction; lane
-// (g, i) of a wave loads 32 bytes of row i, so a wave reads whole 128-byte lines.
+// (g, i) of a wave loads 32 bytes of row i, so a wave reads whole 128-byte lines.  (Of
+// a wide W two such tiles: launch_few8.)
 // The codes are turned into bf16 together with their power of two, which is exact,
 // and multiplied on the bf16 matrix cores: exact products, fp32 sums.  (The 8-bit
 // cores drop bits of a product beside a large one, and would save nothing here.)
@@ -47,9 +48,11 @@ struct Block8 {
   __device__ __forceinline__ bf16x8 part(int j) const { return decode(w[j / 2][j % 2 * 2], w[j / 2][j % 2 * 2 + 1], scale); }
 };
 
-template <typename T, int kRowTiles, bool kGated, bool kRaw, int kWaves>
+// kPair: 32 rows of W per workgroup, not gated.
+template <typename T, int kRowTiles, bool kGated, bool kRaw, int kWaves, bool kPair>
 __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params p) {
-  constexpr int kHalves = kGated ? 2 : 1;
+  static_assert(!(kGated && kPair));
+  constexpr int kHalves = kGated || kPair ? 2 : 1;
   constexpr int kBatch = 2;  // blocks of W on their way
   __shared__ f32x4 part[kWaves][kHalves][kRowTiles][64];
   // x in 8 bits: rows 32 bytes apart in the banks.
@@ -57,7 +60,7 @@ __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params 
   __shared__ uint8_t x_bytes[kRaw ? kRawBytes / 128 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, i = lane & 15;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (kPair ? 32 : 16);
   const int blocks = static_cast<int>(p.depth / 128);
   // Rows past the end: W's repeat the last one (their results are not stored), x's
   // are zeros.
@@ -65,7 +68,7 @@ __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params 
   const uint8_t* w_scale[kHalves];
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
-    const int64_t row = least(n0 + i, p.n - 1) + h * p.n;
+    const int64_t row = kPair ? least(n0 + h * 16 + i, p.n - 1) : least(n0 + i, p.n - 1) + h * p.n;
     w_row[h] = p.weight + row * p.depth + g * 32;
     w_scale[h] = p.weight_scales + row / 128 * p.scale_stride;
   }
@@ -163,17 +166,18 @@ __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params 
 #pragma unroll
     for (int t = 0; t < kRowTiles; ++t) part[wave][h][t][lane] = acc[h][t];
   __syncthreads();
-  // A wave finishes one row tile: lane holds outputs n .. n + 3 of row m.
-  if (wave >= kRowTiles) return;
-  const int m = wave * 16 + i;
-  const int64_t n = n0 + 4 * g;
+  // A wave finishes one row tile (of a pair's half): lane holds outputs n .. n + 3 of row m.
+  if (wave >= kRowTiles * (kPair ? 2 : 1)) return;
+  const int tile = wave % kRowTiles, of = wave / kRowTiles;
+  const int m = tile * 16 + i;
+  const int64_t n = n0 + of * 16 + 4 * g;
   const int left = static_cast<int>(least(p.n - n, 4));
   if (m >= p.rows || left <= 0) return;
   f32x4 z = {0.f, 0.f, 0.f, 0.f}, u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) {
-    z += part[k][0][wave][lane];
-    if constexpr (kGated) u += part[k][1][wave][lane];
+    z += part[k][of][tile][lane];
+    if constexpr (kGated) u += part[k][1][tile][lane];
   }
   if (p.bias) {
 #pragma unroll
@@ -192,19 +196,27 @@ __global__ __launch_bounds__(64 * kWaves) void few8_kernel(const Product8Params 
   vectra_dense::store4(static_cast<T*>(p.out) + m * p.out_stride + n, z, left);
 }
 
-template <typename T, bool kGated, int kWaves>
+template <typename T, bool kGated, int kWaves, bool kPair>
 auto few8_for(int64_t rows, bool raw) {
-  if (raw) return few8_kernel<T, 1, kGated, true, kWaves>;
-  return rows <= 16 ? few8_kernel<T, 1, kGated, false, kWaves> : few8_kernel<T, 2, kGated, false, kWaves>;
+  if constexpr (!kPair) {
+    if (raw) return few8_kernel<T, 1, kGated, true, kWaves, false>;
+  }
+  return rows <= 16 ? few8_kernel<T, 1, kGated, false, kWaves, kPair> : few8_kernel<T, 2, kGated, false, kWaves, kPair>;
 }
 
 template <typename T>
 int launch_few8(const Product8Params& p, bool gated, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>((p.n + 15) / 16));
-  // 16 waves where at most one workgroup of 8 would be on a CU.
+  // 16 waves where at most one workgroup of 8 would be on a CU.  Every workgroup reads all
+  // codes of x, from L2: of 32 rows twice the weight's bytes.  Pairs halve that, where they
+  // leave a workgroup for every CU (us with pairs / without: 32 x 4096 -> 16384 26.0 / 35.8,
+  // 8 rows 20.6 / 21.6; 32 x 8192 -> 28672 80 / 105; 32 x 1024 -> 8192 7.7 / 8.3).
+  const bool pair = !gated && !p.x && p.n >= 32 * 256;
   const int waves = p.n <= 16 * 256 ? 16 : 8;
-  const auto kernel = gated ? (waves == 16 ? few8_for<T, true, 16>(p.rows, p.x) : few8_for<T, true, 8>(p.rows, p.x))
-                            : (waves == 16 ? few8_for<T, false, 16>(p.rows, p.x) : few8_for<T, false, 8>(p.rows, p.x));
+  const dim3 grid(static_cast<uint32_t>((p.n + (pair ? 31 : 15)) / (pair ? 32 : 16)));
+  const auto kernel = gated    ? (waves == 16 ? few8_for<T, true, 16, false>(p.rows, p.x) : few8_for<T, true, 8, false>(p.rows, p.x))
+                      : pair   ? few8_for<T, false, 8, true>(p.rows, false)
+                      : waves == 16 ? few8_for<T, false, 16, false>(p.rows, p.x)
+                                    : few8_for<T, false, 8, false>(p.rows, p.x);
   kernel<<<grid, 64 * waves, 0, stream>>>(p);
   return hipGetLastError() == hipSuccess ? VECTRA_BLOCK_OK : VECTRA_BLOCK_ERR_LAUNCH;
 }

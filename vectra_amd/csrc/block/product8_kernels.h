@@ -30,7 +30,8 @@ enum { kLarge8 = 0, kMedium8 = 1, kSmall8 = 2, kTiles8 = 3 };
 constexpr int kTile8[kTiles8] = {256, 128, 64};  // rows and columns
 
 // Rows up to which a product reads the weight straight into registers, and rows and
-// bytes of them up to which its workgroups bring the input into 8 bits themselves.
+// bytes of them up to which its workgroups bring the input into 8 bits themselves.  (64
+// rows so: 4096 -> 4096 18.9 us, tiles 14.3; 8192 -> 8192 56 and 30.)
 constexpr int kFewRows8 = 32, kFewRaw8 = 16, kRawBytes = 16384;
 
 // One definition per type of result.
