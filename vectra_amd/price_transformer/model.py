@@ -256,10 +256,11 @@ class PriceTransformer(nn.Module):
     def set_norm_kernels(self, enabled: bool = True) -> 'PriceTransformer':
         """Runs the blocks' residual sums and the norms that follow them, dropout
         between them included, through torch.ops.vectra.residual_norm: one pass over
-        the tokens each, forward and backward, also across blocks.  With
-        set_dense_kernels the residual is added there and not in the products'
-        epilogues.  Norms and blocks that carry hooks, and ones that were wrapped or
-        replaced, are called as they are."""
+        the tokens each, forward and backward, also across blocks.  For eager runs and
+        training: torch.compile fuses them by itself.  With set_dense_kernels the
+        residual is added there and not in the products' epilogues.  Norms and blocks
+        that carry hooks, and ones that were wrapped or replaced, are called as they
+        are."""
         if enabled:
             from vectra_amd.kernels import block  # pylint: disable=import-outside-toplevel
 
