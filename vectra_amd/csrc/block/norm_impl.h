@@ -13,11 +13,11 @@
 // an fp32 stream, rms norms on both sides and a gate over all rows, 80 us forward
 // (5.0 TB/s) and 142 backward (4.3); 66560 x 128 bf16, layer norm and dropout, 17.5 us
 // and 34 (3.9, 3.0 TB/s).  Past 4096 columns the registers do not hold a row, its
-// gradients and their sums over the rows: most of the sums are in LDS there, and the
-// vectors over the columns are read again for every row: 4096 x 8192, both norms and a
-// gate, 100 us and 217 (all in registers, spilled: 139 and 405); 2048 x 16384 107 us and
-// 326 (184, 1740).  (A row ahead in registers at two chunks per lane: 96 us with an fp32
-// stream, but 75 instead of 68 with one of 16 bits, so not.)
+// gradients and their sums over the rows: most of the sums are in LDS there, and no row
+// is loaded ahead; past 8192 columns, and in the backward pass with a gate and a post norm,
+// the vectors over the columns are read again for every row.  4096 x 8192, both norms and
+// a gate, 82 us and 214 (all in registers, spilled: 139 and 405; the vectors read again
+// 100 forward); 2048 x 16384 108 us and 337 (184, 1740).
 //
 // Layer norm's variance is the mean of (x - mean)^2, not a difference of squares:
 // within a wave from the wave's own mean, the waves' joined by
@@ -57,7 +57,8 @@ constexpr int kMany = 0;
 constexpr int kMostLanes = 512;
 constexpr int row_threads(int lanes) { return lanes == kMany ? kMostLanes : 256; }  // at most
 
-template <int kLanes, int kChunks_, int kKind>
+// kKeep: the vectors over the columns stay in registers (Held).
+template <int kLanes, int kChunks_, int kKind, bool kKeep>
 struct Row {
   static constexpr int kChunks = kChunks_;
   static constexpr bool kWaves = kLanes == kMany;  // several waves per row, one row per workgroup
@@ -199,14 +200,14 @@ struct Row {
       for (int h = 0; h < 2; ++h) g[j][h] = (g[j][h] - hat[j][h] * along - total) * r;
   }
 
-  // A vector over the columns, from element `at` of it on: held in registers, or with
-  // more than one chunk per lane, whose registers are full, read where it is used (from
-  // L1 and L2: every row reads the same).
+  // A vector over the columns, from element `at` of it on: held in registers (kKeep), or,
+  // where they are full, read where it is used (from L1 and L2: every row reads the
+  // same).
   struct Held {
     Vector from;
     int64_t at;
     float missing;
-    f32x4 value[kChunks == 1 ? 2 : 1];
+    f32x4 value[kKeep ? kChunks * 2 : 1];
   };
   // Chunk j's first column; with several chunks, whose registers are full, known anew at
   // each use: an address for every vector, chunk and type would be held over the loop.
@@ -224,12 +225,19 @@ struct Row {
     v.from = from;
     v.at = at;
     v.missing = missing;
-    if constexpr (kChunks == 1) load_chunk(v, 0, v.value);
+    if constexpr (kKeep)
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        f32x4 chunk[2];
+        load_chunk(v, j, chunk);
+        v.value[j * 2] = chunk[0];
+        v.value[j * 2 + 1] = chunk[1];
+      }
   }
   __device__ __forceinline__ void use(const Held& v, int j, f32x4(&out)[2]) const {
-    if constexpr (kChunks == 1) {
-      out[0] = v.value[0];
-      out[1] = v.value[1];
+    if constexpr (kKeep) {
+      out[0] = v.value[j * 2];
+      out[1] = v.value[j * 2 + 1];
     } else {
       load_chunk(v, j, out);
     }
@@ -253,15 +261,15 @@ struct Row {
       Eight<float> e;
       e.part[0].w = c.w[0];
       e.part[1].w = c.w[1];
-      widen_chunk(e, 0, v.value);
+      widen_chunk(e, 0, reinterpret_cast<f32x4(&)[2]>(v.value));
     } else if (v.from.dtype == VECTRA_BLOCK_F16) {
       Eight<_Float16> e;
       e.part[0].w = c.w[0];
-      widen_chunk(e, 0, v.value);
+      widen_chunk(e, 0, reinterpret_cast<f32x4(&)[2]>(v.value));
     } else {
       Eight<__bf16> e;
       e.part[0].w = c.w[0];
-      widen_chunk(e, 0, v.value);
+      widen_chunk(e, 0, reinterpret_cast<f32x4(&)[2]>(v.value));
     }
   }
   // x * weight + bias in place.
@@ -326,7 +334,7 @@ struct Row {
 
 template <typename T, typename R, int kLanes, int kChunks, int kKind>
 __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormParams p) {
-  using Row = Row<kLanes, kChunks, kKind>;
+  using Row = Row<kLanes, kChunks, kKind, kChunks <= 2>;
   typedef typename Row::Values Values;
   __shared__ f32x4 lds[Row::kLds];
   Row row(p.width, lds);
@@ -352,6 +360,7 @@ __global__ __launch_bounds__(row_threads(kLanes)) void norm_kernel(const NormPar
     if (gate_each) {
       gate.at = static_cast<uint32_t>(at) / static_cast<uint32_t>(p.gate_rows) * p.gate_stride;
       if constexpr (kChunks == 1) row.fetch(gate, gate_next);
+      if constexpr (kChunks == 2) row.hold(p.gate, gate.at, 1.f, gate);
     }
   };
   int64_t base = static_cast<int64_t>(blockIdx.x) * Row::kRows;
@@ -441,7 +450,7 @@ struct Total {
 template <typename T, typename R, int kLanes, int kChunks, int kKind, bool kGate, bool kPost>
 __global__ __launch_bounds__(row_threads(kLanes)) void norm_grad_kernel(const NormGradParams p) {
   constexpr bool kBranch = kGate || kPost || sizeof(R) == 2;
-  using Row = Row<kLanes, kChunks, kKind>;
+  using Row = Row<kLanes, kChunks, kKind, kChunks == 1 || (kChunks == 2 && !(kGate && kPost))>;
   typedef typename Row::Values Values;
   __shared__ f32x4 lds[Row::kLds];
   // The vectors' sums that are in LDS, in order: the weight's, the gate's, the post
