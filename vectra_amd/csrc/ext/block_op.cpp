@@ -1,5 +1,6 @@
 // torch.library registration of the operators between a block's dense products:
 //   dropout                 kept elements scaled, the others zero, by a counter-based generator
+//   dropout_pass            what one pass of a program draws from, counted on
 //   residual_norm           a branch onto the residual stream, and the stream's norm
 //   residual_norm_8bit      the same with the norm in 8-bit rows
 //   residual_norm_backward  residual_norm's gradients
@@ -114,6 +115,19 @@ Tensor factors_cpu(int64_t rows, int64_t width, int32_t threshold, const Tensor&
     }
   }
   return out;
+}
+
+// The generator's state as it is, and counted on in place.  One operator, because of
+// compilers: of a clone and an addition in place they see through the first and
+// leave the backward pass the tensor that the second has changed.
+Tensor dropout_pass(Tensor& state) {
+  TORCH_CHECK(state.scalar_type() == at::kLong && state.dim() == 1 && state.size(0) == 2,
+              "vectra::dropout_pass: state must be two int64, the seed and the offset; got ", state.scalar_type(), " ",
+              state.sizes());
+  c10::DeviceGuard guard(state.device());
+  Tensor rng = state.clone(at::MemoryFormat::Contiguous);
+  state.select(0, 1).add_(1);
+  return rng;
 }
 
 // x * factors, 0 where dropped whatever x holds.
@@ -950,6 +964,7 @@ std::tuple<Tensor, Tensor> residual_norm_autograd(const Tensor& x, const Tensor&
 
 TORCH_LIBRARY_FRAGMENT(vectra, m) {
   m.def("dropout(Tensor x, float p, Tensor rng, int stream=0) -> Tensor");
+  m.def("dropout_pass(Tensor(a!) state) -> Tensor");
   m.def(
       "residual_norm(Tensor x, Tensor residual, Tensor? weight=None, Tensor? bias=None, Tensor? gate=None, "
       "Tensor? post_weight=None, Tensor? post_bias=None, *, str norm='rms', str post='none', float eps=1e-6, "
@@ -973,6 +988,7 @@ TORCH_LIBRARY_FRAGMENT(vectra, m) {
 
 TORCH_LIBRARY_IMPL(vectra, CUDA, m) {
   m.impl("dropout", dropout_hip);
+  m.impl("dropout_pass", dropout_pass);
   m.impl("residual_norm", residual_norm_hip);
   m.impl("residual_norm_8bit", residual_norm_8bit_hip);
   m.impl("residual_norm_backward", residual_norm_backward_hip);
@@ -983,6 +999,7 @@ TORCH_LIBRARY_IMPL(vectra, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(vectra, CPU, m) {
   m.impl("dropout", dropout_cpu);
+  m.impl("dropout_pass", dropout_pass);
   m.impl("residual_norm", residual_norm_cpu);
   m.impl("residual_norm_8bit", residual_norm_8bit_cpu);
   m.impl("residual_norm_backward", residual_norm_backward_cpu);

@@ -2,6 +2,8 @@
 dropout, and the residual stream with its norms; and those operators in 8 bits.
 
   y = torch.ops.vectra.dropout(x, p, rng, stream=0)
+  rng = torch.ops.vectra.dropout_pass(state)
+      a copy of a generator's state, which is counted on in place
   h, n = torch.ops.vectra.residual_norm(
       x, residual, weight=None, bias=None, gate=None, post_weight=None,
       post_bias=None, *, norm='rms', post='none', eps=1e-6,
@@ -41,7 +43,11 @@ its key and counter are the two int64 of `rng`, the seed and an offset (modulo
 2^32), the number `stream` (one for each place of the program that draws) and the
 element's position in x.  No mask is stored: the backward pass draws the same
 again, from the same rng, which must therefore not be changed in place between
-the two (autograd raises if it is).  dropout and residual_norm with equal rng,
+the two (autograd raises if it is): a program keeps a state and draws each pass from
+dropout_pass of it.  (Not from state.clone() followed by state[1].add_(1): the
+compiler behind torch.compile removes the clone, and a compiled backward pass would
+draw from what the addition left, another mask, without an error.)
+dropout and residual_norm with equal rng,
 stream and shape drop the same elements.  rng is read when the kernel runs, so a
 program that replays a captured graph changes it between replays (rng[1].add_(1))
 and draws anew.
@@ -109,6 +115,11 @@ def _dropout_fake(x, p, rng, stream=0):
     return x.new_empty(x.shape)
 
 
+@torch.library.register_fake('vectra::dropout_pass')
+def _dropout_pass_fake(state):
+    return state.new_empty(state.shape)
+
+
 @torch.library.register_fake('vectra::residual_norm')
 def _residual_norm_fake(x, residual, weight=None, bias=None, gate=None, post_weight=None, post_bias=None, *, norm='rms',
                         post='none', eps=1e-6, residual_scale=1.0, p=0.0, rng=None, stream=0):
@@ -157,6 +168,12 @@ def _gated_linear_8bit_fake(x, weight, weight_scales, bias=None, activation='sil
 def dropout(x, p, rng, stream=0):
     """x with elements dropped and the others scaled (torch.ops.vectra.dropout)."""
     return torch.ops.vectra.dropout(x, p, rng, stream)
+
+
+def dropout_pass(state):
+    """What a pass draws from: a copy of `state`, two int64, whose second is counted on
+    (torch.ops.vectra.dropout_pass)."""
+    return torch.ops.vectra.dropout_pass(state)
 
 
 def residual_norm(x, residual, weight=None, bias=None, gate=None, post_weight=None, post_bias=None, **options):

@@ -217,13 +217,11 @@ class PriceTransformer(nn.Module):
         """What this pass's dropout draws from; None where nothing is dropped."""
         if not self.training or not self.config.dropout:
             return None
-        from vectra_amd.kernels import block as _  # pylint: disable=import-outside-toplevel
+        from vectra_amd.kernels import block  # pylint: disable=import-outside-toplevel
 
         # A copy: the backward pass draws from it again, after later passes too.  Counted
         # on the device, so that each replay of a captured pass draws anew.
-        rng = self.dropout_rng.clone()
-        self.dropout_rng[1].add_(1)
-        return rng
+        return block.dropout_pass(self.dropout_rng)
 
     def set_block_dtype(self, dtype: torch.dtype) -> 'PriceTransformer':
         """Runs the Transformer blocks in `dtype`; encoders, geometry and the
