@@ -7,6 +7,8 @@ import copy
 import pytest
 import torch
 
+from torch.utils.checkpoint import checkpoint
+
 from vectra_amd.compiler import backend  # noqa: F401  (registers the backend 'vectra')
 from vectra_amd.kernels import block
 from vectra_amd.price_transformer import model as model_lib
@@ -131,3 +133,73 @@ def test_captured_passes_of_the_model_draw_anew(fused):
             torch.cuda.synchronize()
             assert torch.equal(out, want[i]), i
     assert model.dropout_rng.tolist() == [11, 4]
+
+
+# ------------------------------------------------------------ passes that are run again
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('fused', [False, True])
+def test_a_model_that_is_run_again_drops_the_same_elements(fused, device):
+    """Activation checkpointing of the whole model, of a compiled one and in one; the same
+    operations in the same order where nothing is compiled."""
+    model, inputs = build(device)
+    model.set_norm_kernels(fused).seed_dropout(11)
+    weights = list(model.parameters())
+    outs = [model(*inputs) for _ in range(2)]
+    want = gradients(outs, weights)
+
+    def again(m):
+        return lambda *args: checkpoint(m, *args, use_reentrant=False)
+
+    torch._dynamo.reset()
+    for run, most in ((again(model), 0.0), (again(torch.compile(model)), 1e-4), (torch.compile(again(model)), 1e-4)):
+        model.seed_dropout(11)
+        own = [run(*inputs, model.dropout_pass()) for _ in range(2)]
+        assert model.dropout_rng.tolist() == [11, 2]
+        for got, expected in zip(gradients(own, weights), want):
+            assert all(relative(a, b) <= most for a, b in zip(got, expected))
+        assert model.dropout_rng.tolist() == [11, 2]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('fused', [False, True])
+def test_a_model_that_would_draw_again_in_the_backward_pass_is_refused(fused, device):
+    model, inputs = build(device)
+    model.set_norm_kernels(fused).seed_dropout(11)
+    out = checkpoint(model, *inputs, use_reentrant=False)
+    with pytest.raises(RuntimeError, match='within a backward pass'):
+        out.sum().backward()
+    inputs[0].requires_grad_()
+    out = checkpoint(model, *inputs, use_reentrant=True)
+    with pytest.raises(RuntimeError, match='within a backward pass'):
+        out.sum().backward()
+    torch._dynamo.reset()
+    compiled = torch.compile(model)
+    for run in (lambda *args: checkpoint(compiled, *args, use_reentrant=False),
+                torch.compile(lambda *args: checkpoint(model, *args, use_reentrant=False))):
+        with pytest.raises(RuntimeError):
+            run(*inputs).sum().backward()
+    checkpoint(model.eval(), *inputs, use_reentrant=False).sum().backward()  # (nothing is dropped)
+
+
+def test_single_blocks_that_are_run_again_drop_the_same_elements():
+    model, inputs = build()
+    twin = copy.deepcopy(model)
+    for b in twin.blocks:
+        b.forward = lambda *args, own=b.forward: checkpoint(own, *args, use_reentrant=False)
+    want, got = (gradients([m.seed_dropout(11)(*inputs)], list(m.parameters()))[0] for m in (model, twin))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_draws_that_the_caller_takes():
+    model, inputs = build()
+    with torch.no_grad():
+        rng = model.seed_dropout(11).dropout_pass()
+        assert rng.tolist() == [11, 0] and model.dropout_rng.tolist() == [11, 1]
+        first, again = model(*inputs, rng), model(*inputs, rng=rng)
+        assert torch.equal(first, again) and torch.equal(first, model.seed_dropout(11)(*inputs))
+        assert torch.equal(model.eval()(*inputs, rng), model(*inputs))  # (nothing is dropped)
+        assert model.dropout_pass() is None and model.dropout_rng.tolist() == [11, 1]
+        plain, _ = build(dropout=0.0)
+        assert plain.dropout_pass() is None and torch.equal(plain(*inputs, rng), plain(*inputs))

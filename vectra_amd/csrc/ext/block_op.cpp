@@ -25,6 +25,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
 #include <array>
@@ -120,7 +121,13 @@ Tensor factors_cpu(int64_t rows, int64_t width, int32_t threshold, const Tensor&
 // The generator's state as it is, and counted on in place.  One operator, because of
 // compilers: of a clone and an addition in place they see through the first and
 // leave the backward pass the tensor that the second has changed.
+// A forward pass within a backward one is one run again (activation checkpointing):
+// it has to draw what it drew before, which the state no longer tells.
 Tensor dropout_pass(Tensor& state) {
+  TORCH_CHECK(torch::autograd::get_current_graph_task_id() == -1,
+              "vectra::dropout_pass: called within a backward pass. A forward pass that is run again there, as activation "
+              "checkpointing does, has to drop the same elements: take its draws before the checkpointed function and pass "
+              "them to it as an argument");
   TORCH_CHECK(state.scalar_type() == at::kLong && state.dim() == 1 && state.size(0) == 2,
               "vectra::dropout_pass: state must be two int64, the seed and the offset; got ", state.scalar_type(), " ",
               state.sizes());

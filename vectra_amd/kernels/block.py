@@ -46,7 +46,9 @@ again, from the same rng, which must therefore not be changed in place between
 the two (autograd raises if it is): a program keeps a state and draws each pass from
 dropout_pass of it.  (Not from state.clone() followed by state[1].add_(1): the
 compiler behind torch.compile removes the clone, and a compiled backward pass would
-draw from what the addition left, another mask, without an error.)
+draw from what the addition left, another mask, without an error.)  A function that
+activation checkpointing runs again takes its draws as an argument; dropout_pass
+itself raises within a backward pass, where it would draw others.
 dropout and residual_norm with equal rng,
 stream and shape drop the same elements.  rng is read when the kernel runs, so a
 program that replays a captured graph changes it between replays (rng[1].add_(1))

@@ -213,8 +213,13 @@ class PriceTransformer(nn.Module):
         self.dropout_rng.copy_(torch.tensor([seed, passes]))
         return self
 
-    def _next_rng(self):
-        """What this pass's dropout draws from; None where nothing is dropped."""
+    def dropout_pass(self):
+        """What the next pass's dropout draws from, counted on; None where nothing is
+        dropped.  A pass that is run again in the backward one (activation checkpointing
+        of the whole model) takes it as an argument:
+
+            checkpoint(model, *inputs, model.dropout_pass(), use_reentrant=False)
+        """
         if not self.training or not self.config.dropout:
             return None
         from vectra_amd.kernels import block  # pylint: disable=import-outside-toplevel
@@ -279,8 +284,9 @@ class PriceTransformer(nn.Module):
 
     def forward(self, query_embedding, query_attributes, query_location, query_cell6,
                 valuation_day, radius_km, cand_embedding, cand_attributes, cand_log_price,
-                cand_sale_day, cand_location, cand_cell6, cand_valid) -> torch.Tensor:
-        """Predicted natural-log prices [B]."""
+                cand_sale_day, cand_location, cand_cell6, cand_valid, rng=None) -> torch.Tensor:
+        """Predicted natural-log prices [B].  rng: this pass's dropout_pass(), where the
+        caller has taken it."""
         distance = microhood.haversine_km(query_location, cand_location)
         valid = trim_to_radius(
             distance, radius_km, cand_valid, min(self.config.min_candidates, cand_valid.shape[-1])
@@ -301,7 +307,9 @@ class PriceTransformer(nn.Module):
         key_bias = torch.zeros_like(token_valid, dtype=tokens.dtype).masked_fill(
             ~token_valid, float('-inf')
         )[:, None, None, :]
-        rng, normed = self._next_rng(), None
+        if rng is None or not self.training or not self.config.dropout:
+            rng = self.dropout_pass()
+        normed = None
         for i, block in enumerate(self.blocks):
             following = self._following(i)
             if following is not None:
