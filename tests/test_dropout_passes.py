@@ -7,6 +7,7 @@ import copy
 import pytest
 import torch
 
+from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.checkpoint import checkpoint
 
 from vectra_amd.compiler import backend  # noqa: F401  (registers the backend 'vectra')
@@ -203,3 +204,47 @@ def test_draws_that_the_caller_takes():
         assert model.dropout_pass() is None and model.dropout_rng.tolist() == [11, 1]
         plain, _ = build(dropout=0.0)
         assert plain.dropout_pass() is None and torch.equal(plain(*inputs, rng), plain(*inputs))
+
+
+# ------------------------------------------------------------------ what is dropped
+
+
+class Draws(TorchDispatchMode):
+    """The stream numbers that a run draws with, in order."""
+
+    def __init__(self):
+        super().__init__()
+        self.streams = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        kwargs = kwargs or {}
+        if func is torch.ops.vectra.dropout.default:
+            self.streams.append(args[3] if len(args) > 3 else kwargs.get('stream', 0))
+        elif func is torch.ops.vectra.residual_norm.default and kwargs.get('p', 0.0) > 0:
+            self.streams.append(kwargs.get('stream', 0))
+        return func(*args, **kwargs)
+
+
+def draws(model, inputs):
+    with torch.no_grad(), Draws() as seen:
+        model(*inputs)
+    return seen.streams
+
+
+@pytest.mark.parametrize('fused', [False, True])
+def test_a_block_in_eval_mode_drops_nothing(fused):
+    """As nn.Dropout inside of it would: by its own flag, whatever the model's is."""
+    model, inputs = build(layers=3)
+    model.set_norm_kernels(fused)
+    with torch.no_grad():
+        still = copy.deepcopy(model).eval()(*inputs)
+        model.blocks.eval()
+        assert model.training and draws(model, inputs) == []
+        assert torch.equal(model(*inputs), still) and model.dropout_rng[1] == 0
+        assert torch.equal(model(*inputs, torch.tensor([1, 2])), still)
+        model.blocks[1].train()
+        assert draws(model, inputs) == [2, 3] and model.dropout_rng[1] == 1
+        assert not torch.equal(model(*inputs), still)
+        model.eval()
+        model.blocks[2].train()
+        assert draws(model, inputs) == [4, 5]

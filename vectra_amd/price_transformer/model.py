@@ -135,6 +135,8 @@ class Block(nn.Module):
         """x [B, N, d_model] through both branches.  rng: what dropout draws from (None:
         none is dropped).  normed: norm1(x), where the caller has it.  following: a norm
         of the result, which is returned beside it then."""
+        if not self.training:
+            rng = None
         if normed is None:
             normed = self.norm1(x)
         joined = self.norm_kernels and plain_modules.is_plain_norm(self.norm2, x.shape[-1])
@@ -215,12 +217,12 @@ class PriceTransformer(nn.Module):
 
     def dropout_pass(self):
         """What the next pass's dropout draws from, counted on; None where nothing is
-        dropped.  A pass that is run again in the backward one (activation checkpointing
+        dropped (blocks drop where they are in training, each by itself).  A pass that is run again in the backward one (activation checkpointing
         of the whole model) takes it as an argument:
 
             checkpoint(model, *inputs, model.dropout_pass(), use_reentrant=False)
         """
-        if not self.training or not self.config.dropout:
+        if not self.config.dropout or not any(block.training for block in self.blocks):
             return None
         from vectra_amd.kernels import block  # pylint: disable=import-outside-toplevel
 
@@ -307,7 +309,9 @@ class PriceTransformer(nn.Module):
         key_bias = torch.zeros_like(token_valid, dtype=tokens.dtype).masked_fill(
             ~token_valid, float('-inf')
         )[:, None, None, :]
-        if rng is None or not self.training or not self.config.dropout:
+        if not self.config.dropout:
+            rng = None
+        elif rng is None:
             rng = self.dropout_pass()
         normed = None
         for i, block in enumerate(self.blocks):
@@ -317,7 +321,7 @@ class PriceTransformer(nn.Module):
             elif normed is not None:
                 tokens, normed = block(tokens, key_bias, rng, normed), None
             else:  # (a wrapped block need not take more)
-                tokens = block(tokens, key_bias) if rng is None else block(tokens, key_bias, rng)
+                tokens = block(tokens, key_bias) if rng is None or not block.training else block(tokens, key_bias, rng)
         weights = valid.to(cand_log_price.dtype)
         baseline = (cand_log_price * weights).sum(-1) / weights.sum(-1).clamp_min(1.0)
         readout = self.head(self.norm(tokens[:, 0].float()))
