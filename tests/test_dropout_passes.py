@@ -17,10 +17,10 @@ from vectra_amd.price_transformer import model as model_lib
 DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
 
 
-def build(device='cpu', dropout=0.5, layers=2):
+def build(device='cpu', dropout=0.5, layers=2, gate=False):
     torch.manual_seed(0)
     config = model_lib.ModelConfig(d_model=48, num_heads=4, num_layers=layers, ffn_dim=80, num_candidates=12,
-                                   embedding_dim=24, attribute_dim=7, dropout=dropout)
+                                   embedding_dim=24, attribute_dim=7, ffn_gate=gate, dropout=dropout)
     return model_lib.PriceTransformer(config).to(device), model_lib.example_inputs(config, 9, device, seed=1)
 
 
@@ -248,3 +248,19 @@ def test_a_block_in_eval_mode_drops_nothing(fused):
         model.eval()
         model.blocks[2].train()
         assert draws(model, inputs) == [4, 5]
+
+
+@pytest.mark.parametrize('dense', [False, True])
+@pytest.mark.parametrize('gate', [False, True])
+@pytest.mark.parametrize('fused', [False, True])
+def test_a_run_draws_each_branch_with_a_number_of_its_own(fused, gate, dense):
+    """In a whole forward pass, and as many in its backward one."""
+    model, inputs = build(layers=3, gate=gate)
+    model.set_norm_kernels(fused)
+    if dense:
+        model.set_dense_kernels()
+    assert draws(model, inputs) == [0, 1, 2, 3, 4, 5]
+    with Draws() as seen:
+        model(*inputs).sum().backward()
+    if not fused:  # (the fused backward operator draws the branches that it joins)
+        assert sorted(seen.streams) == [i // 2 for i in range(12)]
