@@ -6,6 +6,9 @@ import copy
 
 import pytest
 import torch
+import torch.distributed as dist
+from torch import multiprocessing
+from torch import nn
 
 from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.checkpoint import checkpoint
@@ -264,3 +267,66 @@ def test_a_run_draws_each_branch_with_a_number_of_its_own(fused, gate, dense):
         model(*inputs).sum().backward()
     if not fused:  # (the fused backward operator draws the branches that it joins)
         assert sorted(seen.streams) == [i // 2 for i in range(12)]
+
+
+# ------------------------------------------------------- where the generator's state is
+
+
+class Loss(torch.nn.Module):
+    """A model inside another, as a loss that wraps it."""
+
+    def __init__(self, model):
+        super().__init__()
+        self.model = model
+
+    def forward(self, *inputs):
+        return self.model(*inputs)
+
+
+def data_parallel_rank(rank, path):
+    """Two replicas with seeds of their own drop by their own seeds and keep equal weights."""
+    dist.init_process_group('gloo', init_method=f'file://{path}', rank=rank, world_size=2)
+    torch.set_num_threads(1)
+    for wrap in (lambda m: m, Loss):
+        model, inputs = build()
+        model.seed_dropout(100 + rank)
+        alone = copy.deepcopy(model)
+        replica = nn.parallel.DistributedDataParallel(wrap(model))
+        for i in range(2):
+            out = replica(*inputs)
+            assert torch.equal(out, alone(*inputs)), (rank, i)
+            assert model.dropout_rng.tolist() == [100 + rank, i + 1]
+            out.sum().backward()
+        grads = [torch.zeros_like(model.head.weight) for _ in range(2)]
+        dist.all_gather(grads, model.head.weight.grad)
+        assert torch.equal(grads[0], grads[1])
+    dist.destroy_process_group()
+
+
+def test_data_parallel_ranks_draw_by_their_own_seeds(tmp_path):
+    multiprocessing.spawn(data_parallel_rank, (str(tmp_path / 'store'),), nprocs=2)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_the_state_moves_with_the_model(device, tmp_path):
+    model, inputs = build()
+    model.seed_dropout(11, 5)
+    with torch.no_grad():
+        want = model(*inputs)
+        model.half().float()
+        assert model.dropout_rng.dtype == torch.int64
+        moved = copy.deepcopy(model).to(device).seed_dropout(11, 5)
+        assert moved.dropout_rng.device.type == device and moved.dropout_rng is not model.dropout_rng
+        moved(*(t.to(device) for t in inputs))
+        assert moved.dropout_rng.tolist() == [11, 6] and moved.to('cpu').dropout_rng.tolist() == [11, 6]
+        # Pickled and restored, and made without memory, which leaves the state as it was made.
+        torch.save(model, tmp_path / 'model.pt')
+        again = torch.load(tmp_path / 'model.pt', weights_only=False)
+        assert again.dropout_rng.tolist() == [11, 6] and torch.equal(again.seed_dropout(11, 5).to('cpu')(*inputs), model.seed_dropout(11, 5)(*inputs))
+        torch.manual_seed(77)
+        with torch.device('meta'):
+            empty = model_lib.PriceTransformer(model.config)
+        assert empty.to_empty(device=device).dropout_rng.tolist() == [77, 0]
+        assert empty.dropout_rng.device.type == device
+    assert relative(want, model.seed_dropout(11, 5)(*inputs)) < 1e-2  # (once through fp16)
+    assert 'dropout_rng' not in model.state_dict()

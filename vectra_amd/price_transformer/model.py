@@ -204,12 +204,20 @@ class PriceTransformer(nn.Module):
             if not 0.0 <= config.dropout < 1.0 - 2 ** -17:  # (in steps of 2^-16)
                 raise ValueError(f'dropout must be at least 0 and at most 1 - 2^-16, not {config.dropout}')
             # The seed of dropout's generator and the number of training passes so far.
-            # Part of a training run, not of the weights: it is not in the state dict.
-            self.register_buffer('dropout_rng', torch.tensor([torch.initial_seed() % 2**63, 0]), persistent=False)
+            # Part of a training run, not of the weights, and of this process's run: no
+            # buffer, which data parallel wrappers would overwrite with the first rank's.
+            self.dropout_rng = torch.tensor([torch.initial_seed() % 2**63, 0], device='cpu')
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.config.dropout:  # (the state goes where the weights go)
+            self.dropout_rng = self.dropout_rng.to(fn(self.dropout_rng).device)
+        return self
 
     def seed_dropout(self, seed: int, passes: int = 0) -> 'PriceTransformer':
         """Dropout's generator: training pass number `passes` of `seed` comes next.  (Data
-        parallel ranks with equal seeds drop the same elements of their batches.)"""
+        parallel ranks with equal seeds drop the same elements of their batches: each
+        gives its own, after wrapping or before.)"""
         if not self.config.dropout:
             raise ValueError('the model has no dropout')
         self.dropout_rng.copy_(torch.tensor([seed, passes]))
