@@ -50,7 +50,8 @@ draw from what the addition left, another mask, without an error.)  A function t
 activation checkpointing runs again takes its draws as an argument; dropout_pass
 itself raises within a backward pass, where it would draw others.
 dropout and residual_norm with equal rng,
-stream and shape drop the same elements.  rng is read when the kernel runs, so a
+stream and shape drop the same elements.  Under torch.vmap, where every sample would draw the same, dropout of what is batched
+is refused unless rng is batched too or randomness is 'same'.  rng is read when the kernel runs, so a
 program that replays a captured graph changes it between replays (rng[1].add_(1))
 and draws anew.
 
@@ -165,6 +166,57 @@ def _linear_8bit_fake(x, weight, weight_scales, bias=None, residual=None, activa
 def _gated_linear_8bit_fake(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None):
     del weight_scales, bias, activation, scales
     return x.new_empty((*x.shape[:-1], weight.shape[0] // 2), dtype=dtype)
+
+
+# Under vmap, where samples would share one mask without a word: as torch's own random
+# operators, refused unless the caller has said how samples draw, here by an rng for each
+# of them or by randomness='same'.  (Within a backward pass, which may be vmapped over
+# gradients of one forward pass, each has to drop the same elements.)  The key is that of
+# operators that draw; below it the operators are looped over the samples as before.
+
+_vmap = torch.library.Library('vectra', 'IMPL')
+
+
+def _check_samples(name, p, rng, x):
+    functorch = torch._C._functorch
+    layer = functorch.peek_interpreter_stack()
+    if layer is None or layer.key() != functorch.TransformType.Vmap:
+        return
+    if round(65536 * p) < 1 or torch._C._current_graph_task_id() != -1:
+        return
+    if functorch.CVmapInterpreterPtr(layer).randomness() == functorch.RandomnessType.Same:
+        return
+
+    def batched(t):
+        return t is not None and functorch.is_batchedtensor(t) and functorch.maybe_get_level(t) == layer.level()
+
+    if batched(x) and not batched(rng):
+        raise RuntimeError(f'vectra::{name}: vmap over dropout would drop the same elements of every sample: give each '
+                           "sample an rng of its own (batch it too), or say randomness='same'")
+
+
+def _below_vmap(op, *args, **kwargs):
+    mode = torch._C.DispatchKeySet(torch._C.DispatchKey.FuncTorchVmapMode)
+    with torch._C._ExcludeDispatchKeyGuard(mode):
+        return op(*args, **kwargs)
+
+
+def _dropout_vmap(x, p, rng, stream=0):
+    _check_samples('dropout', p, rng, x)
+    return _below_vmap(torch.ops.vectra.dropout, x, p, rng, stream)
+
+
+def _norm_vmap(name):
+    def run(x, residual, *vectors, p=0.0, rng=None, **options):
+        _check_samples(name, p, rng, x)
+        return _below_vmap(getattr(torch.ops.vectra, name), x, residual, *vectors, p=p, rng=rng, **options)
+
+    return run
+
+
+_vmap.impl('dropout', _dropout_vmap, 'FuncTorchVmapMode')
+_vmap.impl('residual_norm', _norm_vmap('residual_norm'), 'FuncTorchVmapMode')
+_vmap.impl('residual_norm_8bit', _norm_vmap('residual_norm_8bit'), 'FuncTorchVmapMode')
 
 
 def dropout(x, p, rng, stream=0):
