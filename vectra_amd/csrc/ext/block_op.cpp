@@ -667,8 +667,8 @@ struct Layer8 {
 };
 
 Layer8 check_layer8(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
-                    const OptTensor& residual, const OptTensor& scales, std::optional<at::ScalarType> dtype, bool gated,
-                    const char* op) {
+                    const OptTensor& residual, const OptTensor& scales, std::optional<at::ScalarType> dtype,
+                    std::optional<int64_t> width, bool gated, const char* op) {
   TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && weight_scales.dim() == 2, op,
               ": x must be [..., width], weight and weight_scales matrices; got ", x.sizes(), ", ", weight.sizes(), " and ",
               weight_scales.sizes());
@@ -695,6 +695,9 @@ Layer8 check_layer8(const Tensor& x, const Tensor& weight, const Tensor& weight_
                   weight_scales.size(1) == (l.width + 511) / 512 * 4,
               op, ": weight must be [width_out, width] in tiles of 128 x 128, as quantize_blocks makes it; got ",
               weight.sizes(), " with scales ", weight_scales.sizes(), " for x ", x.sizes());
+  // (Codes and scales tell the weight's width only rounded up to a block.)
+  TORCH_CHECK(!width.has_value() || (has(scales) ? (*width >= 0 && (*width + 127) / 128 * 128 == l.width) : *width == l.width), op,
+              ": x must be ", width.value_or(0), " wide, as the weight is; got ", x.sizes(), has(scales) ? " of codes" : "");
   TORCH_CHECK(!gated || l.n_w % 2 == 0, op, ": weight must hold the gate's rows and as many rows of the up projection; got ",
               weight.sizes());
   TORCH_CHECK(weight.device() == x.device() && weight_scales.device() == x.device(), op, ": weight and weight_scales must be on ",
@@ -717,8 +720,8 @@ Tensor packed(const Tensor& t) {
 
 Tensor layer8_hip(const Tensor& x, const Tensor& weight_in, const Tensor& weight_scales_in, const OptTensor& bias_in,
                   const OptTensor& residual, c10::string_view activation, const OptTensor& scales_in,
-                  std::optional<at::ScalarType> dtype, bool gated, const char* op) {
-  const Layer8 l = check_layer8(x, weight_in, weight_scales_in, bias_in, residual, scales_in, dtype, gated, op);
+                  std::optional<at::ScalarType> dtype, std::optional<int64_t> width, bool gated, const char* op) {
+  const Layer8 l = check_layer8(x, weight_in, weight_scales_in, bias_in, residual, scales_in, dtype, width, gated, op);
   const int32_t act = activation_of(activation, op);
   c10::DeviceGuard guard(x.device());
   const int64_t n = gated ? l.n_w / 2 : l.n_w;
@@ -773,8 +776,8 @@ Tensor values_cpu(const Tensor& codes_in, const Tensor& scales_in, int64_t high)
 
 Tensor layer8_cpu(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
                   const OptTensor& residual, c10::string_view activation, const OptTensor& scales,
-                  std::optional<at::ScalarType> dtype, bool gated, const char* op) {
-  const Layer8 l = check_layer8(x, weight, weight_scales, bias, residual, scales, dtype, gated, op);
+                  std::optional<at::ScalarType> dtype, std::optional<int64_t> width, bool gated, const char* op) {
+  const Layer8 l = check_layer8(x, weight, weight_scales, bias, residual, scales, dtype, width, gated, op);
   const int32_t act = activation_of(activation, op);
   const int64_t rows = rows_of(x), n = gated ? l.n_w / 2 : l.n_w;
   if (rows == 0 || n == 0) return at::empty(with_last(x, n), x.options().dtype(l.dtype));
@@ -798,18 +801,20 @@ Tensor layer8_cpu(const Tensor& x, const Tensor& weight, const Tensor& weight_sc
 }
 
 template <Tensor (*kLayer)(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::string_view,
-                           const OptTensor&, std::optional<at::ScalarType>, bool, const char*)>
+                           const OptTensor&, std::optional<at::ScalarType>, std::optional<int64_t>, bool, const char*)>
 Tensor linear_8bit(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
                    const OptTensor& residual, c10::string_view activation, const OptTensor& scales,
-                   std::optional<at::ScalarType> dtype) {
-  return kLayer(x, weight, weight_scales, bias, residual, activation, scales, dtype, false, "vectra::linear_8bit");
+                   std::optional<at::ScalarType> dtype, std::optional<int64_t> width) {
+  return kLayer(x, weight, weight_scales, bias, residual, activation, scales, dtype, width, false, "vectra::linear_8bit");
 }
 
 template <Tensor (*kLayer)(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::string_view,
-                           const OptTensor&, std::optional<at::ScalarType>, bool, const char*)>
+                           const OptTensor&, std::optional<at::ScalarType>, std::optional<int64_t>, bool, const char*)>
 Tensor gated_linear_8bit(const Tensor& x, const Tensor& weight, const Tensor& weight_scales, const OptTensor& bias,
-                         c10::string_view activation, const OptTensor& scales, std::optional<at::ScalarType> dtype) {
-  return kLayer(x, weight, weight_scales, bias, std::nullopt, activation, scales, dtype, true, "vectra::gated_linear_8bit");
+                         c10::string_view activation, const OptTensor& scales, std::optional<at::ScalarType> dtype,
+                         std::optional<int64_t> width) {
+  return kLayer(x, weight, weight_scales, bias, std::nullopt, activation, scales, dtype, width, true,
+                "vectra::gated_linear_8bit");
 }
 
 // --------------------------------------------------------------- gradients
@@ -987,10 +992,10 @@ TORCH_LIBRARY_FRAGMENT(vectra, m) {
   m.def("quantize_blocks(Tensor x, bool tiles=False) -> (Tensor, Tensor)");
   m.def(
       "linear_8bit(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None, Tensor? residual=None, "
-      "str activation='none', *, Tensor? scales=None, ScalarType? dtype=None) -> Tensor");
+      "str activation='none', *, Tensor? scales=None, ScalarType? dtype=None, int? width=None) -> Tensor");
   m.def(
       "gated_linear_8bit(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None, str activation='silu', *, "
-      "Tensor? scales=None, ScalarType? dtype=None) -> Tensor");
+      "Tensor? scales=None, ScalarType? dtype=None, int? width=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(vectra, CUDA, m) {

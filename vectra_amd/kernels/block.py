@@ -15,10 +15,11 @@ dropout, and the residual stream with its norms; and those operators in 8 bits.
       n in 8-bit rows, as torch.ops.vectra.linear_8bit reads them
   codes, scales = torch.ops.vectra.quantize_blocks(x, tiles=False)
   y = torch.ops.vectra.linear_8bit(x, weight, weight_scales, bias=None,
-      residual=None, activation='none', *, scales=None, dtype=None)
+      residual=None, activation='none', *, scales=None, dtype=None,
+      width=None)
       act(x @ weight.T + bias) + residual, x and weight in 8 bits
   y = torch.ops.vectra.gated_linear_8bit(x, weight, weight_scales, bias=None,
-      activation='silu', *, scales=None, dtype=None)
+      activation='silu', *, scales=None, dtype=None, width=None)
       act(x @ gate.T + b_g) * (x @ up.T + b_u), weight = cat([gate, up])
 
 Dropout and norms.  x [..., width] is float32, float16 or bfloat16 (any strides; views without unit
@@ -70,7 +71,9 @@ rounded up to 128] (zeros behind the width), scales float8_e8m0fnu
 ceil(width / 128) are not used).  A layer takes float32, float16 or bfloat16 inputs,
 which it brings into 8 bits itself, and returns their type; or codes with `scales`
 (residual_norm_8bit's, or quantize_blocks'), and returns `dtype`.  bias is the
-result's type or float32, the residual the result's type.
+result's type or float32, the residual the result's type.  Codes and scales tell a
+weight's width only rounded up to a block of 128: with `width`, the weight's own, an x
+of another is refused; without it, one within the same block is taken as ending in zeros.
 
 float32 results, and those of at most 32 rows, are exact products of the 8-bit values
 in fp32 sums, rounded once.  float16 and bfloat16 results of more rows come from the
@@ -157,14 +160,16 @@ def _quantize_blocks_fake(x, tiles=False):
 
 
 @torch.library.register_fake('vectra::linear_8bit')
-def _linear_8bit_fake(x, weight, weight_scales, bias=None, residual=None, activation='none', *, scales=None, dtype=None):
-    del weight_scales, bias, residual, activation, scales
+def _linear_8bit_fake(x, weight, weight_scales, bias=None, residual=None, activation='none', *, scales=None, dtype=None,
+                      width=None):
+    del weight_scales, bias, residual, activation, scales, width
     return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dtype)
 
 
 @torch.library.register_fake('vectra::gated_linear_8bit')
-def _gated_linear_8bit_fake(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None):
-    del weight_scales, bias, activation, scales
+def _gated_linear_8bit_fake(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None,
+                            width=None):
+    del weight_scales, bias, activation, scales, width
     return x.new_empty((*x.shape[:-1], weight.shape[0] // 2), dtype=dtype)
 
 
@@ -245,11 +250,14 @@ def quantize_blocks(x, tiles=False):
     return torch.ops.vectra.quantize_blocks(x, tiles)
 
 
-def linear_8bit(x, weight, weight_scales, bias=None, residual=None, activation='none', *, scales=None, dtype=None):
+def linear_8bit(x, weight, weight_scales, bias=None, residual=None, activation='none', *, scales=None, dtype=None,
+                width=None):
     """act(x @ weight.T + bias) + residual in 8 bits (torch.ops.vectra.linear_8bit)."""
-    return torch.ops.vectra.linear_8bit(x, weight, weight_scales, bias, residual, activation, scales=scales, dtype=dtype)
+    return torch.ops.vectra.linear_8bit(x, weight, weight_scales, bias, residual, activation, scales=scales, dtype=dtype,
+                                        width=width)
 
 
-def gated_linear_8bit(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None):
+def gated_linear_8bit(x, weight, weight_scales, bias=None, activation='silu', *, scales=None, dtype=None, width=None):
     """act(x @ gate.T + b_g) * (x @ up.T + b_u) in 8 bits (torch.ops.vectra.gated_linear_8bit)."""
-    return torch.ops.vectra.gated_linear_8bit(x, weight, weight_scales, bias, activation, scales=scales, dtype=dtype)
+    return torch.ops.vectra.gated_linear_8bit(x, weight, weight_scales, bias, activation, scales=scales, dtype=dtype,
+                                              width=width)
