@@ -34,6 +34,9 @@
  * Tiles: 128 rows of 128.  codes [rows, depth], depth = width rounded up to 128 (the
  * padding is zero); scales [ceil(rows / 1 or 128), 4 ceil(width / 512)] hold e + 127 as
  * bytes (those past ceil(width / 128) are 0 and not used); rows are adjacent.
+ * Products take any byte b from 0 to 254 as 2^(b - 127), and 255 as NaN.  A code that
+ * stands for more than fp32's largest value, as no call here makes one, counts as infinite
+ * there, or, on the 8-bit matrix cores, as the value that it has.
  *
  * Sums of the products: F32 results, and results of at most 32 rows, are exact products
  * added in fp32.  Larger products with 16-bit results run on the 8-bit matrix cores: of

@@ -68,7 +68,7 @@ whose blocks share a power of two, the smallest that no element exceeds 448 time
 for weights, once when a model is loaded.  codes are float8_e4m3fn [..., width
 rounded up to 128] (zeros behind the width), scales float8_e8m0fnu
 [..., 4 ceil(width / 512)] (a tile's: [ceil(rows / 128), ...]; those past
-ceil(width / 128) are not used).  A layer takes float32, float16 or bfloat16 inputs,
+ceil(width / 128) are not used); a scale of e8m0's NaN makes its block NaN.  A layer takes float32, float16 or bfloat16 inputs,
 which it brings into 8 bits itself, and returns their type; or codes with `scales`
 (residual_norm_8bit's, or quantize_blocks'), and returns `dtype`.  bias is the
 result's type or float32, the residual the result's type.  Codes and scales tell a
