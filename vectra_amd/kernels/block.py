@@ -79,7 +79,10 @@ float32 results, and those of at most 32 rows, are exact products of the 8-bit v
 in fp32 sums, rounded once.  float16 and bfloat16 results of more rows come from the
 8-bit matrix cores, which drop, of the 16 products that they add at a time, what lies
 below 2^-13 of the largest one's power of two: with normal operands 1.6e-5 of a
-result, where the rounding to bfloat16 is 1.7e-3 and to float16 2.1e-4.  They have no
+result, where the rounding to bfloat16 is 1.7e-3 and to float16 2.1e-4; 1e-2 of a result
+beside which products of 500 times its size cancel.  (The rounding of such operands to
+e4m3 is up to 2^-4 of a product, but a program whose values are e4m3 to begin with takes
+dtype=torch.float32, whose sums are exact for any rows, and rounds.)  They have no
 derivative: a backward pass through them raises.  Under torch.autocast they run in
 their input's type.
 
