@@ -170,12 +170,16 @@ __global__ __launch_bounds__(C::kThreads, 2) void product8_kernel(const Product8
   struct Scales {
     uint32_t a[C::kTM], b[C::kTN];
   } now, next;
+  // (Loads that the waits below count: relaxed atomics of this wave's scope, which are
+  // ordinary loads to the memory, but which the compiler may not move past another
+  // access, join or leave out.)
+  const auto load_word = [](const uint32_t* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT); };
   const auto load_scales = [&](Scales& s, int word) {
     const int at = min(word, words - 1);
 #pragma unroll
-    for (int t = 0; t < C::kTM; ++t) s.a[t] = a_scales[a_scale[t] + at];
+    for (int t = 0; t < C::kTM; ++t) s.a[t] = load_word(a_scales + a_scale[t] + at);
 #pragma unroll
-    for (int t = 0; t < C::kTN; ++t) s.b[t] = b_scales[b_scale[t] + at];
+    for (int t = 0; t < C::kTN; ++t) s.b[t] = load_word(b_scales + b_scale[t] + at);
   };
 
   f32x16 acc[C::kTN][C::kTM];
