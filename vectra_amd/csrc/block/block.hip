@@ -284,6 +284,9 @@ int check_norm(const Args& a) {
   return VECTRA_BLOCK_OK;
 }
 
+// Gate rows of a call; one serves at most all rows.  (gate_rows is at least 1.)
+int64_t count_gate_rows(int64_t rows, int64_t gate_rows) { return ceil_div(rows, std::min(gate_rows, std::max<int64_t>(rows, 1))); }
+
 // Whether the gradients read the branch and the residual, or h: h where it tells all that
 // matters, without a gate and a post norm and as the forward pass had it, in fp32.
 bool reads_branch(const vectra_norm_grad_args& a) {
@@ -312,7 +315,7 @@ int check_forward(const vectra_norm_args* a) {
     if (int st = check_stride(a->n_stride, a->width, a->rows)) return st;
   if (a->gate) {
     if (a->gate_rows < 1) return VECTRA_BLOCK_ERR_BAD_SHAPE;
-    if (int st = check_stride(a->gate_stride, a->width, ceil_div(a->rows, a->gate_rows))) return st;
+    if (int st = check_stride(a->gate_stride, a->width, count_gate_rows(a->rows, a->gate_rows))) return st;
   }
   return VECTRA_BLOCK_OK;
 }
@@ -374,12 +377,12 @@ int check_backward(const vectra_norm_grad_args* a) {
   if ((a->dpost_weight || a->dpost_bias) && a->post == VECTRA_BLOCK_NO_NORM) return VECTRA_BLOCK_ERR_BAD_OPTION;
   if (a->gate && a->gate_rows < 1) return VECTRA_BLOCK_ERR_BAD_SHAPE;
   if (a->dgate)
-    if (int st = check_stride(a->dgate_stride, a->width, ceil_div(a->rows, a->gate_rows))) return st;
+    if (int st = check_stride(a->dgate_stride, a->width, count_gate_rows(a->rows, a->gate_rows))) return st;
   if (a->rows == 0) return VECTRA_BLOCK_OK;
   if (branch ? !a->x || !a->residual : !a->h) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
   if (a->threshold && !a->rng) return VECTRA_BLOCK_ERR_NULL_ARGUMENT;
   if (a->gate)
-    if (int st = check_stride(a->gate_stride, a->width, ceil_div(a->rows, a->gate_rows))) return st;
+    if (int st = check_stride(a->gate_stride, a->width, count_gate_rows(a->rows, a->gate_rows))) return st;
   const struct {
     const void* p;
     int64_t stride;
