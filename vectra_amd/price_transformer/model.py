@@ -287,10 +287,12 @@ class PriceTransformer(nn.Module):
     def _following(self, i: int):
         """The norm that block i computes with its result: the next block's first, where
         calls of the two would do nothing besides."""
-        pair = self.blocks[i:i + 2]
-        if len(pair) < 2 or not all(plain_modules.is_plain(b, Block) for b in pair) or not pair[0].norm_kernels:
+        block = self.blocks[i]
+        if i + 1 == len(self.blocks) or not plain_modules.is_plain(block, Block) or not block.norm_kernels:
             return None
-        return pair[1].norm1 if plain_modules.is_plain_norm(pair[1].norm1, self.config.d_model) else None
+        after = self.blocks[i + 1]
+        plain = plain_modules.is_plain(after, Block) and plain_modules.is_plain_norm(after.norm1, self.config.d_model)
+        return after.norm1 if plain else None
 
     def forward(self, query_embedding, query_attributes, query_location, query_cell6,
                 valuation_day, radius_km, cand_embedding, cand_attributes, cand_log_price,
