@@ -48,6 +48,8 @@
  * Contract (as vectra_dense.h):
  *  - Plain pointers, sizes and strides; matrices are row-major with unit element stride
  *    and a row stride in ELEMENTS of at least a row; that of a single row is not read.
+ *    Rows are at most 2^21 wide (of a norm VECTRA_BLOCK_NORM_WIDTH), and rows * (width + 512)
+ *    is below 2^35.
  *    Codes begin at a multiple of 16 bytes, scales of 4.
  *  - Every buffer is owned by the caller.  Calls that need scratch memory take a workspace
  *    whose size the _workspace_bytes function tells; it needs no set-up, holds nothing

@@ -11,9 +11,9 @@ in it (u = 2^-24, a rounding to fp32, relative):
   sum      sum e + depth u sum |v|; a term passes through at most `depth`
            additions
 
-The kernels add at most 16 elements in a lane, 6 times across a wave and 16
-waves: 38; torch's row sums pass through fewer than 64 up to the widths of the
-tests.  Sums over rows pass through at most rows + 80 additions.
+The kernels add at most 32 elements in a lane (four chunks of eight), 6 times
+across a wave, and at most 8 waves: 46; torch's row sums pass through fewer than 64
+up to the widths of the tests.  Sums over rows pass through at most rows + 80 additions.
 """
 
 import dataclasses

@@ -14,7 +14,7 @@ namespace {
 
 // ----------------------------------------------------------------- kernels
 
-// y = k * x: a thread takes kGroups groups of eight elements, kSpan groups apart,
+// y = k * x: a thread takes kGroups groups of eight elements, 256 groups apart,
 // their loads issued together.
 template <typename T, typename Index, int kGroups>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, int64_t rows, int64_t width, int64_t x_stride, T* y,

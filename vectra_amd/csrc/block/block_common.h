@@ -81,16 +81,6 @@ __device__ __forceinline__ void drop(f32x4 (&x)[2], uint32_t kept, float scale) 
   for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = kept >> i & 1 ? x[i / 4][i % 4] * scale : 0.f;
 }
 
-// -------------------------------------------------------------------- 8 bits
-
-// The largest magnitude of eight elements, at least `largest`; NaN counts as nothing.
-__device__ __forceinline__ float largest_magnitude(const f32x4 (&v)[2], float largest) {
-#pragma unroll
-  for (int k = 0; k < 8; k += 2)
-    largest = __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(v[k / 4][k % 4]), __builtin_fabsf(v[k / 4][k % 4 + 1])), largest);
-  return largest;
-}
-
 // ------------------------------------------------------------------ vectors
 
 // Eight elements of a per-column vector from `first` on (`left` of them exist, the

@@ -10,9 +10,10 @@
 // vectors are loaded once per workgroup, and the next row's loads are issued before a
 // row is worked on.  The sums of a row cross lanes by DPP moves and lane swaps, and
 // waves through LDS with one barrier each.  What bounds it is HBM: 8192 x 4096 bf16 on
-// an fp32 stream, rms norms on both sides and a gate over all rows, 80 us forward
-// (5.0 TB/s) and 142 backward (4.3); 66560 x 128 bf16, layer norm and dropout, 17.5 us
-// and 34 (3.9, 3.0 TB/s).  Past 4096 columns the registers do not hold a row, its
+// an fp32 stream, rms norms on both sides and a gate over all rows, 82 us forward
+// (4.9 TB/s) and 140 backward with the joining of its sums (4.3).  Short rows are bound by
+// vector issue beside it: 66560 x 128 bf16, layer norm and dropout, 18.8 us and 34.7
+// (3.6, 2.9 TB/s).  Past 4096 columns the registers do not hold a row, its
 // gradients and their sums over the rows: most of the sums are in LDS there, and no row
 // is loaded ahead; past 8192 columns, and in the backward pass with a gate and a post norm,
 // the vectors over the columns are read again for every row.  4096 x 8192, both norms and
@@ -25,7 +26,8 @@
 //
 // The backward pass computes the normalised rows again, from x and r (h is then not
 // read) or from an fp32 h, in fp32 as the forward pass had them; statistics are
-// not kept.  The vectors' gradients are summed over the rows of a workgroup, then over the workgroups by a second launch in a fixed order.
+// not kept.  The vectors' gradients are summed over the rows of a workgroup, then over the
+// workgroups by a second launch in a fixed order.
 #pragma once
 
 #include "block_common.h"
@@ -732,6 +734,8 @@ template <typename T, typename R>
 int launch_norm(const NormParams& p, int cus, hipStream_t stream) {
   const NormShape shape = norm_shape(p.width);
   const int64_t blocks = (p.rows + shape.rows - 1) / shape.rows;
+  // (A CU's 2048 threads; at 111 to 121 registers of one chunk per lane half of these
+  // workgroups are there at once, and the others follow.)
   const int64_t most_blocks = static_cast<int64_t>(cus) * (2048 / shape.threads);
   with_shape(shape, p.width, [&](auto s) {
     using S = decltype(s);

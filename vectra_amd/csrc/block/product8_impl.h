@@ -20,10 +20,11 @@
 // with their powers of two, which is exact, on their way from LDS, and run on the
 // bf16 cores: exact products, fp32 sums.
 //
-// Staging as in the dense products (dense/gemm_impl.h): tiles go from global memory
-// straight into LDS one ahead of the one being multiplied, two of them there, the
-// fragments of one step of 64 ahead in registers, one barrier per tile of 128.
-// Buffer bounds turn rows past the operand into zeros.
+// Staging: tiles go from global memory straight into LDS, and the fragments of one step
+// of 64 ahead of the products into registers.  The 256-tile takes 128 of the contraction
+// per stage, three stages of x and two of W in LDS, one barrier each; the smaller ones 64,
+// four stages of both, three of them on their way or ahead, one barrier each.  Buffer
+// bounds turn rows past the operand into zeros.
 #pragma once
 
 #include "../dense/gemm_impl.h"

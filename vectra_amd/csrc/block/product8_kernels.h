@@ -30,8 +30,12 @@ enum { kLarge8 = 0, kMedium8 = 1, kSmall8 = 2, kTiles8 = 3 };
 constexpr int kTile8[kTiles8] = {256, 128, 64};  // rows and columns
 
 // Rows up to which a product reads the weight straight into registers, and rows and
-// bytes of them up to which its workgroups bring the input into 8 bits themselves.  (64
-// rows so: 4096 -> 4096 18.9 us, tiles 14.3; 8192 -> 8192 56 and 30.)
+// bytes of them up to which its workgroups bring the input into 8 bits themselves.  The
+// bound is part of the contract (exact sums), and no rule on time: 32 rows so and 33 on
+// tiles, bf16 from codes, us: 4096 -> 4096 11.0 and 12.1, 4096 -> 16384 24.3 and 26.1, but
+// 8192 -> 8192 24.4 and 22.5, 16384 -> 4096 33.9 and 23.4, 8192 -> 28672 81.5 and 68.5,
+// gated 2048 -> 2 x 5632 12.4 and 13.8, 4096 -> 2 x 11008 33.8 and 31.2; 17 rows so 9.0,
+// 21.3, 22.9, 25.8, 68.8, 10.9 and 29.1.  (64 rows so: 4096 -> 4096 18.9, 8192 -> 8192 56.)
 constexpr int kFewRows8 = 32, kFewRaw8 = 16, kRawBytes = 16384;
 
 // One definition per type of result.

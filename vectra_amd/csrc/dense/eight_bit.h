@@ -5,8 +5,6 @@
 
 namespace vectra_dense {
 
-constexpr float kCodeMax = 448.f;
-
 // The exponent byte of a block whose largest finite magnitude is `largest`:
 // the smallest e with largest <= 448 * 2^e, at least `lowest`, plus 127.
 // largest = f * 2^x with f in [1, 2): 448 = 1.75 * 2^8.

@@ -25,7 +25,8 @@ dropout, and the residual stream with its norms; and those operators in 8 bits.
 Dropout and norms.  x [..., width] is float32, float16 or bfloat16 (any strides; views without unit
 element stride are copied); the residual, of x's shape, has x's type or float32
 (a stream wider than its branches), and h has the residual's, n x's.  Rows of a
-norm have at most 16,384 elements.  norm is 'rms' or 'layer', post 'none', 'rms'
+norm have at most 16,384 elements; on the GPU those of every operator here at most
+2^21, and rows * (width + 512) stays below 2^35.  norm is 'rms' or 'layer', post 'none', 'rms'
 or 'layer':
 
   rms    x / sqrt(mean(x^2) + eps) * weight + bias
