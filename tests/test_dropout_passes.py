@@ -328,8 +328,20 @@ def test_the_state_moves_with_the_model(device, tmp_path):
             empty = model_lib.PriceTransformer(model.config)
         assert empty.to_empty(device=device).dropout_rng.tolist() == [77, 0]
         assert empty.dropout_rng.device.type == device
+        assert empty.to('meta').to_empty(device=device).dropout_rng.tolist() == [77, 0]
     assert relative(want, model.seed_dropout(11, 5)(*inputs)) < 1e-2  # (once through fp16)
     assert 'dropout_rng' not in model.state_dict()
+
+
+@pytest.mark.gpu
+def test_the_state_follows_weights_that_are_moved_one_by_one():
+    """As wrappers that shard a model do."""
+    model, inputs = build('cuda')
+    with torch.no_grad():
+        want = model.seed_dropout(11, 5)(*inputs)
+        model.seed_dropout(11, 5).dropout_rng = model.dropout_rng.cpu()
+        assert torch.equal(model(*inputs), want)
+    assert model.dropout_rng.is_cuda and model.dropout_rng.tolist() == [11, 6]
 
 
 @pytest.mark.parametrize('fused', [False, True])

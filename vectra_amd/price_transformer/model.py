@@ -210,9 +210,14 @@ class PriceTransformer(nn.Module):
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        if self.config.dropout:  # (the state goes where the weights go)
-            self.dropout_rng = self.dropout_rng.to(fn(self.dropout_rng).device)
+        if self.config.dropout:
+            self._move_dropout(fn(self.dropout_rng).device)
         return self
+
+    def _move_dropout(self, device):
+        """The state goes where the weights go, but not where it would be lost."""
+        if self.dropout_rng.device != device and device.type != 'meta':
+            self.dropout_rng = self.dropout_rng.to(device)
 
     def seed_dropout(self, seed: int, passes: int = 0) -> 'PriceTransformer':
         """Dropout's generator: training pass number `passes` of `seed` comes next.  (Data
@@ -322,6 +327,7 @@ class PriceTransformer(nn.Module):
         if not self.config.dropout:
             rng = None
         elif rng is None:
+            self._move_dropout(tokens.device)  # (where a wrapper has moved the weights one by one)
             rng = self.dropout_pass()
         normed = None
         for i, block in enumerate(self.blocks):
