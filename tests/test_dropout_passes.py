@@ -339,7 +339,8 @@ def test_the_state_follows_weights_that_are_moved_one_by_one():
     model, inputs = build('cuda')
     with torch.no_grad():
         want = model.seed_dropout(11, 5)(*inputs)
-        model.seed_dropout(11, 5).dropout_rng = model.dropout_rng.cpu()
+        model.seed_dropout(11, 5)
+        model.dropout_rng = model.dropout_rng.cpu()
         assert torch.equal(model(*inputs), want)
     assert model.dropout_rng.is_cuda and model.dropout_rng.tolist() == [11, 6]
 
