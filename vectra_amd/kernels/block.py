@@ -26,8 +26,8 @@ Dropout and norms.  x [..., width] is float32, float16 or bfloat16 (any strides;
 element stride are copied); the residual, of x's shape, has x's type or float32
 (a stream wider than its branches), and h has the residual's, n x's.  Rows of a
 norm have at most 16,384 elements; on the GPU those of every operator here at most
-2^21, and rows * (width + 512) stays below 2^35.  norm is 'rms' or 'layer', post 'none', 'rms'
-or 'layer':
+2^21, and rows * (width + 512) stays below 2^35.  norm is 'rms' or 'layer', post
+'none', 'rms' or 'layer':
 
   rms    x / sqrt(mean(x^2) + eps) * weight + bias
   layer  (x - mean) / sqrt(var + eps) * weight + bias
@@ -50,12 +50,12 @@ dropout_pass of it.  (Not from state.clone() followed by state[1].add_(1): the
 compiler behind torch.compile removes the clone, and a compiled backward pass would
 draw from what the addition left, another mask, without an error.)  A function that
 activation checkpointing runs again takes its draws as an argument; dropout_pass
-itself raises within a backward pass, where it would draw others.
-dropout and residual_norm with equal rng,
-stream and shape drop the same elements.  Under torch.vmap, where every sample would draw the same, dropout of what is batched
-is refused unless rng is batched too or randomness is 'same'.  rng is read when the kernel runs, so a
-program that replays a captured graph changes it between replays (rng[1].add_(1))
-and draws anew.
+itself raises within a backward pass, where it would draw others.  dropout and
+residual_norm with equal rng, stream and shape drop the same elements.  Under
+torch.vmap, where every sample would draw the same, dropout of what is batched is
+refused unless rng is batched too or randomness is 'same'.  rng is read when the
+kernel runs, so a program that replays a captured graph changes it between replays
+(rng[1].add_(1), or dropout_pass in the graph) and draws anew.
 
 dropout and residual_norm have gradients for every tensor argument but rng;
 residual_norm keeps x and the residual for them where there is a gate, a post
@@ -69,8 +69,8 @@ whose blocks share a power of two, the smallest that no element exceeds 448 time
 for weights, once when a model is loaded.  codes are float8_e4m3fn [..., width
 rounded up to 128] (zeros behind the width), scales float8_e8m0fnu
 [..., 4 ceil(width / 512)] (a tile's: [ceil(rows / 128), ...]; those past
-ceil(width / 128) are not used); a scale of e8m0's NaN makes its block NaN.  A layer takes float32, float16 or bfloat16 inputs,
-which it brings into 8 bits itself, and returns their type; or codes with `scales`
+ceil(width / 128) are not used); a scale of e8m0's NaN makes its block NaN.  A layer
+takes float32, float16 or bfloat16 inputs, which it brings into 8 bits itself, and returns their type; or codes with `scales`
 (residual_norm_8bit's, or quantize_blocks'), and returns `dtype`.  bias is the
 result's type or float32, the residual the result's type.  Codes and scales tell a
 weight's width only rounded up to a block of 128: with `width`, the weight's own, an x

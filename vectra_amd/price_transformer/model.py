@@ -230,8 +230,9 @@ class PriceTransformer(nn.Module):
 
     def dropout_pass(self):
         """What the next pass's dropout draws from, counted on; None where nothing is
-        dropped (blocks drop where they are in training, each by itself).  A pass that is run again in the backward one (activation checkpointing
-        of the whole model) takes it as an argument:
+        dropped (blocks drop where they are in training, each by itself).  A pass that is
+        run again in the backward one (activation checkpointing of the whole model) takes
+        it as an argument:
 
             checkpoint(model, *inputs, model.dropout_pass(), use_reentrant=False)
         """
